@@ -381,7 +381,8 @@ def _plain_plan(s):
     # blocks of ended requests go behind the ring's last
     back = torch.where(ended, held, 0)
     behind = (torch.cumsum(back, 0) - back)[:, None] + cols
-    put = (cols < back[:, None]) & (count + behind < size)
+    given = torch.minimum(back, (size - count - behind[:, 0]).clamp(min=0))
+    put = cols < given[:, None]
     ring = torch.cat([s["free"], s["free"][:1]])
     ring.scatter_(0, torch.where(put, (head + count + behind) % size, size).view(-1),
                   s["tables"].view(-1))
@@ -390,9 +391,11 @@ def _plain_plan(s):
     s["held_out"].copy_(torch.where(ended, 0, held + taken))
     total = taken.sum()
     s["state_out"].copy_(torch.stack([(head + total) % size,
-                                      count - total + torch.minimum(back.sum(), size - count)]))
-    s["info"].copy_(torch.stack([torch.where(wide, 2, torch.where(served, 0, 1)), held, taken,
-                                 (head + before) % size], 1))
+                                      count - total + given.sum()]))
+    s["info"].copy_(torch.stack([torch.where(wide, 2, torch.where(served, 0, 1)), held,
+                                 taken - given,
+                                 (head + torch.where(ended, count + behind[:, 0], before)) % size],
+                                1))
     i = torch.arange(n, device=held.device)
     at = lengths[:, None] + i
     ids = s["tables"].long().gather(1, (at // block).clamp(max=m - 1))
