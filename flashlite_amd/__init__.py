@@ -37,4 +37,19 @@ forward_naive = _ext.forward_naive
 forward_flash2_ex = _ext.forward_flash2_ex
 splitkv_workspace_bytes = _ext.splitkv_workspace_bytes
 
-__all__ = ["forward_flash2", "forward_naive", "forward_flash2_ex", "splitkv_workspace_bytes"]
+# Serving over a paged cache: a step's blocks and slots, its drafts' ancestors,
+# rotary positions (and their gradient) with the cache's writes, attention for
+# trees of drafted tokens or one token.
+plan_cache = _ext.plan_cache
+plan_tree = _ext.plan_tree
+forward_rotary = _ext.forward_rotary
+backward_rotary = _ext.backward_rotary
+rotary_to_cache = _ext.rotary_to_cache
+forward_tree = _ext.forward_tree
+tree_workspace_bytes = _ext.tree_workspace_bytes
+
+from .rotary import rotary_frequencies  # noqa: E402
+
+__all__ = ["forward_flash2", "forward_naive", "forward_flash2_ex", "splitkv_workspace_bytes",
+           "plan_cache", "plan_tree", "forward_rotary", "backward_rotary", "rotary_to_cache",
+           "rotary_frequencies", "forward_tree", "tree_workspace_bytes"]

@@ -39,9 +39,16 @@ EXPORTED = (
     "fl_attn_config_id",
     "fl_attn_workspace_bytes",
     "fl_attn_fwd_ws",
+    "fl_attn_cache_plan",
+    "fl_attn_tree_plan",
+    "fl_attn_rotary",
+    "fl_attn_rotary_cache",
+    "fl_attn_tree_workspace_bytes",
+    "fl_attn_tree_fwd",
 )
 
 SCRATCH_BYTES = 8 << 20  # FL_ATTN_SCRATCH_BYTES
+MAX_DRAFTS = 512  # FL_ATTN_MAX_DRAFTS
 
 
 class FlAttnParams(ctypes.Structure):
@@ -72,6 +79,101 @@ class FlAttnParamsEx(ctypes.Structure):
         ("v_stride", ctypes.c_int64 * 3),
         ("o_stride", ctypes.c_int64 * 3),
         ("lse", ctypes.c_void_p),
+    ]
+
+
+class FlCachePlanParams(ctypes.Structure):
+    """Mirror of ``fl_cache_plan_params``."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "lengths", "counts", "block_tables", "held", "held_out", "free_blocks", "free_state",
+        "free_state_out", "positions", "slots", "info")] + [(n, ctypes.c_int64) for n in (
+            "batch", "width", "block_size", "max_blocks", "table_stride", "pool")]
+
+
+class FlTreePlanParams(ctypes.Structure):
+    """Mirror of ``fl_tree_plan_params``."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "parents", "lengths", "counts", "mask", "positions")] + [
+            (n, ctypes.c_int64) for n in ("batch", "drafts", "parent_stride")]
+
+
+class FlRotaryParams(ctypes.Structure):
+    """Mirror of ``fl_rotary_params``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("q_out_stride", ctypes.c_int64 * 3),
+        ("k_out_stride", ctypes.c_int64 * 3),
+        ("positions", ctypes.c_void_p),
+        ("position_stride", ctypes.c_int64 * 2),
+        ("position_bits", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("freqs", ctypes.c_void_p),
+        ("pairs", ctypes.c_int64),
+        ("batch", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("scale", ctypes.c_double),
+        ("interleaved", ctypes.c_int32),
+        ("transpose", ctypes.c_int32),
+    ]
+
+
+class FlCacheStore(ctypes.Structure):
+    """Mirror of ``fl_cache_store``."""
+
+    _fields_ = [
+        ("v", ctypes.c_void_p),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("k_cache_stride", ctypes.c_int64 * 3),
+        ("v_cache_stride", ctypes.c_int64 * 3),
+        ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int64),
+        ("slots", ctypes.c_void_p),
+        ("slot_stride", ctypes.c_int64 * 2),
+    ]
+
+
+class FlTreeParams(ctypes.Structure):
+    """Mirror of ``fl_tree_params``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("o_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("block_tables", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("mask_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("drafts", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int64),
+        ("max_blocks", ctypes.c_int64),
+        ("sm_scale", ctypes.c_double),
+        ("dtype", ctypes.c_int32),
     ]
 
 
@@ -132,6 +234,18 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.fl_attn_splitkv_noalloc_bytes.restype = ctypes.c_int64
     lib.fl_attn_config_id.argtypes = [ctypes.c_char_p]
     lib.fl_attn_config_id.restype = ctypes.c_int
+    for name, args in (("fl_attn_cache_plan", [FlCachePlanParams]),
+                       ("fl_attn_tree_plan", [FlTreePlanParams]),
+                       ("fl_attn_rotary", [FlRotaryParams]),
+                       ("fl_attn_rotary_cache", [FlRotaryParams, FlCacheStore])):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(a) for a in args] + [ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+    lib.fl_attn_tree_workspace_bytes.argtypes = [ctypes.POINTER(FlTreeParams)]
+    lib.fl_attn_tree_workspace_bytes.restype = ctypes.c_int64
+    lib.fl_attn_tree_fwd.argtypes = [ctypes.POINTER(FlTreeParams), ctypes.c_void_p, ctypes.c_int64,
+                                     ctypes.c_void_p]
+    lib.fl_attn_tree_fwd.restype = ctypes.c_int
     _lib = lib
     return lib
 
@@ -211,6 +325,7 @@ def tensor_params_ex(q, k, v, o, sm_scale=0.0, causal=False, lse=None) -> FlAttn
 
 DTYPE_F16 = 0  # FL_DTYPE_F16
 DTYPE_BF16 = 1
+DTYPE_F32 = 2  # the rotary only
 
 
 def workspace_bytes(params: FlAttnParamsEx, dtype: int) -> int:

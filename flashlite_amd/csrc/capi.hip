@@ -34,6 +34,18 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
+}  // namespace
+
+int fl::set_error(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+namespace {
+
 // float(log2 e) widened to double, as the reference multiplies a double
 // sm_scale by its float LOG2_E constant (kernel_flash2.cu:16, :772).
 constexpr double kLog2eF = (double)1.44269504088896340736f;

@@ -149,4 +149,8 @@ hipError_t launch_splitkv_combine(const FwdArgs& a, float* part, int nsplit, hip
 int64_t naive_max_seq(int64_t head_dim);
 hipError_t launch_naive(const FwdArgs& a, hipStream_t stream);
 
+// Records the calling thread's error message (fl_attn_last_error) and returns
+// `code` (capi.hip).
+int set_error(int code, const char* fmt, ...);
+
 }  // namespace fl

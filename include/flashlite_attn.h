@@ -207,6 +207,209 @@ int fl_attn_fwd_f16_splitkv_noalloc(const fl_attn_params_ex* p, int32_t num_spli
 int64_t fl_attn_splitkv_noalloc_bytes(const fl_attn_params_ex* p, int32_t num_splits);
 
 /*
+ * Serving over a paged cache: the blocks and slots of each step's tokens, the
+ * ancestors of drafted tokens, rotary positions with the cache's writes, and
+ * attention for drafted tokens (or one token) over the cache.  No counterpart
+ * in the reference.
+ *
+ * The cache is blocks of block_size rows of every key/value head: k_cache and
+ * v_cache are [num_blocks, kv_heads, block_size, head_dim] views with strides
+ * {block, head, row} in elements (a cache stored [blocks, block_size, heads,
+ * dim] passes as its transpose).  Token t of request b lies in row
+ * t % block_size of block block_tables[b][t / block_size]; its slot is
+ * block * block_size + row.  A cache that is not paged is one block a request.
+ */
+
+/*
+ * Blocks, slots and positions of a step's new tokens, on the GPU from the
+ * requests' lengths.
+ *
+ * lengths[b] tokens are in the cache, counts[b] come (0 .. width; more are
+ * taken as width); counts[b] < 0: the request has ended and gives its blocks
+ * back.  held[b] blocks of row b of block_tables are its own.  The free blocks
+ * are a ring: free_state = {head, count}, the count entries of free_blocks
+ * from head on (modulo pool).  A request that needs more blocks than it holds
+ * (ceil((lengths + counts) / block_size)) takes them from the ring's head, in
+ * the order of the requests; blocks of ended requests are put behind the
+ * ring's last, in order, and are free from the next call on (what a full ring
+ * has no room for is dropped).
+ *
+ * Outputs: block_tables (entries of the blocks taken), held_out and
+ * free_state_out (each may be its input), positions [batch, width] =
+ * lengths[b] + i, slots [batch, width], both -1 where there is no token (i >=
+ * counts[b], a request not served, a negative table entry), and info [batch,
+ * 4]: {0 served, 1 not enough free blocks, 2 the table row is too short;
+ * blocks held before; blocks taken, or minus those put back; the ring's index
+ * of the first of them}.  A request that is not served keeps what it has; one
+ * with nothing to take is always served.  Values out of range (a held count
+ * past the row, a head past the ring) are clamped, never followed.
+ */
+typedef struct fl_cache_plan_params {
+  const int32_t* lengths;
+  const int32_t* counts;
+  int32_t* block_tables; /* rows of max_blocks entries, table_stride apart */
+  const int32_t* held;
+  int32_t* held_out;
+  int32_t* free_blocks;
+  const int32_t* free_state;
+  int32_t* free_state_out;
+  int32_t* positions;
+  int64_t* slots;
+  int32_t* info;
+  int64_t batch;
+  int64_t width;
+  int64_t block_size;
+  int64_t max_blocks;
+  int64_t table_stride;
+  int64_t pool;
+} fl_cache_plan_params;
+
+int fl_attn_cache_plan(const fl_cache_plan_params* p, void* stream);
+
+/*
+ * Ancestors and positions of drafted tokens.  parents[b][i] is the draft that
+ * draft i follows, an earlier one; any other value means that it follows the
+ * request's last token.  mask[b][i] gets the bits of i and its ancestors, in
+ * ceil(drafts / 64) words (bit j % 64 of word j / 64 for draft j), positions
+ * lengths[b] + the number of ancestors.  Drafts from counts[b] on (counts may
+ * be NULL: all are there) get an empty mask and position -1.  At most
+ * FL_ATTN_MAX_DRAFTS drafts a request.
+ */
+#define FL_ATTN_MAX_DRAFTS 512
+typedef struct fl_tree_plan_params {
+  const int32_t* parents; /* rows parent_stride apart */
+  const int32_t* lengths;
+  const int32_t* counts;
+  int64_t* mask;
+  int32_t* positions;
+  int64_t batch;
+  int64_t drafts;
+  int64_t parent_stride;
+} fl_tree_plan_params;
+
+int fl_attn_tree_plan(const fl_tree_plan_params* p, void* stream);
+
+/*
+ * Rotary positions: the pairs of the first 2 * pairs columns of every q and k
+ * row turn by the angle position * freqs[j] (freqs: radians a position,
+ * 64-bit; the angle is reduced in 64 bits, so far positions stay exact), and
+ * are multiplied by `scale`; the other columns are copied.  Pair j is columns
+ * {j, j + pairs}, or {2j, 2j + 1} with interleaved.  With transpose the angle
+ * is negated: the gradient of the same call.  q, k, q_out and k_out are
+ * [batch, heads or kv_heads, rows, head_dim] views with strides {batch, head,
+ * row} in elements; outputs may be their inputs.  k may be NULL (no k).
+ * positions are int32 (or int64: position_bits 64) [batch, rows], strides
+ * {batch, row}.  head_dim 64 or 128; dtype FL_DTYPE_F16, FL_DTYPE_BF16 or (not
+ * with a cache) FL_DTYPE_F32.
+ *
+ * fl_attn_rotary_cache does the same for a step's tokens and stores them:
+ * rotated k and v go to row slots[b][i] of the caches, rotated q to q_out
+ * (k_out is not used).  A token whose slot is negative or past num_blocks *
+ * block_size is passed over: its q_out row and the cache stay as they were.
+ * Two tokens must not have the same slot.
+ */
+#define FL_DTYPE_F32 2
+typedef struct fl_rotary_params {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_out_stride[3];
+  const void* positions;
+  int64_t position_stride[2];
+  int32_t position_bits;
+  int32_t dtype;
+  const double* freqs;
+  int64_t pairs;
+  int64_t batch;
+  int64_t heads;
+  int64_t kv_heads;
+  int64_t rows;
+  int64_t head_dim;
+  double scale;
+  int32_t interleaved;
+  int32_t transpose;
+} fl_rotary_params;
+
+typedef struct fl_cache_store {
+  const void* v;
+  int64_t v_stride[3];
+  void* k_cache;
+  void* v_cache;
+  int64_t k_cache_stride[3];
+  int64_t v_cache_stride[3];
+  int64_t num_blocks;
+  int64_t block_size;
+  const int64_t* slots;
+  int64_t slot_stride[2];
+} fl_cache_store;
+
+int fl_attn_rotary(const fl_rotary_params* p, void* stream);
+int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, void* stream);
+
+/*
+ * Attention of drafted tokens over a paged cache (fp16 or bf16, head_dim 64 or
+ * 128).  Request b has lengths[b] tokens and counts[b] drafts (counts may be
+ * NULL: `drafts` of them), whose keys and values are in the cache behind them,
+ * draft j as token lengths[b] + j.  Draft i sees every token, and draft j
+ * where bit j of its mask is set (mask [batch, drafts, ceil(drafts / 64)]
+ * words, batches mask_stride words apart, 0 for one mask for all; without a
+ * mask the drafts are a chain, draft i sees drafts 0 .. i: a decode step at
+ * drafts = 1, a prompt's chunk beyond).  q and o are [batch, heads, drafts,
+ * head_dim] views with strides {batch, head, row}; heads is a multiple of
+ * kv_heads, head h reads key/value head h / (heads / kv_heads).
+ *
+ * A row that sees nothing is 0 (its log-sum-exp -inf); rows of drafts from
+ * counts[b] on are left as they were, o and lse alike.  A key whose block
+ * table entry is not in [0, num_blocks) is seen by nobody.  What a row does
+ * not see does not reach it, NaN and infinities in k_cache and v_cache
+ * included.  lengths are clamped to the table's rows (max_blocks *
+ * block_size), with the drafts behind them.  lse: optional fp32 [batch, heads,
+ * drafts] (contiguous).
+ *
+ * Few query rows over many keys are split over the CUs; partial results go to
+ * `workspace` (fl_attn_tree_workspace_bytes, from the sizes alone; 0: none
+ * is used, -1: `p` is rejected) and a second kernel merges them.  With less
+ * (or NULL) the call runs without.  The workspace is 16-byte aligned device
+ * memory that needs no initial values; calls that may overlap must not share
+ * one.
+ */
+typedef struct fl_tree_params {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* o;
+  float* lse;
+  int64_t q_stride[3];
+  int64_t o_stride[3];
+  int64_t k_stride[3]; /* {block, head, row} */
+  int64_t v_stride[3];
+  const int32_t* block_tables; /* rows of max_blocks entries, table_stride apart */
+  int64_t table_stride;
+  const int32_t* lengths;
+  const int32_t* counts;
+  const int64_t* mask;
+  int64_t mask_stride;
+  int64_t batch;
+  int64_t heads;
+  int64_t kv_heads;
+  int64_t drafts;
+  int64_t head_dim;
+  int64_t num_blocks;
+  int64_t block_size;
+  int64_t max_blocks;
+  double sm_scale; /* 0.0 means 1/sqrt(head_dim) */
+  int32_t dtype;
+} fl_tree_params;
+
+int64_t fl_attn_tree_workspace_bytes(const fl_tree_params* p);
+int fl_attn_tree_fwd(const fl_tree_params* p, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+
+/*
  * Un-fused baseline: one work-group per query row, scores staged in LDS.
  * Any head_dim >= 1; seq limited by LDS (about 40k keys at D=64).
  * Replaces flash_attn_forward_naive's scale handling and launch
