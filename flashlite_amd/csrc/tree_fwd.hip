@@ -3,7 +3,8 @@
 //
 // The rows of one key/value head are its group of query heads times the drafts
 // (row r: draft r / group, head r % group), so a cached key is read once for
-// all of them.  A unit is 32 such rows of one (request, key/value head).
+// all of them.  A unit is 32 RW such rows of one (request, key/value head): a
+// work-group's 4 waves are RW row blocks times 4 / RW key groups.
 
 #include <cmath>
 
@@ -27,6 +28,11 @@ struct TreeGeom {
   int batch, heads, kv_heads, group, drafts, rows, words, blocks_of_rows;
   int num_blocks, max_blocks;
   FastDiv block;
+  // split launches: partial results [2 * grid][32 RW][kPartStride], and the
+  // least steps of a work-group
+  float* part;
+  int grid, least;
+  int xcds;
 };
 
 __device__ __forceinline__ int divide(int n, const FastDiv& f) {
@@ -166,54 +172,122 @@ __device__ __forceinline__ void fetch4(uint64_t address, const void* lds) {
 
 constexpr int kWaves = 4;
 
-// Four waves own one unit's 32 rows; wave w walks key tiles w, w + 4, ...,
-// each through a K and a V slot of its own, and the partial results meet in
-// LDS.  Keys are found through the block table: lane l looks up key l of a
-// tile (its table entry fetched by DMA two tiles ahead), writes the key's row
-// addresses to a small table in LDS, and each 1 KiB fetch reads its lanes'
-// addresses there, so pages may end anywhere in a tile.
-template <int D, class T>
-__global__ void __launch_bounds__(64 * kWaves, 2)
-tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
-                float cr) {
+// One request: its tokens and its drafts that are there.
+struct Request {
+  int length, count;
+};
+
+__device__ __forceinline__ Request request(const TreeGeom& g, int b) {
+  Request r;
+  r.count = g.counts ? min(max(g.counts[b], 0), g.drafts) : g.drafts;
+  r.length = min(max(g.lengths[b], 0), g.max_blocks * g.block.d);
+  return r;
+}
+
+// Keys that row block rb (of `rows_of_block` rows) of a request walks, 0 where
+// no draft of it is there; with a chain through its last row's draft.
+__device__ __forceinline__ int unit_drafts(const TreeGeom& g, const Request& r, int rb,
+                                           int rows_of_block) {
+  int drafts = min(r.count, g.max_blocks * g.block.d - r.length);
+  if (g.mask == nullptr)
+    drafts = min(drafts, (min((rb + 1) * rows_of_block, g.rows) - 1) / g.group + 1);
+  return drafts;
+}
+
+template <int D, int RW>
+__device__ __forceinline__ int unit_steps(const TreeGeom& g, const Request& r, int rb) {
+  constexpr int kStepKeys = (kWaves / RW) * (D == 64 ? kBc : kBc2);
+  if (rb * 32 * RW / g.group >= r.count) return 0;
+  return (r.length + unit_drafts(g, r, rb, 32 * RW) + kStepKeys - 1) / kStepKeys;
+}
+
+// Steps of all row blocks of one key/value head of a request.
+template <int D, int RW>
+__device__ __forceinline__ long long head_steps(const TreeGeom& g, int b) {
+  const Request r = request(g, b);
+  long long n = 0;
+  for (int rb = 0; rb < g.blocks_of_rows; ++rb) n += unit_steps<D, RW>(g, r, rb);
+  return n;
+}
+
+// Sums over a wave's lanes: inclusive from lane 0, and whole.
+__device__ __forceinline__ long long wave_scan(long long x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const long long y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+// Steps of all requests (each wave by itself).
+template <int D, int RW>
+__device__ __forceinline__ long long all_steps(const TreeGeom& g) {
+  long long n = 0;
+  for (int b0 = 0; b0 < g.batch; b0 += 64) {
+    const int b = b0 + (threadIdx.x & 63);
+    if (b < g.batch) n += head_steps<D, RW>(g, b);
+  }
+  return __shfl(wave_scan(n), 63) * g.kv_heads;
+}
+
+// A split launch deals the steps of all units, in order, evenly to the grid's
+// work-groups; every wave that asks gets the same answer.
+__device__ __forceinline__ long long steps_each(const TreeGeom& g, long long all) {
+  const long long even = (all + g.grid - 1) / g.grid;
+  return even > g.least ? even : g.least;
+}
+
+// The work-group's LDS: key and value tiles, and per wave the row addresses of
+// the next tile's keys and table entries fetched ahead.
+template <int RW>
+struct Shared {
+  static constexpr int kSlots = RW;  // of each key group
+  uint8_t tile[kWaves / RW][kSlots][2][kTileBytes];
+  uint64_t where[kWaves][2][64];
+  int32_t ids[kWaves][RW == 1 ? 2 : kSlots][64];
+  float2 ml[kWaves][64];
+};
+
+// One unit's part over steps [s0, s1) by this work-group: the result goes to O
+// (and lse) with part == nullptr, or unnormalised to `part`.
+template <int D, class T, int RW>
+__device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t* V, T* O,
+                                     const TreeGeom& g, Shared<RW>& sh, int b, int kvh, int rb,
+                                     const Request& req, int s0, int s1, float* part, float cq,
+                                     float cr) {
   using RowsT = TreeRows<D, T>;
   using V8 = typename RowsT::V8;
   constexpr int kKeys = RowsT::kKeys, kRowB = 2 * D;
+  constexpr int KW = kWaves / RW;
   constexpr int kLanes = kRowB / 16;      // lanes a row of a fetch
   constexpr int kSegRows = 64 / kLanes;   // rows a fetch
+  constexpr int kSegs = 8 / RW;           // fetches of a tile by this wave
+  constexpr int kSlots = RW;
   constexpr int kAcc = D / 2;
+  constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
   static_assert(kKeys * kRowB == kTileBytes, "tile size");
-  __shared__ __attribute__((aligned(16))) uint8_t buf[kWaves][2][kTileBytes];
-  __shared__ __attribute__((aligned(16))) uint64_t where[kWaves][2][64];  // K, V row addresses
-  __shared__ __attribute__((aligned(16))) int32_t ids[kWaves][2][64];
-  __shared__ float2 mlbuf[kWaves][64];
 
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // The unit.
-  const int per = g.kv_heads * g.blocks_of_rows;
-  const int b = blockIdx.x / per;
-  const int rest = blockIdx.x - b * per;
-  const int kvh = rest / g.blocks_of_rows, rb = rest - kvh * g.blocks_of_rows;
-  const int capacity = g.max_blocks * g.block.d;
-  const int count = g.counts ? min(max(g.counts[b], 0), g.drafts) : g.drafts;
-  const int length = min(max(g.lengths[b], 0), capacity);
-  const int row0 = 32 * rb;
-  if (row0 / g.group >= count) return;  // no draft of these rows is there
-  int drafts = min(count, capacity - length);  // with keys
-  if (g.mask == nullptr)  // a chain: the rows' last draft sees no later one
-    drafts = min(drafts, (min(row0 + 32, g.rows) - 1) / g.group + 1);
+  const int rw = w % RW, kg = w / RW;  // row block and key group
+  const int length = req.length;
+  const int drafts = unit_drafts(g, req, rb, 32 * RW);
   const int keys = length + drafts;
   const int tiles = (keys + kKeys - 1) / kKeys;
-  const int n = tiles > w ? (tiles - w + kWaves - 1) / kWaves : 0;  // this wave's
+  const int first = s0 * KW + kg;  // this key group's tiles: first, first + KW, ...
+  const int last = min(s1 * KW, tiles);
+  const int n = RW == 1 ? (last > first ? (last - first + KW - 1) / KW : 0) : s1 - s0;
 
   RowsT rows;
   rows.place(lane, cr);
-  const int row = row0 + rows.col;
+  const int local = 32 * rw + rows.col;
+  const int row = 32 * RW * rb + local;
   const int my_row = min(row, g.rows - 1);
   const int draft = my_row / g.group;
   const int head = kvh * g.group + (my_row - draft * g.group);
-  const bool mine = row < g.rows && draft < count;
+  const bool mine = row < g.rows && draft < req.count;
   {
     const T* q = Q + (b * g.q_sb + head * g.q_sh + draft * g.q_sr) + 8 * rows.g;
     const uint32_t sign = cq < 0.0f ? 0x80008000u : 0u;
@@ -227,7 +301,7 @@ tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tree
   }
   const int64_t* const mask =
       g.mask ? g.mask + b * g.mask_stride + (long long)draft * g.words : nullptr;
-  // This lane's row's visible keys of tile [k0, k0 + 64) behind the prefix.
+  // This lane's row's visible keys of tile [k0, k0 + 64) that is not all prefix.
   auto seen_bits = [&](int k0) __attribute__((always_inline)) {
     const int d0 = k0 - length;  // the tile's first draft
     const int from = max(d0, 0);
@@ -235,9 +309,9 @@ tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tree
     if (mask == nullptr) {
       x &= first_bits(draft + 1 - from);
     } else {
-      const int w0 = from >> 6, sh = from & 63;
-      uint64_t m = w0 < g.words ? (uint64_t)mask[w0] >> sh : 0;
-      if (sh != 0 && w0 + 1 < g.words) m |= (uint64_t)mask[w0 + 1] << (64 - sh);
+      const int w0 = from >> 6, shift = from & 63;
+      uint64_t m = w0 < g.words ? (uint64_t)mask[w0] >> shift : 0;
+      if (shift != 0 && w0 + 1 < g.words) m |= (uint64_t)mask[w0 + 1] << (64 - shift);
       x &= m;
     }
     return d0 >= 0 ? x : (d0 > -64 ? x << -d0 : 0) | first_bits(-d0);
@@ -246,75 +320,57 @@ tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tree
   const uint64_t table = (uint64_t)(uintptr_t)(g.tables + b * g.table_stride);
   const uint64_t kbase = (uint64_t)(uintptr_t)(K + kvh * g.k_head);
   const uint64_t vbase = (uint64_t)(uintptr_t)(V + kvh * g.v_head);
-  // Key l of this wave's tile i (past the last: the last again).
+  int32_t(*const ids)[64] = sh.ids[w];
+  uint64_t(*const where)[64] = sh.where[w];
+  // Key l of this key group's tile i (past the last key: the last again).
   auto key_of = [&](int i) __attribute__((always_inline)) {
-    return min((w + kWaves * i) * kKeys + (lane & (kKeys - 1)), keys - 1);
+    return min((first + KW * i) * kKeys + (lane & (kKeys - 1)), keys - 1);
   };
-  auto fetch_ids = [&](int i) __attribute__((always_inline)) {
-    fetch4(table + 4 * (uint64_t)divide(key_of(i), g.block), ids[w][i & 1]);
+  auto fetch_ids = [&](int i, int slot) __attribute__((always_inline)) {
+    fetch4(table + 4 * (uint64_t)divide(key_of(i), g.block), ids[slot]);
   };
   // Row addresses of tile i; the result has a bit per key with a block.
-  auto locate = [&](int i) __attribute__((always_inline)) {
+  auto locate = [&](int i, int slot) __attribute__((always_inline)) {
     const int key = key_of(i);
     const int in = key - divide(key, g.block) * g.block.d;
-    int id = ids[w][i & 1][lane];
+    int id = ids[slot][lane];
     const bool ok = (uint32_t)id < (uint32_t)g.num_blocks;
     id = ok ? id : 0;
-    where[w][0][lane] = kbase + (id * g.k_blk + in * g.k_row);
-    where[w][1][lane] = vbase + (id * g.v_blk + in * g.v_row);
+    where[0][lane] = kbase + (id * g.k_blk + in * g.k_row);
+    where[1][lane] = vbase + (id * g.v_blk + in * g.v_row);
     return __builtin_amdgcn_ballot_w64(ok);
   };
-  auto fetch = [&](int t) __attribute__((always_inline)) {  // 0: K, 1: V
+  auto fetch = [&](int t, uint8_t* tile) __attribute__((always_inline)) {  // 0: K, 1: V
 #pragma unroll
-    for (int seg = 0; seg < 8; ++seg) {
+    for (int i = 0; i < kSegs; ++i) {
+      const int seg = rw * kSegs + i;
       const int r = kSegRows * seg + lane / kLanes;
       const int phys = lane & (kLanes - 1);
       const int chunk = phys ^ (D == 64 ? (t ? v_swz(r) : k_swz(r))
                                         : (t ? v_swz128(r) : k_swz128(r)));
-      fetch16(where[w][t][r] + 16 * chunk, buf[w][t] + 1024 * seg);
+      fetch16(where[t][r] + 16 * chunk, tile + 1024 * seg);
     }
   };
 
-  uint64_t ok = 0;
-  if (n > 0) {
-    fetch_ids(0);
-    fetch_ids(1);
-    asm volatile("s_waitcnt vmcnt(1)" : : : "memory");
-    ok = locate(0);
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-    fetch(0);
-    fetch(1);
-  }
   bool unset = true;
-  for (int i = 0; i < n; ++i) {
-    typename RowsT::Scores s;
-    typename RowsT::Probs p;
-    asm volatile("s_waitcnt vmcnt(8)" : : : "memory");  // K(i), and the ids of i + 1
-    rows.scores(buf[w][0], s);
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // its operands are in registers
-    const bool more = i + 1 < n;
-    uint64_t ok_next = 0;
-    if (more) {
-      ok_next = locate(i + 1);
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      fetch_ids(i + 2);
-      fetch(0);
-    }
-    const int k0 = (w + kWaves * i) * kKeys;
-    const bool checked = k0 + kKeys > length || ~ok != 0;
-    uint64_t seen = ~(uint64_t)0;
+  uint64_t seen = 0;
+  bool checked = false;
+  // Scores of tile i in s to probabilities.
+  auto softmax = [&](int i, uint64_t ok, typename RowsT::Scores& s,
+                     typename RowsT::Probs& p) __attribute__((always_inline)) {
+    const int k0 = (first + KW * i) * kKeys;
+    checked = k0 + kKeys > length || ~ok != 0;
     if (checked) {
       seen = seen_bits(k0) & ok;
       rows.hide(seen, s);
     }
     if (__builtin_amdgcn_ballot_w64(unset) != 0) unset = rows.settle(unset, s);
     rows.softmax(s, p);
-    if (more)
-      asm volatile("s_waitcnt vmcnt(9)" : : : "memory");  // V(i)
-    else
-      asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+  };
+  auto output = [&](const uint8_t* vt, const typename RowsT::Probs& p)
+                    __attribute__((always_inline)) {
     V8 va[8];
-    rows.read_ops(buf[w][1], va);
+    rows.read_ops(vt, va);
     if (checked) {
       // What p = 0 meets must be finite; a visible NaN or infinity is added
       // to the rows that see it.
@@ -333,7 +389,7 @@ tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tree
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
             const int chunk = RowsT::v_phys(j, 2 * c + rows.g);
-            const V8 x = *reinterpret_cast<const V8*>(buf[w][1] + j * kRowB + 16 * chunk);
+            const V8 x = *reinterpret_cast<const V8*>(vt + j * kRowB + 16 * chunk);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float y = (float)x[e];
@@ -345,81 +401,392 @@ tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tree
       }
     }
     rows.output(va, p);
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-    if (more) fetch(1);
-    ok = ok_next;
+  };
+
+  if constexpr (RW == 1) {
+    // Every wave has tiles, and a K and a V slot, of its own: no barrier
+    // orders the walk.  K(i + 1) is fetched as soon as the operands of K(i)
+    // are read, V(i + 1) after those of V(i); table entries two tiles ahead.
+    uint8_t* const kt = sh.tile[w][0][0];
+    uint8_t* const vt = sh.tile[w][0][1];
+    uint64_t ok = 0;
+    if (n > 0) {
+      fetch_ids(0, 0);
+      fetch_ids(1, 1);
+      asm volatile("s_waitcnt vmcnt(1)" : : : "memory");
+      ok = locate(0, 0);
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      fetch(0, kt);
+      fetch(1, vt);
+    }
+    for (int i = 0; i < n; ++i) {
+      typename RowsT::Scores s;
+      typename RowsT::Probs p;
+      asm volatile("s_waitcnt vmcnt(8)" : : : "memory");  // K(i), and the entries of i + 1
+      rows.scores(kt, s);
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // its operands are in registers
+      const bool more = i + 1 < n;
+      uint64_t ok_next = 0;
+      if (more) {
+        ok_next = locate(i + 1, (i + 1) & 1);
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+        fetch_ids(i + 2, i & 1);
+        fetch(0, kt);
+      }
+      softmax(i, ok, s, p);
+      if (more)
+        asm volatile("s_waitcnt vmcnt(9)" : : : "memory");  // V(i)
+      else
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+      output(vt, p);
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      if (more) fetch(1, vt);
+      ok = ok_next;
+    }
+  } else {
+    // RW waves share their key group's tiles, kSlots of them in a ring; each
+    // fetches 1 / RW of a tile, kSlots - 1 tiles ahead, from table entries
+    // fetched kSlots - 1 tiles before that.  One barrier a step: past it tile
+    // i has landed for all, and tile i - 1 is read by none.
+    uint64_t ok[kSlots];  // of tiles i .. i + kSlots - 1
+#pragma unroll
+    for (int j = 0; j < kSlots - 1; ++j) fetch_ids(j, j);
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+#pragma unroll
+    for (int j = 0; j < kSlots - 1; ++j) {
+      fetch_ids(j + kSlots - 1, (j + kSlots - 1) % kSlots);
+      ok[j] = locate(j, j);
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      fetch(0, sh.tile[kg][j][0]);
+      fetch(1, sh.tile[kg][j][1]);
+    }
+    int slot = 0;  // i % kSlots
+    for (int i = 0; i < n; ++i) {
+      sync_ring<(kSlots - 2) * (1 + 2 * kSegs)>();
+      const int behind = slot == 0 ? kSlots - 1 : slot - 1;  // (i + kSlots - 1) % kSlots
+      const int ahead = behind == 0 ? kSlots - 1 : behind - 1;  // (i + 2 kSlots - 2) % kSlots
+      fetch_ids(i + 2 * kSlots - 2, ahead);
+      ok[kSlots - 1] = locate(i + kSlots - 1, behind);
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      fetch(0, sh.tile[kg][behind][0]);
+      fetch(1, sh.tile[kg][behind][1]);
+      if (first + KW * i < tiles) {
+        typename RowsT::Scores s;
+        typename RowsT::Probs p;
+        rows.scores(sh.tile[kg][slot][0], s);
+        softmax(i, ok[0], s, p);
+        output(sh.tile[kg][slot][1], p);
+      }
+#pragma unroll
+      for (int j = 0; j < kSlots - 1; ++j) ok[j] = ok[j + 1];
+      slot = slot + 1 == kSlots ? 0 : slot + 1;
+    }
   }
-  // Nothing may still write this wave's slots: its O goes there.
+  // Nothing may still write the tiles: partial results of the key groups meet
+  // there.
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
-  float4* const mine4 = reinterpret_cast<float4*>(buf[w][0]);
+  float mm, l_tot;
+  float a[KW];
+  if constexpr (KW > 1) {
+    if constexpr (RW > 1) __syncthreads();  // (with RW == 1 a wave's slots are its own)
+    float4* const own = reinterpret_cast<float4*>(sh.tile) + 1024 * w;  // 16 KiB each
 #pragma unroll
-  for (int c = 0; c < kAcc / 4; ++c) {
-    const float16_t& x = rows.o[c >> 2];
-    const int r = 4 * (c & 3);
-    mine4[c * 64 + lane] = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
-  }
-  mlbuf[w][lane] = make_float2(rows.stabiliser(), rows.l);
-  __syncthreads();
-  // Partial results meet at their largest stabiliser; one without a visible
-  // key (l = 0 across the lane pair) is passed over.
-  float mm = ninf(), lt = 0.0f, a[kWaves];
-  float2 ml[kWaves];
-  bool has[kWaves];
+    for (int c = 0; c < kAcc / 4; ++c) {
+      const float16_t& x = rows.o[c >> 2];
+      const int r = 4 * (c & 3);
+      own[c * 64 + lane] = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
+    }
+    sh.ml[w][lane] = make_float2(rows.stabiliser(), rows.l);
+    __syncthreads();
+    // They meet at their largest stabiliser; one without a visible key (l = 0
+    // across the lane pair) is passed over.
+    mm = ninf();
+    float lt = 0.0f;
+    float2 ml[KW];
+    bool has[KW];
 #pragma unroll
-  for (int j = 0; j < kWaves; ++j) {
-    ml[j] = mlbuf[j][lane];
-    has[j] = pair_sum(ml[j].y) != 0.0f;
-    if (has[j]) mm = fmaxf(mm, ml[j].x);
-  }
+    for (int j = 0; j < KW; ++j) {
+      ml[j] = sh.ml[j * RW + rw][lane];
+      has[j] = pair_sum(ml[j].y) != 0.0f;
+      if (has[j]) mm = fmaxf(mm, ml[j].x);
+    }
 #pragma unroll
-  for (int j = 0; j < kWaves; ++j) {
-    a[j] = has[j] ? __builtin_amdgcn_exp2f(ml[j].x - mm) : 0.0f;
-    lt += a[j] * ml[j].y;
+    for (int j = 0; j < KW; ++j) {
+      a[j] = has[j] ? __builtin_amdgcn_exp2f(ml[j].x - mm) : 0.0f;
+      lt += a[j] * ml[j].y;
+    }
+    l_tot = pair_sum(lt);
+  } else {
+    l_tot = pair_sum(rows.l);
+    mm = rows.stabiliser();
   }
-  const float l_tot = pair_sum(lt);
   const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
   T* const orow = O + (b * g.o_sb + head * g.o_sh + draft * g.o_sr);
-  for (int c = w; c < D / 16; c += kWaves) {
-    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  float* const prow = part ? part + (long long)local * kPart : nullptr;
+  // 8 columns of a row: 32 (c / 2) + 16 (c % 2) + 8 g.
+  auto put = [&](int c, const float (&acc)[8]) __attribute__((always_inline)) {
+    const int col = 32 * (c >> 1) + 16 * (c & 1) + 8 * rows.g;
+    if (prow) {
+      *reinterpret_cast<float4*>(prow + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(prow + col + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    } else {
+      V8 out;
 #pragma unroll
-    for (int j = 0; j < kWaves; ++j) {
-      const float4* const pj = reinterpret_cast<const float4*>(buf[j][0]);
-      const float4 x0 = pj[(2 * c) * 64 + lane], x1 = pj[(2 * c + 1) * 64 + lane];
-      acc[0] += a[j] * x0.x;
-      acc[1] += a[j] * x0.y;
-      acc[2] += a[j] * x0.z;
-      acc[3] += a[j] * x0.w;
-      acc[4] += a[j] * x1.x;
-      acc[5] += a[j] * x1.y;
-      acc[6] += a[j] * x1.z;
-      acc[7] += a[j] * x1.w;
+      for (int e = 0; e < 8; ++e) out[e] = (T)(acc[e] * inv);
+      *reinterpret_cast<V8*>(orow + col) = out;
     }
-    if (!mine) continue;
-    V8 out;
+  };
+  if constexpr (KW > 1) {
+    for (int c = kg; c < D / 16; c += KW) {
+      float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = (T)(acc[e] * inv);
-    *reinterpret_cast<V8*>(orow + 32 * (c >> 1) + 16 * (c & 1) + 8 * rows.g) = out;
+      for (int j = 0; j < KW; ++j) {
+        const float4* const pj = reinterpret_cast<const float4*>(sh.tile) + 1024 * (j * RW + rw);
+        const float4 x0 = pj[(2 * c) * 64 + lane], x1 = pj[(2 * c + 1) * 64 + lane];
+        acc[0] += a[j] * x0.x;
+        acc[1] += a[j] * x0.y;
+        acc[2] += a[j] * x0.z;
+        acc[3] += a[j] * x0.w;
+        acc[4] += a[j] * x1.x;
+        acc[5] += a[j] * x1.y;
+        acc[6] += a[j] * x1.z;
+        acc[7] += a[j] * x1.w;
+      }
+      if (mine) put(c, acc);
+    }
+  } else if (mine) {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      float acc[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = rows.o[c >> 1][8 * (c & 1) + e];
+      put(c, acc);
+    }
   }
-  if (w == 0 && rows.g == 0 && mine && g.lse != nullptr)
-    g.lse[((long long)b * g.heads + head) * g.drafts + draft] =
-        l_tot == 0.0f ? ninf() : 0.693147180559945309f * (mm + __builtin_amdgcn_logf(l_tot));
+  if (kg == 0 && rows.g == 0 && mine) {
+    if (prow) {
+      prow[D] = l_tot == 0.0f ? ninf() : mm;
+      prow[D + 1] = l_tot;
+    } else if (g.lse != nullptr) {
+      g.lse[((long long)b * g.heads + head) * g.drafts + draft] =
+          l_tot == 0.0f ? ninf() : 0.693147180559945309f * (mm + __builtin_amdgcn_logf(l_tot));
+    }
+  }
+}
+
+// The launch's work-group, counted so that neighbours run on one XCD.
+__device__ __forceinline__ int group_index(int xcds) {
+  const int per = gridDim.x / xcds;
+  return per * xcds == (int)gridDim.x ? (blockIdx.x % xcds) * per + blockIdx.x / xcds : blockIdx.x;
+}
+
+// A unit a work-group.
+template <int D, class T, int RW>
+__global__ void __launch_bounds__(64 * kWaves, 2)
+tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
+                float cr) {
+  __shared__ __attribute__((aligned(16))) Shared<RW> sh;
+  const int per = g.kv_heads * g.blocks_of_rows;
+  const int unit = group_index(g.xcds);
+  const int b = unit / per, rest = unit - b * per;
+  const int kvh = rest / g.blocks_of_rows, rb = rest - kvh * g.blocks_of_rows;
+  const Request r = request(g, b);
+  const int steps = unit_steps<D, RW>(g, r, rb);
+  if (steps > 0) walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, 0, steps, nullptr, cq, cr);
+}
+
+// Work-group x's steps [x each, (x + 1) each) of all units' steps in order: the
+// end of one unit, whole units, the start of one.  Whole units are stored;
+// partial results go to slot 2 x (its first) or 2 x + 1 (its last, if another).
+template <int D, class T, int RW>
+__global__ void __launch_bounds__(64 * kWaves, 2)
+tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
+                  float cr) {
+  constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
+  __shared__ __attribute__((aligned(16))) Shared<RW> sh;
+  const int x = group_index(g.xcds);
+  const long long all = all_steps<D, RW>(g);
+  const long long each = steps_each(g, all);
+  long long at = x * each;
+  const long long end = min(at + each, all);
+  if (at >= end) return;
+  // The request of step `at`.
+  int b = 0;
+  long long before = 0;  // steps before request b
+  for (int b0 = 0; b0 < g.batch; b0 += 64) {
+    const int mine = b0 + (threadIdx.x & 63);
+    const long long n = mine < g.batch ? head_steps<D, RW>(g, mine) * g.kv_heads : 0;
+    const long long upto = wave_scan(n);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > at);
+    if (past != 0) {
+      const int l = __builtin_ctzll(past);
+      b = b0 + l;
+      before += __shfl(upto - n, l);
+      break;
+    }
+    before += __shfl(upto, 63);
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  Request r = request(g, b);
+  long long head = head_steps<D, RW>(g, b);
+  int kvh = (int)((at - before) / head);
+  long long in = at - before - kvh * head;  // steps into the key/value head's units
+  int rb = 0, steps;
+  while (in >= (steps = unit_steps<D, RW>(g, r, rb))) {
+    in -= steps;
+    ++rb;
+  }
+  int s0 = __builtin_amdgcn_readfirstlane((int)in);
+  kvh = __builtin_amdgcn_readfirstlane(kvh);
+  rb = __builtin_amdgcn_readfirstlane(rb);
+  bool first = true;
+  for (;;) {
+    const int s1 = (int)min((long long)steps, s0 + (end - at));
+    const bool whole = s0 == 0 && s1 == steps;
+    float* const part =
+        whole ? nullptr : g.part + (2LL * x + (first ? 0 : 1)) * (32 * RW) * kPart;
+    walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, s0, s1, part, cq, cr);
+    at += s1 - s0;
+    if (at >= end) return;
+    first = false;
+    s0 = 0;
+    // The next unit with steps.
+    do {
+      if (++rb == g.blocks_of_rows) {
+        rb = 0;
+        if (++kvh == g.kv_heads) {
+          kvh = 0;
+          r = request(g, ++b);
+        }
+      }
+      steps = unit_steps<D, RW>(g, r, rb);
+    } while (steps == 0);
+    __syncthreads();  // the tiles are free again
+  }
+}
+
+// One wave a row: merges the partial results of its unit, if it was split.
+template <int D, class T, int RW>
+__global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g) {
+  constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
+  constexpr int kCols = D / 64;
+  const int lane = threadIdx.x & 63;
+  const long long id = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (id >= (long long)g.batch * g.heads * g.drafts) return;
+  const int b = (int)(id / (g.heads * g.drafts));
+  const int rest = (int)(id - (long long)b * g.heads * g.drafts);
+  const int head = rest / g.drafts, draft = rest - head * g.drafts;
+  const Request r = request(g, b);
+  if (draft >= r.count) return;
+  const int kvh = head / g.group;
+  const int row = draft * g.group + (head - kvh * g.group);
+  const int rb = row / (32 * RW);
+  // Steps of all requests, and of those before b.
+  long long n = 0, before = 0;
+  for (int b0 = 0; b0 < g.batch; b0 += 64) {
+    const int c = b0 + lane;
+    const long long y = c < g.batch ? head_steps<D, RW>(g, c) : 0;
+    n += y;
+    if (c < b) before += y;
+  }
+  n = __shfl(wave_scan(n), 63) * g.kv_heads;
+  before = __shfl(wave_scan(before), 63) * g.kv_heads;
+  const long long each = steps_each(g, n);
+  long long start = before + kvh * head_steps<D, RW>(g, b);
+  for (int i = 0; i < rb; ++i) start += unit_steps<D, RW>(g, r, i);
+  const long long stop = start + unit_steps<D, RW>(g, r, rb);
+  const int x0 = (int)(start / each), x1 = (int)((stop - 1) / each);
+  if (x0 == x1) return;  // one work-group had all of it
+  const float* const base = g.part + (long long)(row - rb * 32 * RW) * kPart;
+  auto slot = [&](int x) __attribute__((always_inline)) {
+    return base + (2LL * x + (x == x0 && start != x0 * each ? 1 : 0)) * (32 * RW) * kPart;
+  };
+  float mx = ninf();
+  for (int x = x0 + lane; x <= x1; x += 64) {
+    const float* const p = slot(x);
+    if (p[D + 1] != 0.0f) mx = fmaxf(mx, p[D]);
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
+  float acc[kCols] = {}, l = 0.0f;
+  for (int x = x0; x <= x1; ++x) {
+    const float* const p = slot(x);
+    const float lx = p[D + 1];
+    if (lx == 0.0f) continue;
+    const float a = __builtin_amdgcn_exp2f(p[D] - mx);
+    l += a * lx;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c] += a * p[lane + 64 * c];
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* const o = O + (b * g.o_sb + head * g.o_sh + draft * g.o_sr);
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) o[lane + 64 * c] = (T)(acc[c] * inv);
+  if (lane == 0 && g.lse != nullptr)
+    g.lse[id] = l == 0.0f ? ninf() : 0.693147180559945309f * (mx + __builtin_amdgcn_logf(l));
+}
+
+// How a call of given sizes runs: row blocks a work-group, and whether the
+// units' steps are dealt to a grid of two work-groups a CU.
+struct TreePlan {
+  int rw, units, grid;
+  bool split;
+  int64_t bytes;
+};
+
+TreePlan tree_plan(const fl_tree_params& p) {
+  TreePlan t;
+  const int64_t rows = p.heads / p.kv_heads * p.drafts;
+  t.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  t.units = (int)((rows + 32 * t.rw - 1) / (32 * t.rw) * p.kv_heads * p.batch);
+  t.grid = 2 * device_cus();
+  t.split = t.units < 2 * t.grid;
+  const int64_t part = p.head_dim == 64 ? kPartStride : kPartStride128;
+  t.bytes = t.split ? 2LL * t.grid * 32 * t.rw * part * (int64_t)sizeof(float) : 0;
+  return t;
+}
+
+template <int D, class T, int RW>
+hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, float cq, float cr,
+                     hipStream_t st) {
+  g.blocks_of_rows = (g.rows + 32 * RW - 1) / (32 * RW);
+  const T* q = static_cast<const T*>(p.q);
+  const uint8_t *k = static_cast<const uint8_t*>(p.k_cache),
+                *v = static_cast<const uint8_t*>(p.v_cache);
+  T* o = static_cast<T*>(p.o);
+  if (g.part == nullptr) {
+    hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW>), dim3((unsigned)t.units), dim3(64 * kWaves), 0,
+                       st, q, k, v, o, g, cq, cr);
+    return hipGetLastError();
+  }
+  g.grid = t.grid;
+  g.least = 1;
+  hipLaunchKernelGGL((tree_split_kernel<D, T, RW>), dim3((unsigned)t.grid), dim3(64 * kWaves), 0,
+                     st, q, k, v, o, g, cq, cr);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t rows = (int64_t)g.batch * g.heads * g.drafts;
+  hipLaunchKernelGGL((tree_merge_kernel<D, T, RW>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0,
+                     st, o, g);
+  return hipGetLastError();
 }
 
 template <int D, class T>
-hipError_t launch_t(const fl_tree_params& p, const TreeGeom& g, float cq, float cr, hipStream_t st) {
-  const unsigned units = (unsigned)(g.batch * g.kv_heads * g.blocks_of_rows);
-  hipLaunchKernelGGL((tree_fwd_kernel<D, T>), dim3(units), dim3(64 * kWaves), 0, st,
-                     static_cast<const T*>(p.q), static_cast<const uint8_t*>(p.k_cache),
-                     static_cast<const uint8_t*>(p.v_cache), static_cast<T*>(p.o), g, cq, cr);
-  return hipGetLastError();
+hipError_t launch_t(const fl_tree_params& p, TreeGeom& g, float cq, float cr, hipStream_t st) {
+  const TreePlan t = tree_plan(p);
+  return t.rw == 1   ? launch_rw<D, T, 1>(p, t, g, cq, cr, st)
+         : t.rw == 2 ? launch_rw<D, T, 2>(p, t, g, cq, cr, st)
+                     : launch_rw<D, T, 4>(p, t, g, cq, cr, st);
 }
 
 }  // namespace
 
-int64_t tree_workspace_bytes(const fl_tree_params&) { return 0; }
+int64_t tree_workspace_bytes(const fl_tree_params& p) { return tree_plan(p).bytes; }
 
-hipError_t launch_tree_fwd(const fl_tree_params& p, void*, hipStream_t st) {
+hipError_t launch_tree_fwd(const fl_tree_params& p, void* ws, hipStream_t st) {
   TreeGeom g = {};
+  g.part = static_cast<float*>(ws);
+  g.xcds = device_xcds();
   g.q_sb = p.q_stride[0];
   g.q_sh = p.q_stride[1];
   g.q_sr = p.q_stride[2];
@@ -446,7 +813,6 @@ hipError_t launch_tree_fwd(const fl_tree_params& p, void*, hipStream_t st) {
   g.drafts = (int)p.drafts;
   g.rows = g.group * g.drafts;
   g.words = (g.drafts + 63) / 64;
-  g.blocks_of_rows = (g.rows + 31) / 32;
   g.num_blocks = (int)p.num_blocks;
   g.max_blocks = (int)p.max_blocks;
   g.block = fast_div((int)p.block_size);
