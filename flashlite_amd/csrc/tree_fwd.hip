@@ -28,9 +28,10 @@ struct TreeGeom {
   int batch, heads, kv_heads, group, drafts, rows, words, blocks_of_rows;
   int num_blocks, max_blocks;
   FastDiv block;
-  // split launches: partial results [2 * grid][32 RW][kPartStride], and the
-  // least steps of a work-group
+  // split launches: partial results [2 * grid][32 RW][kPartStride], per unit
+  // where they are, and the least steps of a work-group
   float* part;
+  int2* parts;
   int grid, least;
   int xcds;
 };
@@ -598,6 +599,8 @@ tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tree
 // Work-group x's steps [x each, (x + 1) each) of all units' steps in order: the
 // end of one unit, whole units, the start of one.  Whole units are stored;
 // partial results go to slot 2 x (its first) or 2 x + 1 (its last, if another).
+// Whoever has a unit's first step says in parts[unit] where its partial results
+// begin and how many there are (the others are slots 2 (x + 1), 2 (x + 2), ...).
 template <int D, class T, int RW>
 __global__ void __launch_bounds__(64 * kWaves, 2)
 tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
@@ -643,8 +646,11 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
   for (;;) {
     const int s1 = (int)min((long long)steps, s0 + (end - at));
     const bool whole = s0 == 0 && s1 == steps;
-    float* const part =
-        whole ? nullptr : g.part + (2LL * x + (first ? 0 : 1)) * (32 * RW) * kPart;
+    const int slot = 2 * x + (first ? 0 : 1);
+    if (s0 == 0 && threadIdx.x == 0)
+      g.parts[(b * g.kv_heads + kvh) * g.blocks_of_rows + rb] =
+          make_int2(slot, (int)((steps - s1 + each - 1) / each) + 1);
+    float* const part = whole ? nullptr : g.part + (long long)slot * (32 * RW) * kPart;
     walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, s0, s1, part, cq, cr);
     at += s1 - s0;
     if (at >= end) return;
@@ -669,59 +675,80 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
 template <int D, class T, int RW>
 __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g) {
   constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
-  constexpr int kCols = D / 64;
+  constexpr int kCols = D / 64, kBatch = 8;
   const int lane = threadIdx.x & 63;
+  const int per = g.heads * g.drafts;
   const long long id = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (id >= (long long)g.batch * g.heads * g.drafts) return;
-  const int b = (int)(id / (g.heads * g.drafts));
-  const int rest = (int)(id - (long long)b * g.heads * g.drafts);
+  if (id >= (long long)g.batch * per) return;
+  const int b = (int)(id / per);
+  const int rest = (int)(id - (long long)b * per);
   const int head = rest / g.drafts, draft = rest - head * g.drafts;
-  const Request r = request(g, b);
-  if (draft >= r.count) return;
   const int kvh = head / g.group;
   const int row = draft * g.group + (head - kvh * g.group);
   const int rb = row / (32 * RW);
-  // Steps of all requests, and of those before b.
-  long long n = 0, before = 0;
-  for (int b0 = 0; b0 < g.batch; b0 += 64) {
-    const int c = b0 + lane;
-    const long long y = c < g.batch ? head_steps<D, RW>(g, c) : 0;
-    n += y;
-    if (c < b) before += y;
-  }
-  n = __shfl(wave_scan(n), 63) * g.kv_heads;
-  before = __shfl(wave_scan(before), 63) * g.kv_heads;
-  const long long each = steps_each(g, n);
-  long long start = before + kvh * head_steps<D, RW>(g, b);
-  for (int i = 0; i < rb; ++i) start += unit_steps<D, RW>(g, r, i);
-  const long long stop = start + unit_steps<D, RW>(g, r, rb);
-  const int x0 = (int)(start / each), x1 = (int)((stop - 1) / each);
-  if (x0 == x1) return;  // one work-group had all of it
+  const int count = g.counts ? g.counts[b] : g.drafts;
+  const int2 parts = g.parts[(b * g.kv_heads + kvh) * g.blocks_of_rows + rb];
+  if (draft >= count) return;  // (its unit's entry may not be there either)
+  const int n = parts.y;
+  if (n == 1) return;  // one work-group had all of it
+  // Part j: the first in slot parts.x, then the first slots of the work-groups
+  // that follow.
+  const int x0 = parts.x >> 1;
   const float* const base = g.part + (long long)(row - rb * 32 * RW) * kPart;
-  auto slot = [&](int x) __attribute__((always_inline)) {
-    return base + (2LL * x + (x == x0 && start != x0 * each ? 1 : 0)) * (32 * RW) * kPart;
+  auto at = [&](int j) __attribute__((always_inline)) {
+    return base + (long long)(j == 0 ? parts.x : 2 * (x0 + j)) * (32 * RW) * kPart;
   };
-  float mx = ninf();
-  for (int x = x0 + lane; x <= x1; x += 64) {
-    const float* const p = slot(x);
-    if (p[D + 1] != 0.0f) mx = fmaxf(mx, p[D]);
-  }
+  float acc[kCols] = {}, l = 0.0f, mx = ninf();
+  for (int j0 = 0; j0 < n; j0 += 64) {
+    // Lane j's part's stabiliser and sum; O of the first parts meanwhile.
+    float m = ninf(), lj = 0.0f;
+    if (j0 + lane < n) {
+      const float* const p = at(j0 + lane);
+      m = p[D];
+      lj = p[D + 1];
+    }
+    float o[kBatch][kCols];
+    const int most = min(n - j0, 64);
+    auto load = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-  float acc[kCols] = {}, l = 0.0f;
-  for (int x = x0; x <= x1; ++x) {
-    const float* const p = slot(x);
-    const float lx = p[D + 1];
-    if (lx == 0.0f) continue;
-    const float a = __builtin_amdgcn_exp2f(p[D] - mx);
-    l += a * lx;
+      for (int u = 0; u < kBatch; ++u) {
+        const float* const p = at(j0 + min(from + u, most - 1));
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] += a * p[lane + 64 * c];
+        for (int c = 0; c < kCols; ++c) o[u][c] = p[lane + 64 * c];
+      }
+    };
+    load(0);
+    float top = lj != 0.0f ? m : ninf();
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    top = fmaxf(top, mx);
+    const float again = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
+    mx = top;
+    l *= again;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c] *= again;
+    // (weights are not negative: -1 marks a part without a visible key)
+    const float a = lj != 0.0f ? __builtin_amdgcn_exp2f(m - mx) : -1.0f;
+    float sum = a < 0.0f ? 0.0f : a * lj;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    l += sum;
+    for (int from = 0; from < most; from += kBatch) {
+      if (from > 0) load(from);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const float w = from + u < most
+                            ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), from + u))
+                            : -1.0f;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) acc[c] += w < 0.0f ? 0.0f : w * o[u][c];
+      }
+    }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  T* const o = O + (b * g.o_sb + head * g.o_sh + draft * g.o_sr);
+  T* const out = O + (b * g.o_sb + head * g.o_sh + draft * g.o_sr);
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) o[lane + 64 * c] = (T)(acc[c] * inv);
+  for (int c = 0; c < kCols; ++c) out[lane + 64 * c] = (T)(acc[c] * inv);
   if (lane == 0 && g.lse != nullptr)
     g.lse[id] = l == 0.0f ? ninf() : 0.693147180559945309f * (mx + __builtin_amdgcn_logf(l));
 }
@@ -742,7 +769,9 @@ TreePlan tree_plan(const fl_tree_params& p) {
   t.grid = 2 * device_cus();
   t.split = t.units < 2 * t.grid;
   const int64_t part = p.head_dim == 64 ? kPartStride : kPartStride128;
-  t.bytes = t.split ? 2LL * t.grid * 32 * t.rw * part * (int64_t)sizeof(float) : 0;
+  t.bytes = t.split ? 2LL * t.grid * 32 * t.rw * part * (int64_t)sizeof(float) +
+                          t.units * (int64_t)sizeof(int2)
+                    : 0;
   return t;
 }
 
@@ -761,6 +790,8 @@ hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, fl
   }
   g.grid = t.grid;
   g.least = 1;
+  g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.grid * 32 * RW *
+                                                 (D == 64 ? kPartStride : kPartStride128));
   hipLaunchKernelGGL((tree_split_kernel<D, T, RW>), dim3((unsigned)t.grid), dim3(64 * kWaves), 0,
                      st, q, k, v, o, g, cq, cr);
   const hipError_t e = hipGetLastError();
