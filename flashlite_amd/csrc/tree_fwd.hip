@@ -25,14 +25,14 @@ struct TreeGeom {
   const int64_t* mask;
   long long mask_stride;
   float* lse;
-  int batch, heads, kv_heads, group, drafts, rows, words, blocks_of_rows;
-  int num_blocks, max_blocks;
-  FastDiv block;
-  // split launches: partial results [2 * grid][32 RW][kPartStride], per unit
-  // where they are, and the least steps of a work-group
+  int batch, heads, kv_heads, drafts, rows, words, blocks_of_rows;
+  int num_blocks, capacity;  // capacity: keys of a table row
+  FastDiv block, group, by_drafts;
+  // split launches: partial results [2 * grid][32 RW][kPartStride], and per
+  // unit where they begin and end
   float* part;
   int2* parts;
-  int grid, least;
+  int least_log2;  // least steps of a work-group
   int xcds;
 };
 
@@ -180,64 +180,49 @@ struct Request {
 
 __device__ __forceinline__ Request request(const TreeGeom& g, int b) {
   Request r;
-  r.count = g.counts ? min(max(g.counts[b], 0), g.drafts) : g.drafts;
-  r.length = min(max(g.lengths[b], 0), g.max_blocks * g.block.d);
+  r.length = g.lengths[b];
+  r.count = g.drafts;
+  if (g.counts) r.count = min(max(g.counts[b], 0), g.drafts);
+  r.length = min(max(r.length, 0), g.capacity);
   return r;
 }
 
-// Keys that row block rb (of `rows_of_block` rows) of a request walks, 0 where
-// no draft of it is there; with a chain through its last row's draft.
+// Drafts whose keys row block rb (of `block` rows) of a request walks; with a
+// chain through its last row's draft.
 __device__ __forceinline__ int unit_drafts(const TreeGeom& g, const Request& r, int rb,
-                                           int rows_of_block) {
-  int drafts = min(r.count, g.max_blocks * g.block.d - r.length);
+                                           int block) {
+  int drafts = min(r.count, g.capacity - r.length);
   if (g.mask == nullptr)
-    drafts = min(drafts, (min((rb + 1) * rows_of_block, g.rows) - 1) / g.group + 1);
+    drafts = min(drafts, divide(min((rb + 1) * block, g.rows) - 1, g.group) + 1);
   return drafts;
 }
 
+// Steps of a unit's walk, 0 where no draft of its rows is there.
 template <int D, int RW>
 __device__ __forceinline__ int unit_steps(const TreeGeom& g, const Request& r, int rb) {
   constexpr int kStepKeys = (kWaves / RW) * (D == 64 ? kBc : kBc2);
-  if (rb * 32 * RW / g.group >= r.count) return 0;
+  if (rb * 32 * RW >= r.count * g.group.d) return 0;
   return (r.length + unit_drafts(g, r, rb, 32 * RW) + kStepKeys - 1) / kStepKeys;
 }
 
 // Steps of all row blocks of one key/value head of a request.
 template <int D, int RW>
-__device__ __forceinline__ long long head_steps(const TreeGeom& g, int b) {
-  const Request r = request(g, b);
-  long long n = 0;
+__device__ __forceinline__ int head_steps(const TreeGeom& g, const Request& r) {
+  int n = 0;
+#pragma unroll 1
   for (int rb = 0; rb < g.blocks_of_rows; ++rb) n += unit_steps<D, RW>(g, r, rb);
   return n;
 }
 
-// Sums over a wave's lanes: inclusive from lane 0, and whole.
-__device__ __forceinline__ long long wave_scan(long long x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const long long y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+// Inclusive sum over a wave's lanes: within rows of 16, then over the rows.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);  // row_bcast:31
   return x;
-}
-
-// Steps of all requests (each wave by itself).
-template <int D, int RW>
-__device__ __forceinline__ long long all_steps(const TreeGeom& g) {
-  long long n = 0;
-  for (int b0 = 0; b0 < g.batch; b0 += 64) {
-    const int b = b0 + (threadIdx.x & 63);
-    if (b < g.batch) n += head_steps<D, RW>(g, b);
-  }
-  return __shfl(wave_scan(n), 63) * g.kv_heads;
-}
-
-// A split launch deals the steps of all units, in order, evenly to the grid's
-// work-groups; every wave that asks gets the same answer.
-__device__ __forceinline__ long long steps_each(const TreeGeom& g, long long all) {
-  const long long even = (all + g.grid - 1) / g.grid;
-  return even > g.least ? even : g.least;
 }
 
 // The work-group's LDS: key and value tiles, and per wave the row addresses of
@@ -286,10 +271,12 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   const int local = 32 * rw + rows.col;
   const int row = 32 * RW * rb + local;
   const int my_row = min(row, g.rows - 1);
-  const int draft = my_row / g.group;
-  const int head = kvh * g.group + (my_row - draft * g.group);
+  const int draft = divide(my_row, g.group);
+  const int head = kvh * g.group.d + (my_row - draft * g.group.d);
   const bool mine = row < g.rows && draft < req.count;
-  {
+  // Q, and whatever was fetched before it: the loads are waited for here, not
+  // among the fetches.
+  auto load_q = [&]() __attribute__((always_inline)) {
     const T* q = Q + (b * g.q_sb + head * g.q_sh + draft * g.q_sr) + 8 * rows.g;
     const uint32_t sign = cq < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
@@ -299,7 +286,8 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     }
 #pragma unroll
     for (int st = 0; st < RowsT::kSteps; ++st) asm volatile("" : "+v"(rows.qf[st]));
-  }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+  };
   const int64_t* const mask =
       g.mask ? g.mask + b * g.mask_stride + (long long)draft * g.words : nullptr;
   // This lane's row's visible keys of tile [k0, k0 + 64) that is not all prefix.
@@ -414,7 +402,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     if (n > 0) {
       fetch_ids(0, 0);
       fetch_ids(1, 1);
-      asm volatile("s_waitcnt vmcnt(1)" : : : "memory");
+      load_q();
       ok = locate(0, 0);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
       fetch(0, kt);
@@ -452,7 +440,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     uint64_t ok[kSlots];  // of tiles i .. i + kSlots - 1
 #pragma unroll
     for (int j = 0; j < kSlots - 1; ++j) fetch_ids(j, j);
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    load_q();
 #pragma unroll
     for (int j = 0; j < kSlots - 1; ++j) {
       fetch_ids(j + kSlots - 1, (j + kSlots - 1) % kSlots);
@@ -596,65 +584,90 @@ tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tree
   if (steps > 0) walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, 0, steps, nullptr, cq, cr);
 }
 
-// Work-group x's steps [x each, (x + 1) each) of all units' steps in order: the
-// end of one unit, whole units, the start of one.  Whole units are stored;
-// partial results go to slot 2 x (its first) or 2 x + 1 (its last, if another).
-// Whoever has a unit's first step says in parts[unit] where its partial results
-// begin and how many there are (the others are slots 2 (x + 1), 2 (x + 2), ...).
+// The steps of all units, in order, are dealt evenly to the work-groups: each
+// has the end of one unit, whole units, the start of one.  Whole units are
+// stored; partial results go to slot 2 x of work-group x (its first unit's) or
+// 2 x + 1 (its last's, if another).  Whoever has a unit's first step says in
+// parts[unit].x in which slot its results begin, whoever has its last in .y
+// which work-group that was; between them each work-group has one in its first
+// slot.  (Fewer than 2^31 steps: tree_plan.)
 template <int D, class T, int RW>
 __global__ void __launch_bounds__(64 * kWaves, 2)
 tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
                   float cr) {
   constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
   __shared__ __attribute__((aligned(16))) Shared<RW> sh;
-  const int x = group_index(g.xcds);
-  const long long all = all_steps<D, RW>(g);
-  const long long each = steps_each(g, all);
-  long long at = x * each;
-  const long long end = min(at + each, all);
-  if (at >= end) return;
-  // The request of step `at`.
-  int b = 0;
-  long long before = 0;  // steps before request b
-  for (int b0 = 0; b0 < g.batch; b0 += 64) {
-    const int mine = b0 + (threadIdx.x & 63);
-    const long long n = mine < g.batch ? head_steps<D, RW>(g, mine) * g.kv_heads : 0;
-    const long long upto = wave_scan(n);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > at);
-    if (past != 0) {
-      const int l = __builtin_ctzll(past);
-      b = b0 + l;
-      before += __shfl(upto - n, l);
-      break;
-    }
-    before += __shfl(upto, 63);
+  const int lane = threadIdx.x & 63;
+  // Steps of one key/value head of requests b0 .. b0 + 63, one a lane.
+  Request c;
+  int n, upto;
+  auto chunk = [&](int b0) __attribute__((always_inline)) {
+    c = request(g, min(b0 + lane, g.batch - 1));
+    n = b0 + lane < g.batch ? head_steps<D, RW>(g, c) : 0;
+    upto = wave_scan(n);
+  };
+  auto last_lane = [](int x) __attribute__((always_inline)) {
+    return __builtin_amdgcn_readlane(x, 63);
+  };
+  int all = 0;
+#pragma unroll 1
+  for (int b0 = (g.batch - 1) & ~63; b0 >= 0; b0 -= 64) {  // (ends with the first 64)
+    chunk(b0);
+    all += last_lane(upto);
   }
-  b = __builtin_amdgcn_readfirstlane(b);
-  Request r = request(g, b);
-  long long head = head_steps<D, RW>(g, b);
-  int kvh = (int)((at - before) / head);
-  long long in = at - before - kvh * head;  // steps into the key/value head's units
-  int rb = 0, steps;
-  while (in >= (steps = unit_steps<D, RW>(g, r, rb))) {
-    in -= steps;
+  all *= g.kv_heads;
+  // `busy` work-groups have steps, `even` or one more; neighbours run on one
+  // XCD, all XCDs alike.
+  const int busy = min((int)gridDim.x, max(all >> g.least_log2, min(all, 1)));
+  const int apiece = (busy + g.xcds - 1) / g.xcds;
+  const int k = blockIdx.x / g.xcds;
+  const int x = (blockIdx.x - k * g.xcds) * apiece + k;
+  if (k >= apiece || x >= busy) return;
+  const int even = (uint32_t)all / (uint32_t)busy, more = all - even * busy;
+  int at = x * even + min(x, more);
+  const int end = at + even + (x < more ? 1 : 0);
+  // The request of step `at`, and where in it that is.
+  int b0 = 0, before = 0;
+  uint64_t past;
+#pragma unroll 1
+  while ((past = __builtin_amdgcn_ballot_w64(before + upto * g.kv_heads > at)) == 0) {
+    before += last_lane(upto) * g.kv_heads;
+    b0 += 64;
+    chunk(b0);
+  }
+  const int l = __builtin_ctzll(past);
+  int b = b0 + l;
+  Request r;
+  r.length = __builtin_amdgcn_readlane(c.length, l);
+  r.count = __builtin_amdgcn_readlane(c.count, l);
+  const int head = __builtin_amdgcn_readlane(n, l);
+  int s0 = at - before - __builtin_amdgcn_readlane(upto - n, l) * g.kv_heads;
+  int kvh = 0, rb = 0, steps;
+#pragma unroll 1
+  while (s0 >= head) {
+    s0 -= head;
+    ++kvh;
+  }
+#pragma unroll 1
+  while (s0 >= (steps = unit_steps<D, RW>(g, r, rb))) {
+    s0 -= steps;
     ++rb;
   }
-  int s0 = __builtin_amdgcn_readfirstlane((int)in);
-  kvh = __builtin_amdgcn_readfirstlane(kvh);
-  rb = __builtin_amdgcn_readfirstlane(rb);
-  bool first = true;
+  int slot = 2 * x;
+#pragma unroll 1
   for (;;) {
-    const int s1 = (int)min((long long)steps, s0 + (end - at));
-    const bool whole = s0 == 0 && s1 == steps;
-    const int slot = 2 * x + (first ? 0 : 1);
-    if (s0 == 0 && threadIdx.x == 0)
-      g.parts[(b * g.kv_heads + kvh) * g.blocks_of_rows + rb] =
-          make_int2(slot, (int)((steps - s1 + each - 1) / each) + 1);
-    float* const part = whole ? nullptr : g.part + (long long)slot * (32 * RW) * kPart;
+    const int s1 = min(steps, s0 + (end - at));
+    if (threadIdx.x == 0) {
+      int2* const where = g.parts + (b * g.kv_heads + kvh) * g.blocks_of_rows + rb;
+      if (s0 == 0) where->x = slot;
+      if (s1 == steps) where->y = x;
+    }
+    float* const part =
+        s0 == 0 && s1 == steps ? nullptr : g.part + (long long)slot * (32 * RW) * kPart;
     walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, s0, s1, part, cq, cr);
     at += s1 - s0;
     if (at >= end) return;
-    first = false;
+    slot = 2 * x + 1;
     s0 = 0;
     // The next unit with steps.
     do {
@@ -677,64 +690,61 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g)
   constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
   constexpr int kCols = D / 64, kBatch = 8;
   const int lane = threadIdx.x & 63;
-  const int per = g.heads * g.drafts;
-  const long long id = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (id >= (long long)g.batch * per) return;
-  const int b = (int)(id / per);
-  const int rest = (int)(id - (long long)b * per);
-  const int head = rest / g.drafts, draft = rest - head * g.drafts;
-  const int kvh = head / g.group;
-  const int row = draft * g.group + (head - kvh * g.group);
+  const int b = blockIdx.y;
+  const int rest = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (rest >= g.heads * g.drafts) return;
+  const int head = divide(rest, g.by_drafts), draft = rest - head * g.drafts;
+  const int kvh = divide(head, g.group);
+  const int row = draft * g.group.d + (head - kvh * g.group.d);
   const int rb = row / (32 * RW);
   const int count = g.counts ? g.counts[b] : g.drafts;
   const int2 parts = g.parts[(b * g.kv_heads + kvh) * g.blocks_of_rows + rb];
   if (draft >= count) return;  // (its unit's entry may not be there either)
-  const int n = parts.y;
-  if (n == 1) return;  // one work-group had all of it
   // Part j: the first in slot parts.x, then the first slots of the work-groups
   // that follow.
-  const int x0 = parts.x >> 1;
+  const int x0 = parts.x >> 1, n = parts.y - x0 + 1;
+  if (n == 1) return;  // one work-group had all of it
   const float* const base = g.part + (long long)(row - rb * 32 * RW) * kPart;
   auto at = [&](int j) __attribute__((always_inline)) {
     return base + (long long)(j == 0 ? parts.x : 2 * (x0 + j)) * (32 * RW) * kPart;
   };
   float acc[kCols] = {}, l = 0.0f, mx = ninf();
+#pragma unroll 1
   for (int j0 = 0; j0 < n; j0 += 64) {
     // Lane j's part's stabiliser and sum; O of the first parts meanwhile.
-    float m = ninf(), lj = 0.0f;
+    float m = ninf(), lj = 0.0f, a = 0.0f;
     if (j0 + lane < n) {
-      const float* const p = at(j0 + lane);
-      m = p[D];
-      lj = p[D + 1];
+      const float2 ml = *reinterpret_cast<const float2*>(at(j0 + lane) + D);
+      m = ml.x;
+      lj = ml.y;
     }
-    float o[kBatch][kCols];
     const int most = min(n - j0, 64);
-    auto load = [&](int from) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int from = 0; from < most; from += kBatch) {
+      float o[kBatch][kCols];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const float* const p = at(j0 + min(from + u, most - 1));
 #pragma unroll
         for (int c = 0; c < kCols; ++c) o[u][c] = p[lane + 64 * c];
       }
-    };
-    load(0);
-    float top = lj != 0.0f ? m : ninf();
+      if (from == 0) {
+        float top = lj != 0.0f ? m : ninf();
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    top = fmaxf(top, mx);
-    const float again = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
-    mx = top;
-    l *= again;
+        for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+        top = fmaxf(top, mx);
+        const float again = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
+        mx = top;
+        l *= again;
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] *= again;
-    // (weights are not negative: -1 marks a part without a visible key)
-    const float a = lj != 0.0f ? __builtin_amdgcn_exp2f(m - mx) : -1.0f;
-    float sum = a < 0.0f ? 0.0f : a * lj;
+        for (int c = 0; c < kCols; ++c) acc[c] *= again;
+        // (weights are not negative: -1 marks a part without a visible key)
+        a = lj != 0.0f ? __builtin_amdgcn_exp2f(m - mx) : -1.0f;
+        float sum = a < 0.0f ? 0.0f : a * lj;
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    l += sum;
-    for (int from = 0; from < most; from += kBatch) {
-      if (from > 0) load(from);
+        for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+        l += sum;
+      }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const float w = from + u < most
@@ -750,7 +760,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g)
 #pragma unroll
   for (int c = 0; c < kCols; ++c) out[lane + 64 * c] = (T)(acc[c] * inv);
   if (lane == 0 && g.lse != nullptr)
-    g.lse[id] = l == 0.0f ? ninf() : 0.693147180559945309f * (mx + __builtin_amdgcn_logf(l));
+    g.lse[(long long)b * g.heads * g.drafts + rest] =
+        l == 0.0f ? ninf() : 0.693147180559945309f * (mx + __builtin_amdgcn_logf(l));
 }
 
 // How a call of given sizes runs: row blocks a work-group, and whether the
@@ -778,27 +789,29 @@ TreePlan tree_plan(const fl_tree_params& p) {
 template <int D, class T, int RW>
 hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, float cq, float cr,
                      hipStream_t st) {
+  constexpr int kStepKeys = (kWaves / RW) * (D == 64 ? kBc : kBc2);
   g.blocks_of_rows = (g.rows + 32 * RW - 1) / (32 * RW);
   const T* q = static_cast<const T*>(p.q);
   const uint8_t *k = static_cast<const uint8_t*>(p.k_cache),
                 *v = static_cast<const uint8_t*>(p.v_cache);
   T* o = static_cast<T*>(p.o);
-  if (g.part == nullptr) {
+  // A split launch counts steps in 32 bits.
+  const bool counted = t.units * (((int64_t)g.capacity + g.drafts) / kStepKeys + 1) < (1LL << 30);
+  if (g.part == nullptr || !counted) {
     hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW>), dim3((unsigned)t.units), dim3(64 * kWaves), 0,
                        st, q, k, v, o, g, cq, cr);
     return hipGetLastError();
   }
-  g.grid = t.grid;
-  g.least = 1;
+  g.least_log2 = 0;
   g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.grid * 32 * RW *
                                                  (D == 64 ? kPartStride : kPartStride128));
   hipLaunchKernelGGL((tree_split_kernel<D, T, RW>), dim3((unsigned)t.grid), dim3(64 * kWaves), 0,
                      st, q, k, v, o, g, cq, cr);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t rows = (int64_t)g.batch * g.heads * g.drafts;
-  hipLaunchKernelGGL((tree_merge_kernel<D, T, RW>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0,
-                     st, o, g);
+  const unsigned rows = (unsigned)(g.heads * g.drafts);
+  hipLaunchKernelGGL((tree_merge_kernel<D, T, RW>), dim3((rows + 3) / 4, (unsigned)g.batch),
+                     dim3(256), 0, st, o, g);
   return hipGetLastError();
 }
 
@@ -840,12 +853,13 @@ hipError_t launch_tree_fwd(const fl_tree_params& p, void* ws, hipStream_t st) {
   g.batch = (int)p.batch;
   g.heads = (int)p.heads;
   g.kv_heads = (int)p.kv_heads;
-  g.group = (int)(p.heads / p.kv_heads);
   g.drafts = (int)p.drafts;
-  g.rows = g.group * g.drafts;
+  g.group = fast_div((int)(p.heads / p.kv_heads));
+  g.by_drafts = fast_div(g.drafts);
+  g.rows = g.group.d * g.drafts;
   g.words = (g.drafts + 63) / 64;
   g.num_blocks = (int)p.num_blocks;
-  g.max_blocks = (int)p.max_blocks;
+  g.capacity = (int)(p.max_blocks * p.block_size);
   g.block = fast_div((int)p.block_size);
   const double s = p.sm_scale == 0.0 ? (double)(1.0f / std::sqrt((float)p.head_dim)) : p.sm_scale;
   const float cr = (float)(std::fabs(s) * 1.44269504088896340736), cq = s < 0.0 ? -1.0f : 1.0f;
