@@ -232,7 +232,8 @@ struct Shared {
   static constexpr int kSlots = RW;  // of each key group
   uint8_t tile[kWaves / RW][kSlots][2][kTileBytes];
   uint64_t where[kWaves][2][64];
-  int32_t ids[kWaves][RW == 1 ? 2 : kSlots][64];
+  int32_t ids[kWaves][RW == 1 ? 2 : 1][64];
+  uint64_t ok[kWaves];
   float2 ml[kWaves][64];
 };
 
@@ -310,7 +311,6 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   const uint64_t kbase = (uint64_t)(uintptr_t)(K + kvh * g.k_head);
   const uint64_t vbase = (uint64_t)(uintptr_t)(V + kvh * g.v_head);
   int32_t(*const ids)[64] = sh.ids[w];
-  uint64_t(*const where)[64] = sh.where[w];
   // Key l of this key group's tile i (past the last key: the last again).
   auto key_of = [&](int i) __attribute__((always_inline)) {
     return min((first + KW * i) * kKeys + (lane & (kKeys - 1)), keys - 1);
@@ -318,18 +318,23 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   auto fetch_ids = [&](int i, int slot) __attribute__((always_inline)) {
     fetch4(table + 4 * (uint64_t)divide(key_of(i), g.block), ids[slot]);
   };
-  // Row addresses of tile i; the result has a bit per key with a block.
+  // Row addresses of tile i, and a bit per key with a block, to this wave's
+  // entries.
   auto locate = [&](int i, int slot) __attribute__((always_inline)) {
     const int key = key_of(i);
     const int in = key - divide(key, g.block) * g.block.d;
     int id = ids[slot][lane];
     const bool ok = (uint32_t)id < (uint32_t)g.num_blocks;
     id = ok ? id : 0;
-    where[0][lane] = kbase + (id * g.k_blk + in * g.k_row);
-    where[1][lane] = vbase + (id * g.v_blk + in * g.v_row);
-    return __builtin_amdgcn_ballot_w64(ok);
+    sh.where[w][0][lane] = kbase + (id * g.k_blk + in * g.k_row);
+    sh.where[w][1][lane] = vbase + (id * g.v_blk + in * g.v_row);
+    const uint64_t all = __builtin_amdgcn_ballot_w64(ok);
+    if constexpr (RW > 1) sh.ok[w] = all;
+    return all;
   };
-  auto fetch = [&](int t, uint8_t* tile) __attribute__((always_inline)) {  // 0: K, 1: V
+  // This wave's share of the K (t = 0) or V (1) tile whose rows wave
+  // kg * RW + from looked up.
+  auto fetch = [&](int t, int from, uint8_t* tile) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kSegs; ++i) {
       const int seg = rw * kSegs + i;
@@ -337,7 +342,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       const int phys = lane & (kLanes - 1);
       const int chunk = phys ^ (D == 64 ? (t ? v_swz(r) : k_swz(r))
                                         : (t ? v_swz128(r) : k_swz128(r)));
-      fetch16(where[t][r] + 16 * chunk, tile + 1024 * seg);
+      fetch16(sh.where[kg * RW + from][t][r] + 16 * chunk, tile + 1024 * seg);
     }
   };
 
@@ -405,8 +410,8 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       load_q();
       ok = locate(0, 0);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      fetch(0, kt);
-      fetch(1, vt);
+      fetch(0, 0, kt);
+      fetch(1, 0, vt);
     }
     for (int i = 0; i < n; ++i) {
       typename RowsT::Scores s;
@@ -420,7 +425,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
         ok_next = locate(i + 1, (i + 1) & 1);
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
         fetch_ids(i + 2, i & 1);
-        fetch(0, kt);
+        fetch(0, 0, kt);
       }
       softmax(i, ok, s, p);
       if (more)
@@ -429,40 +434,43 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
       output(vt, p);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      if (more) fetch(1, vt);
+      if (more) fetch(1, 0, vt);
       ok = ok_next;
     }
   } else {
     // RW waves share their key group's tiles, kSlots of them in a ring; each
-    // fetches 1 / RW of a tile, kSlots - 1 tiles ahead, from table entries
-    // fetched kSlots - 1 tiles before that.  One barrier a step: past it tile
-    // i has landed for all, and tile i - 1 is read by none.
+    // fetches 1 / RW of a tile, kSlots - 1 tiles ahead.  Wave j % RW looks up
+    // the rows of tile j one step before that, from table entries it fetched
+    // kSlots steps earlier.  One barrier a step: past it tile i has landed for
+    // all, tile i - 1 is read by none, and the next tile's addresses are there.
     uint64_t ok[kSlots];  // of tiles i .. i + kSlots - 1
-#pragma unroll
-    for (int j = 0; j < kSlots - 1; ++j) fetch_ids(j, j);
+    auto fetch_tile = [&](int slot) __attribute__((always_inline)) {
+      fetch(0, slot, sh.tile[kg][slot][0]);
+      fetch(1, slot, sh.tile[kg][slot][1]);
+      return sh.ok[kg * RW + slot];
+    };
+    fetch_ids(rw, 0);
     load_q();
+    locate(rw, 0);
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    fetch_ids(rw + kSlots, 0);
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kSlots - 1; ++j) {
-      fetch_ids(j + kSlots - 1, (j + kSlots - 1) % kSlots);
-      ok[j] = locate(j, j);
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      fetch(0, sh.tile[kg][j][0]);
-      fetch(1, sh.tile[kg][j][1]);
-    }
+    for (int j = 0; j < kSlots - 1; ++j) ok[j] = fetch_tile(j);
     int slot = 0;  // i % kSlots
     for (int i = 0; i < n; ++i) {
-      sync_ring<(kSlots - 2) * (1 + 2 * kSegs)>();
-      const int behind = slot == 0 ? kSlots - 1 : slot - 1;  // (i + kSlots - 1) % kSlots
-      const int ahead = behind == 0 ? kSlots - 1 : behind - 1;  // (i + 2 kSlots - 2) % kSlots
-      fetch_ids(i + 2 * kSlots - 2, ahead);
-      ok[kSlots - 1] = locate(i + kSlots - 1, behind);
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      fetch(0, sh.tile[kg][behind][0]);
-      fetch(1, sh.tile[kg][behind][1]);
-      if (first + KW * i < tiles) {
-        typename RowsT::Scores s;
+      sync_ring<(kSlots - 2) * 2 * kSegs>();
+      const bool busy = first + KW * i < tiles;
+      typename RowsT::Scores s;
+      if (busy) rows.scores(sh.tile[kg][slot][0], s);
+      ok[kSlots - 1] = fetch_tile(slot == 0 ? kSlots - 1 : slot - 1);
+      if (rw == slot) {
+        locate(i + kSlots, 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+        fetch_ids(i + 2 * kSlots, 0);
+      }
+      if (busy) {
         typename RowsT::Probs p;
-        rows.scores(sh.tile[kg][slot][0], s);
         softmax(i, ok[0], s, p);
         output(sh.tile[kg][slot][1], p);
       }
