@@ -58,105 +58,133 @@ __device__ __forceinline__ typename Elem<T>::v8 finite_only(const typename Elem<
   return __builtin_bit_cast(typename Elem<T>::v8, x);
 }
 
-// One wave's 32 rows: Rows / Rows128 (non-causal) with scores masked by bits,
-// a stabiliser that waits for a row's first visible key, and a product with V
-// that hidden rows of V do not reach.
+// Where a lane's operands lie: those of Rows (head dim 64) and Rows128.
 template <int D, class T>
-struct TreeRows;
-
+struct TreeLayout;
 template <class T>
-struct TreeRows<64, T> : Rows<false, true, T> {
-  using Base = Rows<false, true, T>;
-  using V8 = typename Base::V8;
-  static constexpr int kKeys = kBc, kSteps = 4, kOps = 8;
+struct TreeLayout<64, T> {
+  using type = Rows<false, true, T>;
+};
+template <class T>
+struct TreeLayout<128, T> {
+  using type = Rows128<false, T>;
+};
+
+// One wave's 32 rows.  Scores stay raw in the accumulators and the stabiliser
+// mc (base-2 logit units) is subtracted with the scale's multiply.  mc is the
+// row max of the first tile in which the row sees a key, and later only moves
+// when a tile would push p out of fp16's range; it never passes the running
+// max.
+template <int D, class T>
+struct TreeRows : TreeLayout<D, T>::type {
+  using Base = typename TreeLayout<D, T>::type;
+  using E = Elem<T>;
+  using V8 = typename E::v8;
+  static constexpr int kBlocks = D == 64 ? 2 : 1;  // 32-key blocks of a tile
+  static constexpr int kKeys = 32 * kBlocks, kSteps = D / 16;
   struct Scores {
-    float16_t s[2];
+    float16_t s[kBlocks];
   };
   struct Probs {
-    V8 p[2][2];
+    V8 p[2 * kBlocks];
   };
-  __device__ __forceinline__ void place(int lane, float cr) {
+  float mc;
+
+  __device__ __forceinline__ void start(int lane, float cr) {
     Base::place(lane, 0, 0, 0, 0, cr);
     this->reset();
+    mc = 0.0f;
   }
   __device__ __forceinline__ void scores(const uint8_t* kt, Scores& s) const {
-    V8 ka[2][4];
-    this->read_k(kt, ka);
-    this->gemm1(ka, s.s);
+    V8 ka[kBlocks][kSteps];
+#pragma unroll
+    for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        if constexpr (D == 64)
+          ka[kb][st] = this->read_k_op(kt, kb, st);
+        else
+          ka[kb][st] = this->read_k_op(kt, st);
+      }
+    const float16_t zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int kb = 0; kb < kBlocks; ++kb)
+        s.s[kb] = E::mfma(ka[kb][st], this->qf[st], st == 0 ? zero : s.s[kb]);
   }
+  // Scores of hidden keys become -inf (bit j: key j of the tile is visible).
   __device__ __forceinline__ void hide(uint64_t seen, Scores& s) const {
     const uint64_t x = seen >> (4 * this->g);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int kb = 0; kb < kBlocks; ++kb) {
+      const uint32_t word = (uint32_t)(x >> (32 * kb));
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const uint32_t word = kb ? (uint32_t)(x >> 32) : (uint32_t)x;
+      for (int r = 0; r < 16; ++r)
         s.s[kb][r] = (word >> (8 * (r >> 2) + (r & 3))) & 1 ? s.s[kb][r] : ninf();
-      }
+    }
+  }
+  // Row max of a tile in base-2 logit units (both halves of the row).
+  __device__ __forceinline__ float tile_max(const Scores& s) const {
+    float mx = ninf();
+#pragma unroll
+    for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s.s[kb][r]);
+    return pair_max(mx) * this->cr;
   }
   // Rows without a stabiliser take the tile's row max, if they see a key.
-  __device__ __forceinline__ bool settle(bool unset, Scores& s) {
-    const float mx = this->tile_max(s.s);
+  __device__ __forceinline__ bool settle(bool unset, const Scores& s) {
+    const float mx = tile_max(s);
     const bool now = unset && mx != ninf();
-    const float d = now ? mx : 0.0f;
-    this->sub(s.s, d);
-    this->set_m(this->m + d);
+    if (now) mc = mx;
     return unset && !now;
   }
-  __device__ __forceinline__ void softmax(Scores& s, Probs& p) { this->softmax_checked(s.s, p.p); }
-  __device__ __forceinline__ void read_ops(const uint8_t* vt, V8 (&va)[8]) const {
+  // p = 2^(s cr - mc); returns this lane's sum of the unrounded p.
+  __device__ __forceinline__ float exponentiate(const Scores& s, Probs& p) const {
+    float sum[2 * kBlocks];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) va[u] = this->read_v_op(vt, u & 1, u >> 1);
-  }
-  __device__ __forceinline__ void output(const V8 (&va)[8], const Probs& p) {
+    for (int h = 0; h < 2 * kBlocks; ++h) {
+      sum[h] = 0.0f;
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      this->o[u & 1] = Base::E::mfma(va[u], p.p[u >> 2][(u >> 1) & 1], this->o[u & 1]);
+      for (int e = 0; e < 8; ++e) {
+        const float x =
+            __builtin_amdgcn_exp2f(__builtin_fmaf(s.s[h >> 1][8 * (h & 1) + e], this->cr, -mc));
+        p.p[h][e] = (T)x;
+        sum[h] += x;
+      }
+    }
+    float all = sum[0] + sum[1];
+    if constexpr (kBlocks == 2) all += sum[2] + sum[3];
+    return all;
   }
-  __device__ __forceinline__ float stabiliser() const { return this->m * this->cr; }
-  __device__ __forceinline__ static int v_phys(int row, int chunk) { return chunk ^ v_swz(row); }
-};
-
-template <class T>
-struct TreeRows<128, T> : Rows128<false, T> {
-  using Base = Rows128<false, T>;
-  using V8 = typename Base::V8;
-  static constexpr int kKeys = kBc2, kSteps = 8, kOps = 8;
-  struct Scores {
-    float16_t s;
-  };
-  struct Probs {
-    V8 p[2];
-  };
-  __device__ __forceinline__ void place(int lane, float cr) {
-    Base::place(lane, 0, 0, 0, 0, cr);
-  }
-  __device__ __forceinline__ void scores(const uint8_t* kt, Scores& s) const {
-    this->gemm1(kt, s.s);
-  }
-  __device__ __forceinline__ void hide(uint64_t seen, Scores& s) const {
-    const uint32_t x = (uint32_t)seen >> (4 * this->g);
+  // Ends a tile's softmax: where a lane's sum left the range that keeps p
+  // finite (or is NaN), mc moves up to the row max and p is taken again.
+  __device__ __forceinline__ void settle_sum(float sum, const Scores& s, Probs& p) {
+    if (__builtin_amdgcn_ballot_w64(!(sum <= kSumLimit)) != 0) {
+      const float d = fmaxf(tile_max(s) - mc, 0.0f);
+      const float alpha = __builtin_amdgcn_exp2f(-d);
+      this->l *= alpha;
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      s.s[r] = (x >> (8 * (r >> 2) + (r & 3))) & 1 ? s.s[r] : ninf();
-  }
-  __device__ __forceinline__ bool settle(bool unset, Scores& s) {
-    const float mx = this->tile_max(s.s);
-    const bool now = unset && mx != ninf();
-    if (now) this->mc = mx;
-    return unset && !now;
-  }
-  __device__ __forceinline__ void softmax(Scores& s, Probs& p) { this->softmax_checked(s.s, p.p); }
-  __device__ __forceinline__ void read_ops(const uint8_t* vt, V8 (&va)[8]) const {
+      for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-    for (int u = 0; u < 8; ++u) va[u] = this->read_v_op(vt, u & 3, u >> 2);
+        for (int r = 0; r < 16; ++r) this->o[db][r] *= alpha;
+      mc += d;
+      sum = exponentiate(s, p);
+    }
+    this->l += sum;
   }
-  __device__ __forceinline__ void output(const V8 (&va)[8], const Probs& p) {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) this->o[u & 3] = Base::E::mfma(va[u], p.p[u >> 2], this->o[u & 3]);
+  // V operand u of the tile: head-dim block u % (D / 32) at 16-key step
+  // u / (D / 32).
+  __device__ __forceinline__ V8 v_op(const uint8_t* vt, int u) const {
+    return this->read_v_op(vt, u % (D / 32), u / (D / 32));
   }
-  __device__ __forceinline__ float stabiliser() const { return this->mc; }
-  __device__ __forceinline__ static int v_phys(int row, int chunk) { return chunk ^ v_swz128(row); }
+  __device__ __forceinline__ void output(int u, const V8& v, const Probs& p) {
+    this->o[u % (D / 32)] = E::mfma(v, p.p[u / (D / 32)], this->o[u % (D / 32)]);
+  }
+  __device__ __forceinline__ static int v_phys(int row, int chunk) {
+    return chunk ^ (D == 64 ? v_swz(row) : v_swz128(row));
+  }
 };
 
 // 16 (or 4) bytes a lane from a 64-bit address of its own into LDS at
@@ -214,6 +242,12 @@ __device__ __forceinline__ int head_steps(const TreeGeom& g, const Request& r) {
   return n;
 }
 
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32));
+  return (uint64_t)hi << 32 | lo;
+}
+
 // Inclusive sum over a wave's lanes: within rows of 16, then over the rows.
 __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
@@ -231,9 +265,10 @@ template <int RW>
 struct Shared {
   static constexpr int kSlots = RW;  // of each key group
   uint8_t tile[kWaves / RW][kSlots][2][kTileBytes];
-  uint64_t where[kWaves][2][64];
-  int32_t ids[kWaves][RW == 1 ? 2 : 1][64];
-  uint64_t ok[kWaves];
+  static constexpr int kRing = RW == 1 ? 1 : 2 * kSlots;  // looked-up tiles
+  uint64_t where[kWaves / RW][kRing][2][64];
+  uint64_t ok[kWaves / RW][kRing];
+  int32_t ids[kWaves][2][64];
   float2 ml[kWaves][64];
 };
 
@@ -268,7 +303,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   const int n = RW == 1 ? (last > first ? (last - first + KW - 1) / KW : 0) : s1 - s0;
 
   RowsT rows;
-  rows.place(lane, cr);
+  rows.start(lane, cr);
   const int local = 32 * rw + rows.col;
   const int row = 32 * RW * rb + local;
   const int my_row = min(row, g.rows - 1);
@@ -318,40 +353,41 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   auto fetch_ids = [&](int i, int slot) __attribute__((always_inline)) {
     fetch4(table + 4 * (uint64_t)divide(key_of(i), g.block), ids[slot]);
   };
-  // Row addresses of tile i, and a bit per key with a block, to this wave's
-  // entries.
-  auto locate = [&](int i, int slot) __attribute__((always_inline)) {
+  // Row addresses of tile i, from table entries in ids[slot], and a bit per
+  // key with a block, to entry `to` of the key group's.
+  auto locate = [&](int i, int slot, int to) __attribute__((always_inline)) {
     const int key = key_of(i);
     const int in = key - divide(key, g.block) * g.block.d;
     int id = ids[slot][lane];
     const bool ok = (uint32_t)id < (uint32_t)g.num_blocks;
     id = ok ? id : 0;
-    sh.where[w][0][lane] = kbase + (id * g.k_blk + in * g.k_row);
-    sh.where[w][1][lane] = vbase + (id * g.v_blk + in * g.v_row);
+    sh.where[kg][to][0][lane] = kbase + (id * g.k_blk + in * g.k_row);
+    sh.where[kg][to][1][lane] = vbase + (id * g.v_blk + in * g.v_row);
     const uint64_t all = __builtin_amdgcn_ballot_w64(ok);
-    if constexpr (RW > 1) sh.ok[w] = all;
+    if constexpr (RW > 1) sh.ok[kg][to] = all;
     return all;
   };
-  // This wave's share of the K (t = 0) or V (1) tile whose rows wave
-  // kg * RW + from looked up.
+  // This wave's share of the K (t = 0) or V (1) tile whose rows are in entry
+  // `from`.
   auto fetch = [&](int t, int from, uint8_t* tile) __attribute__((always_inline)) {
+    uint64_t at[kSegs];
 #pragma unroll
     for (int i = 0; i < kSegs; ++i) {
-      const int seg = rw * kSegs + i;
-      const int r = kSegRows * seg + lane / kLanes;
+      const int r = kSegRows * (rw * kSegs + i) + lane / kLanes;
       const int phys = lane & (kLanes - 1);
       const int chunk = phys ^ (D == 64 ? (t ? v_swz(r) : k_swz(r))
                                         : (t ? v_swz128(r) : k_swz128(r)));
-      fetch16(sh.where[kg * RW + from][t][r] + 16 * chunk, tile + 1024 * seg);
+      at[i] = sh.where[kg][from][t][r] + 16 * chunk;
     }
+#pragma unroll
+    for (int i = 0; i < kSegs; ++i) fetch16(at[i], tile + 1024 * (rw * kSegs + i));
   };
 
   bool unset = true;
   uint64_t seen = 0;
   bool checked = false;
-  // Scores of tile i in s to probabilities.
-  auto softmax = [&](int i, uint64_t ok, typename RowsT::Scores& s,
-                     typename RowsT::Probs& p) __attribute__((always_inline)) {
+  // Before tile i's exponentials: hidden keys, and rows' first stabilisers.
+  auto prepare = [&](int i, uint64_t ok, typename RowsT::Scores& s) __attribute__((always_inline)) {
     const int k0 = (first + KW * i) * kKeys;
     checked = k0 + kKeys > length || ~ok != 0;
     if (checked) {
@@ -359,24 +395,24 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       rows.hide(seen, s);
     }
     if (__builtin_amdgcn_ballot_w64(unset) != 0) unset = rows.settle(unset, s);
-    rows.softmax(s, p);
   };
   auto output = [&](const uint8_t* vt, const typename RowsT::Probs& p)
                     __attribute__((always_inline)) {
     V8 va[8];
-    rows.read_ops(vt, va);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) va[u] = rows.v_op(vt, u);
     if (checked) {
       // What p = 0 meets must be finite; a visible NaN or infinity is added
       // to the rows that see it.
-      bool odd = false;
+      uint32_t odd = 0;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const V8 f = finite_only<T>(va[u]);
-        const u32x4_t x = __builtin_bit_cast(u32x4_t, f) ^ __builtin_bit_cast(u32x4_t, va[u]);
-        odd |= (x[0] | x[1] | x[2] | x[3]) != 0;
-        va[u] = f;
+        const u32x4_t x = __builtin_bit_cast(u32x4_t, va[u]);
+        va[u] = finite_only<T>(va[u]);
+        const u32x4_t y = __builtin_bit_cast(u32x4_t, va[u]) ^ x;
+        odd |= y[0] | y[1] | y[2] | y[3];
       }
-      if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+      if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
 #pragma unroll 1
         for (int j = 0; j < kKeys; ++j) {
           const bool sees = (seen >> j) & 1;
@@ -394,7 +430,8 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
         }
       }
     }
-    rows.output(va, p);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) rows.output(u, va[u], p);
   };
 
   if constexpr (RW == 1) {
@@ -408,7 +445,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       fetch_ids(0, 0);
       fetch_ids(1, 1);
       load_q();
-      ok = locate(0, 0);
+      ok = locate(0, 0, 0);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
       fetch(0, 0, kt);
       fetch(1, 0, vt);
@@ -422,12 +459,13 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       const bool more = i + 1 < n;
       uint64_t ok_next = 0;
       if (more) {
-        ok_next = locate(i + 1, (i + 1) & 1);
+        ok_next = locate(i + 1, (i + 1) & 1, 0);
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
         fetch_ids(i + 2, i & 1);
         fetch(0, 0, kt);
       }
-      softmax(i, ok, s, p);
+      prepare(i, ok, s);
+      rows.settle_sum(rows.exponentiate(s, p), s, p);
       if (more)
         asm volatile("s_waitcnt vmcnt(9)" : : : "memory");  // V(i)
       else
@@ -438,45 +476,55 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       ok = ok_next;
     }
   } else {
-    // RW waves share their key group's tiles, kSlots of them in a ring; each
-    // fetches 1 / RW of a tile, kSlots - 1 tiles ahead.  Wave j % RW looks up
-    // the rows of tile j one step before that, from table entries it fetched
-    // kSlots steps earlier.  One barrier a step: past it tile i has landed for
-    // all, tile i - 1 is read by none, and the next tile's addresses are there.
-    uint64_t ok[kSlots];  // of tiles i .. i + kSlots - 1
-    auto fetch_tile = [&](int slot) __attribute__((always_inline)) {
-      fetch(0, slot, sh.tile[kg][slot][0]);
-      fetch(1, slot, sh.tile[kg][slot][1]);
-      return sh.ok[kg * RW + slot];
+    // RW waves share their key group's tiles, kSlots of K and of V in rings;
+    // each fetches 1 / RW of a tile.  Step i fetches V(i + kSlots - 1) and
+    // K(i + kSlots), multiplies K(i + 1) while it exponentiates the scores of
+    // tile i, then V(i).  Wave j % RW looks up the rows of tile j a step before
+    // K(j) is fetched, from table entries it fetched kSlots steps earlier.  One
+    // barrier a step: past it K(i + 1) and V(i) have landed for all, K(i) and
+    // V(i - 1) are read by none, and the next addresses are there.
+    constexpr int kRing = Shared<RW>::kRing;
+    auto fetch_k = [&](int j) __attribute__((always_inline)) {
+      fetch(0, j & (kRing - 1), sh.tile[kg][j & (kSlots - 1)][0]);
+    };
+    auto fetch_v = [&](int j) __attribute__((always_inline)) {
+      fetch(1, j & (kRing - 1), sh.tile[kg][j & (kSlots - 1)][1]);
+    };
+    auto look_up = [&](int j) __attribute__((always_inline)) {  // wave j % RW
+      const int half = (j / kSlots) & 1;
+      locate(j, half, j & (kRing - 1));
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      return half;
     };
     fetch_ids(rw, 0);
+    fetch_ids(rw + kSlots, 1);
     load_q();
-    locate(rw, 0);
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-    fetch_ids(rw + kSlots, 0);
+    fetch_ids(rw + 2 * kSlots, look_up(rw));
+    if (rw == 0) fetch_ids(3 * kSlots, look_up(kSlots));
     __syncthreads();
+    fetch_k(0);
 #pragma unroll
-    for (int j = 0; j < kSlots - 1; ++j) ok[j] = fetch_tile(j);
-    int slot = 0;  // i % kSlots
+    for (int j = 0; j < kSlots - 1; ++j) {
+      fetch_v(j);
+      fetch_k(j + 1);
+    }
+    sync_ring<(kSlots - 1) * 2 * kSegs>();
+    typename RowsT::Scores s;
+    rows.scores(sh.tile[kg][0][0], s);
     for (int i = 0; i < n; ++i) {
       sync_ring<(kSlots - 2) * 2 * kSegs>();
-      const bool busy = first + KW * i < tiles;
-      typename RowsT::Scores s;
-      if (busy) rows.scores(sh.tile[kg][slot][0], s);
-      ok[kSlots - 1] = fetch_tile(slot == 0 ? kSlots - 1 : slot - 1);
-      if (rw == slot) {
-        locate(i + kSlots, 0);
-        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-        fetch_ids(i + 2 * kSlots, 0);
-      }
-      if (busy) {
-        typename RowsT::Probs p;
-        softmax(i, ok[0], s, p);
-        output(sh.tile[kg][slot][1], p);
-      }
-#pragma unroll
-      for (int j = 0; j < kSlots - 1; ++j) ok[j] = ok[j + 1];
-      slot = slot + 1 == kSlots ? 0 : slot + 1;
+      fetch_v(i + kSlots - 1);
+      fetch_k(i + kSlots);
+      const uint64_t ok = uniform(sh.ok[kg][i & (kRing - 1)]);
+      prepare(i, ok, s);
+      typename RowsT::Scores next;
+      typename RowsT::Probs p;
+      rows.scores(sh.tile[kg][(i + 1) & (kSlots - 1)][0], next);
+      rows.settle_sum(rows.exponentiate(s, p), s, p);
+      output(sh.tile[kg][i & (kSlots - 1)][1], p);
+      if (rw == ((i + 1) & (RW - 1)))
+        fetch_ids(i + 3 * kSlots + 1, look_up(i + kSlots + 1));
+      s = next;
     }
   }
   // Nothing may still write the tiles: partial results of the key groups meet
@@ -493,7 +541,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       const int r = 4 * (c & 3);
       own[c * 64 + lane] = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
     }
-    sh.ml[w][lane] = make_float2(rows.stabiliser(), rows.l);
+    sh.ml[w][lane] = make_float2(rows.mc, rows.l);
     __syncthreads();
     // They meet at their largest stabiliser; one without a visible key (l = 0
     // across the lane pair) is passed over.
@@ -515,7 +563,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     l_tot = pair_sum(lt);
   } else {
     l_tot = pair_sum(rows.l);
-    mm = rows.stabiliser();
+    mm = rows.mc;
   }
   const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
   T* const orow = O + (b * g.o_sb + head * g.o_sh + draft * g.o_sr);
