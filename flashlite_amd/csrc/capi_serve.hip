@@ -128,7 +128,13 @@ int check_tree(const fl_tree_params* p, const char* who) {
   if (rc == FL_OK) rc = check_view(p->o_stride, 8, "o", who);
   if (rc == FL_OK) rc = check_view(p->k_stride, 8, "k_cache", who);
   if (rc == FL_OK) rc = check_view(p->v_stride, 8, "v_cache", who);
-  return rc;
+  if (rc != FL_OK) return rc;
+  // Rows are found by 32-bit block and row strides in bytes.
+  for (int i = 0; i < 3; i += 2)
+    if (p->k_stride[i] > INT32_MAX || p->v_stride[i] > INT32_MAX)
+      return set_error(FL_ERR_UNSUPPORTED,
+                       "%s: block and row strides of the caches must be below 2^31 elements", who);
+  return FL_OK;
 }
 
 bool empty_tree(const fl_tree_params* p) { return p->batch == 0 || p->heads == 0 || p->drafts == 0; }

@@ -17,7 +17,8 @@ namespace {
 
 struct TreeGeom {
   long long q_sb, q_sh, q_sr, o_sb, o_sh, o_sr;  // elements
-  long long k_blk, k_head, k_row, v_blk, v_head, v_row;  // bytes
+  long long k_head, v_head;             // bytes
+  uint32_t k_blk, k_row, v_blk, v_row;  // bytes
   const int32_t* tables;
   long long table_stride;
   const int32_t* lengths;
@@ -199,7 +200,8 @@ __device__ __forceinline__ void fetch4(uint64_t address, const void* lds) {
   asm volatile("global_load_lds_dword %0, off" : : "v"(address), "{m0}"(base) : "memory");
 }
 
-constexpr int kWaves = 4;
+// Waves of a work-group of RW row blocks: 4, two work-groups a CU, or 8.
+constexpr int waves_of(int rw) { return rw == 8 ? 8 : 4; }
 
 // One request: its tokens and its drafts that are there.
 struct Request {
@@ -228,7 +230,7 @@ __device__ __forceinline__ int unit_drafts(const TreeGeom& g, const Request& r, 
 // Steps of a unit's walk, 0 where no draft of its rows is there.
 template <int D, int RW>
 __device__ __forceinline__ int unit_steps(const TreeGeom& g, const Request& r, int rb) {
-  constexpr int kStepKeys = (kWaves / RW) * (D == 64 ? kBc : kBc2);
+  constexpr int kStepKeys = (waves_of(RW) / RW) * (D == 64 ? kBc : kBc2);
   if (rb * 32 * RW >= r.count * g.group.d) return 0;
   return (r.length + unit_drafts(g, r, rb, 32 * RW) + kStepKeys - 1) / kStepKeys;
 }
@@ -261,13 +263,19 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 // The work-group's LDS: key and value tiles, and per wave the row addresses of
 // the next tile's keys and table entries fetched ahead.
-template <int RW>
+template <int D, int RW>
 struct Shared {
+  static constexpr int kWaves = waves_of(RW);
+  static constexpr int kGroups = kWaves / RW;
   static constexpr int kSlots = RW;  // of each key group
-  uint8_t tile[kWaves / RW][kSlots][2][kTileBytes];
-  static constexpr int kRing = RW == 1 ? 1 : 2 * kSlots;  // looked-up tiles
-  uint64_t where[kWaves / RW][kRing][2][64];
-  uint64_t ok[kWaves / RW][kRing];
+  // Tiles a wave looks up at once (64 keys, but for RW == 1), and entries of
+  // the ring of looked-up ones: those of tiles i .. i + kSlots + 2.
+  static constexpr int kPer = RW > 1 && D == 128 ? 2 : 1;
+  static constexpr int kRing =
+      RW == 1 ? 1 : RW == 2 ? 4 : RW == 4 || D == 128 ? 8 : 16;
+  uint8_t tile[kGroups][kSlots][2][kTileBytes];
+  uint64_t where[kGroups][kRing][2][64];
+  uint64_t ok[kGroups][kRing];
   int32_t ids[kWaves][2][64];
   float2 ml[kWaves][64];
 };
@@ -276,13 +284,13 @@ struct Shared {
 // (and lse) with part == nullptr, or unnormalised to `part`.
 template <int D, class T, int RW>
 __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t* V, T* O,
-                                     const TreeGeom& g, Shared<RW>& sh, int b, int kvh, int rb,
+                                     const TreeGeom& g, Shared<D, RW>& sh, int b, int kvh, int rb,
                                      const Request& req, int s0, int s1, float* part, float cq,
                                      float cr) {
   using RowsT = TreeRows<D, T>;
   using V8 = typename RowsT::V8;
   constexpr int kKeys = RowsT::kKeys, kRowB = 2 * D;
-  constexpr int KW = kWaves / RW;
+  constexpr int KW = waves_of(RW) / RW;
   constexpr int kLanes = kRowB / 16;      // lanes a row of a fetch
   constexpr int kSegRows = 64 / kLanes;   // rows a fetch
   constexpr int kSegs = 8 / RW;           // fetches of a tile by this wave
@@ -346,30 +354,38 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   const uint64_t kbase = (uint64_t)(uintptr_t)(K + kvh * g.k_head);
   const uint64_t vbase = (uint64_t)(uintptr_t)(V + kvh * g.v_head);
   int32_t(*const ids)[64] = sh.ids[w];
-  // Key l of this key group's tile i (past the last key: the last again).
-  auto key_of = [&](int i) __attribute__((always_inline)) {
-    return min((first + KW * i) * kKeys + (lane & (kKeys - 1)), keys - 1);
+  using Sh = Shared<D, RW>;
+  constexpr int kPer = Sh::kPer, kRing = Sh::kRing;
+  // The key that lane l looks up for the key group's tiles kPer m ..: key
+  // l % kKeys of tile kPer m + l / kKeys (past the last key: the last again).
+  auto key_of = [&](int m) __attribute__((always_inline)) {
+    const int tile = kPer * m + (kPer == 2 ? lane / kKeys : 0);
+    return min((first + KW * tile) * kKeys + (lane & (kKeys - 1)), keys - 1);
   };
-  auto fetch_ids = [&](int i, int slot) __attribute__((always_inline)) {
-    fetch4(table + 4 * (uint64_t)divide(key_of(i), g.block), ids[slot]);
+  auto fetch_ids = [&](int m, int buffer) __attribute__((always_inline)) {
+    fetch4(table + 4 * (uint64_t)divide(key_of(m), g.block), ids[buffer]);
   };
-  // Row addresses of tile i, from table entries in ids[slot], and a bit per
-  // key with a block, to entry `to` of the key group's.
-  auto locate = [&](int i, int slot, int to) __attribute__((always_inline)) {
-    const int key = key_of(i);
-    const int in = key - divide(key, g.block) * g.block.d;
-    int id = ids[slot][lane];
-    const bool ok = (uint32_t)id < (uint32_t)g.num_blocks;
-    id = ok ? id : 0;
-    sh.where[kg][to][0][lane] = kbase + (id * g.k_blk + in * g.k_row);
-    sh.where[kg][to][1][lane] = vbase + (id * g.v_blk + in * g.v_row);
-    const uint64_t all = __builtin_amdgcn_ballot_w64(ok);
+  // Their rows' addresses, from table entries in ids[buffer], and a bit per
+  // key with a block, to the ring.
+  auto look_up = [&](int m, int buffer) __attribute__((always_inline)) {
+    const int key = key_of(m);
+    const uint32_t in = key - divide(key, g.block) * g.block.d;
+    uint32_t id = ids[buffer][lane];
+    const bool good = id < (uint32_t)g.num_blocks;
+    id = good ? id : 0;
+    const int to = m & (kRing - 1);
+    sh.where[kg][to][0][lane] = kbase + ((uint64_t)id * g.k_blk + (uint64_t)in * g.k_row);
+    sh.where[kg][to][1][lane] = vbase + ((uint64_t)id * g.v_blk + (uint64_t)in * g.v_row);
+    const uint64_t all = __builtin_amdgcn_ballot_w64(good);
     if constexpr (RW > 1) sh.ok[kg][to] = all;
     return all;
   };
-  // This wave's share of the K (t = 0) or V (1) tile whose rows are in entry
-  // `from`.
-  auto fetch = [&](int t, int from, uint8_t* tile) __attribute__((always_inline)) {
+  // This wave's share of the K (t = 0) or V (1) tile j, whose rows are in the
+  // ring.
+  auto fetch = [&](int t, int j) __attribute__((always_inline)) {
+    uint8_t* const tile = sh.tile[kg][j & (kSlots - 1)][t];
+    const uint64_t* const from =
+        sh.where[kg][(j / kPer) & (kRing - 1)][t] + (kPer == 2 ? (j & 1) * kKeys : 0);
     uint64_t at[kSegs];
 #pragma unroll
     for (int i = 0; i < kSegs; ++i) {
@@ -377,13 +393,13 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       const int phys = lane & (kLanes - 1);
       const int chunk = phys ^ (D == 64 ? (t ? v_swz(r) : k_swz(r))
                                         : (t ? v_swz128(r) : k_swz128(r)));
-      at[i] = sh.where[kg][from][t][r] + 16 * chunk;
+      at[i] = from[r] + 16 * chunk;
     }
 #pragma unroll
     for (int i = 0; i < kSegs; ++i) fetch16(at[i], tile + 1024 * (rw * kSegs + i));
   };
 
-  bool unset = true;
+  bool unset = true, fresh = true;  // this lane's row, some row has no stabiliser yet
   uint64_t seen = 0;
   bool checked = false;
   // Before tile i's exponentials: hidden keys, and rows' first stabilisers.
@@ -394,13 +410,17 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       seen = seen_bits(k0) & ok;
       rows.hide(seen, s);
     }
-    if (__builtin_amdgcn_ballot_w64(unset) != 0) unset = rows.settle(unset, s);
+    if (fresh) {
+      unset = rows.settle(unset, s);
+      fresh = __builtin_amdgcn_ballot_w64(unset) != 0;
+    }
   };
-  auto output = [&](const uint8_t* vt, const typename RowsT::Probs& p)
-                    __attribute__((always_inline)) {
-    V8 va[8];
+  auto read_v = [&](const uint8_t* vt, V8 (&va)[8]) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) va[u] = rows.v_op(vt, u);
+  };
+  auto output = [&](const uint8_t* vt, V8 (&va)[8], const typename RowsT::Probs& p)
+                    __attribute__((always_inline)) {
     if (checked) {
       // What p = 0 meets must be finite; a visible NaN or infinity is added
       // to the rows that see it.
@@ -445,10 +465,10 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       fetch_ids(0, 0);
       fetch_ids(1, 1);
       load_q();
-      ok = locate(0, 0, 0);
+      ok = look_up(0, 0);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      fetch(0, 0, kt);
-      fetch(1, 0, vt);
+      fetch(0, 0);
+      fetch(1, 0);
     }
     for (int i = 0; i < n; ++i) {
       typename RowsT::Scores s;
@@ -459,10 +479,10 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       const bool more = i + 1 < n;
       uint64_t ok_next = 0;
       if (more) {
-        ok_next = locate(i + 1, (i + 1) & 1, 0);
+        ok_next = look_up(i + 1, (i + 1) & 1);
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
         fetch_ids(i + 2, i & 1);
-        fetch(0, 0, kt);
+        fetch(0, i + 1);
       }
       prepare(i, ok, s);
       rows.settle_sum(rows.exponentiate(s, p), s, p);
@@ -470,60 +490,71 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
         asm volatile("s_waitcnt vmcnt(9)" : : : "memory");  // V(i)
       else
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-      output(vt, p);
+      V8 va[8];
+      read_v(vt, va);
+      output(vt, va, p);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      if (more) fetch(1, 0, vt);
+      if (more) fetch(1, i + 1);
       ok = ok_next;
     }
   } else {
     // RW waves share their key group's tiles, kSlots of K and of V in rings;
     // each fetches 1 / RW of a tile.  Step i fetches V(i + kSlots - 1) and
     // K(i + kSlots), multiplies K(i + 1) while it exponentiates the scores of
-    // tile i, then V(i).  Wave j % RW looks up the rows of tile j a step before
-    // K(j) is fetched, from table entries it fetched kSlots steps earlier.  One
-    // barrier a step: past it K(i + 1) and V(i) have landed for all, K(i) and
-    // V(i - 1) are read by none, and the next addresses are there.
-    constexpr int kRing = Shared<RW>::kRing;
-    auto fetch_k = [&](int j) __attribute__((always_inline)) {
-      fetch(0, j & (kRing - 1), sh.tile[kg][j & (kSlots - 1)][0]);
-    };
-    auto fetch_v = [&](int j) __attribute__((always_inline)) {
-      fetch(1, j & (kRing - 1), sh.tile[kg][j & (kSlots - 1)][1]);
-    };
-    auto look_up = [&](int j) __attribute__((always_inline)) {  // wave j % RW
-      const int half = (j / kSlots) & 1;
-      locate(j, half, j & (kRing - 1));
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      return half;
-    };
+    // tile i, then V(i).  A step before K(j) is fetched, wave (j / kPer) % RW
+    // looks up its rows (and the next tile's), from table entries it fetched
+    // when it last did.  One barrier a step: past it K(i + 1) and V(i) have
+    // landed for all, K(i) and V(i - 1) are read by none, and the next
+    // addresses are there.
+    constexpr int kFirst = kPer == 2 ? kSlots / 2 : kSlots;  // lookups 0 .. kFirst at once
     fetch_ids(rw, 0);
-    fetch_ids(rw + kSlots, 1);
+    fetch_ids(rw + RW, 1);
     load_q();
-    fetch_ids(rw + 2 * kSlots, look_up(rw));
-    if (rw == 0) fetch_ids(3 * kSlots, look_up(kSlots));
+    if (rw <= kFirst) {
+      look_up(rw, 0);
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      fetch_ids(rw + 2 * RW, 0);
+    }
+    if (kFirst == RW && rw == 0) {
+      look_up(RW, 1);
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      fetch_ids(3 * RW, 1);
+    }
     __syncthreads();
-    fetch_k(0);
+    fetch(0, 0);
 #pragma unroll
     for (int j = 0; j < kSlots - 1; ++j) {
-      fetch_v(j);
-      fetch_k(j + 1);
+      fetch(1, j);
+      fetch(0, j + 1);
     }
     sync_ring<(kSlots - 1) * 2 * kSegs>();
     typename RowsT::Scores s;
     rows.scores(sh.tile[kg][0][0], s);
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
       sync_ring<(kSlots - 2) * 2 * kSegs>();
-      fetch_v(i + kSlots - 1);
-      fetch_k(i + kSlots);
-      const uint64_t ok = uniform(sh.ok[kg][i & (kRing - 1)]);
+      uint64_t ok = uniform(sh.ok[kg][(i / kPer) & (kRing - 1)]);
+      if constexpr (kPer == 2)
+        ok = (i & 1 ? ok >> 32 : ok) | 0xFFFFFFFF00000000u;  // (bits of 32 keys)
       prepare(i, ok, s);
+      const uint8_t* const vt = sh.tile[kg][i & (kSlots - 1)][1];
       typename RowsT::Scores next;
       typename RowsT::Probs p;
+      V8 va[8];
       rows.scores(sh.tile[kg][(i + 1) & (kSlots - 1)][0], next);
-      rows.settle_sum(rows.exponentiate(s, p), s, p);
-      output(sh.tile[kg][i & (kSlots - 1)][1], p);
-      if (rw == ((i + 1) & (RW - 1)))
-        fetch_ids(i + 3 * kSlots + 1, look_up(i + kSlots + 1));
+      const float sum = rows.exponentiate(s, p);
+      fetch(1, i + kSlots - 1);
+      fetch(0, i + kSlots);
+      read_v(vt, va);
+      rows.settle_sum(sum, s, p);
+      output(vt, va, p);
+      const int m = (i + kSlots + 1) / kPer;
+      if ((kPer == 1 || (i & 1) != 0) && rw == (m & (RW - 1))) {
+        const int buffer = (m / RW) & 1;
+        look_up(m, buffer);
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+        fetch_ids(m + 2 * RW, buffer);
+      }
       s = next;
     }
   }
@@ -627,10 +658,10 @@ __device__ __forceinline__ int group_index(int xcds) {
 
 // A unit a work-group.
 template <int D, class T, int RW>
-__global__ void __launch_bounds__(64 * kWaves, 2)
+__global__ void __launch_bounds__(64 * waves_of(RW), 2)
 tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
                 float cr) {
-  __shared__ __attribute__((aligned(16))) Shared<RW> sh;
+  __shared__ __attribute__((aligned(16))) Shared<D, RW> sh;
   const int per = g.kv_heads * g.blocks_of_rows;
   const int unit = group_index(g.xcds);
   const int b = unit / per, rest = unit - b * per;
@@ -648,11 +679,11 @@ tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tree
 // which work-group that was; between them each work-group has one in its first
 // slot.  (Fewer than 2^31 steps: tree_plan.)
 template <int D, class T, int RW>
-__global__ void __launch_bounds__(64 * kWaves, 2)
+__global__ void __launch_bounds__(64 * waves_of(RW), 2)
 tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
                   float cr) {
   constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
-  __shared__ __attribute__((aligned(16))) Shared<RW> sh;
+  __shared__ __attribute__((aligned(16))) Shared<D, RW> sh;
   const int lane = threadIdx.x & 63;
   // Steps of one key/value head of requests b0 .. b0 + 63, one a lane.
   Request c;
@@ -831,9 +862,9 @@ struct TreePlan {
 TreePlan tree_plan(const fl_tree_params& p) {
   TreePlan t;
   const int64_t rows = p.heads / p.kv_heads * p.drafts;
-  t.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  t.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
   t.units = (int)((rows + 32 * t.rw - 1) / (32 * t.rw) * p.kv_heads * p.batch);
-  t.grid = 2 * device_cus();
+  t.grid = (t.rw == 8 ? 1 : 2) * device_cus();
   t.split = t.units < 2 * t.grid;
   const int64_t part = p.head_dim == 64 ? kPartStride : kPartStride128;
   t.bytes = t.split ? 2LL * t.grid * 32 * t.rw * part * (int64_t)sizeof(float) +
@@ -845,7 +876,7 @@ TreePlan tree_plan(const fl_tree_params& p) {
 template <int D, class T, int RW>
 hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, float cq, float cr,
                      hipStream_t st) {
-  constexpr int kStepKeys = (kWaves / RW) * (D == 64 ? kBc : kBc2);
+  constexpr int kStepKeys = (waves_of(RW) / RW) * (D == 64 ? kBc : kBc2);
   g.blocks_of_rows = (g.rows + 32 * RW - 1) / (32 * RW);
   const T* q = static_cast<const T*>(p.q);
   const uint8_t *k = static_cast<const uint8_t*>(p.k_cache),
@@ -854,14 +885,14 @@ hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, fl
   // A split launch counts steps in 32 bits.
   const bool counted = t.units * (((int64_t)g.capacity + g.drafts) / kStepKeys + 1) < (1LL << 30);
   if (g.part == nullptr || !counted) {
-    hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW>), dim3((unsigned)t.units), dim3(64 * kWaves), 0,
+    hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW>), dim3((unsigned)t.units), dim3(64 * waves_of(RW)), 0,
                        st, q, k, v, o, g, cq, cr);
     return hipGetLastError();
   }
   g.least_log2 = 0;
   g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.grid * 32 * RW *
                                                  (D == 64 ? kPartStride : kPartStride128));
-  hipLaunchKernelGGL((tree_split_kernel<D, T, RW>), dim3((unsigned)t.grid), dim3(64 * kWaves), 0,
+  hipLaunchKernelGGL((tree_split_kernel<D, T, RW>), dim3((unsigned)t.grid), dim3(64 * waves_of(RW)), 0,
                      st, q, k, v, o, g, cq, cr);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
@@ -876,7 +907,8 @@ hipError_t launch_t(const fl_tree_params& p, TreeGeom& g, float cq, float cr, hi
   const TreePlan t = tree_plan(p);
   return t.rw == 1   ? launch_rw<D, T, 1>(p, t, g, cq, cr, st)
          : t.rw == 2 ? launch_rw<D, T, 2>(p, t, g, cq, cr, st)
-                     : launch_rw<D, T, 4>(p, t, g, cq, cr, st);
+         : t.rw == 4 ? launch_rw<D, T, 4>(p, t, g, cq, cr, st)
+                     : launch_rw<D, T, 8>(p, t, g, cq, cr, st);
 }
 
 }  // namespace
@@ -893,12 +925,12 @@ hipError_t launch_tree_fwd(const fl_tree_params& p, void* ws, hipStream_t st) {
   g.o_sb = p.o_stride[0];
   g.o_sh = p.o_stride[1];
   g.o_sr = p.o_stride[2];
-  g.k_blk = 2 * p.k_stride[0];
+  g.k_blk = (uint32_t)(2 * p.k_stride[0]);
   g.k_head = 2 * p.k_stride[1];
-  g.k_row = 2 * p.k_stride[2];
-  g.v_blk = 2 * p.v_stride[0];
+  g.k_row = (uint32_t)(2 * p.k_stride[2]);
+  g.v_blk = (uint32_t)(2 * p.v_stride[0]);
   g.v_head = 2 * p.v_stride[1];
-  g.v_row = 2 * p.v_stride[2];
+  g.v_row = (uint32_t)(2 * p.v_stride[2]);
   g.tables = p.block_tables;
   g.table_stride = p.table_stride;
   g.lengths = p.lengths;
