@@ -864,7 +864,7 @@ TreePlan tree_plan(const fl_tree_params& p) {
   const int64_t rows = p.heads / p.kv_heads * p.drafts;
   t.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
   t.units = (int)((rows + 32 * t.rw - 1) / (32 * t.rw) * p.kv_heads * p.batch);
-  t.grid = (t.rw == 8 ? 1 : 2) * device_cus();
+  t.grid = device_cus();
   t.split = t.units < 2 * t.grid;
   const int64_t part = p.head_dim == 64 ? kPartStride : kPartStride128;
   t.bytes = t.split ? 2LL * t.grid * 32 * t.rw * part * (int64_t)sizeof(float) +
