@@ -6,6 +6,7 @@
 // requests moves a few KiB.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fl_serve.h"
 
@@ -13,29 +14,42 @@ namespace fl {
 
 namespace {
 
-// Sum over the lanes below (exclusive) within the work-group; `total` gets the
-// whole sum.  `part` holds a value per wave.
-template <int kWaves>
-__device__ __forceinline__ long long group_scan(long long x, long long* part, long long& total) {
+// Inclusive sum over a wave's lanes: within rows of 16, then over the rows.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);  // row_bcast:31
+  return x;
+}
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+
+// Exclusive sums of two values over the work-group, and their totals.
+struct Sums {
+  int before[2], total[2];
+};
+
+__device__ __forceinline__ Sums group_scan(int x, int y, int2 (&part)[kWaves]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  long long s = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const long long y = __shfl_up(s, d);
-    if (lane >= d) s += y;
-  }
-  if (lane == 63) part[w] = s;
+  const int sx = wave_scan(x), sy = wave_scan(y);
+  __syncthreads();  // the last call's parts are read
+  if (lane == 63) part[w] = make_int2(sx, sy);
   __syncthreads();
-  long long before = 0;
-  total = 0;
+  Sums s = {{sx - x, sy - y}, {0, 0}};
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) {
-    const long long y = part[i];
-    if (i < w) before += y;
-    total += y;
+    const int2 p = part[i];
+    if (i < w) {
+      s.before[0] += p.x;
+      s.before[1] += p.y;
+    }
+    s.total[0] += p.x;
+    s.total[1] += p.y;
   }
-  __syncthreads();
-  return before + s - x;
+  return s;
 }
 
 struct PlanGeom {
@@ -52,7 +66,7 @@ struct PlanGeom {
   int32_t* info;
   long long table_stride;
   int batch, width, max_blocks, pool;
-  FastDiv block;
+  FastDiv block, by_width;
 };
 
 __device__ __forceinline__ int divide(int n, const FastDiv& f) {
@@ -81,73 +95,71 @@ __device__ __forceinline__ Want want(const PlanGeom& g, int b) {
   return r;
 }
 
-constexpr int kScanThreads = 1024;
+// What a call does with one request (fl_attn_cache_plan's info).
+struct Move {
+  int status, held, moved, first;
+};
 
-// One work-group: prefix sums of the blocks needed and given back over the
-// requests, 1024 at a time.
-__global__ void __launch_bounds__(kScanThreads) cache_plan_scan_kernel(const PlanGeom g) {
-  constexpr int kWaves = kScanThreads / 64;
-  __shared__ long long part[kWaves];
+// The moves of all requests, 256 at a time: put(b, move) is called for each by
+// one thread; returns the ring's new head and count.  Every thread of the
+// work-group takes part, and has read the state and every held count when it
+// returns.
+template <class F>
+__device__ __forceinline__ int2 plan(const PlanGeom& g, F&& put) {
+  __shared__ int2 part[kWaves];
   const int count = min(max(g.state[1], 0), g.pool);
   const int head = (int)((unsigned)max(g.state[0], 0) % (unsigned)g.pool);
-  long long before = 0, back_before = 0, taken_sum = 0, given_sum = 0;
-  for (int b0 = 0; b0 < g.batch; b0 += kScanThreads) {
+  int needed = 0, backs = 0, taken = 0, given = 0;
+#pragma unroll 1
+  for (int b0 = 0; b0 < g.batch; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
     Want r = {};
     if (b < g.batch) r = want(g, b);
     const int back = r.ended ? r.held : 0;
-    long long sum_need, sum_back, sum_taken, sum_given;
-    const long long off = before + group_scan<kWaves>(r.need, part, sum_need);
-    const long long roff = back_before + group_scan<kWaves>(back, part, sum_back);
-    const bool served = !r.wide && (r.need == 0 || off + r.need <= count);
-    const int taken = served ? r.need : 0;
-    const long long room = (long long)g.pool - count - roff;
-    const int given = (int)min((long long)back, max(room, 0LL));
-    group_scan<kWaves>(taken, part, sum_taken);
-    group_scan<kWaves>(given, part, sum_given);
-    if (b < g.batch) {
-      g.held_out[b] = r.ended ? 0 : r.held + taken;
-      int32_t* const info = g.info + 4LL * b;
-      info[0] = r.wide ? 2 : served ? 0 : 1;
-      info[1] = r.held;
-      info[2] = taken - given;
-      info[3] = (int)((head + (r.ended ? count + roff : off)) % g.pool);
-    }
-    before += sum_need;
-    back_before += sum_back;
-    taken_sum += sum_taken;
-    given_sum += sum_given;
+    const Sums s = group_scan(r.need, back, part);
+    const int off = needed + s.before[0], behind = backs + s.before[1];
+    const bool served = !r.wide && (r.need == 0 || (long long)off + r.need <= count);
+    Move m;
+    m.status = r.wide ? 2 : served ? 0 : 1;
+    m.held = r.held;
+    m.moved = r.ended ? -min(back, max(g.pool - count - behind, 0)) : served ? r.need : 0;
+    m.first = (int)((head + (r.ended ? (long long)count + behind : (long long)off)) % g.pool);
+    if (b < g.batch) put(b, m);
+    needed += s.total[0];
+    backs += s.total[1];
+    const Sums t = group_scan(max(m.moved, 0), max(-m.moved, 0), part);
+    taken += t.total[0];
+    given += t.total[1];
   }
-  __syncthreads();  // every thread has read the state
-  if (threadIdx.x == 0) {
-    g.state_out[0] = (int)((head + taken_sum) % g.pool);
-    g.state_out[1] = (int)(count - taken_sum + given_sum);
-  }
+  return make_int2((int)(((long long)head + taken) % g.pool), count - taken + given);
 }
 
-// Request blockIdx.y: its taken blocks' table entries, or its blocks put back
-// on the ring (the first work-group), and its share of positions and slots.
-__global__ void __launch_bounds__(256) cache_plan_fill_kernel(const PlanGeom g) {
-  const int b = blockIdx.y;
-  const int32_t* const info = g.info + 4LL * b;
-  const int status = info[0], held = info[1], moved = info[2], first = info[3];
+// The held count and info of request b.
+__device__ __forceinline__ void note(const PlanGeom& g, int b, const Move& m, bool ended) {
+  g.held_out[b] = ended ? 0 : m.held + max(m.moved, 0);
+  *reinterpret_cast<int4*>(g.info + 4LL * b) = make_int4(m.status, m.held, m.moved, m.first);
+}
+
+// Request b's table entries, or its blocks back to the ring.
+__device__ __forceinline__ void move_blocks(const PlanGeom& g, int b, const Move& m) {
   int32_t* const table = g.tables + b * g.table_stride;
-  if (blockIdx.x == 0) {
-    for (int k = threadIdx.x; k < moved; k += 256)
-      table[held + k] = g.ring[((long long)first + k) % g.pool];
-    for (int k = threadIdx.x; k < -moved; k += 256)
-      g.ring[((long long)first + k) % g.pool] = table[k];
-  }
-  const int length = max(g.lengths[b], 0);
-  const int fresh = status == 0 ? min(max(g.counts[b], 0), g.width) : 0;
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= g.width) return;
+  for (int k = threadIdx.x; k < m.moved; k += kThreads)
+    table[m.held + k] = g.ring[((long long)m.first + k) % g.pool];
+  for (int k = threadIdx.x; k < -m.moved; k += kThreads)
+    g.ring[((long long)m.first + k) % g.pool] = table[k];
+}
+
+// Position and slot of new token i of request b.  (Blocks that this call takes
+// are read from the ring, which it writes nowhere else.)
+__device__ __forceinline__ void place(const PlanGeom& g, int b, int i, const Move& m) {
   int position = -1;
   long long slot = -1;
+  const int fresh = m.status == 0 ? min(g.counts[b], g.width) : 0;
   if (i < fresh) {
-    const int at = length + i;
+    const int at = max(g.lengths[b], 0) + i;
     const int k = divide(at, g.block);
-    const int id = k < held ? table[k] : g.ring[((long long)first + (k - held)) % g.pool];
+    const int id = k < m.held ? g.tables[b * g.table_stride + k]
+                              : g.ring[((long long)m.first + (k - m.held)) % g.pool];
     if (id >= 0) {
       position = at;
       slot = (long long)id * g.block.d + (at - k * g.block.d);
@@ -158,49 +170,109 @@ __global__ void __launch_bounds__(256) cache_plan_fill_kernel(const PlanGeom g) 
   g.slots[o] = slot;
 }
 
-// One work-group a request.  seen[i] starts as draft i's own bit and up[i] as
-// its parent; each round seen[i] |= seen[up[i]], up[i] = up[up[i]], after
-// which seen[i] holds i's 2^round nearest ancestors.  (A round may already
-// read a neighbour's new words: they only hold more of the same ancestors.)
-__global__ void __launch_bounds__(256)
+// Up to kKept requests in one launch: every work-group finds all moves and
+// keeps them in LDS, the first notes them, and the requests' blocks and the
+// tokens are dealt to all.  With several work-groups the new held counts and
+// ring state must not be the old ones' memory, which another may still read.
+constexpr int kKept = 2048;
+__global__ void __launch_bounds__(kThreads) cache_plan_kernel(const PlanGeom g) {
+  __shared__ Move moves[kKept];
+  const int2 state = plan(g, [&](int b, const Move& m) __attribute__((always_inline)) {
+    moves[b] = m;
+  });
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int b = threadIdx.x; b < g.batch; b += kThreads) note(g, b, moves[b], g.counts[b] < 0);
+    if (threadIdx.x == 0) {
+      g.state_out[0] = state.x;
+      g.state_out[1] = state.y;
+    }
+  }
+  for (int b = blockIdx.x; b < g.batch; b += gridDim.x) move_blocks(g, b, moves[b]);
+  const uint32_t all = (uint32_t)g.batch * (uint32_t)g.width, step = gridDim.x * kThreads;
+  for (uint32_t e = blockIdx.x * kThreads + threadIdx.x; e < all; e += step) {
+    const int b = divide((int)e, g.by_width);
+    place(g, b, (int)e - b * g.width, moves[b]);
+  }
+}
+
+// Otherwise in two: the moves by one work-group, then a work-group's threads
+// each token of request blockIdx.y (the first also its blocks).
+__global__ void __launch_bounds__(kThreads) cache_plan_scan_kernel(const PlanGeom g) {
+  const int2 state = plan(g, [&](int b, const Move& m) __attribute__((always_inline)) {
+    note(g, b, m, g.counts[b] < 0);
+  });
+  if (threadIdx.x == 0) {
+    g.state_out[0] = state.x;
+    g.state_out[1] = state.y;
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) cache_plan_fill_kernel(const PlanGeom g) {
+  const int b = blockIdx.y;
+  const int4 info = *reinterpret_cast<const int4*>(g.info + 4LL * b);
+  const Move m = {info.x, info.y, info.z, info.w};
+  if (blockIdx.x == 0) move_blocks(g, b, m);
+  const int i = blockIdx.x * kThreads + threadIdx.x;
+  if (i < g.width) place(g, b, i, m);
+}
+
+// One work-group a request, a thread a draft.  seen[w][i] starts as draft i's
+// own bit and up[i] as its parent; each round seen[.][i] |= seen[.][up[i]],
+// up[i] = up[up[i]], after which it holds i's 2^round nearest ancestors, until
+// no draft has further ones: about log2 of the tree's depth rounds.  (A round
+// may already read a neighbour's new words: they only hold more of the same
+// ancestors.)  Word w has bits of drafts from 64 w on only.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS)
 tree_plan_kernel(const int32_t* parents, long long parent_stride, const int32_t* lengths,
                  const int32_t* counts, int64_t* mask, int32_t* positions, int n) {
-  extern __shared__ uint64_t seen[];  // [n][words], then up[2][n]
+  constexpr int kWords = THREADS / 64;
+  __shared__ uint64_t seen[kWords][THREADS];
+  __shared__ int up[2][THREADS];
   const int words = (n + 63) / 64;
-  int* const up0 = reinterpret_cast<int*>(seen + n * words);
-  const int b = blockIdx.x;
+  const int b = blockIdx.x, i = threadIdx.x;
   const int count = counts ? min(max(counts[b], 0), n) : n;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const int p = parents[b * parent_stride + i];
-    up0[i] = p >= 0 && p < i ? p : -1;
-  }
-  for (int x = threadIdx.x; x < n * words; x += 256) {
-    const int i = x / words, w = x - i * words;
-    seen[x] = i >> 6 == w ? (uint64_t)1 << (i & 63) : 0;
-  }
-  __syncthreads();
-  int cur = 0;
-  for (int reach = 1; reach < n; reach <<= 1) {
-    const int* const up = up0 + cur * n;
-    int* const next = up0 + (cur ^ 1) * n;
-    for (int x = threadIdx.x; x < n * words; x += 256) {
-      const int i = x / words;
-      const int u = up[i];
-      if (u >= 0) seen[x] |= seen[u * words + (x - i * words)];
-    }
-    for (int i = threadIdx.x; i < n; i += 256) next[i] = up[i] >= 0 ? up[up[i]] : -1;
-    cur ^= 1;
-    __syncthreads();
-  }
   const int length = max(lengths[b], 0);
-  for (int i = threadIdx.x; i < n; i += 256) {
-    int above = -1;
-    for (int w = 0; w < words; ++w) above += __popcll(seen[i * words + w]);
-    positions[(long long)b * n + i] = i < count ? length + above : -1;
+  int u = i < n ? parents[b * parent_stride + i] : -1;
+  u = u >= 0 && u < i ? u : -1;
+  up[0][i] = u;
+  uint64_t own[kWords];
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) {
+    own[w] = w == i >> 6 ? (uint64_t)1 << (i & 63) : 0;
+    seen[w][i] = own[w];
   }
-  for (int x = threadIdx.x; x < n * words; x += 256)
-    mask[(long long)b * n * words + x] = x / words < count ? (int64_t)seen[x] : 0;
+  int cur = 0;
+#pragma unroll 1
+  while (__syncthreads_or(u >= 0)) {
+    int next = -1;
+    if (u >= 0) {
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        own[w] |= seen[w][u];
+        seen[w][i] = own[w];
+      }
+      next = up[cur][u];
+    }
+    cur ^= 1;
+    u = next;
+    up[cur][i] = u;
+  }
+  if (i >= n) return;
+  int above = -1;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w) above += __popcll(own[w]);
+  const bool there = i < count;
+  positions[(long long)b * n + i] = there ? length + above : -1;
+  int64_t* const out = mask + ((long long)b * n + i) * words;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w)
+    if (w < words) out[w] = there ? (int64_t)own[w] : 0;
 }
+
+// Tokens a work-group of the one-launch form.
+constexpr int kEach = 2048;
 
 }  // namespace
 
@@ -223,20 +295,37 @@ hipError_t launch_cache_plan(const fl_cache_plan_params& p, hipStream_t stream) 
   g.max_blocks = (int)p.max_blocks;
   g.pool = (int)p.pool;
   g.block = fast_div((int)p.block_size);
-  hipLaunchKernelGGL(cache_plan_scan_kernel, dim3(1), dim3(kScanThreads), 0, stream, g);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.batch == 0) return e;
-  const unsigned across = (unsigned)std::max<int64_t>(1, (p.width + 255) / 256);
-  hipLaunchKernelGGL(cache_plan_fill_kernel, dim3(across, (unsigned)p.batch), dim3(256), 0, stream,
-                     g);
+  g.by_width = fast_div((int)std::max<int64_t>(1, p.width));
+  const int64_t all = p.batch * p.width;
+  const int64_t groups = std::max<int64_t>(1, std::min<int64_t>((all + kEach - 1) / kEach, 1024));
+  const bool in_place = p.held == p.held_out || p.free_state == p.free_state_out;
+  if (p.batch <= kKept && all <= INT32_MAX && (groups == 1 || !in_place)) {
+    hipLaunchKernelGGL(cache_plan_kernel, dim3((unsigned)groups), dim3(kThreads), 0, stream, g);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(cache_plan_scan_kernel, dim3(1), dim3(kThreads), 0, stream, g);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const unsigned across = (unsigned)std::max<int64_t>(1, (p.width + kThreads - 1) / kThreads);
+  hipLaunchKernelGGL(cache_plan_fill_kernel, dim3(across, (unsigned)p.batch), dim3(kThreads), 0,
+                     stream, g);
   return hipGetLastError();
 }
 
 hipError_t launch_tree_plan(const fl_tree_plan_params& p, hipStream_t stream) {
-  const int n = (int)p.drafts, words = (n + 63) / 64;
-  const size_t lds = (size_t)n * words * 8 + 2 * (size_t)n * 4;
-  hipLaunchKernelGGL(tree_plan_kernel, dim3((unsigned)p.batch), dim3(256), lds, stream, p.parents,
-                     (long long)p.parent_stride, p.lengths, p.counts, p.mask, p.positions, n);
+  const int n = (int)p.drafts;
+  auto go = [&](auto threads) {
+    constexpr int kThreads = decltype(threads)::value;
+    hipLaunchKernelGGL(tree_plan_kernel<kThreads>, dim3((unsigned)p.batch), dim3(kThreads), 0,
+                       stream, p.parents, (long long)p.parent_stride, p.lengths, p.counts, p.mask,
+                       p.positions, n);
+  };
+  if (n <= 64)
+    go(std::integral_constant<int, 64>{});
+  else if (n <= 256)
+    go(std::integral_constant<int, 256>{});
+  else
+    go(std::integral_constant<int, FL_ATTN_MAX_DRAFTS>{});
   return hipGetLastError();
 }
 

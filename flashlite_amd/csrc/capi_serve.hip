@@ -154,6 +154,8 @@ int fl_attn_cache_plan(const fl_cache_plan_params* p, void* stream) {
       !fits32(p->max_blocks) || p->max_blocks > INT32_MAX / p->block_size)
     return set_error(FL_ERR_UNSUPPORTED, "%s: batch must be at most 65535, and width, pool and "
                      "max_blocks * block_size fit in int32", who);
+  if (p->batch > 0 && p->max_blocks > INT32_MAX / p->batch)
+    return set_error(FL_ERR_UNSUPPORTED, "%s: batch * max_blocks must fit in int32", who);
   if (p->batch > 1 && p->table_stride < p->max_blocks)
     return set_error(FL_ERR_INVALID_ARGUMENT, "%s: table_stride %lld is below max_blocks %lld", who,
                      (long long)p->table_stride, (long long)p->max_blocks);
@@ -169,8 +171,8 @@ int fl_attn_cache_plan(const fl_cache_plan_params* p, void* stream) {
   for (const void* x : four)
     if (!aligned(x, 4))
       return set_error(FL_ERR_MISALIGNED, "%s: int32 pointers must be 4-byte aligned", who);
-  if (!aligned(p->slots, 8))
-    return set_error(FL_ERR_MISALIGNED, "%s: slots must be 8-byte aligned", who);
+  if (!aligned(p->slots, 8) || !aligned(p->info, 16))
+    return set_error(FL_ERR_MISALIGNED, "%s: slots must be 8-byte aligned, info 16", who);
   return launched(fl::launch_cache_plan(*p, static_cast<hipStream_t>(stream)), who);
 }
 

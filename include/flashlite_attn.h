@@ -241,8 +241,10 @@ int64_t fl_attn_splitkv_noalloc_bytes(const fl_attn_params_ex* p, int32_t num_sp
  * 4]: {0 served, 1 not enough free blocks, 2 the table row is too short;
  * blocks held before; blocks taken, or minus those put back; the ring's index
  * of the first of them}.  A request that is not served keeps what it has; one
- * with nothing to take is always served.  Values out of range (a held count
- * past the row, a head past the ring) are clamped, never followed.
+ * with nothing to take is always served.  Values out of range are brought into
+ * it, never followed (a held count past the row, a count of free blocks past
+ * the ring: clamped; a head past it: modulo pool).  info is 16-byte aligned;
+ * batch is at most 65535.
  */
 typedef struct fl_cache_plan_params {
   const int32_t* lengths;
@@ -368,7 +370,8 @@ int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, voi
  * not see does not reach it, NaN and infinities in k_cache and v_cache
  * included.  lengths are clamped to the table's rows (max_blocks *
  * block_size), with the drafts behind them.  lse: optional fp32 [batch, heads,
- * drafts] (contiguous).
+ * drafts] (contiguous).  Block and row strides of the caches are below 2^31
+ * elements.
  *
  * Few query rows over many keys are split over the CUs; partial results go to
  * `workspace` (fl_attn_tree_workspace_bytes, from the sizes alone; 0: none
