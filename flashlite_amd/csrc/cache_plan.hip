@@ -35,7 +35,6 @@ struct Sums {
 __device__ __forceinline__ Sums group_scan(int x, int y, int2 (&part)[kWaves]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int sx = wave_scan(x), sy = wave_scan(y);
-  __syncthreads();  // the last call's parts are read
   if (lane == 63) part[w] = make_int2(sx, sy);
   __syncthreads();
   Sums s = {{sx - x, sy - y}, {0, 0}};
@@ -100,38 +99,49 @@ struct Move {
   int status, held, moved, first;
 };
 
+// Index i of the ring, i < 2 pool.
+__device__ __forceinline__ int wrap(const PlanGeom& g, uint32_t i) {
+  return (int)(i >= (uint32_t)g.pool ? i - (uint32_t)g.pool : i);
+}
+
 // The moves of all requests, 256 at a time: put(b, move) is called for each by
 // one thread; returns the ring's new head and count.  Every thread of the
 // work-group takes part, and has read the state and every held count when it
 // returns.
 template <class F>
 __device__ __forceinline__ int2 plan(const PlanGeom& g, F&& put) {
-  __shared__ int2 part[kWaves];
+  __shared__ int2 part[2][kWaves];
+  __shared__ int most;
+  const uint32_t pool = (uint32_t)g.pool;
   const int count = min(max(g.state[1], 0), g.pool);
-  const int head = (int)((unsigned)max(g.state[0], 0) % (unsigned)g.pool);
-  int needed = 0, backs = 0, taken = 0, given = 0;
+  const uint32_t head = (uint32_t)max(g.state[0], 0) % pool;
+  const int tail = wrap(g, head + (uint32_t)count), room = g.pool - count;
+  int needed = 0, backs = 0;
+  if (threadIdx.x == 0) most = 0;
 #pragma unroll 1
   for (int b0 = 0; b0 < g.batch; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
     Want r = {};
     if (b < g.batch) r = want(g, b);
     const int back = r.ended ? r.held : 0;
-    const Sums s = group_scan(r.need, back, part);
+    // (two sets of parts: the last call's may still be read)
+    const Sums s = group_scan(r.need, back, part[(b0 / kThreads) & 1]);
     const int off = needed + s.before[0], behind = backs + s.before[1];
     const bool served = !r.wide && (r.need == 0 || (long long)off + r.need <= count);
     Move m;
     m.status = r.wide ? 2 : served ? 0 : 1;
     m.held = r.held;
-    m.moved = r.ended ? -min(back, max(g.pool - count - behind, 0)) : served ? r.need : 0;
-    m.first = (int)((head + (r.ended ? (long long)count + behind : (long long)off)) % g.pool);
+    m.moved = r.ended ? -min(back, max(room - behind, 0)) : served ? r.need : 0;
+    m.first = (int)((r.ended ? (uint32_t)tail + (uint32_t)behind : head + (uint32_t)off) % pool);
+    // Who takes blocks is a prefix of those in need of them.
+    if (m.moved > 0) atomicMax(&most, off + m.moved);
     if (b < g.batch) put(b, m);
     needed += s.total[0];
     backs += s.total[1];
-    const Sums t = group_scan(max(m.moved, 0), max(-m.moved, 0), part);
-    taken += t.total[0];
-    given += t.total[1];
   }
-  return make_int2((int)(((long long)head + taken) % g.pool), count - taken + given);
+  __syncthreads();
+  const int taken = most;
+  return make_int2(wrap(g, head + (uint32_t)taken), count - taken + min(backs, room));
 }
 
 // The held count and info of request b.
@@ -144,9 +154,9 @@ __device__ __forceinline__ void note(const PlanGeom& g, int b, const Move& m, bo
 __device__ __forceinline__ void move_blocks(const PlanGeom& g, int b, const Move& m) {
   int32_t* const table = g.tables + b * g.table_stride;
   for (int k = threadIdx.x; k < m.moved; k += kThreads)
-    table[m.held + k] = g.ring[((long long)m.first + k) % g.pool];
+    table[m.held + k] = g.ring[wrap(g, (uint32_t)m.first + (uint32_t)k)];
   for (int k = threadIdx.x; k < -m.moved; k += kThreads)
-    g.ring[((long long)m.first + k) % g.pool] = table[k];
+    g.ring[wrap(g, (uint32_t)m.first + (uint32_t)k)] = table[k];
 }
 
 // Position and slot of new token i of request b.  (Blocks that this call takes
@@ -159,7 +169,7 @@ __device__ __forceinline__ void place(const PlanGeom& g, int b, int i, const Mov
     const int at = max(g.lengths[b], 0) + i;
     const int k = divide(at, g.block);
     const int id = k < m.held ? g.tables[b * g.table_stride + k]
-                              : g.ring[((long long)m.first + (k - m.held)) % g.pool];
+                              : g.ring[wrap(g, (uint32_t)m.first + (uint32_t)(k - m.held))];
     if (id >= 0) {
       position = at;
       slot = (long long)id * g.block.d + (at - k * g.block.d);
@@ -180,7 +190,6 @@ __global__ void __launch_bounds__(kThreads) cache_plan_kernel(const PlanGeom g) 
   const int2 state = plan(g, [&](int b, const Move& m) __attribute__((always_inline)) {
     moves[b] = m;
   });
-  __syncthreads();
   if (blockIdx.x == 0) {
     for (int b = threadIdx.x; b < g.batch; b += kThreads) note(g, b, moves[b], g.counts[b] < 0);
     if (threadIdx.x == 0) {

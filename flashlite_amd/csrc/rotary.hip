@@ -15,7 +15,9 @@ namespace {
 
 // Work-groups that a launch should have, by fewer heads a thread: the sines
 // and cosines of a token are then computed more often, but the chip is full.
-constexpr int kLeastBlocks = 1024;
+constexpr int kLeastBlocks = 256;
+// Heads side by side, and lanes that they take at most.
+constexpr int kAcross = 4, kAcrossLanes = 32;
 
 struct RotaryGeom {
   const void *q, *k, *v;
@@ -29,7 +31,7 @@ struct RotaryGeom {
   const double* freqs;
   int pos64, pairs, heads, kv_heads;
   uint32_t tokens;  // batch * rows
-  int heads_per_thread;
+  int heads_per_thread, across_log2;
   float scale, sign;
   FastDiv rows, block;
 };
@@ -45,16 +47,16 @@ __device__ __forceinline__ void store(T* p, const T (&x)[N]) {
 
 // A thread owns V columns at c0 and V at c1 of one token, the V pairs between
 // them (V / 2 within each when interleaved: neighbouring threads then read
-// neighbouring columns in both layouts), or 2 V columns behind the rotated
-// ones.  Head h of the launch: q heads, then k heads, then (with a cache) v
+// neighbouring columns in both layouts), or V of either half of the columns
+// behind the rotated ones.  Head h of the launch: q heads, then k heads, then (with a cache) v
 // heads.
-template <class T, int D, bool INTER, int V, bool CACHE>
+template <class T, int D, bool INTER, int V, bool CACHE, int UNROLL>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryGeom g) {
   constexpr uint32_t kThreads = D / (2 * V);  // a row
-  constexpr int kUnroll = 4;
   const uint32_t x = blockIdx.x * 256 + threadIdx.x;
-  const uint32_t token = x / kThreads;
+  const uint32_t token = x / kThreads >> g.across_log2;
   const int j = (int)(x % kThreads);
+  const int across = 1 << g.across_log2;  // heads side by side
   if (token >= g.tokens) return;
   const int b = (int)((__umulhi(g.rows.mul, token) + token) >> g.rows.shift);
   const int i = (int)token - b * g.rows.d;
@@ -70,8 +72,42 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryGeom g) {
   }
   const bool turns = j * V < g.pairs;
   constexpr bool kHalves = !INTER || V > 1;
-  const int c0 = turns && kHalves ? j * V : 2 * j * V;
-  const int c1 = turns && kHalves ? g.pairs + j * V : c0 + V;
+  const int rest = D - 2 * g.pairs;  // columns that are copied
+  const int c0 = turns ? (kHalves ? j * V : 2 * j) : g.pairs + j * V;
+  const int c1 = turns ? (kHalves ? g.pairs + j * V : 2 * j + 1) : c0 + rest / 2;
+  const long long q_in = b * g.q_st[0] + i * g.q_st[2], k_in = b * g.k_st[0] + i * g.k_st[2],
+                  v_in = CACHE ? b * g.v_st[0] + i * g.v_st[2] : 0;
+  const long long q_to = b * g.qo_st[0] + i * g.qo_st[2],
+                  k_to = blk * g.ko_st[0] + row * g.ko_st[2],
+                  v_to = CACHE ? blk * g.vo_st[0] + row * g.vo_st[2] : 0;
+  const int total = g.heads + g.kv_heads * (CACHE ? 2 : 1);
+  // This thread's heads: h, h + across, .. below h1.
+  const int span = g.heads_per_thread << g.across_log2;
+  int h = blockIdx.y * span + (int)(x / kThreads & (uint32_t)(across - 1));
+  const int h1 = min((int)(blockIdx.y + 1) * span, total);
+  if (h >= h1) return;
+  T x0[UNROLL][V], x1[UNROLL][V];
+  T* to[UNROLL];
+  auto fetch = [&]() __attribute__((always_inline)) {  // (past h1: the first again)
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int hu = h + u * across, hh = hu < h1 ? hu : h, hk = hh - g.heads;
+      const T* from;
+      if (hk < 0) {
+        from = static_cast<const T*>(g.q) + (q_in + hh * g.q_st[1]);
+        to[u] = static_cast<T*>(g.q_out) + (q_to + hh * g.qo_st[1]);
+      } else if (!CACHE || hk < g.kv_heads) {
+        from = static_cast<const T*>(g.k) + (k_in + hk * g.k_st[1]);
+        to[u] = static_cast<T*>(g.k_out) + (k_to + hk * g.ko_st[1]);
+      } else {
+        from = static_cast<const T*>(g.v) + (v_in + (hk - g.kv_heads) * g.v_st[1]);
+        to[u] = static_cast<T*>(g.v_out) + (v_to + (hk - g.kv_heads) * g.vo_st[1]);
+      }
+      load<T, V>(from + c0, x0[u]);
+      load<T, V>(from + c1, x1[u]);
+    }
+  };
+  fetch();
   float cs[V], sn[V];
   if (turns) {
     const long long at = b * g.pos_sb + i * g.pos_sr;
@@ -91,39 +127,11 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryGeom g) {
       sn[e] = g.scale * g.sign * __builtin_amdgcn_sinf((float)t);
     }
   }
-  const long long q_in = b * g.q_st[0] + i * g.q_st[2], k_in = b * g.k_st[0] + i * g.k_st[2],
-                  v_in = CACHE ? b * g.v_st[0] + i * g.v_st[2] : 0;
-  const long long q_to = b * g.qo_st[0] + i * g.qo_st[2],
-                  k_to = blk * g.ko_st[0] + row * g.ko_st[2],
-                  v_to = CACHE ? blk * g.vo_st[0] + row * g.vo_st[2] : 0;
-  const int total = g.heads + g.kv_heads * (CACHE ? 2 : 1);
-  const int h0 = blockIdx.y * g.heads_per_thread;
-  const int h1 = min(h0 + g.heads_per_thread, total);
-#pragma unroll 1
-  for (int h = h0; h < h1; h += kUnroll) {
-    T x0[kUnroll][V], x1[kUnroll][V];
-    T* to[kUnroll];
-    // (past the last head: the last again, not stored)
+  for (;;) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int hh = min(h + u, h1 - 1), hk = hh - g.heads;
-      const T* from;
-      if (hk < 0) {
-        from = static_cast<const T*>(g.q) + (q_in + hh * g.q_st[1]);
-        to[u] = static_cast<T*>(g.q_out) + (q_to + hh * g.qo_st[1]);
-      } else if (!CACHE || hk < g.kv_heads) {
-        from = static_cast<const T*>(g.k) + (k_in + hk * g.k_st[1]);
-        to[u] = static_cast<T*>(g.k_out) + (k_to + hk * g.ko_st[1]);
-      } else {
-        from = static_cast<const T*>(g.v) + (v_in + (hk - g.kv_heads) * g.v_st[1]);
-        to[u] = static_cast<T*>(g.v_out) + (v_to + (hk - g.kv_heads) * g.vo_st[1]);
-      }
-      load<T, V>(from + c0, x0[u]);
-      load<T, V>(from + c1, x1[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (turns && (!CACHE || h + u < g.heads + g.kv_heads)) {
+    for (int u = 0; u < UNROLL; ++u) {
+      const int hu = h + u * across;
+      if (turns && (!CACHE || hu < g.heads + g.kv_heads)) {
         if constexpr (INTER && V > 1) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
@@ -141,20 +149,51 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryGeom g) {
           }
         }
       }
-      if (h + u < h1) {
+      if (hu < h1) {
         store<T, V>(to[u] + c0, x0[u]);
         store<T, V>(to[u] + c1, x1[u]);
       }
     }
+    h += UNROLL * across;
+    if (h >= h1) return;
+    fetch();
   }
 }
 
-template <class T, bool CACHE, int D, int V>
-void launch(const RotaryGeom& g, bool inter, dim3 grid, hipStream_t stream) {
+template <class T, bool CACHE, int D, int V, int UNROLL>
+void launch_unroll(const RotaryGeom& g, bool inter, dim3 grid, hipStream_t stream) {
   if (inter)
-    hipLaunchKernelGGL((rotary_kernel<T, D, true, V, CACHE>), grid, dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((rotary_kernel<T, D, true, V, CACHE, UNROLL>), grid, dim3(256), 0, stream, g);
   else
-    hipLaunchKernelGGL((rotary_kernel<T, D, false, V, CACHE>), grid, dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((rotary_kernel<T, D, false, V, CACHE, UNROLL>), grid, dim3(256), 0, stream,
+                       g);
+}
+
+// Neighbouring threads go on to the next token, or where a token's heads lie
+// closer together than its rows (projections [B, N, H, D]) first to the next of
+// up to kAcross heads, so that a wave's accesses are whole pieces of memory.
+// Heads a thread: as many as leave kLeastBlocks work-groups, at most 8; four
+// of them (or one) in flight.
+template <class T, bool CACHE, int D, int V>
+void launch(RotaryGeom& g, bool inter, hipStream_t stream) {
+  const int total = g.heads + g.kv_heads * (CACHE ? 2 : 1);
+  g.across_log2 = 0;
+  if (g.q_st[1] < g.q_st[2])
+    while (1 << g.across_log2 < kAcross && 2 << g.across_log2 <= total &&
+           (D / (2 * V)) << (g.across_log2 + 1) <= kAcrossLanes &&
+           ((int64_t)g.tokens * (D / (2 * V)) << (g.across_log2 + 1)) < (1LL << 32) - 256)
+      ++g.across_log2;  // (threads are counted in 32 bits)
+  const int64_t blocks =
+      (((int64_t)g.tokens << g.across_log2) * (D / (2 * V)) + 255) / 256;
+  const int each = (total + (1 << g.across_log2) - 1) >> g.across_log2;
+  int per = 8;
+  while (per > 1 && blocks * ((each + per - 1) / per) < kLeastBlocks) per /= 2;
+  g.heads_per_thread = per;
+  const dim3 grid((unsigned)blocks, (unsigned)((each + per - 1) / per));
+  if (per >= 4)
+    launch_unroll<T, CACHE, D, V, 4>(g, inter, grid, stream);
+  else
+    launch_unroll<T, CACHE, D, V, 1>(g, inter, grid, stream);
 }
 
 template <class T, bool CACHE, int D>
@@ -162,21 +201,14 @@ void launch_dim(RotaryGeom& g, bool inter, hipStream_t stream) {
   constexpr int kMost = 16 / (int)sizeof(T);
   int v = kMost;  // columns a load: 16 bytes where the pairs divide
   while (g.pairs % v != 0) v /= 2;
-  const int64_t threads = (int64_t)g.tokens * (D / (2 * v));
-  const int64_t blocks = (threads + 255) / 256;
-  const int total = g.heads + g.kv_heads * (CACHE ? 2 : 1);
-  int per = 8;
-  while (per > 1 && blocks * ((total + per - 1) / per) < kLeastBlocks) per /= 2;
-  g.heads_per_thread = per;
-  const dim3 grid((unsigned)blocks, (unsigned)((total + per - 1) / per));
   if (v == 8) {
-    if constexpr (kMost == 8) launch<T, CACHE, D, 8>(g, inter, grid, stream);
+    if constexpr (kMost == 8) launch<T, CACHE, D, 8>(g, inter, stream);
   } else if (v == 4) {
-    launch<T, CACHE, D, 4>(g, inter, grid, stream);
+    launch<T, CACHE, D, 4>(g, inter, stream);
   } else if (v == 2) {
-    launch<T, CACHE, D, 2>(g, inter, grid, stream);
+    launch<T, CACHE, D, 2>(g, inter, stream);
   } else {
-    launch<T, CACHE, D, 1>(g, inter, grid, stream);
+    launch<T, CACHE, D, 1>(g, inter, stream);
   }
 }
 
