@@ -73,7 +73,7 @@ __device__ __forceinline__ int divide(int n, const FastDiv& f) {
 }
 
 // Request b's blocks: what it holds, and what its length with its new tokens
-// needs (64-bit: a length near 2^31 with `width` more).
+// needs.
 struct Want {
   int length, fresh, held;
   bool ended, wide;
@@ -87,16 +87,18 @@ __device__ __forceinline__ Want want(const PlanGeom& g, int b) {
   r.ended = c < 0;
   r.fresh = min(max(c, 0), g.width);
   r.held = min(max(g.held[b], 0), g.max_blocks);
-  const long long blocks =
-      ((long long)r.length + r.fresh + g.block.d - 1) / (long long)g.block.d;
+  // The last new token's block (past 2^31 tokens it is past the table's row).
+  const uint32_t last = (uint32_t)r.length + (uint32_t)r.fresh - 1;
+  const int blocks = last >> 31 ? g.max_blocks + 1 : divide((int)last, g.block) + 1;
   r.wide = r.fresh > 0 && blocks > g.max_blocks;
-  r.need = r.fresh > 0 && !r.wide ? max((int)(blocks - r.held), 0) : 0;
+  r.need = r.fresh > 0 && !r.wide ? max(blocks - r.held, 0) : 0;
   return r;
 }
 
-// What a call does with one request (fl_attn_cache_plan's info).
+// What a call does with one request (fl_attn_cache_plan's info), its length and
+// the tokens that get slots.
 struct Move {
-  int status, held, moved, first;
+  int status, held, moved, first, length, fresh;
 };
 
 // Index i of the ring, i < 2 pool.
@@ -131,6 +133,8 @@ __device__ __forceinline__ int2 plan(const PlanGeom& g, F&& put) {
     Move m;
     m.status = r.wide ? 2 : served ? 0 : 1;
     m.held = r.held;
+    m.length = r.length;
+    m.fresh = served ? r.fresh : 0;
     m.moved = r.ended ? -min(back, max(room - behind, 0)) : served ? r.need : 0;
     m.first = (int)((r.ended ? (uint32_t)tail + (uint32_t)behind : head + (uint32_t)off) % pool);
     // Who takes blocks is a prefix of those in need of them.
@@ -150,13 +154,39 @@ __device__ __forceinline__ void note(const PlanGeom& g, int b, const Move& m, bo
   *reinterpret_cast<int4*>(g.info + 4LL * b) = make_int4(m.status, m.held, m.moved, m.first);
 }
 
-// Request b's table entries, or its blocks back to the ring.
-__device__ __forceinline__ void move_blocks(const PlanGeom& g, int b, const Move& m) {
+// Block k of request b: its table entry, or back to the ring.
+__device__ __forceinline__ void move_block(const PlanGeom& g, int b, const Move& m, int k) {
   int32_t* const table = g.tables + b * g.table_stride;
-  for (int k = threadIdx.x; k < m.moved; k += kThreads)
-    table[m.held + k] = g.ring[wrap(g, (uint32_t)m.first + (uint32_t)k)];
-  for (int k = threadIdx.x; k < -m.moved; k += kThreads)
-    g.ring[wrap(g, (uint32_t)m.first + (uint32_t)k)] = table[k];
+  int32_t* const ring = g.ring + wrap(g, (uint32_t)m.first + (uint32_t)k);
+  if (m.moved > 0)
+    table[m.held + k] = *ring;
+  else
+    *ring = table[k];
+}
+
+// The blocks of the requests first, first + step, ..: a few by the thread that
+// has the request, many by its wave.
+template <class F>
+__device__ __forceinline__ void move_blocks(const PlanGeom& g, int first, int step, F&& move_of) {
+  constexpr int kFew = 4;
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int b0 = first; b0 < g.batch; b0 += kThreads * step) {
+    const int b = b0 + threadIdx.x * step;
+    Move m = {};
+    if (b < g.batch) m = move_of(b);
+    const int n = max(m.moved, -m.moved);
+#pragma unroll 1
+    for (int k = 0; k < min(n, kFew); ++k) move_block(g, b, m, k);
+    uint64_t many = __builtin_amdgcn_ballot_w64(n > kFew);
+#pragma unroll 1
+    for (; many != 0; many &= many - 1) {
+      const int l = __builtin_ctzll(many);
+      const int of = __builtin_amdgcn_readlane(b, l), all = __builtin_amdgcn_readlane(n, l);
+      const Move o = move_of(of);
+      for (int k = kFew + lane; k < all; k += 64) move_block(g, of, o, k);
+    }
+  }
 }
 
 // Position and slot of new token i of request b.  (Blocks that this call takes
@@ -164,9 +194,8 @@ __device__ __forceinline__ void move_blocks(const PlanGeom& g, int b, const Move
 __device__ __forceinline__ void place(const PlanGeom& g, int b, int i, const Move& m) {
   int position = -1;
   long long slot = -1;
-  const int fresh = m.status == 0 ? min(g.counts[b], g.width) : 0;
-  if (i < fresh) {
-    const int at = max(g.lengths[b], 0) + i;
+  if (i < m.fresh) {
+    const int at = m.length + i;
     const int k = divide(at, g.block);
     const int id = k < m.held ? g.tables[b * g.table_stride + k]
                               : g.ring[wrap(g, (uint32_t)m.first + (uint32_t)(k - m.held))];
@@ -197,7 +226,8 @@ __global__ void __launch_bounds__(kThreads) cache_plan_kernel(const PlanGeom g) 
       g.state_out[1] = state.y;
     }
   }
-  for (int b = blockIdx.x; b < g.batch; b += gridDim.x) move_blocks(g, b, moves[b]);
+  move_blocks(g, blockIdx.x, gridDim.x,
+              [&](int b) __attribute__((always_inline)) { return moves[b]; });
   const uint32_t all = (uint32_t)g.batch * (uint32_t)g.width, step = gridDim.x * kThreads;
   for (uint32_t e = blockIdx.x * kThreads + threadIdx.x; e < all; e += step) {
     const int b = divide((int)e, g.by_width);
@@ -220,8 +250,12 @@ __global__ void __launch_bounds__(kThreads) cache_plan_scan_kernel(const PlanGeo
 __global__ void __launch_bounds__(kThreads) cache_plan_fill_kernel(const PlanGeom g) {
   const int b = blockIdx.y;
   const int4 info = *reinterpret_cast<const int4*>(g.info + 4LL * b);
-  const Move m = {info.x, info.y, info.z, info.w};
-  if (blockIdx.x == 0) move_blocks(g, b, m);
+  Move m = {info.x, info.y, info.z, info.w, max(g.lengths[b], 0), 0};
+  if (m.status == 0) m.fresh = min(max(g.counts[b], 0), g.width);
+  if (blockIdx.x == 0) {
+    const int n = max(m.moved, -m.moved);
+    for (int k = threadIdx.x; k < n; k += kThreads) move_block(g, b, m, k);
+  }
   const int i = blockIdx.x * kThreads + threadIdx.x;
   if (i < g.width) place(g, b, i, m);
 }
@@ -281,7 +315,7 @@ tree_plan_kernel(const int32_t* parents, long long parent_stride, const int32_t*
 }
 
 // Tokens a work-group of the one-launch form.
-constexpr int kEach = 2048;
+constexpr int kEach = 512;
 
 }  // namespace
 
