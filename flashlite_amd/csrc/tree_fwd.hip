@@ -33,7 +33,6 @@ struct TreeGeom {
   // unit where they begin and end
   float* part;
   int2* parts;
-  int least_log2;  // least steps of a work-group
   int xcds;
 };
 
@@ -235,12 +234,21 @@ __device__ __forceinline__ int unit_steps(const TreeGeom& g, const Request& r, i
   return (r.length + unit_drafts(g, r, rb, 32 * RW) + kStepKeys - 1) / kStepKeys;
 }
 
-// Steps of all row blocks of one key/value head of a request.
+// A unit's cost to a split launch, in steps: its walk and what starting one
+// takes (the first tiles' latency, the merge of partial results).
+constexpr int start_of(int rw) { return rw == 1 ? 1 : rw == 2 ? 6 : 10; }
+
+template <int RW>
+__device__ __forceinline__ int cost_of(int steps) {
+  return steps > 0 ? steps + start_of(RW) : 0;
+}
+
+// Costs of all row blocks of one key/value head of a request.
 template <int D, int RW>
-__device__ __forceinline__ int head_steps(const TreeGeom& g, const Request& r) {
+__device__ __forceinline__ int head_cost(const TreeGeom& g, const Request& r) {
   int n = 0;
 #pragma unroll 1
-  for (int rb = 0; rb < g.blocks_of_rows; ++rb) n += unit_steps<D, RW>(g, r, rb);
+  for (int rb = 0; rb < g.blocks_of_rows; ++rb) n += cost_of<RW>(unit_steps<D, RW>(g, r, rb));
   return n;
 }
 
@@ -294,7 +302,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   constexpr int kLanes = kRowB / 16;      // lanes a row of a fetch
   constexpr int kSegRows = 64 / kLanes;   // rows a fetch
   constexpr int kSegs = 8 / RW;           // fetches of a tile by this wave
-  constexpr int kSlots = RW;
+  constexpr int kSlots = Shared<D, RW>::kSlots;
   constexpr int kAcc = D / 2;
   constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
   static_assert(kKeys * kRowB == kTileBytes, "tile size");
@@ -458,8 +466,8 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     // Every wave has tiles, and a K and a V slot, of its own: no barrier
     // orders the walk.  K(i + 1) is fetched as soon as the operands of K(i)
     // are read, V(i + 1) after those of V(i); table entries two tiles ahead.
-    uint8_t* const kt = sh.tile[w][0][0];
-    uint8_t* const vt = sh.tile[w][0][1];
+    // (Two slots each, 128 KiB, measured 1 us slower for short calls and 3%
+    // for long ones.)
     uint64_t ok = 0;
     if (n > 0) {
       fetch_ids(0, 0);
@@ -470,11 +478,12 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       fetch(0, 0);
       fetch(1, 0);
     }
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
       typename RowsT::Scores s;
       typename RowsT::Probs p;
       asm volatile("s_waitcnt vmcnt(8)" : : : "memory");  // K(i), and the entries of i + 1
-      rows.scores(kt, s);
+      rows.scores(sh.tile[kg][0][0], s);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // its operands are in registers
       const bool more = i + 1 < n;
       uint64_t ok_next = 0;
@@ -491,8 +500,8 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       else
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
       V8 va[8];
-      read_v(vt, va);
-      output(vt, va, p);
+      read_v(sh.tile[kg][0][1], va);
+      output(sh.tile[kg][0][1], va, p);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
       if (more) fetch(1, i + 1);
       ok = ok_next;
@@ -565,7 +574,8 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   float a[KW];
   if constexpr (KW > 1) {
     if constexpr (RW > 1) __syncthreads();  // (with RW == 1 a wave's slots are its own)
-    float4* const own = reinterpret_cast<float4*>(sh.tile) + 1024 * w;  // 16 KiB each
+    // (16 KiB a wave: its own slots, with RW == 1)
+    float4* const own = reinterpret_cast<float4*>(sh.tile) + 1024 * w;
 #pragma unroll
     for (int c = 0; c < kAcc / 4; ++c) {
       const float16_t& x = rows.o[c >> 2];
@@ -668,16 +678,17 @@ tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tree
   const int kvh = rest / g.blocks_of_rows, rb = rest - kvh * g.blocks_of_rows;
   const Request r = request(g, b);
   const int steps = unit_steps<D, RW>(g, r, rb);
-  if (steps > 0) walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, 0, steps, nullptr, cq, cr);
+  if (steps > 0)
+    walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, 0, steps, nullptr, cq, cr);
 }
 
-// The steps of all units, in order, are dealt evenly to the work-groups: each
+// The costs of all units, in order, are dealt evenly to the work-groups: each
 // has the end of one unit, whole units, the start of one.  Whole units are
 // stored; partial results go to slot 2 x of work-group x (its first unit's) or
 // 2 x + 1 (its last's, if another).  Whoever has a unit's first step says in
 // parts[unit].x in which slot its results begin, whoever has its last in .y
 // which work-group that was; between them each work-group has one in its first
-// slot.  (Fewer than 2^31 steps: tree_plan.)
+// slot.  (The sum is below 2^31: tree_plan.)
 template <int D, class T, int RW>
 __global__ void __launch_bounds__(64 * waves_of(RW), 2)
 tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
@@ -685,12 +696,12 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
   constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
   __shared__ __attribute__((aligned(16))) Shared<D, RW> sh;
   const int lane = threadIdx.x & 63;
-  // Steps of one key/value head of requests b0 .. b0 + 63, one a lane.
+  // Cost of one key/value head of requests b0 .. b0 + 63, one a lane.
   Request c;
   int n, upto;
   auto chunk = [&](int b0) __attribute__((always_inline)) {
     c = request(g, min(b0 + lane, g.batch - 1));
-    n = b0 + lane < g.batch ? head_steps<D, RW>(g, c) : 0;
+    n = b0 + lane < g.batch ? head_cost<D, RW>(g, c) : 0;
     upto = wave_scan(n);
   };
   auto last_lane = [](int x) __attribute__((always_inline)) {
@@ -703,9 +714,9 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
     all += last_lane(upto);
   }
   all *= g.kv_heads;
-  // `busy` work-groups have steps, `even` or one more; neighbours run on one
+  // `busy` work-groups have a share, `even` or one more; neighbours run on one
   // XCD, all XCDs alike.
-  const int busy = min((int)gridDim.x, max(all >> g.least_log2, min(all, 1)));
+  const int busy = min((int)gridDim.x, all);
   const int apiece = (busy + g.xcds - 1) / g.xcds;
   const int k = blockIdx.x / g.xcds;
   const int x = (blockIdx.x - k * g.xcds) * apiece + k;
@@ -713,7 +724,7 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
   const int even = (uint32_t)all / (uint32_t)busy, more = all - even * busy;
   int at = x * even + min(x, more);
   const int end = at + even + (x < more ? 1 : 0);
-  // The request of step `at`, and where in it that is.
+  // The request of `at`, and where in it that is.
   int b0 = 0, before = 0;
   uint64_t past;
 #pragma unroll 1
@@ -728,34 +739,38 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
   r.length = __builtin_amdgcn_readlane(c.length, l);
   r.count = __builtin_amdgcn_readlane(c.count, l);
   const int head = __builtin_amdgcn_readlane(n, l);
-  int s0 = at - before - __builtin_amdgcn_readlane(upto - n, l) * g.kv_heads;
-  int kvh = 0, rb = 0, steps;
+  int in = at - before - __builtin_amdgcn_readlane(upto - n, l) * g.kv_heads;
+  int kvh = 0, rb = 0, steps, cost;
 #pragma unroll 1
-  while (s0 >= head) {
-    s0 -= head;
+  while (in >= head) {
+    in -= head;
     ++kvh;
   }
 #pragma unroll 1
-  while (s0 >= (steps = unit_steps<D, RW>(g, r, rb))) {
-    s0 -= steps;
+  while (in >= (cost = cost_of<RW>(steps = unit_steps<D, RW>(g, r, rb)))) {
+    in -= cost;
     ++rb;
   }
   int slot = 2 * x;
 #pragma unroll 1
   for (;;) {
-    const int s1 = min(steps, s0 + (end - at));
-    if (threadIdx.x == 0) {
-      int2* const where = g.parts + (b * g.kv_heads + kvh) * g.blocks_of_rows + rb;
-      if (s0 == 0) where->x = slot;
-      if (s1 == steps) where->y = x;
+    // Costs [in, upto) of the unit; its start comes first.
+    const int to = min(cost, in + (end - at));
+    const int s0 = max(in - start_of(RW), 0), s1 = to - start_of(RW);
+    if (s1 > s0) {
+      if (threadIdx.x == 0) {
+        int2* const where = g.parts + (b * g.kv_heads + kvh) * g.blocks_of_rows + rb;
+        if (s0 == 0) where->x = slot;
+        if (s1 == steps) where->y = x;
+      }
+      float* const part =
+          s0 == 0 && s1 == steps ? nullptr : g.part + (long long)slot * (32 * RW) * kPart;
+      walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, s0, s1, part, cq, cr);
+      slot = 2 * x + 1;
     }
-    float* const part =
-        s0 == 0 && s1 == steps ? nullptr : g.part + (long long)slot * (32 * RW) * kPart;
-    walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, s0, s1, part, cq, cr);
-    at += s1 - s0;
+    at += to - in;
     if (at >= end) return;
-    slot = 2 * x + 1;
-    s0 = 0;
+    in = 0;
     // The next unit with steps.
     do {
       if (++rb == g.blocks_of_rows) {
@@ -765,8 +780,8 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
           r = request(g, ++b);
         }
       }
-      steps = unit_steps<D, RW>(g, r, rb);
-    } while (steps == 0);
+      cost = cost_of<RW>(steps = unit_steps<D, RW>(g, r, rb));
+    } while (cost == 0);
     __syncthreads();  // the tiles are free again
   }
 }
@@ -882,14 +897,14 @@ hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, fl
   const uint8_t *k = static_cast<const uint8_t*>(p.k_cache),
                 *v = static_cast<const uint8_t*>(p.v_cache);
   T* o = static_cast<T*>(p.o);
-  // A split launch counts steps in 32 bits.
-  const bool counted = t.units * (((int64_t)g.capacity + g.drafts) / kStepKeys + 1) < (1LL << 30);
+  // A split launch adds up costs in 32 bits.
+  const bool counted =
+      t.units * (((int64_t)g.capacity + g.drafts) / kStepKeys + 1 + start_of(RW)) < (1LL << 30);
   if (g.part == nullptr || !counted) {
     hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW>), dim3((unsigned)t.units), dim3(64 * waves_of(RW)), 0,
                        st, q, k, v, o, g, cq, cr);
     return hipGetLastError();
   }
-  g.least_log2 = 0;
   g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.grid * 32 * RW *
                                                  (D == 64 ? kPartStride : kPartStride128));
   hipLaunchKernelGGL((tree_split_kernel<D, T, RW>), dim3((unsigned)t.grid), dim3(64 * waves_of(RW)), 0,
