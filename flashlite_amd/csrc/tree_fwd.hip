@@ -276,14 +276,14 @@ struct Shared {
   static constexpr int kWaves = waves_of(RW);
   static constexpr int kGroups = kWaves / RW;
   static constexpr int kSlots = RW;  // of each key group
-  // Tiles a wave looks up at once (64 keys, but for RW == 1), and entries of
-  // the ring of looked-up ones: those of tiles i .. i + kSlots + 2.
-  static constexpr int kPer = RW > 1 && D == 128 ? 2 : 1;
-  static constexpr int kRing =
-      RW == 1 ? 1 : RW == 2 ? 4 : RW == 4 || D == 128 ? 8 : 16;
+  // Rows of a tile that a wave fetches, and tiles whose rows it looks up at
+  // once, a row a lane.
+  static constexpr int kRows = (D == 64 ? kBc : kBc2) / RW;
+  static constexpr int kPer = 64 / kRows;
   uint8_t tile[kGroups][kSlots][2][kTileBytes];
-  uint64_t where[kGroups][kRing][2][64];
-  uint64_t ok[kGroups][kRing];
+  uint64_t where[kWaves][2][2][64];  // K and V row addresses of two lookups
+  uint64_t good[kWaves][2];          // their keys that have a block
+  int bad[kWaves];                   // whether a key so far had none
   int32_t ids[kWaves][2][64];
   float2 ml[kWaves][64];
 };
@@ -363,37 +363,49 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   const uint64_t vbase = (uint64_t)(uintptr_t)(V + kvh * g.v_head);
   int32_t(*const ids)[64] = sh.ids[w];
   using Sh = Shared<D, RW>;
-  constexpr int kPer = Sh::kPer, kRing = Sh::kRing;
-  // The key that lane l looks up for the key group's tiles kPer m ..: key
-  // l % kKeys of tile kPer m + l / kKeys (past the last key: the last again).
+  constexpr int kPer = Sh::kPer, kRows = Sh::kRows;
+  // The key that lane l looks up for the key group's tiles kPer m ..: this
+  // wave's row l % kRows of tile kPer m + l / kRows (past the last key: the
+  // last again).
   auto key_of = [&](int m) __attribute__((always_inline)) {
-    const int tile = kPer * m + (kPer == 2 ? lane / kKeys : 0);
-    return min((first + KW * tile) * kKeys + (lane & (kKeys - 1)), keys - 1);
+    const int tile = first + KW * (kPer * m + lane / kRows);
+    return min(tile * kKeys + rw * kRows + lane % kRows, keys - 1);
   };
-  auto fetch_ids = [&](int m, int buffer) __attribute__((always_inline)) {
-    fetch4(table + 4 * (uint64_t)divide(key_of(m), g.block), ids[buffer]);
+  auto fetch_ids = [&](int m) __attribute__((always_inline)) {
+    fetch4(table + 4 * (uint64_t)divide(key_of(m), g.block), ids[m & 1]);
   };
-  // Their rows' addresses, from table entries in ids[buffer], and a bit per
-  // key with a block, to the ring.
-  auto look_up = [&](int m, int buffer) __attribute__((always_inline)) {
+  // Their rows' addresses, from the table entries, and a bit per key with a
+  // block; then the table entries of lookup m + 2.
+  int bad = 0;
+  auto look_up = [&](int m) __attribute__((always_inline)) {
     const int key = key_of(m);
     const uint32_t in = key - divide(key, g.block) * g.block.d;
-    uint32_t id = ids[buffer][lane];
+    uint32_t id = ids[m & 1][lane];
     const bool good = id < (uint32_t)g.num_blocks;
     id = good ? id : 0;
-    const int to = m & (kRing - 1);
-    sh.where[kg][to][0][lane] = kbase + ((uint64_t)id * g.k_blk + (uint64_t)in * g.k_row);
-    sh.where[kg][to][1][lane] = vbase + ((uint64_t)id * g.v_blk + (uint64_t)in * g.v_row);
+    sh.where[w][m & 1][0][lane] = kbase + ((uint64_t)id * g.k_blk + (uint64_t)in * g.k_row);
+    sh.where[w][m & 1][1][lane] = vbase + ((uint64_t)id * g.v_blk + (uint64_t)in * g.v_row);
     const uint64_t all = __builtin_amdgcn_ballot_w64(good);
-    if constexpr (RW > 1) sh.ok[kg][to] = all;
-    return all;
+    bad |= ~all != 0;
+    sh.good[w][m & 1] = all;
+    sh.bad[w] = bad;
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    fetch_ids(m + 2);
   };
-  // This wave's share of the K (t = 0) or V (1) tile j, whose rows are in the
-  // ring.
+  // Keys of the key group's tile i with a block.
+  auto good_keys = [&](int i) __attribute__((always_inline)) {
+    uint64_t x = 0;
+#pragma unroll 1
+    for (int q = 0; q < RW; ++q) {
+      const uint64_t y = uniform(sh.good[kg * RW + q][(i / kPer) & 1]) >> (i % kPer * kRows);
+      x |= (y & (kRows == 64 ? ~(uint64_t)0 : ((uint64_t)1 << kRows) - 1)) << (q * kRows);
+    }
+    return x;
+  };
+  // This wave's share of the K (t = 0) or V (1) tile j.
   auto fetch = [&](int t, int j) __attribute__((always_inline)) {
     uint8_t* const tile = sh.tile[kg][j & (kSlots - 1)][t];
-    const uint64_t* const from =
-        sh.where[kg][(j / kPer) & (kRing - 1)][t] + (kPer == 2 ? (j & 1) * kKeys : 0);
+    const uint64_t* const from = sh.where[w][(j / kPer) & 1][t] + j % kPer * kRows;
     uint64_t at[kSegs];
 #pragma unroll
     for (int i = 0; i < kSegs; ++i) {
@@ -401,7 +413,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       const int phys = lane & (kLanes - 1);
       const int chunk = phys ^ (D == 64 ? (t ? v_swz(r) : k_swz(r))
                                         : (t ? v_swz128(r) : k_swz128(r)));
-      at[i] = from[r] + 16 * chunk;
+      at[i] = from[kSegRows * i + lane / kLanes] + 16 * chunk;
     }
 #pragma unroll
     for (int i = 0; i < kSegs; ++i) fetch16(at[i], tile + 1024 * (rw * kSegs + i));
@@ -411,11 +423,14 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   uint64_t seen = 0;
   bool checked = false;
   // Before tile i's exponentials: hidden keys, and rows' first stabilisers.
-  auto prepare = [&](int i, uint64_t ok, typename RowsT::Scores& s) __attribute__((always_inline)) {
+  // `some_bad`: a key of this walk may have no block.
+  auto prepare = [&](int i, bool some_bad, typename RowsT::Scores& s)
+                     __attribute__((always_inline)) {
     const int k0 = (first + KW * i) * kKeys;
-    checked = k0 + kKeys > length || ~ok != 0;
+    checked = k0 + kKeys > length || some_bad;
     if (checked) {
-      seen = seen_bits(k0) & ok;
+      seen = seen_bits(k0);
+      if (some_bad) seen &= good_keys(i);
       rows.hide(seen, s);
     }
     if (fresh) {
@@ -468,13 +483,11 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     // are read, V(i + 1) after those of V(i); table entries two tiles ahead.
     // (Two slots each, 128 KiB, measured 1 us slower for short calls and 3%
     // for long ones.)
-    uint64_t ok = 0;
     if (n > 0) {
-      fetch_ids(0, 0);
-      fetch_ids(1, 1);
+      fetch_ids(0);
+      fetch_ids(1);
       load_q();
-      ok = look_up(0, 0);
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      look_up(0);
       fetch(0, 0);
       fetch(1, 0);
     }
@@ -482,54 +495,38 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     for (int i = 0; i < n; ++i) {
       typename RowsT::Scores s;
       typename RowsT::Probs p;
-      asm volatile("s_waitcnt vmcnt(8)" : : : "memory");  // K(i), and the entries of i + 1
+      asm volatile("s_waitcnt vmcnt(8)" : : : "memory");  // K(i), and the next table entries
       rows.scores(sh.tile[kg][0][0], s);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // its operands are in registers
-      const bool more = i + 1 < n;
-      uint64_t ok_next = 0;
+      const bool more = i + 1 < n, next = (i + 1) % kPer == 0;
+      prepare(i, bad != 0, s);
       if (more) {
-        ok_next = look_up(i + 1, (i + 1) & 1);
-        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-        fetch_ids(i + 2, i & 1);
+        if (next) look_up((i + 1) / kPer);
         fetch(0, i + 1);
       }
-      prepare(i, ok, s);
       rows.settle_sum(rows.exponentiate(s, p), s, p);
-      if (more)
-        asm volatile("s_waitcnt vmcnt(9)" : : : "memory");  // V(i)
+      if (!more)
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // V(i)
+      else if (next)
+        asm volatile("s_waitcnt vmcnt(9)" : : : "memory");
       else
-        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        asm volatile("s_waitcnt vmcnt(8)" : : : "memory");
       V8 va[8];
       read_v(sh.tile[kg][0][1], va);
       output(sh.tile[kg][0][1], va, p);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
       if (more) fetch(1, i + 1);
-      ok = ok_next;
     }
   } else {
     // RW waves share their key group's tiles, kSlots of K and of V in rings;
-    // each fetches 1 / RW of a tile.  Step i fetches V(i + kSlots - 1) and
-    // K(i + kSlots), multiplies K(i + 1) while it exponentiates the scores of
-    // tile i, then V(i).  A step before K(j) is fetched, wave (j / kPer) % RW
-    // looks up its rows (and the next tile's), from table entries it fetched
-    // when it last did.  One barrier a step: past it K(i + 1) and V(i) have
-    // landed for all, K(i) and V(i - 1) are read by none, and the next
-    // addresses are there.
-    constexpr int kFirst = kPer == 2 ? kSlots / 2 : kSlots;  // lookups 0 .. kFirst at once
-    fetch_ids(rw, 0);
-    fetch_ids(rw + RW, 1);
+    // each fetches 1 / RW of a tile.  Step i multiplies K(i + 1) while it
+    // exponentiates the scores of tile i, then V(i), and fetches V(i + kSlots
+    // - 1) and K(i + kSlots).  One barrier a step: past it K(i + 1) and V(i)
+    // have landed for all, and K(i) and V(i - 1) are read by none.
+    fetch_ids(0);
+    fetch_ids(1);
     load_q();
-    if (rw <= kFirst) {
-      look_up(rw, 0);
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      fetch_ids(rw + 2 * RW, 0);
-    }
-    if (kFirst == RW && rw == 0) {
-      look_up(RW, 1);
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      fetch_ids(3 * RW, 1);
-    }
-    __syncthreads();
+    look_up(0);
     fetch(0, 0);
 #pragma unroll
     for (int j = 0; j < kSlots - 1; ++j) {
@@ -539,31 +536,25 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     sync_ring<(kSlots - 1) * 2 * kSegs>();
     typename RowsT::Scores s;
     rows.scores(sh.tile[kg][0][0], s);
+    int flag = sh.bad[kg * RW + (lane & (RW - 1))];
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
       sync_ring<(kSlots - 2) * 2 * kSegs>();
-      uint64_t ok = uniform(sh.ok[kg][(i / kPer) & (kRing - 1)]);
-      if constexpr (kPer == 2)
-        ok = (i & 1 ? ok >> 32 : ok) | 0xFFFFFFFF00000000u;  // (bits of 32 keys)
-      prepare(i, ok, s);
+      prepare(i, __builtin_amdgcn_ballot_w64(flag != 0) != 0, s);
       const uint8_t* const vt = sh.tile[kg][i & (kSlots - 1)][1];
       typename RowsT::Scores next;
       typename RowsT::Probs p;
       V8 va[8];
       rows.scores(sh.tile[kg][(i + 1) & (kSlots - 1)][0], next);
       const float sum = rows.exponentiate(s, p);
-      fetch(1, i + kSlots - 1);
-      fetch(0, i + kSlots);
       read_v(vt, va);
+      // (of tile i + 1, or a later one's)
+      flag = sh.bad[kg * RW + (lane & (RW - 1))];
+      fetch(1, i + kSlots - 1);
+      if ((i + kSlots) % kPer == 0) look_up((i + kSlots) / kPer);
+      fetch(0, i + kSlots);
       rows.settle_sum(sum, s, p);
       output(vt, va, p);
-      const int m = (i + kSlots + 1) / kPer;
-      if ((kPer == 1 || (i & 1) != 0) && rw == (m & (RW - 1))) {
-        const int buffer = (m / RW) & 1;
-        look_up(m, buffer);
-        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-        fetch_ids(m + 2 * RW, buffer);
-      }
       s = next;
     }
   }
