@@ -547,6 +547,10 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       V8 va[8];
       rows.scores(sh.tile[kg][(i + 1) & (kSlots - 1)][0], next);
       const float sum = rows.exponentiate(s, p);
+      // Keeps the exponentials here, among the products (they would be sunk
+      // past the next branch).
+#pragma unroll
+      for (int h = 0; h < 2 * RowsT::kBlocks; ++h) asm volatile("" : : "v"(p.p[h]));
       read_v(vt, va);
       // (of tile i + 1, or a later one's)
       flag = sh.bad[kg * RW + (lane & (RW - 1))];
