@@ -6,6 +6,7 @@
 // all of them.  A unit is 32 RW such rows of one (request, key/value head): a
 // work-group's 4 waves are RW row blocks times 4 / RW key groups.
 
+#include <algorithm>
 #include <cmath>
 
 #include "fa2_d128.h"
@@ -862,7 +863,14 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g)
 }
 
 // How a call of given sizes runs: row blocks a work-group, and whether the
-// units' steps are dealt to a grid of two work-groups a CU.
+// units' steps are dealt to a grid of one work-group a CU, at most
+// kMostParts of them to a unit.  The merge reads a row's partial results one
+// batch after another, so past some parts it takes longer than the walks they
+// shorten.  8 heads over one KV head (D 128, bf16), one token after 32000: 31
+// us with 256 parts, 17.0 with 64, 18.6 with 32, 25.0 with 16; 64 drafts there
+// (f16) 39.9, 35.7, 45.4 and 69.9.
+constexpr int kMostParts = 64;
+
 struct TreePlan {
   int rw, units, grid;
   bool split;
@@ -874,7 +882,7 @@ TreePlan tree_plan(const fl_tree_params& p) {
   const int64_t rows = p.heads / p.kv_heads * p.drafts;
   t.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
   t.units = (int)((rows + 32 * t.rw - 1) / (32 * t.rw) * p.kv_heads * p.batch);
-  t.grid = device_cus();
+  t.grid = (int)std::min<int64_t>(device_cus(), (int64_t)kMostParts * t.units);
   t.split = t.units < 2 * t.grid;
   const int64_t part = p.head_dim == 64 ? kPartStride : kPartStride128;
   t.bytes = t.split ? 2LL * t.grid * 32 * t.rw * part * (int64_t)sizeof(float) +
@@ -895,7 +903,22 @@ hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, fl
   // A split launch adds up costs in 32 bits.
   const bool counted =
       t.units * (((int64_t)g.capacity + g.drafts) / kStepKeys + 1 + start_of(RW)) < (1LL << 30);
-  if (g.part == nullptr || !counted) {
+  // Splitting costs the partial results' way through memory and a second
+  // launch, about four microseconds; it saves the steps by which the longest
+  // unit that the table has room for passes an even share.  Up to kFewSaved
+  // one pass is no slower: 16 requests x 16 heads of 600 keys (D 128, f16)
+  // 18.8 us against 22.2, 4 x 16 drafts of 16/4 heads after 300 keys 10.2
+  // against 13.2, 1 head of 1000 keys 8.2 against 9.7; with twice that bound 8
+  // drafts of 32/8 heads after 1000 keys lose, 12.8 against 11.8.  With as many
+  // units as work-groups the share says nothing about requests of unlike
+  // lengths, so kMostSteps bounds what waiting for the longest can cost: up to
+  // it 32 drafts of 32 x 32/8 heads after 500 keys take 24.0 us against 29.4,
+  // while 16 heads and 1 to 16384 keys (128 steps) lose, 129 against 110.
+  constexpr int kFewSaved = 6, kMostSteps = 32;
+  const int64_t most = ((int64_t)g.capacity + g.drafts) / kStepKeys + 1;
+  const bool whole =
+      most <= kMostSteps && most - (most * t.units + t.grid - 1) / t.grid <= kFewSaved;
+  if (g.part == nullptr || !counted || whole) {
     hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW>), dim3((unsigned)t.units), dim3(64 * waves_of(RW)), 0,
                        st, q, k, v, o, g, cq, cr);
     return hipGetLastError();
