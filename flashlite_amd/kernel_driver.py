@@ -51,6 +51,19 @@ a one pass runs ``--config``'s configuration, by default the dispatcher's;
 and reports the K/V read rate against 8 TB/s: bytes = 2 * B*H*NK*64*2
 (K and V once) + Q and O.
 
+``--serve B H HK LEN`` runs one step of serving over a paged cache: B requests
+of LEN tokens, H query heads over HK key/value heads, ``--drafts N`` drafted
+tokens a request (1: a decode step; ``--chain`` for a prompt's chunk instead
+of a tree), ``--block``, ``--head-dim`` and ``--dtype``, through
+``plan_cache``, ``plan_tree`` (trees only), ``rotary_to_cache`` and
+``forward_tree``.  The requests' blocks lie in random order.  Prints each
+operator's mean time and the whole step's, launched eagerly and as a replayed
+HIP graph.
+
+``--rotary B H HK N`` turns q and k of that shape by their positions
+(``forward_rotary``) and back (``backward_rotary``), ``--head-dim`` and
+``--dtype``, and prints both times and rates.
+
 ``--mfma-clock ROUNDS`` runs the clock calibration of the diagnostic
 library (``libflashlite_diag.so``, ``csrc/diag.hip``): every wave issues
 ROUNDS x 16 independent ``v_mfma_f32_32x32x16_f16`` (``--groups`` work-groups
@@ -87,6 +100,11 @@ def main(argv=None):
     ap.add_argument("--dtype", choices=("fp16", "bf16"), default="fp16")
     ap.add_argument("--head-dim", type=int, default=0, help="override the workload's head dim")
     ap.add_argument("--shape", type=int, nargs=3, metavar=("B", "H", "N"), default=None)
+    ap.add_argument("--serve", type=int, nargs=4, metavar=("B", "H", "HK", "LEN"), default=None)
+    ap.add_argument("--drafts", type=int, default=1, metavar="N")
+    ap.add_argument("--chain", action="store_true")
+    ap.add_argument("--block", type=int, default=16)
+    ap.add_argument("--rotary", type=int, nargs=4, metavar=("B", "H", "HK", "N"), default=None)
     ap.add_argument("--mfma-clock", type=int, default=0, metavar="ROUNDS")
     ap.add_argument("--groups", type=int, default=256)
     ap.add_argument("--waves", type=int, default=4)
@@ -116,6 +134,10 @@ def main(argv=None):
         return _quarter_timeline(args, torch)
     if args.decode:
         return _decode(args, torch)
+    if args.serve:
+        return _serve(args, torch)
+    if args.rotary:
+        return _rotary(args, torch)
 
     if args.copy_mib:
         n = args.copy_mib * (1 << 20) // 2
@@ -223,6 +245,91 @@ def _decode(args, torch):
           f"{' cold' if args.cold_mib else ''}: "
           f"{us:.2f} us/call, {nbytes / us / 1e3:.1f} GB/s ({nbytes / us / 1e3 / 8000:.1%} of 8 TB/s)",
           flush=True)
+    return 0
+
+
+def _serve(args, torch):
+    import numpy as np
+
+    import flashlite_amd as fl
+
+    b, h, hk, length = args.serve
+    n, block, d = args.drafts, args.block, args.head_dim or 64
+    dt = torch.bfloat16 if args.dtype == "bf16" else torch.float16
+    dev = torch.device("cuda:0")
+    rs = np.random.RandomState(11)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    own, most = -(-length // block), -(-(length + n) // block)
+    ids = rs.permutation(b * most)
+    tables = np.full((b, most), -1)
+    tables[:, :own] = ids[:b * own].reshape(b, own)
+    ring = np.concatenate([ids[b * own:], ids[:b * own]])
+    torch.manual_seed(11)
+    k_cache, v_cache = (torch.randn((b * most, block, hk, d), device=dev, dtype=dt).transpose(1, 2)
+                        for _ in range(2))
+    q, k, v = (torch.randn((b, n, x, d), device=dev, dtype=dt).transpose(1, 2) for x in (h, hk, hk))
+    freqs, scale = fl.rotary_frequencies(d, device=dev)
+    lengths, counts, held = i32([length] * b), i32([n] * b), i32([own] * b)
+    # the state goes to outputs of its own: a repeated call takes the same blocks
+    plan = dict(held_out=torch.empty_like(held), state_out=torch.empty_like(i32([0, 0])),
+                positions=torch.empty((b, n), dtype=torch.int32, device=dev),
+                slots=torch.empty((b, n), dtype=torch.int64, device=dev),
+                info=torch.empty((b, 4), dtype=torch.int32, device=dev))
+    tables, ring, state = i32(tables), i32(ring), i32([0, b * (most - own)])
+    tree = n > 1 and not args.chain
+    parents = i32(np.floor(rs.rand(b, n) * (np.arange(n) + 1)).astype(int) - 1)
+    mask = torch.empty((b, n, -(-n // 64)), dtype=torch.int64, device=dev) if tree else None
+    turned, out = torch.empty_like(q), torch.empty_like(q)
+    ws = torch.empty(max(fl.tree_workspace_bytes(q, k_cache), 16) // 4, device=dev)
+
+    steps = {"plan_cache": lambda: fl.plan_cache(lengths, counts, tables, held, ring, state, block,
+                                                 n, **plan)}
+    if tree:
+        steps["plan_tree"] = lambda: fl.plan_tree(parents, lengths, None, mask, plan["positions"])
+    steps["rotary_to_cache"] = lambda: fl.rotary_to_cache(
+        q, k, v, plan["positions"], plan["slots"], freqs, k_cache, v_cache, scale=scale, out=turned)
+    steps["forward_tree"] = lambda: fl.forward_tree(turned, k_cache, v_cache, tables, lengths, mask,
+                                                    out=out, workspace=ws)
+
+    def step():
+        for run in steps.values():
+            run()
+
+    step()
+    if bool((plan["info"][:, 0] != 0).any()):
+        raise RuntimeError("the plan refused a request")
+    for name, run in steps.items():
+        print(f"{name}: {_time_launches(run, args, torch):.2f} us", flush=True)
+    eager = _time_launches(step, args, torch)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    replayed = _time_launches(graph.replay, args, torch)
+    nbytes = 2 * b * hk * (length + n) * d * 2
+    print(f"serve B{b} H{h}/{hk} len {length} drafts {n}{'' if tree or n == 1 else ' (chain)'} "
+          f"D={d} {args.dtype} block {block}{' cold' if args.cold_mib else ''}: {eager:.2f} us/step, "
+          f"{replayed:.2f} us replayed, K/V {nbytes / replayed / 1e3:.1f} GB/s", flush=True)
+    return 0
+
+
+def _rotary(args, torch):
+    import flashlite_amd as fl
+
+    b, h, hk, n = args.rotary
+    d = args.head_dim or 64
+    dt = torch.bfloat16 if args.dtype == "bf16" else torch.float16
+    dev = torch.device("cuda:0")
+    torch.manual_seed(13)
+    q, k = (torch.randn((b, n, x, d), device=dev, dtype=dt).transpose(1, 2) for x in (h, hk))
+    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    positions = torch.arange(n, dtype=torch.int32, device=dev)[None].expand(b, n)
+    freqs, scale = fl.rotary_frequencies(d, device=dev)
+    nbytes = 2 * 2 * b * (h + hk) * n * d
+    for name, turn in (("forward_rotary", fl.forward_rotary), ("backward_rotary", fl.backward_rotary)):
+        us = _time_launches(lambda: turn(q, k, positions, freqs, scale=scale, q_out=qo, k_out=ko),
+                            args, torch)
+        print(f"{name} B{b} H{h}/{hk} N{n} D={d} {args.dtype}{' cold' if args.cold_mib else ''}: "
+              f"{us:.2f} us/launch, {nbytes / us / 1e3:.1f} GB/s", flush=True)
     return 0
 
 
