@@ -200,7 +200,9 @@ __device__ __forceinline__ void fetch4(uint64_t address, const void* lds) {
   asm volatile("global_load_lds_dword %0, off" : : "v"(address), "{m0}"(base) : "memory");
 }
 
-// Waves of a work-group of RW row blocks: 4, two work-groups a CU, or 8.
+// Waves of a work-group of RW row blocks, and slots for tiles of each of its
+// key groups (DEEP: for long walks, see launch_rw).
+constexpr int slots_of(int d, int rw, bool deep) { return rw == 2 && d == 128 && deep ? 4 : rw; }
 constexpr int waves_of(int rw) { return rw == 8 ? 8 : 4; }
 
 // One request: its tokens and its drafts that are there.
@@ -228,7 +230,7 @@ __device__ __forceinline__ int unit_drafts(const TreeGeom& g, const Request& r, 
 }
 
 // Steps of a unit's walk, 0 where no draft of its rows is there.
-template <int D, int RW>
+template <int D, int RW, bool DEEP>
 __device__ __forceinline__ int unit_steps(const TreeGeom& g, const Request& r, int rb) {
   constexpr int kStepKeys = (waves_of(RW) / RW) * (D == 64 ? kBc : kBc2);
   if (rb * 32 * RW >= r.count * g.group.d) return 0;
@@ -245,11 +247,11 @@ __device__ __forceinline__ int cost_of(int steps) {
 }
 
 // Costs of all row blocks of one key/value head of a request.
-template <int D, int RW>
+template <int D, int RW, bool DEEP>
 __device__ __forceinline__ int head_cost(const TreeGeom& g, const Request& r) {
   int n = 0;
 #pragma unroll 1
-  for (int rb = 0; rb < g.blocks_of_rows; ++rb) n += cost_of<RW>(unit_steps<D, RW>(g, r, rb));
+  for (int rb = 0; rb < g.blocks_of_rows; ++rb) n += cost_of<RW>(unit_steps<D, RW, DEEP>(g, r, rb));
   return n;
 }
 
@@ -272,11 +274,11 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 // The work-group's LDS: key and value tiles, and per wave the row addresses of
 // the next tile's keys and table entries fetched ahead.
-template <int D, int RW>
+template <int D, int RW, bool DEEP>
 struct Shared {
   static constexpr int kWaves = waves_of(RW);
   static constexpr int kGroups = kWaves / RW;
-  static constexpr int kSlots = RW;  // of each key group
+  static constexpr int kSlots = slots_of(D, RW, DEEP);
   // Rows of a tile that a wave fetches, and tiles whose rows it looks up at
   // once, a row a lane.
   static constexpr int kRows = (D == 64 ? kBc : kBc2) / RW;
@@ -291,9 +293,9 @@ struct Shared {
 
 // One unit's part over steps [s0, s1) by this work-group: the result goes to O
 // (and lse) with part == nullptr, or unnormalised to `part`.
-template <int D, class T, int RW>
+template <int D, class T, int RW, bool DEEP>
 __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t* V, T* O,
-                                     const TreeGeom& g, Shared<D, RW>& sh, int b, int kvh, int rb,
+                                     const TreeGeom& g, Shared<D, RW, DEEP>& sh, int b, int kvh, int rb,
                                      const Request& req, int s0, int s1, float* part, float cq,
                                      float cr) {
   using RowsT = TreeRows<D, T>;
@@ -303,7 +305,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   constexpr int kLanes = kRowB / 16;      // lanes a row of a fetch
   constexpr int kSegRows = 64 / kLanes;   // rows a fetch
   constexpr int kSegs = 8 / RW;           // fetches of a tile by this wave
-  constexpr int kSlots = Shared<D, RW>::kSlots;
+  constexpr int kSlots = Shared<D, RW, DEEP>::kSlots;
   constexpr int kAcc = D / 2;
   constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
   static_assert(kKeys * kRowB == kTileBytes, "tile size");
@@ -363,7 +365,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   const uint64_t kbase = (uint64_t)(uintptr_t)(K + kvh * g.k_head);
   const uint64_t vbase = (uint64_t)(uintptr_t)(V + kvh * g.v_head);
   int32_t(*const ids)[64] = sh.ids[w];
-  using Sh = Shared<D, RW>;
+  using Sh = Shared<D, RW, DEEP>;
   constexpr int kPer = Sh::kPer, kRows = Sh::kRows;
   // The key that lane l looks up for the key group's tiles kPer m ..: this
   // wave's row l % kRows of tile kPer m + l / kRows (past the last key: the
@@ -663,19 +665,19 @@ __device__ __forceinline__ int group_index(int xcds) {
 }
 
 // A unit a work-group.
-template <int D, class T, int RW>
+template <int D, class T, int RW, bool DEEP>
 __global__ void __launch_bounds__(64 * waves_of(RW), 2)
 tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
                 float cr) {
-  __shared__ __attribute__((aligned(16))) Shared<D, RW> sh;
+  __shared__ __attribute__((aligned(16))) Shared<D, RW, DEEP> sh;
   const int per = g.kv_heads * g.blocks_of_rows;
   const int unit = group_index(g.xcds);
   const int b = unit / per, rest = unit - b * per;
   const int kvh = rest / g.blocks_of_rows, rb = rest - kvh * g.blocks_of_rows;
   const Request r = request(g, b);
-  const int steps = unit_steps<D, RW>(g, r, rb);
+  const int steps = unit_steps<D, RW, DEEP>(g, r, rb);
   if (steps > 0)
-    walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, 0, steps, nullptr, cq, cr);
+    walk<D, T, RW, DEEP>(Q, K, V, O, g, sh, b, kvh, rb, r, 0, steps, nullptr, cq, cr);
 }
 
 // The costs of all units, in order, are dealt evenly to the work-groups: each
@@ -685,19 +687,19 @@ tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tree
 // parts[unit].x in which slot its results begin, whoever has its last in .y
 // which work-group that was; between them each work-group has one in its first
 // slot.  (The sum is below 2^31: tree_plan.)
-template <int D, class T, int RW>
+template <int D, class T, int RW, bool DEEP>
 __global__ void __launch_bounds__(64 * waves_of(RW), 2)
 tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
                   float cr) {
   constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
-  __shared__ __attribute__((aligned(16))) Shared<D, RW> sh;
+  __shared__ __attribute__((aligned(16))) Shared<D, RW, DEEP> sh;
   const int lane = threadIdx.x & 63;
   // Cost of one key/value head of requests b0 .. b0 + 63, one a lane.
   Request c;
   int n, upto;
   auto chunk = [&](int b0) __attribute__((always_inline)) {
     c = request(g, min(b0 + lane, g.batch - 1));
-    n = b0 + lane < g.batch ? head_cost<D, RW>(g, c) : 0;
+    n = b0 + lane < g.batch ? head_cost<D, RW, DEEP>(g, c) : 0;
     upto = wave_scan(n);
   };
   auto last_lane = [](int x) __attribute__((always_inline)) {
@@ -743,7 +745,7 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
     ++kvh;
   }
 #pragma unroll 1
-  while (in >= (cost = cost_of<RW>(steps = unit_steps<D, RW>(g, r, rb)))) {
+  while (in >= (cost = cost_of<RW>(steps = unit_steps<D, RW, DEEP>(g, r, rb)))) {
     in -= cost;
     ++rb;
   }
@@ -761,7 +763,7 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
       }
       float* const part =
           s0 == 0 && s1 == steps ? nullptr : g.part + (long long)slot * (32 * RW) * kPart;
-      walk<D, T, RW>(Q, K, V, O, g, sh, b, kvh, rb, r, s0, s1, part, cq, cr);
+      walk<D, T, RW, DEEP>(Q, K, V, O, g, sh, b, kvh, rb, r, s0, s1, part, cq, cr);
       slot = 2 * x + 1;
     }
     at += to - in;
@@ -776,7 +778,7 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
           r = request(g, ++b);
         }
       }
-      cost = cost_of<RW>(steps = unit_steps<D, RW>(g, r, rb));
+      cost = cost_of<RW>(steps = unit_steps<D, RW, DEEP>(g, r, rb));
     } while (cost == 0);
     __syncthreads();  // the tiles are free again
   }
@@ -891,42 +893,22 @@ TreePlan tree_plan(const fl_tree_params& p) {
   return t;
 }
 
-template <int D, class T, int RW>
-hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, float cq, float cr,
-                     hipStream_t st) {
-  constexpr int kStepKeys = (waves_of(RW) / RW) * (D == 64 ? kBc : kBc2);
-  g.blocks_of_rows = (g.rows + 32 * RW - 1) / (32 * RW);
+// One pass, or (split) the units' steps dealt to work-groups and joined.
+template <int D, class T, int RW, bool DEEP>
+hipError_t launch_walk(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, bool split,
+                       float cq, float cr, hipStream_t st) {
+  const dim3 threads(64 * waves_of(RW));
   const T* q = static_cast<const T*>(p.q);
   const uint8_t *k = static_cast<const uint8_t*>(p.k_cache),
                 *v = static_cast<const uint8_t*>(p.v_cache);
   T* o = static_cast<T*>(p.o);
-  // A split launch adds up costs in 32 bits.
-  const bool counted =
-      t.units * (((int64_t)g.capacity + g.drafts) / kStepKeys + 1 + start_of(RW)) < (1LL << 30);
-  // Splitting costs the partial results' way through memory and a second
-  // launch, about four microseconds; it saves the steps by which the longest
-  // unit that the table has room for passes an even share.  Up to kFewSaved
-  // one pass is no slower: 16 requests x 16 heads of 600 keys (D 128, f16)
-  // 18.8 us against 22.2, 4 x 16 drafts of 16/4 heads after 300 keys 10.2
-  // against 13.2, 1 head of 1000 keys 8.2 against 9.7; with twice that bound 8
-  // drafts of 32/8 heads after 1000 keys lose, 12.8 against 11.8.  With as many
-  // units as work-groups the share says nothing about requests of unlike
-  // lengths, so kMostSteps bounds what waiting for the longest can cost: up to
-  // it 32 drafts of 32 x 32/8 heads after 500 keys take 24.0 us against 29.4,
-  // while 16 heads and 1 to 16384 keys (128 steps) lose, 129 against 110.
-  constexpr int kFewSaved = 6, kMostSteps = 32;
-  const int64_t most = ((int64_t)g.capacity + g.drafts) / kStepKeys + 1;
-  const bool whole =
-      most <= kMostSteps && most - (most * t.units + t.grid - 1) / t.grid <= kFewSaved;
-  if (g.part == nullptr || !counted || whole) {
-    hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW>), dim3((unsigned)t.units), dim3(64 * waves_of(RW)), 0,
-                       st, q, k, v, o, g, cq, cr);
+  if (!split) {
+    hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW, DEEP>), dim3((unsigned)t.units), threads, 0, st,
+                       q, k, v, o, g, cq, cr);
     return hipGetLastError();
   }
-  g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.grid * 32 * RW *
-                                                 (D == 64 ? kPartStride : kPartStride128));
-  hipLaunchKernelGGL((tree_split_kernel<D, T, RW>), dim3((unsigned)t.grid), dim3(64 * waves_of(RW)), 0,
-                     st, q, k, v, o, g, cq, cr);
+  hipLaunchKernelGGL((tree_split_kernel<D, T, RW, DEEP>), dim3((unsigned)t.grid), threads, 0, st, q,
+                     k, v, o, g, cq, cr);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const unsigned rows = (unsigned)(g.heads * g.drafts);
@@ -935,9 +917,46 @@ hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, fl
   return hipGetLastError();
 }
 
+template <int D, class T, int RW>
+hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, float cq, float cr,
+                     hipStream_t st) {
+  constexpr int kStepKeys = waves_of(RW) / RW * (D == 64 ? kBc : kBc2);
+  // Steps of the longest unit that the table has room for.
+  const int64_t most = ((int64_t)g.capacity + g.drafts) / kStepKeys + 1;
+  // A split launch adds up costs in 32 bits.
+  const bool counted = t.units * (most + start_of(RW)) < (1LL << 30);
+  // Splitting costs the partial results' way through memory and a second
+  // launch, about four microseconds; it saves the steps by which the longest
+  // unit passes an even share.  Up to kFewSaved one pass is no slower: 16
+  // requests x 16 heads of 600 keys (D 128, f16) 18.8 us against 22.2, 4 x 16
+  // drafts of 16/4 heads after 300 keys 10.2 against 13.2, 1 head of 1000 keys
+  // 8.2 against 9.7; with twice that bound 8 drafts of 32/8 heads after 1000
+  // keys lose, 12.8 against 11.8.  With as many units as work-groups the share
+  // says nothing about requests of unlike lengths, so kMostSteps bounds what
+  // waiting for the longest can cost: up to it 32 drafts of 32 x 32/8 heads
+  // after 500 keys take 24.0 us against 29.4, while 16 heads and 1 to 16384
+  // keys (128 steps) lose, 129 against 110.
+  constexpr int kFewSaved = 6, kMostSteps = 32;
+  const int64_t share = (most * t.units + t.grid - 1) / t.grid;
+  const bool split =
+      g.part != nullptr && counted && (most > kMostSteps || most - share > kFewSaved);
+  // Long walks of 64 rows (D 128) are bound by the keys on their way: 4 slots
+  // instead of 2.  Short ones pay for the longer start.  12 drafts of 32/8
+  // heads (bf16) for 16 requests of 2000-4000 tokens 56.5 us against 64.7, for
+  // 8 of 1000-2000 23.7 against 25.8 (shares of 16 steps), for 4 of 1500-3000
+  // 21.9 against 20.7, for 4 x 16/4 heads of 300 11.5 against 10.0.
+  if constexpr (slots_of(D, RW, true) != slots_of(D, RW, false)) {
+    if (split && share >= 8) return launch_walk<D, T, RW, true>(p, t, g, split, cq, cr, st);
+  }
+  return launch_walk<D, T, RW, false>(p, t, g, split, cq, cr, st);
+}
+
 template <int D, class T>
 hipError_t launch_t(const fl_tree_params& p, TreeGeom& g, float cq, float cr, hipStream_t st) {
   const TreePlan t = tree_plan(p);
+  g.blocks_of_rows = (g.rows + 32 * t.rw - 1) / (32 * t.rw);
+  g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.grid * 32 * t.rw *
+                                                 (D == 64 ? kPartStride : kPartStride128));
   return t.rw == 1   ? launch_rw<D, T, 1>(p, t, g, cq, cr, st)
          : t.rw == 2 ? launch_rw<D, T, 2>(p, t, g, cq, cr, st)
          : t.rw == 4 ? launch_rw<D, T, 4>(p, t, g, cq, cr, st)
