@@ -874,7 +874,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g)
 constexpr int kMostParts = 64;
 
 struct TreePlan {
-  int rw, units, grid;
+  int rw, units, grid, most_grid;  // most_grid: what the workspace has room for
   bool split;
   int64_t bytes;
 };
@@ -885,30 +885,35 @@ TreePlan tree_plan(const fl_tree_params& p) {
   t.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
   t.units = (int)((rows + 32 * t.rw - 1) / (32 * t.rw) * p.kv_heads * p.batch);
   t.grid = (int)std::min<int64_t>(device_cus(), (int64_t)kMostParts * t.units);
+  // (see launch_rw)
+  t.most_grid = t.rw == 2 && p.head_dim == 64
+                    ? (int)std::min<int64_t>(2 * device_cus(), (int64_t)kMostParts * t.units)
+                    : t.grid;
   t.split = t.units < 2 * t.grid;
   const int64_t part = p.head_dim == 64 ? kPartStride : kPartStride128;
-  t.bytes = t.split ? 2LL * t.grid * 32 * t.rw * part * (int64_t)sizeof(float) +
+  t.bytes = t.split ? 2LL * t.most_grid * 32 * t.rw * part * (int64_t)sizeof(float) +
                           t.units * (int64_t)sizeof(int2)
                     : 0;
   return t;
 }
 
-// One pass, or (split) the units' steps dealt to work-groups and joined.
+// One pass, or (grid > 0) the units' steps dealt to `grid` work-groups and
+// joined.
 template <int D, class T, int RW, bool DEEP>
-hipError_t launch_walk(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, bool split,
+hipError_t launch_walk(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, int grid,
                        float cq, float cr, hipStream_t st) {
   const dim3 threads(64 * waves_of(RW));
   const T* q = static_cast<const T*>(p.q);
   const uint8_t *k = static_cast<const uint8_t*>(p.k_cache),
                 *v = static_cast<const uint8_t*>(p.v_cache);
   T* o = static_cast<T*>(p.o);
-  if (!split) {
+  if (grid == 0) {
     hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW, DEEP>), dim3((unsigned)t.units), threads, 0, st,
                        q, k, v, o, g, cq, cr);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL((tree_split_kernel<D, T, RW, DEEP>), dim3((unsigned)t.grid), threads, 0, st, q,
-                     k, v, o, g, cq, cr);
+  hipLaunchKernelGGL((tree_split_kernel<D, T, RW, DEEP>), dim3((unsigned)grid), threads, 0, st, q, k,
+                     v, o, g, cq, cr);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const unsigned rows = (unsigned)(g.heads * g.drafts);
@@ -940,22 +945,28 @@ hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, fl
   const int64_t share = (most * t.units + t.grid - 1) / t.grid;
   const bool split =
       g.part != nullptr && counted && (most > kMostSteps || most - share > kFewSaved);
-  // Long walks of 64 rows (D 128) are bound by the keys on their way: 4 slots
-  // instead of 2.  Short ones pay for the longer start.  12 drafts of 32/8
-  // heads (bf16) for 16 requests of 2000-4000 tokens 56.5 us against 64.7, for
-  // 8 of 1000-2000 23.7 against 25.8 (shares of 16 steps), for 4 of 1500-3000
-  // 21.9 against 20.7, for 4 x 16/4 heads of 300 11.5 against 10.0.
-  if constexpr (slots_of(D, RW, true) != slots_of(D, RW, false)) {
-    if (split && share >= 8) return launch_walk<D, T, RW, true>(p, t, g, split, cq, cr, st);
+  int grid = split ? t.grid : 0;
+  // Long walks of 64 rows are bound by the keys on their way: at D 128 4 slots
+  // instead of 2, at D 64 two work-groups a CU.  Short ones pay for the longer
+  // start, or the parts.  12 drafts of 32/8 heads (bf16) for 16 requests of
+  // 2000-4000 tokens 56.5 us against 64.7 (D 64: 35.9 against 42.6), for 8 of
+  // 1000-2000 23.7 against 25.8 (D 64: 17.9 against 18.0), for 4 of 1500-3000
+  // 21.9 against 20.7 (D 64: 17.8 against 16.6).
+  if constexpr (RW == 2) {
+    if (split && share * kStepKeys >= 512) {
+      if constexpr (slots_of(D, RW, true) != slots_of(D, RW, false))
+        return launch_walk<D, T, RW, true>(p, t, g, grid, cq, cr, st);
+      grid = t.most_grid;
+    }
   }
-  return launch_walk<D, T, RW, false>(p, t, g, split, cq, cr, st);
+  return launch_walk<D, T, RW, false>(p, t, g, grid, cq, cr, st);
 }
 
 template <int D, class T>
 hipError_t launch_t(const fl_tree_params& p, TreeGeom& g, float cq, float cr, hipStream_t st) {
   const TreePlan t = tree_plan(p);
   g.blocks_of_rows = (g.rows + 32 * t.rw - 1) / (32 * t.rw);
-  g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.grid * 32 * t.rw *
+  g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.most_grid * 32 * t.rw *
                                                  (D == 64 ? kPartStride : kPartStride128));
   return t.rw == 1   ? launch_rw<D, T, 1>(p, t, g, cq, cr, st)
          : t.rw == 2 ? launch_rw<D, T, 2>(p, t, g, cq, cr, st)
