@@ -35,6 +35,15 @@ int check_view(const int64_t st[3], int64_t unit, const char* name, const char* 
   return FL_OK;
 }
 
+// Rows that are written: no two in one place.
+int check_apart(const int64_t st[3], int64_t n0, int64_t n1, int64_t n2, const char* name,
+                const char* who) {
+  if ((n0 > 1 && st[0] == 0) || (n1 > 1 && st[1] == 0) || (n2 > 1 && st[2] == 0))
+    return set_error(FL_ERR_INVALID_ARGUMENT, "%s: %s is written, its rows must not overlap", who,
+                     name);
+  return FL_OK;
+}
+
 int check_pages(int64_t num_blocks, int64_t block_size, const char* who) {
   if (num_blocks < 1 || block_size < 1)
     return set_error(FL_ERR_INVALID_ARGUMENT,
@@ -71,6 +80,9 @@ int check_rotary(const fl_rotary_params* p, bool cache, const char* who) {
   if (rc == FL_OK) rc = check_view(p->q_out_stride, unit, "q_out", who);
   if (rc == FL_OK && p->k) rc = check_view(p->k_stride, unit, "k", who);
   if (rc == FL_OK && p->k && !cache) rc = check_view(p->k_out_stride, unit, "k_out", who);
+  if (rc == FL_OK) rc = check_apart(p->q_out_stride, p->batch, p->heads, p->rows, "q_out", who);
+  if (rc == FL_OK && p->k && !cache)
+    rc = check_apart(p->k_out_stride, p->batch, p->kv_heads, p->rows, "k_out", who);
   return rc;
 }
 
@@ -108,8 +120,10 @@ int check_tree(const fl_tree_params* p, const char* who) {
   if (rc != FL_OK) return rc;
   if (p->max_blocks < 1)
     return set_error(FL_ERR_INVALID_ARGUMENT, "%s: the block tables need entries", who);
-  if (p->max_blocks > INT32_MAX / p->block_size || p->max_blocks * p->block_size > INT32_MAX - 256)
-    return set_error(FL_ERR_UNSUPPORTED, "%s: max_blocks * block_size must be below 2^31 - 256",
+  // (keys are counted in 32 bits, those of lookups past the last one too)
+  if (p->max_blocks > INT32_MAX / p->block_size ||
+      p->max_blocks * p->block_size >= (INT64_C(1) << 31) - 65536)
+    return set_error(FL_ERR_UNSUPPORTED, "%s: max_blocks * block_size must be below 2^31 - 65536",
                      who);
   if (!fits32(p->batch) || !fits32(p->heads) || !fits32(p->drafts) ||
       (p->drafts > 0 && p->heads > INT32_MAX / 2 / p->drafts))
@@ -218,6 +232,10 @@ int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, voi
   if (rc == FL_OK) rc = check_view(c->v_stride, 8, "v", who);
   if (rc == FL_OK) rc = check_view(c->k_cache_stride, 8, "k_cache", who);
   if (rc == FL_OK) rc = check_view(c->v_cache_stride, 8, "v_cache", who);
+  if (rc == FL_OK)
+    rc = check_apart(c->k_cache_stride, c->num_blocks, p->kv_heads, c->block_size, "k_cache", who);
+  if (rc == FL_OK)
+    rc = check_apart(c->v_cache_stride, c->num_blocks, p->kv_heads, c->block_size, "v_cache", who);
   if (rc != FL_OK) return rc;
   if (p->batch == 0 || p->rows == 0 || p->heads + p->kv_heads == 0) return FL_OK;
   if (!p->k || !c->v || !c->k_cache || !c->v_cache || !c->slots)
@@ -252,6 +270,8 @@ int fl_attn_tree_fwd(const fl_tree_params* p, void* workspace, int64_t workspace
       !aligned(p->lse, 4) || !aligned(p->mask, 8))
     return set_error(FL_ERR_MISALIGNED,
                      "%s: block_tables, lengths, counts and lse must be 4-byte aligned, mask 8", who);
+  const int apart = check_apart(p->o_stride, p->batch, p->heads, p->drafts, "o", who);
+  if (apart != FL_OK) return apart;
   const int64_t need = fl::tree_workspace_bytes(*p);
   void* const ws = need > 0 && workspace_bytes >= need ? workspace : nullptr;
   if (!aligned(ws, 16))

@@ -903,6 +903,7 @@ template <int D, class T, int RW, bool DEEP>
 hipError_t launch_walk(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, int grid,
                        float cq, float cr, hipStream_t st) {
   const dim3 threads(64 * waves_of(RW));
+  if (grid % g.xcds != 0) g.xcds = 1;  // (all XCDs alike, or none told apart)
   const T* q = static_cast<const T*>(p.q);
   const uint8_t *k = static_cast<const uint8_t*>(p.k_cache),
                 *v = static_cast<const uint8_t*>(p.v_cache);

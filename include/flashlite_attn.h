@@ -299,7 +299,7 @@ int fl_attn_tree_plan(const fl_tree_plan_params* p, void* stream);
  * {j, j + pairs}, or {2j, 2j + 1} with interleaved.  With transpose the angle
  * is negated: the gradient of the same call.  q, k, q_out and k_out are
  * [batch, heads or kv_heads, rows, head_dim] views with strides {batch, head,
- * row} in elements; outputs may be their inputs.  k may be NULL (no k).
+ * row} in elements; outputs may be their inputs (no other overlap).  k may be NULL (no k).
  * positions are int32 (or int64: position_bits 64) [batch, rows], strides
  * {batch, row}.  head_dim 64 or 128; dtype FL_DTYPE_F16, FL_DTYPE_BF16 or (not
  * with a cache) FL_DTYPE_F32.
@@ -368,7 +368,7 @@ int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, voi
  * counts[b] on are left as they were, o and lse alike.  A key whose block
  * table entry is not in [0, num_blocks) is seen by nobody.  What a row does
  * not see does not reach it, NaN and infinities in k_cache and v_cache
- * included.  lengths are clamped to the table's rows (max_blocks *
+ * included.  max_blocks * block_size is below 2^31 - 65536.  lengths are clamped to the table's rows (max_blocks *
  * block_size), with the drafts behind them.  lse: optional fp32 [batch, heads,
  * drafts] (contiguous).  Block and row strides of the caches are below 2^31
  * elements.

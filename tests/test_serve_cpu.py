@@ -101,6 +101,8 @@ def rotary_params(**kw):
     (dict(batch=1 << 20, rows=1 << 20), capi.FL_ERR_UNSUPPORTED, "2^26"),
     (dict(q_stride=T3(6400, 64, 12)), capi.FL_ERR_UNSUPPORTED, "q strides"),
     (dict(k_out_stride=T3(6400, 64, -64)), capi.FL_ERR_UNSUPPORTED, "k_out strides"),
+    (dict(q_out_stride=T3(0, 6400, 64)), capi.FL_ERR_INVALID_ARGUMENT, "q_out is written"),
+    (dict(k_out_stride=T3(51200, 0, 64)), capi.FL_ERR_INVALID_ARGUMENT, "k_out is written"),
     (dict(q=0), capi.FL_ERR_INVALID_ARGUMENT, "non-NULL"),
     (dict(k_out=0), capi.FL_ERR_INVALID_ARGUMENT, "non-NULL"),
     (dict(positions=0), capi.FL_ERR_INVALID_ARGUMENT, "non-NULL"),
@@ -125,6 +127,8 @@ def test_rotary_null_and_empty():
     ({}, dict(num_blocks=0), capi.FL_ERR_INVALID_ARGUMENT, "blocks"),
     ({}, dict(block_size=1 << 31), capi.FL_ERR_UNSUPPORTED, "int32"),
     ({}, dict(v_cache_stride=T3(64, 64, 4)), capi.FL_ERR_UNSUPPORTED, "v_cache strides"),
+    ({}, dict(k_cache_stride=T3(0, 1024, 64)), capi.FL_ERR_INVALID_ARGUMENT, "k_cache is written"),
+    ({}, dict(v_cache_stride=T3(8192, 1024, 0)), capi.FL_ERR_INVALID_ARGUMENT, "v_cache is written"),
     ({}, dict(slots=0), capi.FL_ERR_INVALID_ARGUMENT, "slots"),
     (dict(k=0), {}, capi.FL_ERR_INVALID_ARGUMENT, "non-NULL"),
     ({}, dict(v=A + 4), capi.FL_ERR_MISALIGNED, "16-byte"),
@@ -171,6 +175,7 @@ TREE_REFUSALS = [
     (dict(num_blocks=0), capi.FL_ERR_INVALID_ARGUMENT, "blocks"),
     (dict(max_blocks=0), capi.FL_ERR_INVALID_ARGUMENT, "tables"),
     (dict(max_blocks=1 << 27, table_stride=1 << 27), capi.FL_ERR_UNSUPPORTED, "2^31"),
+    (dict(max_blocks=1, block_size=(1 << 31) - 65536), capi.FL_ERR_UNSUPPORTED, "2^31"),
     (dict(table_stride=19), capi.FL_ERR_INVALID_ARGUMENT, "table_stride"),
     (dict(mask_stride=-1), capi.FL_ERR_INVALID_ARGUMENT, "mask_stride"),
     (dict(k_stride=T3(2048, 1024, 60)), capi.FL_ERR_UNSUPPORTED, "k_cache strides"),
@@ -191,6 +196,7 @@ def test_tree_refusals(change, code, text):
 @pytest.mark.parametrize("change,code,text", [
     (dict(lengths=0), capi.FL_ERR_INVALID_ARGUMENT, "non-NULL"),
     (dict(o=0), capi.FL_ERR_INVALID_ARGUMENT, "non-NULL"),
+    (dict(o_stride=T3(2560, 320, 0)), capi.FL_ERR_INVALID_ARGUMENT, "o is written"),
     (dict(v_cache=A + 8), capi.FL_ERR_MISALIGNED, "16-byte"),
     (dict(mask=A + 4), capi.FL_ERR_MISALIGNED, "mask"),
     (dict(lse=A + 1), capi.FL_ERR_MISALIGNED, "lse"),
