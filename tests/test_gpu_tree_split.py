@@ -145,3 +145,49 @@ def test_workspace_too_small_is_refused(cuda):
         fl.forward_tree(workspace=torch.empty(need - 4, dtype=torch.uint8, device=cuda), **args)
     with pytest.raises(RuntimeError, match="workspace"):
         fl.forward_tree(workspace=torch.empty(need), **args)
+
+
+@pytest.mark.parametrize("dtype,d", KINDS)
+@pytest.mark.parametrize("group,n", ROWS)
+@pytest.mark.parametrize("room", [0, ROOM])
+def test_infinite_scores(cuda, dtype, d, group, n, room):
+    """Scores of -inf weigh nothing, a whole tile's or part's included; one of
+    +inf makes its row NaN."""
+    p = Problem(70 + n, dtype, 2, group, 1, n, d, 16, [900, 260], "tree", table_pad=room)
+    for b, gone in ((0, 700), (1, 200)):  # the first tokens' scores: -inf or inf
+        for t in range(gone):
+            p.k[int(p.tables[b, t // 16]), 0, t % 16, 0] = float("inf")
+    low = np.random.RandomState(n).rand(2, group, n) < 0.8
+    import torch
+
+    sign = torch.from_numpy(np.where(low, -1.0, 1.0))
+    p.q[..., 0] = (p.q[..., 0].abs() + 0.1) * sign.to(p.q.dtype)
+    ref = p.reference()
+    assert np.isnan(ref[0]).any() and np.isfinite(ref[0]).any()
+    check(*run(p, cuda), p, ref)
+
+
+@pytest.mark.parametrize("dtype,d", KINDS)
+@pytest.mark.parametrize("b,h,hk,n,lengths,tree,room", [
+    (1, 2, 2, 512, [40], "tree", 0),       # the widest mask plan_tree makes
+    (2, 1, 1, 512, [0, 300], "any", ROOM),
+    (1, 1, 1, 700, [33], None, 0),         # a prompt's chunk
+    (1, 1, 1, 700, [0], None, ROOM),
+])
+def test_many_drafts(cuda, dtype, d, b, h, hk, n, lengths, tree, room):
+    p = Problem(71 + n, dtype, b, h, hk, n, d, 16, lengths, tree, ragged=b > 1, table_pad=room)
+    check(*run(p, cuda), p)
+
+
+def test_outputs_that_overlap_are_refused(cuda):
+    import torch
+
+    p = Problem(72, "float16", 2, 2, 1, 3, 64, 16, [20, 5], "tree")
+    args = p.device(cuda)
+    one = torch.empty((1, 2, 3, 64), dtype=torch.float16, device=cuda).expand(2, 2, 3, 64)
+    with pytest.raises(RuntimeError, match="overlap"):
+        fl.forward_tree(out=one, **args)
+    pos = torch.zeros((2, 3), dtype=torch.int32, device=cuda)
+    freqs, _ = fl.rotary_frequencies(64, device=cuda)
+    with pytest.raises(RuntimeError, match="overlap"):
+        fl.forward_rotary(args["q"], None, pos, freqs, q_out=one)
