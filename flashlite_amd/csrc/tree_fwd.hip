@@ -27,7 +27,7 @@ struct TreeGeom {
   const int64_t* mask;
   long long mask_stride;
   float* lse;
-  int batch, heads, kv_heads, drafts, rows, words, blocks_of_rows;
+  int batch, heads, kv_units, drafts, rows, words, blocks_of_rows;
   int num_blocks, capacity;  // capacity: keys of a table row
   FastDiv block, group, by_drafts;
   // split launches: partial results [2 * grid][32 RW][kPartStride], and per
@@ -201,9 +201,12 @@ __device__ __forceinline__ void fetch4(uint64_t address, const void* lds) {
 }
 
 // Waves of a work-group of RW row blocks, and slots for tiles of each of its
-// key groups (DEEP: for long walks, see launch_rw).
+// key groups.  DEEP: for long walks, see launch_rw.
 constexpr int slots_of(int d, int rw, bool deep) { return rw == 2 && d == 128 && deep ? 4 : rw; }
 constexpr int waves_of(int rw) { return rw == 8 ? 8 : 4; }
+// Key/value heads of a work-group, side by side.
+constexpr int heads_of(int rw, bool deep) { return rw == 1 && deep ? 4 : 1; }
+constexpr int key_groups_of(int rw, bool deep) { return waves_of(rw) / (rw * heads_of(rw, deep)); }
 
 // One request: its tokens and its drafts that are there.
 struct Request {
@@ -232,7 +235,7 @@ __device__ __forceinline__ int unit_drafts(const TreeGeom& g, const Request& r, 
 // Steps of a unit's walk, 0 where no draft of its rows is there.
 template <int D, int RW, bool DEEP>
 __device__ __forceinline__ int unit_steps(const TreeGeom& g, const Request& r, int rb) {
-  constexpr int kStepKeys = (waves_of(RW) / RW) * (D == 64 ? kBc : kBc2);
+  constexpr int kStepKeys = key_groups_of(RW, DEEP) * (D == 64 ? kBc : kBc2);
   if (rb * 32 * RW >= r.count * g.group.d) return 0;
   return (r.length + unit_drafts(g, r, rb, 32 * RW) + kStepKeys - 1) / kStepKeys;
 }
@@ -301,7 +304,8 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   using RowsT = TreeRows<D, T>;
   using V8 = typename RowsT::V8;
   constexpr int kKeys = RowsT::kKeys, kRowB = 2 * D;
-  constexpr int KW = waves_of(RW) / RW;
+  constexpr int KW = key_groups_of(RW, DEEP);
+  constexpr int kHeads = heads_of(RW, DEEP);
   constexpr int kLanes = kRowB / 16;      // lanes a row of a fetch
   constexpr int kSegRows = 64 / kLanes;   // rows a fetch
   constexpr int kSegs = 8 / RW;           // fetches of a tile by this wave
@@ -312,7 +316,10 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
 
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rw = w % RW, kg = w / RW;  // row block and key group
+  // Row block, head of those side by side, key group, and which wave (of a row
+  // block) or key group's tiles are its.
+  const int rw = w % RW, hw = w / RW % kHeads, kg = w / (RW * kHeads), own = w / RW;
+  kvh += hw;
   const int length = req.length;
   const int drafts = unit_drafts(g, req, rb, 32 * RW);
   const int keys = length + drafts;
@@ -323,8 +330,8 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
 
   RowsT rows;
   rows.start(lane, cr);
-  const int local = 32 * rw + rows.col;
-  const int row = 32 * RW * rb + local;
+  const int local = 32 * (rw + hw) + rows.col;  // (one of them is 0)
+  const int row = 32 * (RW * rb + rw) + rows.col;
   const int my_row = min(row, g.rows - 1);
   const int draft = divide(my_row, g.group);
   const int head = kvh * g.group.d + (my_row - draft * g.group.d);
@@ -400,14 +407,14 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     uint64_t x = 0;
 #pragma unroll 1
     for (int q = 0; q < RW; ++q) {
-      const uint64_t y = uniform(sh.good[kg * RW + q][(i / kPer) & 1]) >> (i % kPer * kRows);
+      const uint64_t y = uniform(sh.good[own * RW + q][(i / kPer) & 1]) >> (i % kPer * kRows);
       x |= (y & (kRows == 64 ? ~(uint64_t)0 : ((uint64_t)1 << kRows) - 1)) << (q * kRows);
     }
     return x;
   };
   // This wave's share of the K (t = 0) or V (1) tile j.
   auto fetch = [&](int t, int j) __attribute__((always_inline)) {
-    uint8_t* const tile = sh.tile[kg][j & (kSlots - 1)][t];
+    uint8_t* const tile = sh.tile[own][j & (kSlots - 1)][t];
     const uint64_t* const from = sh.where[w][(j / kPer) & 1][t] + j % kPer * kRows;
     uint64_t at[kSegs];
 #pragma unroll
@@ -499,7 +506,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       typename RowsT::Scores s;
       typename RowsT::Probs p;
       asm volatile("s_waitcnt vmcnt(8)" : : : "memory");  // K(i), and the next table entries
-      rows.scores(sh.tile[kg][0][0], s);
+      rows.scores(sh.tile[own][0][0], s);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // its operands are in registers
       const bool more = i + 1 < n, next = (i + 1) % kPer == 0;
       prepare(i, bad != 0, s);
@@ -515,8 +522,8 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       else
         asm volatile("s_waitcnt vmcnt(8)" : : : "memory");
       V8 va[8];
-      read_v(sh.tile[kg][0][1], va);
-      output(sh.tile[kg][0][1], va, p);
+      read_v(sh.tile[own][0][1], va);
+      output(sh.tile[own][0][1], va, p);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
       if (more) fetch(1, i + 1);
     }
@@ -538,17 +545,17 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     }
     sync_ring<(kSlots - 1) * 2 * kSegs>();
     typename RowsT::Scores s;
-    rows.scores(sh.tile[kg][0][0], s);
-    int flag = sh.bad[kg * RW + (lane & (RW - 1))];
+    rows.scores(sh.tile[own][0][0], s);
+    int flag = sh.bad[own * RW + (lane & (RW - 1))];
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
       sync_ring<(kSlots - 2) * 2 * kSegs>();
       prepare(i, __builtin_amdgcn_ballot_w64(flag != 0) != 0, s);
-      const uint8_t* const vt = sh.tile[kg][i & (kSlots - 1)][1];
+      const uint8_t* const vt = sh.tile[own][i & (kSlots - 1)][1];
       typename RowsT::Scores next;
       typename RowsT::Probs p;
       V8 va[8];
-      rows.scores(sh.tile[kg][(i + 1) & (kSlots - 1)][0], next);
+      rows.scores(sh.tile[own][(i + 1) & (kSlots - 1)][0], next);
       const float sum = rows.exponentiate(s, p);
       // Keeps the exponentials here, among the products (they would be sunk
       // past the next branch).
@@ -556,7 +563,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
       for (int h = 0; h < 2 * RowsT::kBlocks; ++h) asm volatile("" : : "v"(p.p[h]));
       read_v(vt, va);
       // (of tile i + 1, or a later one's)
-      flag = sh.bad[kg * RW + (lane & (RW - 1))];
+      flag = sh.bad[own * RW + (lane & (RW - 1))];
       fetch(1, i + kSlots - 1);
       if ((i + kSlots) % kPer == 0) look_up((i + kSlots) / kPer);
       fetch(0, i + kSlots);
@@ -573,12 +580,12 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   if constexpr (KW > 1) {
     if constexpr (RW > 1) __syncthreads();  // (with RW == 1 a wave's slots are its own)
     // (16 KiB a wave: its own slots, with RW == 1)
-    float4* const own = reinterpret_cast<float4*>(sh.tile) + 1024 * w;
+    float4* const to = reinterpret_cast<float4*>(sh.tile) + 1024 * w;
 #pragma unroll
     for (int c = 0; c < kAcc / 4; ++c) {
       const float16_t& x = rows.o[c >> 2];
       const int r = 4 * (c & 3);
-      own[c * 64 + lane] = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
+      to[c * 64 + lane] = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
     }
     sh.ml[w][lane] = make_float2(rows.mc, rows.l);
     __syncthreads();
@@ -665,19 +672,19 @@ __device__ __forceinline__ int group_index(int xcds) {
 }
 
 // A unit a work-group.
-template <int D, class T, int RW, bool DEEP>
+template <int D, class T, int RW>
 __global__ void __launch_bounds__(64 * waves_of(RW), 2)
 tree_fwd_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
                 float cr) {
-  __shared__ __attribute__((aligned(16))) Shared<D, RW, DEEP> sh;
-  const int per = g.kv_heads * g.blocks_of_rows;
+  __shared__ __attribute__((aligned(16))) Shared<D, RW, false> sh;
+  const int per = g.kv_units * g.blocks_of_rows;
   const int unit = group_index(g.xcds);
   const int b = unit / per, rest = unit - b * per;
   const int kvh = rest / g.blocks_of_rows, rb = rest - kvh * g.blocks_of_rows;
   const Request r = request(g, b);
-  const int steps = unit_steps<D, RW, DEEP>(g, r, rb);
+  const int steps = unit_steps<D, RW, false>(g, r, rb);
   if (steps > 0)
-    walk<D, T, RW, DEEP>(Q, K, V, O, g, sh, b, kvh, rb, r, 0, steps, nullptr, cq, cr);
+    walk<D, T, RW, false>(Q, K, V, O, g, sh, b, kvh, rb, r, 0, steps, nullptr, cq, cr);
 }
 
 // The costs of all units, in order, are dealt evenly to the work-groups: each
@@ -691,6 +698,7 @@ template <int D, class T, int RW, bool DEEP>
 __global__ void __launch_bounds__(64 * waves_of(RW), 2)
 tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
                   float cr) {
+  constexpr int kHeads = heads_of(RW, DEEP);
   constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
   __shared__ __attribute__((aligned(16))) Shared<D, RW, DEEP> sh;
   const int lane = threadIdx.x & 63;
@@ -711,7 +719,7 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
     chunk(b0);
     all += last_lane(upto);
   }
-  all *= g.kv_heads;
+  all *= g.kv_units;
   // `busy` work-groups have a share, `even` or one more; neighbours run on one
   // XCD, all XCDs alike.
   const int busy = min((int)gridDim.x, all);
@@ -726,8 +734,8 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
   int b0 = 0, before = 0;
   uint64_t past;
 #pragma unroll 1
-  while ((past = __builtin_amdgcn_ballot_w64(before + upto * g.kv_heads > at)) == 0) {
-    before += last_lane(upto) * g.kv_heads;
+  while ((past = __builtin_amdgcn_ballot_w64(before + upto * g.kv_units > at)) == 0) {
+    before += last_lane(upto) * g.kv_units;
     b0 += 64;
     chunk(b0);
   }
@@ -737,7 +745,7 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
   r.length = __builtin_amdgcn_readlane(c.length, l);
   r.count = __builtin_amdgcn_readlane(c.count, l);
   const int head = __builtin_amdgcn_readlane(n, l);
-  int in = at - before - __builtin_amdgcn_readlane(upto - n, l) * g.kv_heads;
+  int in = at - before - __builtin_amdgcn_readlane(upto - n, l) * g.kv_units;
   int kvh = 0, rb = 0, steps, cost;
 #pragma unroll 1
   while (in >= head) {
@@ -757,13 +765,13 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
     const int s0 = max(in - start_of(RW), 0), s1 = to - start_of(RW);
     if (s1 > s0) {
       if (threadIdx.x == 0) {
-        int2* const where = g.parts + (b * g.kv_heads + kvh) * g.blocks_of_rows + rb;
+        int2* const where = g.parts + (b * g.kv_units + kvh) * g.blocks_of_rows + rb;
         if (s0 == 0) where->x = slot;
         if (s1 == steps) where->y = x;
       }
       float* const part =
-          s0 == 0 && s1 == steps ? nullptr : g.part + (long long)slot * (32 * RW) * kPart;
-      walk<D, T, RW, DEEP>(Q, K, V, O, g, sh, b, kvh, rb, r, s0, s1, part, cq, cr);
+          s0 == 0 && s1 == steps ? nullptr : g.part + (long long)slot * (32 * RW * kHeads) * kPart;
+      walk<D, T, RW, DEEP>(Q, K, V, O, g, sh, b, kvh * kHeads, rb, r, s0, s1, part, cq, cr);
       slot = 2 * x + 1;
     }
     at += to - in;
@@ -773,7 +781,7 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
     do {
       if (++rb == g.blocks_of_rows) {
         rb = 0;
-        if (++kvh == g.kv_heads) {
+        if (++kvh == g.kv_units) {
           kvh = 0;
           r = request(g, ++b);
         }
@@ -785,7 +793,7 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
 }
 
 // One wave a row: merges the partial results of its unit, if it was split.
-template <int D, class T, int RW>
+template <int D, class T, int RW, int HEADS>
 __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g) {
   constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
   constexpr int kCols = D / 64, kBatch = 8;
@@ -798,15 +806,16 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g)
   const int row = draft * g.group.d + (head - kvh * g.group.d);
   const int rb = row / (32 * RW);
   const int count = g.counts ? g.counts[b] : g.drafts;
-  const int2 parts = g.parts[(b * g.kv_heads + kvh) * g.blocks_of_rows + rb];
+  const int2 parts = g.parts[(b * g.kv_units + kvh / HEADS) * g.blocks_of_rows + rb];
   if (draft >= count) return;  // (its unit's entry may not be there either)
   // Part j: the first in slot parts.x, then the first slots of the work-groups
   // that follow.
   const int x0 = parts.x >> 1, n = parts.y - x0 + 1;
   if (n == 1) return;  // one work-group had all of it
-  const float* const base = g.part + (long long)(row - rb * 32 * RW) * kPart;
+  const float* const base =
+      g.part + (long long)(row - rb * 32 * RW + kvh % HEADS * 32) * kPart;
   auto at = [&](int j) __attribute__((always_inline)) {
-    return base + (long long)(j == 0 ? parts.x : 2 * (x0 + j)) * (32 * RW) * kPart;
+    return base + (long long)(j == 0 ? parts.x : 2 * (x0 + j)) * (32 * RW * HEADS) * kPart;
   };
   float acc[kCols] = {}, l = 0.0f, mx = ninf();
 #pragma unroll 1
@@ -874,7 +883,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g)
 constexpr int kMostParts = 64;
 
 struct TreePlan {
-  int rw, units, grid, most_grid;  // most_grid: what the workspace has room for
+  int rw, units, grid;
+  int most_grid, heads;  // what the workspace has room for: work-groups, heads of each
   bool split;
   int64_t bytes;
 };
@@ -889,9 +899,10 @@ TreePlan tree_plan(const fl_tree_params& p) {
   t.most_grid = t.rw == 2 && p.head_dim == 64
                     ? (int)std::min<int64_t>(2 * device_cus(), (int64_t)kMostParts * t.units)
                     : t.grid;
-  t.split = t.units < 2 * t.grid;
+  t.heads = t.rw == 1 && p.kv_heads % heads_of(1, true) == 0 ? heads_of(1, true) : 1;
+  t.split = t.units < 2 * t.grid || t.heads > 1;
   const int64_t part = p.head_dim == 64 ? kPartStride : kPartStride128;
-  t.bytes = t.split ? 2LL * t.most_grid * 32 * t.rw * part * (int64_t)sizeof(float) +
+  t.bytes = t.split ? 2LL * t.most_grid * 32 * t.rw * t.heads * part * (int64_t)sizeof(float) +
                           t.units * (int64_t)sizeof(int2)
                     : 0;
   return t;
@@ -903,22 +914,25 @@ template <int D, class T, int RW, bool DEEP>
 hipError_t launch_walk(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, int grid,
                        float cq, float cr, hipStream_t st) {
   const dim3 threads(64 * waves_of(RW));
+  g.kv_units = (int)p.kv_heads / heads_of(RW, DEEP);
   if (grid % g.xcds != 0) g.xcds = 1;  // (all XCDs alike, or none told apart)
   const T* q = static_cast<const T*>(p.q);
   const uint8_t *k = static_cast<const uint8_t*>(p.k_cache),
                 *v = static_cast<const uint8_t*>(p.v_cache);
   T* o = static_cast<T*>(p.o);
-  if (grid == 0) {
-    hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW, DEEP>), dim3((unsigned)t.units), threads, 0, st,
-                       q, k, v, o, g, cq, cr);
-    return hipGetLastError();
+  if constexpr (!DEEP) {
+    if (grid == 0) {
+      hipLaunchKernelGGL((tree_fwd_kernel<D, T, RW>), dim3((unsigned)t.units), threads, 0, st, q, k,
+                         v, o, g, cq, cr);
+      return hipGetLastError();
+    }
   }
   hipLaunchKernelGGL((tree_split_kernel<D, T, RW, DEEP>), dim3((unsigned)grid), threads, 0, st, q, k,
                      v, o, g, cq, cr);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const unsigned rows = (unsigned)(g.heads * g.drafts);
-  hipLaunchKernelGGL((tree_merge_kernel<D, T, RW>), dim3((rows + 3) / 4, (unsigned)g.batch),
+  hipLaunchKernelGGL((tree_merge_kernel<D, T, RW, heads_of(RW, DEEP)>), dim3((rows + 3) / 4, (unsigned)g.batch),
                      dim3(256), 0, st, o, g);
   return hipGetLastError();
 }
@@ -926,7 +940,7 @@ hipError_t launch_walk(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, 
 template <int D, class T, int RW>
 hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, float cq, float cr,
                      hipStream_t st) {
-  constexpr int kStepKeys = waves_of(RW) / RW * (D == 64 ? kBc : kBc2);
+  constexpr int kStepKeys = key_groups_of(RW, false) * (D == 64 ? kBc : kBc2);
   // Steps of the longest unit that the table has room for.
   const int64_t most = ((int64_t)g.capacity + g.drafts) / kStepKeys + 1;
   // A split launch adds up costs in 32 bits.
@@ -944,8 +958,9 @@ hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, fl
   // keys (128 steps) lose, 129 against 110.
   constexpr int kFewSaved = 6, kMostSteps = 32;
   const int64_t share = (most * t.units + t.grid - 1) / t.grid;
-  const bool split =
-      g.part != nullptr && counted && (most > kMostSteps || most - share > kFewSaved);
+  const bool can = g.part != nullptr && counted;
+  const bool split = can && t.units < 2 * t.grid &&
+                     (most > kMostSteps || most - share > kFewSaved);
   int grid = split ? t.grid : 0;
   // Long walks of 64 rows are bound by the keys on their way: at D 128 4 slots
   // instead of 2, at D 64 two work-groups a CU.  Short ones pay for the longer
@@ -960,6 +975,21 @@ hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, fl
       grid = t.most_grid;
     }
   }
+  // Up to 32 rows over long walks are bound by memory, and where a token's
+  // heads lie side by side (the cache's rows first) a head's row is 128 or 256
+  // bytes of it: 4 heads at once read 4 times that in one piece, a wave each.
+  // One token after 8000 of 32 requests, 32/8 heads (bf16): D 64 98.7 us
+  // against 109.7, D 128 181 against 191; 16 requests of 2000-4000: 26.5
+  // against 29.9, 43.7 against 45.8.  Heads first they lose, 96 against 91, as
+  // do shares (4 requests of 2000-4000: 16.2 against 14.1) or walks that are
+  // short (512 of 100-500: 70 against 65), and units too few for kMostParts
+  // each (1 of 64000: 39.2 against 36.3).
+  if constexpr (RW == 1) {
+    const int64_t units = t.units / heads_of(RW, true);
+    if (can && t.heads > 1 && p.k_stride[1] < p.k_stride[2] && share * kStepKeys >= 2048 &&
+        most * kStepKeys > 2048 && units * kMostParts >= t.grid)
+      return launch_walk<D, T, RW, true>(p, t, g, t.grid, cq, cr, st);
+  }
   return launch_walk<D, T, RW, false>(p, t, g, grid, cq, cr, st);
 }
 
@@ -967,7 +997,7 @@ template <int D, class T>
 hipError_t launch_t(const fl_tree_params& p, TreeGeom& g, float cq, float cr, hipStream_t st) {
   const TreePlan t = tree_plan(p);
   g.blocks_of_rows = (g.rows + 32 * t.rw - 1) / (32 * t.rw);
-  g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.most_grid * 32 * t.rw *
+  g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.most_grid * 32 * t.rw * t.heads *
                                                  (D == 64 ? kPartStride : kPartStride128));
   return t.rw == 1   ? launch_rw<D, T, 1>(p, t, g, cq, cr, st)
          : t.rw == 2 ? launch_rw<D, T, 2>(p, t, g, cq, cr, st)
@@ -1004,7 +1034,6 @@ hipError_t launch_tree_fwd(const fl_tree_params& p, void* ws, hipStream_t st) {
   g.lse = p.lse;
   g.batch = (int)p.batch;
   g.heads = (int)p.heads;
-  g.kv_heads = (int)p.kv_heads;
   g.drafts = (int)p.drafts;
   g.group = fast_div((int)(p.heads / p.kv_heads));
   g.by_drafts = fast_div(g.drafts);

@@ -191,3 +191,23 @@ def test_outputs_that_overlap_are_refused(cuda):
     freqs, _ = fl.rotary_frequencies(64, device=cuda)
     with pytest.raises(RuntimeError, match="overlap"):
         fl.forward_rotary(args["q"], None, pos, freqs, q_out=one)
+
+
+@pytest.mark.parametrize("dtype,d", KINDS)
+@pytest.mark.parametrize("b,h,hk,n,lengths,tree", [
+    (2, 8, 8, 1, [3000, 0], None),
+    (1, 16, 16, 1, [2500], None),
+    (5, 8, 4, 3, [100, 0, 1700, 5, 64], "tree"),
+    (3, 12, 12, 20, [7, 600, 0], "any"),
+    (2, 32, 4, 4, [900, 2000], None),
+])
+@pytest.mark.parametrize("rows_first", [True, False])
+def test_heads_side_by_side(cuda, dtype, d, b, h, hk, n, lengths, tree, rows_first):
+    """Long tables of caches whose heads lie side by side, and of others; blocks
+    nobody has and NaN rows among them."""
+    p = Problem(73 + n, dtype, b, h, hk, n, d, 16, lengths, tree, ragged=n > 1, table_pad=ROOM,
+                rows_first=rows_first)
+    p.tables[0, 2] = -1
+    p.k[int(p.tables[0, 3]), hk - 1, 5, 1] = float("nan")   # one head's rows
+    p.v[int(p.tables[0, 4]), 0, 5, 1] = float("inf")
+    check(*run(p, cuda), p)
