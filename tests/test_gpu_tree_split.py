@@ -211,3 +211,51 @@ def test_heads_side_by_side(cuda, dtype, d, b, h, hk, n, lengths, tree, rows_fir
     p.k[int(p.tables[0, 3]), hk - 1, 5, 1] = float("nan")   # one head's rows
     p.v[int(p.tables[0, 4]), 0, 5, 1] = float("inf")
     check(*run(p, cuda), p)
+
+
+@pytest.mark.parametrize("group,n", ROWS)
+def test_less_workspace_runs_one_pass(cuda, group, n):
+    """The C entry with no workspace, one byte too little, and enough; one
+    that is not aligned is refused; the memory behind a workspace stays."""
+    import ctypes
+
+    import torch
+
+    from flashlite_amd import capi
+
+    p = Problem(74 + n, "bfloat16", 2, 4 * group, 4, n, 64, 16, [1800, 40], "tree", table_pad=ROOM)
+    ref = p.reference()
+    a = p.device(cuda)
+    out = torch.zeros_like(a["q"])
+    t3 = ctypes.c_int64 * 3
+    f = capi.FlTreeParams(
+        q=a["q"].data_ptr(), k_cache=a["k_cache"].data_ptr(), v_cache=a["v_cache"].data_ptr(),
+        o=out.data_ptr(), lse=None, q_stride=t3(*a["q"].stride()[:3]),
+        o_stride=t3(*out.stride()[:3]), k_stride=t3(*a["k_cache"].stride()[:3]),
+        v_stride=t3(*a["v_cache"].stride()[:3]), block_tables=a["block_tables"].data_ptr(),
+        table_stride=a["block_tables"].stride(0), lengths=a["lengths"].data_ptr(), counts=None,
+        mask=a["mask"].data_ptr(), mask_stride=a["mask"].stride(0), batch=2, heads=4 * group,
+        kv_heads=4, drafts=n, head_dim=64, num_blocks=a["k_cache"].shape[0], block_size=16,
+        max_blocks=a["block_tables"].shape[1], sm_scale=0.0, dtype=capi.DTYPE_BF16)
+    lib = capi.load()
+    lib.fl_attn_tree_workspace_bytes.restype = ctypes.c_int64
+    need = lib.fl_attn_tree_workspace_bytes(ctypes.byref(f))
+    assert need > 0 and need == fl.tree_workspace_bytes(a["q"], a["k_cache"])
+    ws = torch.full((need + 4096,), 77, dtype=torch.uint8, device=cuda)
+    st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def call(at, size):
+        out.zero_()
+        rc = lib.fl_attn_tree_fwd(ctypes.byref(f), ctypes.c_void_p(at), ctypes.c_int64(size), st)
+        torch.cuda.synchronize()
+        return rc
+
+    for at, size in ((None, 0), (None, need), (ws.data_ptr(), need - 1)):
+        assert call(at, size) == capi.FL_OK
+        check(out, None, p, ref)
+        assert bool((ws == 77).all())
+    assert call(ws.data_ptr() + 4, need) == capi.FL_ERR_MISALIGNED
+    assert bool((out == 0).all())
+    assert call(ws.data_ptr(), need) == capi.FL_OK
+    check(out, None, p, ref)
+    assert bool((ws[need:] == 77).all()) and not bool((ws[:need] == 77).all())
