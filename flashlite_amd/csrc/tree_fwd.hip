@@ -69,6 +69,23 @@ __device__ __forceinline__ typename Elem<T>::v8 finite_only(const typename Elem<
   return __builtin_bit_cast(typename Elem<T>::v8, x);
 }
 
+// Whether one of a tile's V operands is NaN or infinite: the largest of their
+// bits, signs aside.
+template <class T>
+__device__ __forceinline__ bool any_odd(const typename Elem<T>::v8 (&v)[8]) {
+  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+  constexpr uint16_t kExp = __is_same(T, _Float16) ? 0x7C00 : 0x7F80;
+  u16x2_t top = {0, 0};
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const u32x4_t x = __builtin_bit_cast(u32x4_t, v[u]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, x[i] & 0x7FFF7FFFu));
+  }
+  return top[0] >= kExp || top[1] >= kExp;
+}
+
 // Where a lane's operands lie: those of Rows (head dim 64) and Rows128.
 template <int D, class T>
 struct TreeLayout;
@@ -379,6 +396,13 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
     return d0 >= 0 ? x : (d0 > -64 ? x << -d0 : 0) | first_bits(-d0);
   };
 
+  // The keys that every row of this wave sees: the tokens, and in a chain the
+  // drafts up to the first row's.
+  const int open =
+      mask != nullptr
+          ? length
+          : length + min(drafts, divide(min(32 * (RW * rb + rw), g.rows - 1), g.group) + 1);
+
   const uint64_t table = (uint64_t)(uintptr_t)(g.tables + b * g.table_stride);
   const uint64_t kbase = (uint64_t)(uintptr_t)(K + kvh * g.k_head);
   const uint64_t vbase = (uint64_t)(uintptr_t)(V + kvh * g.v_head);
@@ -448,7 +472,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   auto prepare = [&](int i, bool some_bad, typename RowsT::Scores& s)
                      __attribute__((always_inline)) {
     const int k0 = (first + KW * i) * kKeys;
-    checked = k0 + kKeys > length || some_bad;
+    checked = k0 + kKeys > open || some_bad;
     if (checked) {
       seen = seen_bits(k0);
       if (some_bad) seen &= good_keys(i);
@@ -465,18 +489,12 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
   };
   auto output = [&](const uint8_t* vt, V8 (&va)[8], const typename RowsT::Probs& p)
                     __attribute__((always_inline)) {
+    // What p = 0 meets must be finite; a visible NaN or infinity is added to
+    // the rows that see it.
     if (checked) {
-      // What p = 0 meets must be finite; a visible NaN or infinity is added
-      // to the rows that see it.
-      uint32_t odd = 0;
+      if (__builtin_amdgcn_ballot_w64(any_odd<T>(va)) != 0) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const u32x4_t x = __builtin_bit_cast(u32x4_t, va[u]);
-        va[u] = finite_only<T>(va[u]);
-        const u32x4_t y = __builtin_bit_cast(u32x4_t, va[u]) ^ x;
-        odd |= y[0] | y[1] | y[2] | y[3];
-      }
-      if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
+        for (int u = 0; u < 8; ++u) va[u] = finite_only<T>(va[u]);
 #pragma unroll 1
         for (int j = 0; j < kKeys; ++j) {
           const bool sees = (seen >> j) & 1;
