@@ -337,6 +337,16 @@ __device__ __forceinline__ void chunk_coords(int nqb, int nsplit, int xcds, int&
   chunk = c - bh * nsplit;
 }
 
+// 16 bytes a lane from `rs` at byte offset `voff` into LDS at slot + 16 * lane,
+// asynchronously (vmcnt).  A load directly behind the write of M0 may take the
+// old LDS address: one wait state belongs between them, which the compiler
+// does not add before inline assembly.
+__device__ __forceinline__ void load_lds16(const i32x4_t& rs, int voff, const uint8_t* slot) {
+  const uint32_t lds_base = (uint32_t)(uintptr_t)slot;
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               : : "v"(voff), "s"(rs), "{m0}"(lds_base));
+}
+
 // Asynchronous fetch of tile t (clamped to the last tile the work-group
 // needs) straight into LDS with buffer_load_dwordx4 ... lds: each wave moves
 // `kSegs` 1 KiB segments (8 rows); lane i of a segment lands at byte 16*i,
@@ -382,8 +392,7 @@ __device__ __forceinline__ void fetch_tile_z(const i32x4_t& rs, const uint8_t* s
   for (int i = 0; i < kSegs; ++i) {
     const int seg = wave * kSegs + i;
     const int voff = tb + f.lane[i];
-    const uint32_t lds_base = (uint32_t)(uintptr_t)(slot + 1024 * seg);
-    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rs), "{m0}"(lds_base));
+    load_lds16(rs, voff, slot + 1024 * seg);
   }
 }
 
@@ -393,8 +402,7 @@ template <int kSegs>
 __device__ __forceinline__ void fetch_seg(const i32x4_t& rs, const uint8_t* slot, int tb, int i,
                                           int wave, const FetchOff<kSegs>& f) {
   const int voff = tb + f.lane[i];
-  const uint32_t lds_base = (uint32_t)(uintptr_t)(slot + 1024 * (wave * kSegs + i));
-  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rs), "{m0}"(lds_base));
+  load_lds16(rs, voff, slot + 1024 * (wave * kSegs + i));
 }
 
 // The 32 query rows [q, q + 32) of a head (rows >= N_q read as zeros) into
@@ -437,8 +445,7 @@ __device__ __forceinline__ void fetch_tile(const i32x4_t& rs, const uint8_t* slo
   for (int i = 0; i < kSegs; ++i) {
     const int seg = wave * kSegs + i;
     const int voff = tb + f.lane[i];
-    const uint32_t lds_base = (uint32_t)(uintptr_t)(slot + 1024 * seg);
-    asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rs), "{m0}"(lds_base));
+    load_lds16(rs, voff, slot + 1024 * seg);
   }
 }
 

@@ -125,18 +125,10 @@ fa2_fwd_stream_kernel(const T* Q, const T* __restrict__ K, const T* __restrict__
     const i32x4_t rq =
         buffer_rsrc(hp.q + (long long)q0 * geom.q_sr, (valid - 1) * qrow_bytes + kRowBytes);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lds_base = (uint32_t)(uintptr_t)(qdst + 1024 * i);
-      asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(qoff[i]), "s"(rq),
-                   "{m0}"(lds_base));
-    }
+    for (int i = 0; i < 4; ++i) load_lds16(rq, qoff[i], qdst + 1024 * i);
     if (kShare && mate) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t lds_base = (uint32_t)(uintptr_t)(qdst + 4 * 4096 + 1024 * i);
-        asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(qoff2[i]), "s"(rq),
-                     "{m0}"(lds_base));
-      }
+      for (int i = 0; i < 4; ++i) load_lds16(rq, qoff2[i], qdst + 4 * 4096 + 1024 * i);
     }
   };
   auto issue_loads = [&](int u, int b, bool mate) __attribute__((always_inline)) {

@@ -217,14 +217,17 @@ struct TreeRows : TreeLayout<D, T>::type {
 
 // 16 (or 4) bytes a lane from a 64-bit address of its own into LDS at
 // base + 16 (4) * lane, asynchronously (vmcnt).  Inline assembly, so that the
-// compiler does not guard reads of other slots with waits on it.
+// compiler does not guard reads of other slots with waits on it.  The wait state
+// before the load is the one that it needs behind the write of M0 (load_lds16).
 __device__ __forceinline__ void fetch16(uint64_t address, const void* lds) {
   const uint32_t base = (uint32_t)(uintptr_t)lds;
-  asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(address), "{m0}"(base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               : : "v"(address), "{m0}"(base) : "memory");
 }
 __device__ __forceinline__ void fetch4(uint64_t address, const void* lds) {
   const uint32_t base = (uint32_t)(uintptr_t)lds;
-  asm volatile("global_load_lds_dword %0, off" : : "v"(address), "{m0}"(base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off"
+               : : "v"(address), "{m0}"(base) : "memory");
 }
 
 // Waves of a work-group of RW row blocks, and slots for tiles of each of its
