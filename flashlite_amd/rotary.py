@@ -48,8 +48,9 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, method: str | None =
         def pair(turns):  # the (fractional) pair that turns so often over `trained` positions
             return rot_dim * math.log(trained / (2 * math.pi * turns)) / (2 * math.log(base))
 
+        # (the ramp may end past the last pair, which then is not divided in full)
         lo = max(math.floor(pair(fast)), 0)
-        hi = min(math.ceil(pair(slow)), rot_dim // 2 - 1)
+        hi = min(math.ceil(pair(slow)), rot_dim - 1)
         ramp = ((j - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
         freqs = freqs * (1.0 - ramp) + freqs / factor * ramp
         scale = 0.1 * math.log(factor) + 1.0
