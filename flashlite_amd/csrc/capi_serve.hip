@@ -1,8 +1,10 @@
 // C-ABI entry points of the paged-cache operators: argument checks and the
 // launch.  No counterpart in the reference.
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <utility>
 
 #include "fl_serve.h"
 
@@ -35,12 +37,21 @@ int check_view(const int64_t st[3], int64_t unit, const char* name, const char* 
   return FL_OK;
 }
 
-// Rows that are written: no two in one place.
-int check_apart(const int64_t st[3], int64_t n0, int64_t n1, int64_t n2, const char* name,
-                const char* who) {
-  if ((n0 > 1 && st[0] == 0) || (n1 > 1 && st[1] == 0) || (n2 > 1 && st[2] == 0))
-    return set_error(FL_ERR_INVALID_ARGUMENT, "%s: %s is written, its rows must not overlap", who,
-                     name);
+// Rows of head_dim columns that are written: no two may share a place.  The
+// dimensions must nest: each stride reaches past everything that the smaller
+// ones span.
+int check_apart(const int64_t st[3], int64_t n0, int64_t n1, int64_t n2, int64_t head_dim,
+                const char* name, const char* who) {
+  std::pair<int64_t, int64_t> dim[3] = {{st[0], n0}, {st[1], n1}, {st[2], n2}};
+  std::sort(dim, dim + 3);
+  __int128 span = head_dim;
+  for (const auto& [stride, n] : dim) {
+    if (n <= 1) continue;
+    if (stride < span)
+      return set_error(FL_ERR_INVALID_ARGUMENT, "%s: %s is written, its rows must not overlap", who,
+                       name);
+    span += (__int128)stride * (n - 1);
+  }
   return FL_OK;
 }
 
@@ -80,9 +91,10 @@ int check_rotary(const fl_rotary_params* p, bool cache, const char* who) {
   if (rc == FL_OK) rc = check_view(p->q_out_stride, unit, "q_out", who);
   if (rc == FL_OK && p->k) rc = check_view(p->k_stride, unit, "k", who);
   if (rc == FL_OK && p->k && !cache) rc = check_view(p->k_out_stride, unit, "k_out", who);
-  if (rc == FL_OK) rc = check_apart(p->q_out_stride, p->batch, p->heads, p->rows, "q_out", who);
+  if (rc == FL_OK)
+    rc = check_apart(p->q_out_stride, p->batch, p->heads, p->rows, p->head_dim, "q_out", who);
   if (rc == FL_OK && p->k && !cache)
-    rc = check_apart(p->k_out_stride, p->batch, p->kv_heads, p->rows, "k_out", who);
+    rc = check_apart(p->k_out_stride, p->batch, p->kv_heads, p->rows, p->head_dim, "k_out", who);
   return rc;
 }
 
@@ -233,9 +245,11 @@ int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, voi
   if (rc == FL_OK) rc = check_view(c->k_cache_stride, 8, "k_cache", who);
   if (rc == FL_OK) rc = check_view(c->v_cache_stride, 8, "v_cache", who);
   if (rc == FL_OK)
-    rc = check_apart(c->k_cache_stride, c->num_blocks, p->kv_heads, c->block_size, "k_cache", who);
+    rc = check_apart(c->k_cache_stride, c->num_blocks, p->kv_heads, c->block_size, p->head_dim,
+                     "k_cache", who);
   if (rc == FL_OK)
-    rc = check_apart(c->v_cache_stride, c->num_blocks, p->kv_heads, c->block_size, "v_cache", who);
+    rc = check_apart(c->v_cache_stride, c->num_blocks, p->kv_heads, c->block_size, p->head_dim,
+                     "v_cache", who);
   if (rc != FL_OK) return rc;
   if (p->batch == 0 || p->rows == 0 || p->heads + p->kv_heads == 0) return FL_OK;
   if (!p->k || !c->v || !c->k_cache || !c->v_cache || !c->slots)
@@ -270,7 +284,8 @@ int fl_attn_tree_fwd(const fl_tree_params* p, void* workspace, int64_t workspace
       !aligned(p->lse, 4) || !aligned(p->mask, 8))
     return set_error(FL_ERR_MISALIGNED,
                      "%s: block_tables, lengths, counts and lse must be 4-byte aligned, mask 8", who);
-  const int apart = check_apart(p->o_stride, p->batch, p->heads, p->drafts, "o", who);
+  const int apart =
+      check_apart(p->o_stride, p->batch, p->heads, p->drafts, p->head_dim, "o", who);
   if (apart != FL_OK) return apart;
   const int64_t need = fl::tree_workspace_bytes(*p);
   void* const ws = need > 0 && workspace_bytes >= need ? workspace : nullptr;

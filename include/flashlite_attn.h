@@ -218,6 +218,8 @@ int64_t fl_attn_splitkv_noalloc_bytes(const fl_attn_params_ex* p, int32_t num_sp
  * dim] passes as its transpose).  Token t of request b lies in row
  * t % block_size of block block_tables[b][t / block_size]; its slot is
  * block * block_size + row.  A cache that is not paged is one block a request.
+ * Rows that a call writes must not overlap: a written view's strides nest, each
+ * at least what the smaller ones span (views of dense memory do).
  */
 
 /*

@@ -1,0 +1,83 @@
+"""Strides of the paged-cache operators' arguments at the C ABI: which written
+views overlap.  No call here reaches a launch (fake addresses, and a refusal
+that comes after the check of strides)."""
+
+import ctypes
+
+import pytest
+
+from flashlite_amd import capi
+
+A = 0x7F0000000000
+T3, T2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
+D = 64
+
+# {batch, head, row} strides of 2 x 4 x 5 rows of 64 columns, and whether two rows meet
+VIEWS = [
+    ((1280, 320, 64), False),       # contiguous
+    ((1280, 64, 256), False),       # a token's heads side by side
+    ((64, 640, 128), False),        # batches innermost
+    ((1 << 40, 1 << 20, 4096), False),
+    ((1280, 320, 8), True),         # rows closer together than their columns
+    ((1280, 320, 56), True),
+    ((1280, 312, 64), True),        # a head begins in the last one's last row
+    ((1272, 64, 256), True),
+    ((1280, 8, 256), True),
+    ((1280, 320, 320), True),       # two dimensions of one stride
+    ((1280, 64, 192), True),        # a token's heads reach into the next one's
+    ((1280, 320, 0), True),
+]
+
+
+def tree_call(o):
+    q = T3(1280, 320, 64)
+    kv = T3(2 * 16 * D, 16 * D, D)
+    p = capi.FlTreeParams(
+        q=A, k_cache=A, v_cache=A, o=A, lse=0, q_stride=q, o_stride=T3(*o), k_stride=kv,
+        v_stride=kv, block_tables=A, table_stride=20, lengths=A, batch=2, heads=4, kv_heads=2,
+        drafts=5, head_dim=D, num_blocks=70, block_size=16, max_blocks=20, dtype=capi.DTYPE_F16)
+    # (a workspace that is not aligned is refused last)
+    return capi.load().fl_attn_tree_fwd(ctypes.byref(p), A + 4, 1 << 40, None), "workspace"
+
+
+def rotary_call(name, st):
+    views = dict.fromkeys(("q_stride", "k_stride", "q_out_stride", "k_out_stride"),
+                          T3(1280, 320, 64))
+    views[name] = T3(*st)
+    p = capi.FlRotaryParams(q=A, k=A, q_out=A, k_out=A, positions=A, position_stride=T2(5, 1),
+                            position_bits=32, dtype=capi.DTYPE_F16, freqs=A + 4, pairs=32, batch=2,
+                            heads=4, kv_heads=4, rows=5, head_dim=D, scale=1.0, **views)
+    return capi.load().fl_attn_rotary(ctypes.byref(p), None), "freqs"
+
+
+def cache_call(name, st):
+    v = T3(1280, 320, 64)
+    p = capi.FlRotaryParams(q=A, k=A, q_out=A, q_stride=v, k_stride=v, q_out_stride=v,
+                            positions=A, position_stride=T2(5, 1), position_bits=32,
+                            dtype=capi.DTYPE_F16, freqs=A, pairs=32, batch=2, heads=4, kv_heads=4,
+                            rows=5, head_dim=D, scale=1.0)
+    views = dict.fromkeys(("k_cache_stride", "v_cache_stride"), v)
+    views[name] = T3(*st)
+    c = capi.FlCacheStore(v=A, v_stride=v, k_cache=A, v_cache=A, num_blocks=2, block_size=5,
+                          slots=A + 4, slot_stride=T2(5, 1), **views)
+    return capi.load().fl_attn_rotary_cache(ctypes.byref(p), ctypes.byref(c), None), "slots"
+
+
+CALLS = {
+    "o": tree_call,
+    "q_out": lambda st: rotary_call("q_out_stride", st),
+    "k_out": lambda st: rotary_call("k_out_stride", st),
+    "k_cache": lambda st: cache_call("k_cache_stride", st),
+    "v_cache": lambda st: cache_call("v_cache_stride", st),
+}
+
+
+@pytest.mark.parametrize("what", CALLS)
+@pytest.mark.parametrize("strides,overlap", VIEWS)
+def test_written_rows_do_not_overlap(what, strides, overlap):
+    rc, later = CALLS[what](strides)
+    if overlap:
+        assert rc == capi.FL_ERR_INVALID_ARGUMENT
+        assert f"{what} is written, its rows must not overlap" in capi.last_error()
+    else:
+        assert rc == capi.FL_ERR_MISALIGNED and later in capi.last_error()
