@@ -40,10 +40,11 @@ struct TreeGeom {
   int batch, heads, kv_units, drafts, rows, words, blocks_of_rows;
   int num_blocks, capacity;  // capacity: keys of a table row
   FastDiv block, group, by_drafts;
-  // split launches: partial results [2 * grid][32 RW][kPartStride], and per
-  // unit where they begin and end
+  // split launches: partial results, part_size floats each ([heads side by side]
+  // [part_rows][kPartStride]), and per unit where they begin and end
   float* part;
   int2* parts;
+  int part_rows, part_size;
   int xcds;
 };
 
@@ -361,7 +362,7 @@ __device__ __forceinline__ void walk(const T* Q, const uint8_t* K, const uint8_t
 
   RowsT rows;
   rows.start(lane, cr);
-  const int local = 32 * (rw + hw) + rows.col;  // (one of them is 0)
+  const int local = 32 * rw + g.part_rows * hw + rows.col;  // (of the unit's rows in a part)
   const int row = 32 * (RW * rb + rw) + rows.col;
   const int my_row = min(row, g.rows - 1);
   const int draft = divide(my_row, g.group);
@@ -731,7 +732,6 @@ __global__ void __launch_bounds__(64 * waves_of(RW), 2)
 tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const TreeGeom g, float cq,
                   float cr) {
   constexpr int kHeads = heads_of(RW, DEEP);
-  constexpr int kPart = D == 64 ? kPartStride : kPartStride128;
   __shared__ __attribute__((aligned(16))) Shared<D, RW, DEEP> sh;
   const int lane = threadIdx.x & 63;
   // Cost of one key/value head of requests b0 .. b0 + 63, one a lane.
@@ -802,7 +802,7 @@ tree_split_kernel(const T* Q, const uint8_t* K, const uint8_t* V, T* O, const Tr
         if (s1 == steps) where->y = x;
       }
       float* const part =
-          s0 == 0 && s1 == steps ? nullptr : g.part + (long long)slot * (32 * RW * kHeads) * kPart;
+          s0 == 0 && s1 == steps ? nullptr : g.part + (long long)slot * g.part_size;
       walk<D, T, RW, DEEP>(Q, K, V, O, g, sh, b, kvh * kHeads, rb, r, s0, s1, part, cq, cr);
       slot = 2 * x + 1;
     }
@@ -845,9 +845,9 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g)
   const int x0 = parts.x >> 1, n = parts.y - x0 + 1;
   if (n == 1) return;  // one work-group had all of it
   const float* const base =
-      g.part + (long long)(row - rb * 32 * RW + kvh % HEADS * 32) * kPart;
+      g.part + (long long)(row - rb * 32 * RW + kvh % HEADS * g.part_rows) * kPart;
   auto at = [&](int j) __attribute__((always_inline)) {
-    return base + (long long)(j == 0 ? parts.x : 2 * (x0 + j)) * (32 * RW * HEADS) * kPart;
+    return base + (long long)(j == 0 ? parts.x : 2 * (x0 + j)) * g.part_size;
   };
   float acc[kCols] = {}, l = 0.0f, mx = ninf();
 #pragma unroll 1
@@ -913,12 +913,15 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g)
 // us with 256 parts, 17.0 with 64, 18.6 with 32, 25.0 with 16; 64 drafts there
 // (f16) 39.9, 35.7, 45.4 and 69.9.
 constexpr int kMostParts = 64;
+// Floats of a cache line, on which a partial result begins.
+constexpr int kPartUnit = 32;
 
 struct TreePlan {
   int rw, units, grid;
-  int most_grid, heads;  // what the workspace has room for: work-groups, heads of each
+  int most_grid, heads;  // what the workspace has room for: work-groups, heads of each;
+  int part_rows, part_size;  // rows of each, floats of a partial result
   bool split;
-  int64_t bytes;
+  int64_t parts_at, bytes;
 };
 
 TreePlan tree_plan(const fl_tree_params& p) {
@@ -931,12 +934,15 @@ TreePlan tree_plan(const fl_tree_params& p) {
   t.most_grid = t.rw == 2 && p.head_dim == 64
                     ? (int)std::min<int64_t>(2 * device_cus(), (int64_t)kMostParts * t.units)
                     : t.grid;
-  t.heads = t.rw == 1 && p.kv_heads % heads_of(1, true) == 0 ? heads_of(1, true) : 1;
+  t.heads = t.rw == 1 && p.kv_heads % heads_of(1, true) == 0 && p.k_stride[1] < p.k_stride[2]
+                ? heads_of(1, true)
+                : 1;
+  t.part_rows = (int)std::min<int64_t>(rows, 32 * t.rw);
   t.split = t.units < 2 * t.grid || t.heads > 1;
   const int64_t part = p.head_dim == 64 ? kPartStride : kPartStride128;
-  t.bytes = t.split ? 2LL * t.most_grid * 32 * t.rw * t.heads * part * (int64_t)sizeof(float) +
-                          t.units * (int64_t)sizeof(int2)
-                    : 0;
+  t.part_size = (int)((t.part_rows * t.heads * part + kPartUnit - 1) / kPartUnit * kPartUnit);
+  t.parts_at = 2LL * t.most_grid * t.part_size * (int64_t)sizeof(float);
+  t.bytes = t.split ? t.parts_at + t.units * (int64_t)sizeof(int2) : 0;
   return t;
 }
 
@@ -1018,8 +1024,8 @@ hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, fl
   // each (1 of 64000: 39.2 against 36.3).
   if constexpr (RW == 1) {
     const int64_t units = t.units / heads_of(RW, true);
-    if (can && t.heads > 1 && p.k_stride[1] < p.k_stride[2] && share * kStepKeys >= 2048 &&
-        most * kStepKeys > 2048 && units * kMostParts >= t.grid)
+    if (can && t.heads > 1 && share * kStepKeys >= 2048 && most * kStepKeys > 2048 &&
+        units * kMostParts >= t.grid)
       return launch_walk<D, T, RW, true>(p, t, g, t.grid, cq, cr, st);
   }
   return launch_walk<D, T, RW, false>(p, t, g, grid, cq, cr, st);
@@ -1029,8 +1035,9 @@ template <int D, class T>
 hipError_t launch_t(const fl_tree_params& p, TreeGeom& g, float cq, float cr, hipStream_t st) {
   const TreePlan t = tree_plan(p);
   g.blocks_of_rows = (g.rows + 32 * t.rw - 1) / (32 * t.rw);
-  g.parts = reinterpret_cast<int2*>(g.part + 2LL * t.most_grid * 32 * t.rw * t.heads *
-                                                 (D == 64 ? kPartStride : kPartStride128));
+  g.part_rows = t.part_rows;
+  g.part_size = t.part_size;
+  g.parts = reinterpret_cast<int2*>(reinterpret_cast<uint8_t*>(g.part) + t.parts_at);
   return t.rw == 1   ? launch_rw<D, T, 1>(p, t, g, cq, cr, st)
          : t.rw == 2 ? launch_rw<D, T, 2>(p, t, g, cq, cr, st)
          : t.rw == 4 ? launch_rw<D, T, 4>(p, t, g, cq, cr, st)

@@ -376,7 +376,8 @@ int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, voi
  * elements.
  *
  * Few query rows over many keys are split over the CUs; partial results go to
- * `workspace` (fl_attn_tree_workspace_bytes, from the sizes alone; 0: none
+ * `workspace` (fl_attn_tree_workspace_bytes, from the sizes and whether heads
+ * or rows are closer together in k_cache; 0: none
  * is used, -1: `p` is rejected) and a second kernel merges them.  With less
  * (or NULL) the call runs without.  The workspace is 16-byte aligned device
  * memory that needs no initial values; calls that may overlap must not share
