@@ -2,8 +2,9 @@
 // stores rotated k and v in a paged cache (fl_attn_rotary, fl_attn_rotary_cache).
 //
 // Bound by memory: a row is read and written once (B1 H16/16 N16384 D 128
-// fp16 5.5-6.2 TB/s, into a cache B4 H32/8 N4096 5.4); small calls by their
-// launch.  A thread owns V pairs of
+// fp16 5.5-6.2 TB/s, fp32 5.3, into a cache B4 H32/8 N4096 5.4); small calls by
+// their launch, and in fp32 by 64-bit sines (B2 H8/8 N1999 D 64 7.4 us, 6.9 with
+// the hardware's, which are not exact enough for it).  A thread owns V pairs of
 // one token and walks a few heads with their sines and cosines in registers,
 // the loads of four heads at a time in flight.
 
@@ -35,6 +36,7 @@ struct RotaryGeom {
   uint32_t tokens;  // batch * rows
   int heads_per_thread, across_log2;
   float scale, sign;
+  double scale64;
   FastDiv rows, block;
 };
 
@@ -120,13 +122,22 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryGeom g) {
       const int pair = !INTER ? j * V + e
                        : V == 1 ? j
                                 : (e < V / 2 ? c0 / 2 + e : c1 / 2 + e - V / 2);
-      // Turns in 64 bits, reduced to [-1/2, 1/2] before the rounding to 32:
-      // far positions lose nothing.  The hardware's sine and cosine take turns
-      // and are off by at most 1.24e-7 there (measured over 2^20 points).
+      // Turns in 64 bits, reduced to [-1/2, 1/2], so that far positions keep
+      // what 64 bits have of them.  16-bit rows take the hardware's sine and
+      // cosine of the turns in 32 bits: at most 2^-22 off, of a half step of
+      // 2^-11 or more.  32-bit rows round the scaled sine and cosine once from
+      // 64 bits.
       double t = position * (g.freqs[pair] * 0.15915494309189533577);
       t -= rint(t);
-      cs[e] = g.scale * __builtin_amdgcn_cosf((float)t);
-      sn[e] = g.scale * g.sign * __builtin_amdgcn_sinf((float)t);
+      if constexpr (sizeof(T) == 4) {
+        double s64, c64;
+        sincospi(2.0 * t, &s64, &c64);
+        cs[e] = (float)(g.scale64 * c64);
+        sn[e] = g.sign * (float)(g.scale64 * s64);
+      } else {
+        cs[e] = g.scale * __builtin_amdgcn_cosf((float)t);
+        sn[e] = g.scale * g.sign * __builtin_amdgcn_sinf((float)t);
+      }
     }
   }
   for (;;) {
@@ -247,6 +258,7 @@ hipError_t launch_rotary(const fl_rotary_params& p, const fl_cache_store* c, hip
   g.tokens = (uint32_t)(p.batch * p.rows);
   g.rows = fast_div((int)p.rows);
   g.scale = (float)p.scale;
+  g.scale64 = p.scale;
   g.sign = p.transpose ? -1.0f : 1.0f;
   const bool inter = p.interleaved != 0;
   const int d = (int)p.head_dim;
