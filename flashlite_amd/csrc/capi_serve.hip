@@ -25,11 +25,13 @@ bool fits32(int64_t x) { return x >= 0 && x <= INT32_MAX; }
 
 bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
-// Strides of a [.., .., rows, head_dim] view: non-negative, and rows of whole
-// 16-byte pieces.
-int check_view(const int64_t st[3], int64_t unit, const char* name, const char* who) {
+// Strides of an [n0, n1, n2, head_dim] view: non-negative, and rows of whole
+// 16-byte pieces.  (Those of one entry step nowhere.)
+int check_view(const int64_t st[3], int64_t n0, int64_t n1, int64_t n2, int64_t unit,
+               const char* name, const char* who) {
+  const int64_t n[3] = {n0, n1, n2};
   for (int i = 0; i < 3; ++i)
-    if (st[i] < 0 || st[i] % unit != 0)
+    if (n[i] > 1 && (st[i] < 0 || st[i] % unit != 0))
       return set_error(FL_ERR_UNSUPPORTED,
                        "%s: %s strides must be non-negative multiples of %lld elements (got %lld, "
                        "%lld, %lld)", who, name, (long long)unit, (long long)st[0],
@@ -87,10 +89,13 @@ int check_rotary(const fl_rotary_params* p, bool cache, const char* who) {
     return set_error(FL_ERR_UNSUPPORTED, "%s: batch * rows must be below 2^26 and heads at most "
                      "16384", who);
   const int64_t unit = p->dtype == FL_DTYPE_F32 ? 4 : 8;
-  int rc = check_view(p->q_stride, unit, "q", who);
-  if (rc == FL_OK) rc = check_view(p->q_out_stride, unit, "q_out", who);
-  if (rc == FL_OK && p->k) rc = check_view(p->k_stride, unit, "k", who);
-  if (rc == FL_OK && p->k && !cache) rc = check_view(p->k_out_stride, unit, "k_out", who);
+  auto view = [&](const int64_t st[3], int64_t heads, const char* name) {
+    return check_view(st, p->batch, heads, p->rows, unit, name, who);
+  };
+  int rc = view(p->q_stride, p->heads, "q");
+  if (rc == FL_OK) rc = view(p->q_out_stride, p->heads, "q_out");
+  if (rc == FL_OK && p->k) rc = view(p->k_stride, p->kv_heads, "k");
+  if (rc == FL_OK && p->k && !cache) rc = view(p->k_out_stride, p->kv_heads, "k_out");
   if (rc == FL_OK)
     rc = check_apart(p->q_out_stride, p->batch, p->heads, p->rows, p->head_dim, "q_out", who);
   if (rc == FL_OK && p->k && !cache)
@@ -150,14 +155,21 @@ int check_tree(const fl_tree_params* p, const char* who) {
                      (long long)p->table_stride, (long long)p->max_blocks);
   if (p->mask_stride < 0)
     return set_error(FL_ERR_INVALID_ARGUMENT, "%s: mask_stride must be non-negative", who);
-  rc = check_view(p->q_stride, 8, "q", who);
-  if (rc == FL_OK) rc = check_view(p->o_stride, 8, "o", who);
-  if (rc == FL_OK) rc = check_view(p->k_stride, 8, "k_cache", who);
-  if (rc == FL_OK) rc = check_view(p->v_stride, 8, "v_cache", who);
+  auto view = [&](const int64_t st[3], const char* name) {
+    return check_view(st, p->batch, p->heads, p->drafts, 8, name, who);
+  };
+  auto cache = [&](const int64_t st[3], const char* name) {
+    return check_view(st, p->num_blocks, p->kv_heads, p->block_size, 8, name, who);
+  };
+  rc = view(p->q_stride, "q");
+  if (rc == FL_OK) rc = view(p->o_stride, "o");
+  if (rc == FL_OK) rc = cache(p->k_stride, "k_cache");
+  if (rc == FL_OK) rc = cache(p->v_stride, "v_cache");
   if (rc != FL_OK) return rc;
   // Rows are found by 32-bit block and row strides in bytes.
   for (int i = 0; i < 3; i += 2)
-    if (p->k_stride[i] > INT32_MAX || p->v_stride[i] > INT32_MAX)
+    if ((i == 0 ? p->num_blocks : p->block_size) > 1 &&
+        (p->k_stride[i] > INT32_MAX || p->v_stride[i] > INT32_MAX))
       return set_error(FL_ERR_UNSUPPORTED,
                        "%s: block and row strides of the caches must be below 2^31 elements", who);
   return FL_OK;
@@ -241,9 +253,12 @@ int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, voi
   if (p->transpose)
     return set_error(FL_ERR_INVALID_ARGUMENT, "%s: transpose is not for a cache", who);
   rc = check_pages(c->num_blocks, c->block_size, who);
-  if (rc == FL_OK) rc = check_view(c->v_stride, 8, "v", who);
-  if (rc == FL_OK) rc = check_view(c->k_cache_stride, 8, "k_cache", who);
-  if (rc == FL_OK) rc = check_view(c->v_cache_stride, 8, "v_cache", who);
+  if (rc == FL_OK) rc = check_view(c->v_stride, p->batch, p->kv_heads, p->rows, 8, "v", who);
+  auto cache = [&](const int64_t st[3], const char* name) {
+    return check_view(st, c->num_blocks, p->kv_heads, c->block_size, 8, name, who);
+  };
+  if (rc == FL_OK) rc = cache(c->k_cache_stride, "k_cache");
+  if (rc == FL_OK) rc = cache(c->v_cache_stride, "v_cache");
   if (rc == FL_OK)
     rc = check_apart(c->k_cache_stride, c->num_blocks, p->kv_heads, c->block_size, p->head_dim,
                      "k_cache", who);

@@ -81,3 +81,40 @@ def test_written_rows_do_not_overlap(what, strides, overlap):
         assert f"{what} is written, its rows must not overlap" in capi.last_error()
     else:
         assert rc == capi.FL_ERR_MISALIGNED and later in capi.last_error()
+
+
+# --- dimensions of one entry -------------------------------------------------
+# Their strides step nowhere, and torch leaves any number there.
+
+ODD = (1, 12, -8, 1 << 40)
+
+
+@pytest.mark.parametrize("stride", ODD)
+@pytest.mark.parametrize("dim,sizes", [(0, (1, 4, 5)), (1, (2, 1, 5)), (2, (2, 4, 1))])
+def test_strides_of_one_entry_are_not_looked_at(stride, dim, sizes):
+    b, h, n = sizes
+    st = [h * n * D, n * D, D]
+    st[dim] = stride
+    st = T3(*st)
+    p = capi.FlRotaryParams(q=A, k=A, q_out=A, k_out=A, q_stride=st, k_stride=st, q_out_stride=st,
+                            k_out_stride=st, positions=A, position_stride=T2(5, 1),
+                            position_bits=32, dtype=capi.DTYPE_F16, freqs=A + 4, pairs=32, batch=b,
+                            heads=h, kv_heads=h, rows=n, head_dim=D, scale=1.0)
+    lib = capi.load()
+    assert lib.fl_attn_rotary(ctypes.byref(p), None) == capi.FL_ERR_MISALIGNED
+    assert "freqs" in capi.last_error()
+    # a cache of b blocks of n rows
+    c = capi.FlCacheStore(v=A, v_stride=st, k_cache=A, v_cache=A, k_cache_stride=st,
+                          v_cache_stride=st, num_blocks=b, block_size=n, slots=A + 4,
+                          slot_stride=T2(5, 1))
+    p.freqs = A
+    assert lib.fl_attn_rotary_cache(ctypes.byref(p), ctypes.byref(c), None) == \
+        capi.FL_ERR_MISALIGNED
+    assert "slots" in capi.last_error()
+    t = capi.FlTreeParams(
+        q=A, k_cache=A, v_cache=A, o=A, q_stride=st, o_stride=st, k_stride=st, v_stride=st,
+        block_tables=A, table_stride=20, lengths=A, batch=b, heads=h, kv_heads=h, drafts=n,
+        head_dim=D, num_blocks=b, block_size=n, max_blocks=20, dtype=capi.DTYPE_F16)
+    assert lib.fl_attn_tree_workspace_bytes(ctypes.byref(t)) > 0
+    assert lib.fl_attn_tree_fwd(ctypes.byref(t), A + 4, 1 << 40, None) == capi.FL_ERR_MISALIGNED
+    assert "workspace" in capi.last_error()
