@@ -203,6 +203,13 @@ int fl_attn_cache_plan(const fl_cache_plan_params* p, void* stream) {
                        (p->max_blocks > 0 && !p->block_tables) ||
                        (p->width > 0 && (!p->positions || !p->slots))))
     return set_error(FL_ERR_INVALID_ARGUMENT, "%s: the requests' pointers must be non-NULL", who);
+  // (work-groups read the old ones while others write the new)
+  auto meet = [](const int32_t* x, const int32_t* y, int64_t n) {
+    return x != y && (uintptr_t)x < (uintptr_t)y + 4 * n && (uintptr_t)y < (uintptr_t)x + 4 * n;
+  };
+  if (meet(p->held, p->held_out, p->batch) || meet(p->free_state, p->free_state_out, 2))
+    return set_error(FL_ERR_INVALID_ARGUMENT,
+                     "%s: held_out and free_state_out must be in place or apart", who);
   const void* const four[] = {p->lengths, p->counts, p->block_tables, p->held, p->held_out,
                               p->free_blocks, p->free_state, p->free_state_out, p->positions,
                               p->info};

@@ -237,7 +237,7 @@ int64_t fl_attn_splitkv_noalloc_bytes(const fl_attn_params_ex* p, int32_t num_sp
  * has no room for is dropped).
  *
  * Outputs: block_tables (entries of the blocks taken), held_out and
- * free_state_out (each may be its input), positions [batch, width] =
+ * free_state_out (each its input, or apart from it), positions [batch, width] =
  * lengths[b] + i, slots [batch, width], both -1 where there is no token (i >=
  * counts[b], a request not served, a negative table entry), and info [batch,
  * 4]: {0 served, 1 not enough free blocks, 2 the table row is too short;
