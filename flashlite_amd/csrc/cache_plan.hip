@@ -15,17 +15,6 @@ namespace fl {
 
 namespace {
 
-// Inclusive sum over a wave's lanes: within rows of 16, then over the rows.
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);  // row_shr:2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);  // row_shr:4
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);  // row_shr:8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // row_bcast:15
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);  // row_bcast:31
-  return x;
-}
-
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 
 // Exclusive sums of two values over the work-group, and their totals.
@@ -68,10 +57,6 @@ struct PlanGeom {
   int batch, width, max_blocks, pool;
   FastDiv block, by_width;
 };
-
-__device__ __forceinline__ int divide(int n, const FastDiv& f) {
-  return (int)((__umulhi(f.mul, (uint32_t)n) + (uint32_t)n) >> f.shift);
-}
 
 // Request b's blocks: what it holds, and what its length with its new tokens
 // needs.

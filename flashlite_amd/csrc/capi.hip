@@ -26,14 +26,6 @@ namespace {
 
 thread_local char g_err[512] = "";
 
-int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return code;
-}
-
 }  // namespace
 
 int fl::set_error(int code, const char* fmt, ...) {
@@ -45,6 +37,8 @@ int fl::set_error(int code, const char* fmt, ...) {
 }
 
 namespace {
+
+constexpr auto& fail = fl::set_error;
 
 // float(log2 e) widened to double, as the reference multiplies a double
 // sm_scale by its float LOG2_E constant (kernel_flash2.cu:16, :772).

@@ -27,6 +27,21 @@ inline FastDiv fast_div(int d) {
   return f;
 }
 
+__device__ __forceinline__ int divide(int n, const FastDiv& f) {
+  return (int)((__umulhi(f.mul, (uint32_t)n) + (uint32_t)n) >> f.shift);
+}
+
+// Inclusive sum over a wave's lanes: within rows of 16, then over the rows.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);  // row_bcast:31
+  return x;
+}
+
 hipError_t launch_cache_plan(const fl_cache_plan_params& p, hipStream_t stream);  // cache_plan.hip
 hipError_t launch_tree_plan(const fl_tree_plan_params& p, hipStream_t stream);    // cache_plan.hip
 

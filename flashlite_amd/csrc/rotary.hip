@@ -62,14 +62,14 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryGeom g) {
   const int j = (int)(x % kThreads);
   const int across = 1 << g.across_log2;  // heads side by side
   if (token >= g.tokens) return;
-  const int b = (int)((__umulhi(g.rows.mul, token) + token) >> g.rows.shift);
+  const int b = divide((int)token, g.rows);
   const int i = (int)token - b * g.rows.d;
   long long blk = b, row = i;  // where k (and v) go
   if constexpr (CACHE) {
     const long long slot = g.slots[b * g.slot_sb + i * g.slot_sr];
     if (slot < 0 || slot >= g.num_slots) return;
     if (((uint64_t)slot >> 31) == 0)
-      blk = (long long)((__umulhi(g.block.mul, (uint32_t)slot) + (uint32_t)slot) >> g.block.shift);
+      blk = divide((int)slot, g.block);
     else
       blk = slot / g.block.d;
     row = slot - blk * g.block.d;

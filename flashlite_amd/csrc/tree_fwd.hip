@@ -48,10 +48,6 @@ struct TreeGeom {
   int xcds;
 };
 
-__device__ __forceinline__ int divide(int n, const FastDiv& f) {
-  return (int)((__umulhi(f.mul, (uint32_t)n) + (uint32_t)n) >> f.shift);
-}
-
 // The first n of 64 bits.
 __device__ __forceinline__ uint64_t first_bits(int n) {
   return n <= 0 ? 0 : n >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << n) - 1;
@@ -293,17 +289,6 @@ __device__ __forceinline__ uint64_t uniform(uint64_t x) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x);
   const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32));
   return (uint64_t)hi << 32 | lo;
-}
-
-// Inclusive sum over a wave's lanes: within rows of 16, then over the rows.
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);  // row_shr:2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);  // row_shr:4
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);  // row_shr:8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // row_bcast:15
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);  // row_bcast:31
-  return x;
 }
 
 // The work-group's LDS: key and value tiles, and per wave the row addresses of
