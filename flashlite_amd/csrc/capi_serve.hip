@@ -104,7 +104,9 @@ int check_rotary(const fl_rotary_params* p, bool cache, const char* who) {
 }
 
 int check_rotary_pointers(const fl_rotary_params* p, bool cache, const char* who) {
-  if (!p->q || !p->q_out || (!cache && p->k && !p->k_out) ||
+  // (what has no heads has no memory)
+  if ((p->heads > 0 && (!p->q || !p->q_out)) ||
+      (!cache && p->k && p->kv_heads > 0 && !p->k_out) ||
       (p->pairs > 0 && (!p->positions || !p->freqs)))
     return set_error(FL_ERR_INVALID_ARGUMENT,
                      "%s: q, the outputs, positions and freqs must be non-NULL", who);
@@ -274,7 +276,7 @@ int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, voi
                      "v_cache", who);
   if (rc != FL_OK) return rc;
   if (p->batch == 0 || p->rows == 0 || p->heads + p->kv_heads == 0) return FL_OK;
-  if (!p->k || !c->v || !c->k_cache || !c->v_cache || !c->slots)
+  if (!c->slots || (p->kv_heads > 0 && (!p->k || !c->v || !c->k_cache || !c->v_cache)))
     return set_error(FL_ERR_INVALID_ARGUMENT, "%s: k, v, the caches and slots must be non-NULL", who);
   rc = check_rotary_pointers(p, true, who);
   if (rc != FL_OK) return rc;

@@ -190,8 +190,9 @@ void launch_unroll(const RotaryGeom& g, bool inter, dim3 grid, hipStream_t strea
 template <class T, bool CACHE, int D, int V>
 void launch(RotaryGeom& g, bool inter, hipStream_t stream) {
   const int total = g.heads + g.kv_heads * (CACHE ? 2 : 1);
+  const long long* const st = g.heads > 0 ? g.q_st : g.k_st;
   g.across_log2 = 0;
-  if (g.q_st[1] < g.q_st[2])
+  if (st[1] < st[2])
     while (1 << g.across_log2 < kAcross && 2 << g.across_log2 <= total &&
            (D / (2 * V)) << (g.across_log2 + 1) <= kAcrossLanes &&
            ((int64_t)g.tokens * (D / (2 * V)) << (g.across_log2 + 1)) < (1LL << 32) - 256)

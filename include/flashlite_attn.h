@@ -301,7 +301,8 @@ int fl_attn_tree_plan(const fl_tree_plan_params* p, void* stream);
  * {j, j + pairs}, or {2j, 2j + 1} with interleaved.  With transpose the angle
  * is negated: the gradient of the same call.  q, k, q_out and k_out are
  * [batch, heads or kv_heads, rows, head_dim] views with strides {batch, head,
- * row} in elements; outputs may be their inputs (no other overlap).  k may be NULL (no k).
+ * row} in elements; outputs may be their inputs (no other overlap).  k may be
+ * NULL (no k), and q where heads is 0.
  * positions are int32 (or int64: position_bits 64) [batch, rows], strides
  * {batch, row}.  head_dim 64 or 128; dtype FL_DTYPE_F16, FL_DTYPE_BF16 or (not
  * with a cache) FL_DTYPE_F32.

@@ -118,3 +118,28 @@ def test_strides_of_one_entry_are_not_looked_at(stride, dim, sizes):
     assert lib.fl_attn_tree_workspace_bytes(ctypes.byref(t)) > 0
     assert lib.fl_attn_tree_fwd(ctypes.byref(t), A + 4, 1 << 40, None) == capi.FL_ERR_MISALIGNED
     assert "workspace" in capi.last_error()
+
+
+def test_no_query_heads():
+    """Without query heads only k and v are stored: q and out have no memory."""
+    v = T3(1280, 320, 64)
+    p = capi.FlRotaryParams(q=0, k=A, q_out=0, q_stride=v, k_stride=v, q_out_stride=v,
+                            positions=A, position_stride=T2(5, 1), position_bits=32,
+                            dtype=capi.DTYPE_F16, freqs=A, pairs=32, batch=2, heads=0, kv_heads=4,
+                            rows=5, head_dim=D, scale=1.0)
+    c = capi.FlCacheStore(v=A, v_stride=v, k_cache=A, v_cache=A, k_cache_stride=v,
+                          v_cache_stride=v, num_blocks=2, block_size=5, slots=A + 4,
+                          slot_stride=T2(5, 1))
+    lib = capi.load()
+    assert lib.fl_attn_rotary_cache(ctypes.byref(p), ctypes.byref(c), None) == \
+        capi.FL_ERR_MISALIGNED
+    p.k_out, p.k_out_stride, p.freqs = A, v, A + 4
+    assert lib.fl_attn_rotary(ctypes.byref(p), None) == capi.FL_ERR_MISALIGNED
+    # nor key heads
+    p.q, p.q_out, p.k, p.k_out, p.heads, p.kv_heads = A, A, 0, 0, 4, 0
+    assert lib.fl_attn_rotary(ctypes.byref(p), None) == capi.FL_ERR_MISALIGNED
+    p.freqs = A
+    assert lib.fl_attn_rotary_cache(ctypes.byref(p), ctypes.byref(c), None) == \
+        capi.FL_ERR_MISALIGNED
+    p.q = 0
+    assert lib.fl_attn_rotary(ctypes.byref(p), None) == capi.FL_ERR_INVALID_ARGUMENT
