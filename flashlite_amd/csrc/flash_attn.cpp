@@ -685,14 +685,14 @@ PYBIND11_MODULE(flash_attn_wmma, m) {
         "Rotary positions of q and k (or None) [B, H, N, D] views, D 64 or 128, fp16, bf16 or "
         "fp32: pairs {j, j + len(freqs)}, or {2j, 2j + 1} with interleaved, turn by "
         "positions * freqs[j] (float64 radians) and are multiplied by scale; the outputs may be "
-        "the inputs",
+        "the inputs. Not recorded by autograd: the gradient is backward_rotary",
         py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("freqs"),
         py::arg("interleaved") = false, py::arg("scale") = 1.0, py::arg("q_out") = py::none(),
         py::arg("k_out") = py::none());
 
   m.def("backward_rotary", &flash_attn::backward_rotary,
         "The gradient of forward_rotary: the same call on the outputs' gradients, the angles "
-        "negated",
+        "negated. Not recorded by autograd itself",
         py::arg("dq"), py::arg("dk"), py::arg("positions"), py::arg("freqs"),
         py::arg("interleaved") = false, py::arg("scale") = 1.0, py::arg("q_out") = py::none(),
         py::arg("k_out") = py::none());
