@@ -222,7 +222,8 @@ __global__ void __launch_bounds__(kThreads) cache_plan_kernel(const PlanGeom g) 
 }
 
 // Otherwise in two: the moves by one work-group, then a work-group's threads
-// each token of request blockIdx.y (the first also its blocks).
+// each token of request blockIdx.y (the first also its blocks).  64 prompts of
+// 4096 tokens 7.6 us, 5.0 in one launch; 1024 requests of 4 tokens 8.5 and 5.5.
 __global__ void __launch_bounds__(kThreads) cache_plan_scan_kernel(const PlanGeom g) {
   const int2 state = plan(g, [&](int b, const Move& m) __attribute__((always_inline)) {
     note(g, b, m, g.counts[b] < 0);

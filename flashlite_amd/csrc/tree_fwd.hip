@@ -13,8 +13,8 @@
 // token after 256-8192 of 32 requests, 32/8 heads, D 128: 5.3 TB/s), more by
 // the matrix cores and what feeds them (64 drafts after 16000 of 8 requests,
 // 32/8 heads: 0.7 PFLOP/s, matrix cores 42% busy), and short calls by the chain
-// lengths, table entry, key row and by the launches (one token after 4096, B2
-// H8 D 64: 12.8 us).
+// lengths, table entry, key row and by the second launch (one token after 4096,
+// B2 H8 D 64: 12.1-12.9 us, of them the merge 3.1-3.8).
 
 #include <algorithm>
 #include <cmath>
@@ -165,7 +165,12 @@ struct TreeRows : TreeLayout<D, T>::type {
     if (now) mc = mx;
     return unset && !now;
   }
-  // p = 2^(s cr - mc); returns this lane's sum of the unrounded p.
+  // p = 2^(s cr - mc); returns this lane's sum of the unrounded p.  For the
+  // product with V p is rounded to the element type, half a step of it a key:
+  // the matrix cores take 16-bit operands, and a second product with what the
+  // rounding left would double half of the work.  Against 64 bits outputs are
+  // off by 2.6-2.9e-4 (fp16) and 2.3e-3 (bf16) where their own rounding alone
+  // makes 2.0e-4 and 1.7e-3.
   __device__ __forceinline__ float exponentiate(const Scores& s, Probs& p) const {
     float sum[2 * kBlocks];
 #pragma unroll
@@ -891,12 +896,13 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(T* O, const TreeGeom g)
 }
 
 // How a call of given sizes runs: row blocks a work-group, and whether the
-// units' steps are dealt to a grid of one work-group a CU, at most
-// kMostParts of them to a unit.  The merge reads a row's partial results one
-// batch after another, so past some parts it takes longer than the walks they
+// units' steps are dealt to a grid of one work-group a CU, of kMostParts to a
+// unit on average at most.  The merge reads a row's partial results one batch
+// after another, so past some parts it takes longer than the walks they
 // shorten.  8 heads over one KV head (D 128, bf16), one token after 32000: 31
 // us with 256 parts, 17.0 with 64, 18.6 with 32, 25.0 with 16; 64 drafts there
-// (f16) 39.9, 35.7, 45.4 and 69.9.
+// (f16) 39.9, 35.7, 45.4 and 69.9.  (The host does not know the lengths: beside
+// 3 requests of 1 token that one unit still gets some 250 parts, 30.3 us.)
 constexpr int kMostParts = 64;
 // Floats of a cache line, on which a partial result begins.
 constexpr int kPartUnit = 32;
@@ -971,14 +977,16 @@ hipError_t launch_rw(const fl_tree_params& p, const TreePlan& t, TreeGeom& g, fl
   // Splitting costs the partial results' way through memory and a second
   // launch, about four microseconds; it saves the steps by which the longest
   // unit passes an even share.  Up to kFewSaved one pass is no slower: 16
-  // requests x 16 heads of 600 keys (D 128, f16) 18.8 us against 22.2, 4 x 16
-  // drafts of 16/4 heads after 300 keys 10.2 against 13.2, 1 head of 1000 keys
+  // requests x 16 heads of 600 keys (D 128, f16) 15.5 us against 20.4, 4 x 16
+  // drafts of 16/4 heads after 300 keys 9.4 against 13.3, 1 head of 1000 keys
   // 8.2 against 9.7; with twice that bound 8 drafts of 32/8 heads after 1000
   // keys lose, 12.8 against 11.8.  With as many units as work-groups the share
   // says nothing about requests of unlike lengths, so kMostSteps bounds what
   // waiting for the longest can cost: up to it 32 drafts of 32 x 32/8 heads
-  // after 500 keys take 24.0 us against 29.4, while 16 heads and 1 to 16384
-  // keys (128 steps) lose, 129 against 110.
+  // after 500 keys take 21.3 us against 26.5, while 16 heads and 1 to 16384
+  // keys (128 steps) lose, 129 against 110.  The longest unit is taken to be as
+  // long as the tables have room for: in tables 4 times as wide as the requests
+  // need, short calls take the other side's time.
   constexpr int kFewSaved = 6, kMostSteps = 32;
   const int64_t share = (most * t.units + t.grid - 1) / t.grid;
   const bool can = g.part != nullptr && counted;

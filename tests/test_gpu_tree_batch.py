@@ -1,11 +1,12 @@
-"""forward_tree over more requests than a launch has work-groups along its second
-dimension (65535)."""
+"""forward_tree over more requests than 65535 (what some launches allow along a
+dimension), and over part of a table's columns."""
 
 import math
 
 import pytest
 
 import flashlite_amd as fl
+from tree_util import Problem, check
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +53,15 @@ def test_more_than_65535_requests(cuda, rows_first):
         assert bool((off <= delta[..., 0] + 80 * 2.0 ** -24
                      + 2.0 ** -21 * (logs.abs() + reach + 1)).all())
     assert worst <= 1.0
+
+
+@pytest.mark.parametrize("n,tree", [(1, None), (30, "tree")])
+def test_the_first_columns_of_a_wide_table(cuda, n, tree):
+    """A caller that knows its longest request hands over fewer columns."""
+    p = Problem(95, "bfloat16", 3, 8, 2, n, 128, 16, [600, 0, 333], tree, table_pad=3000)
+    args = p.device(cuda)
+    ref = p.reference()
+    for m in (args["block_tables"].shape[1], -(-(600 + n) // 16)):
+        out, lse = fl.forward_tree(return_lse=True,
+                                   **{**args, "block_tables": args["block_tables"][:, :m]})
+        check(out, lse, p, ref)
