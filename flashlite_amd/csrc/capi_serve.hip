@@ -44,6 +44,7 @@ int check_view(const int64_t st[3], int64_t n0, int64_t n1, int64_t n2, int64_t 
 // ones span.
 int check_apart(const int64_t st[3], int64_t n0, int64_t n1, int64_t n2, int64_t head_dim,
                 const char* name, const char* who) {
+  if (n0 == 0 || n1 == 0 || n2 == 0) return FL_OK;
   std::pair<int64_t, int64_t> dim[3] = {{st[0], n0}, {st[1], n1}, {st[2], n2}};
   std::sort(dim, dim + 3);
   __int128 span = head_dim;

@@ -143,3 +143,19 @@ def test_no_query_heads():
         capi.FL_ERR_MISALIGNED
     p.q = 0
     assert lib.fl_attn_rotary(ctypes.byref(p), None) == capi.FL_ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("sizes", [(0, 4, 5), (2, 0, 5), (2, 4, 0)])
+def test_views_without_rows_do_not_overlap(sizes):
+    """Nothing is written: no stride is too small, and the call does nothing."""
+    b, h, n = sizes
+    st = T3(8, 8, 8)
+    p = capi.FlRotaryParams(q_stride=st, k_stride=st, q_out_stride=st, k_out_stride=st,
+                            position_bits=32, dtype=capi.DTYPE_F16, pairs=32, batch=b, heads=h,
+                            kv_heads=h, rows=n, head_dim=D, scale=1.0)
+    assert capi.load().fl_attn_rotary(ctypes.byref(p), None) == capi.FL_OK
+    kv = T3(2 * 16 * D, 16 * D, D)
+    t = capi.FlTreeParams(q_stride=st, o_stride=st, k_stride=kv, v_stride=kv, table_stride=20,
+                          batch=b, heads=h, kv_heads=2, drafts=n, head_dim=D, num_blocks=70,
+                          block_size=16, max_blocks=20, dtype=capi.DTYPE_F16)
+    assert capi.load().fl_attn_tree_fwd(ctypes.byref(t), None, 0, None) == capi.FL_OK
