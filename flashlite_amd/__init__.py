@@ -48,8 +48,22 @@ rotary_to_cache = _ext.rotary_to_cache
 forward_tree = _ext.forward_tree
 tree_workspace_bytes = _ext.tree_workspace_bytes
 
-from .rotary import rotary_frequencies  # noqa: E402
+# Norms of q and k for each head with the rotary positions (of one or several
+# axes) in the same pass, their gradients, and the form that stores k and v.
+forward_norm_rotary = _ext.forward_norm_rotary
+backward_norm_rotary = _ext.backward_norm_rotary
+norm_rotary_to_cache = _ext.norm_rotary_to_cache
+norm_rotary_workspace_bytes = _ext.norm_rotary_workspace_bytes
+
+# Attention over packed sequences of different lengths, and its gradients.
+forward_packed = _ext.forward_packed
+backward_packed = _ext.backward_packed
+packed_workspace_bytes = _ext.packed_workspace_bytes
+
+from .rotary import rotary_axes, rotary_frequencies  # noqa: E402
 
 __all__ = ["forward_flash2", "forward_naive", "forward_flash2_ex", "splitkv_workspace_bytes",
            "plan_cache", "plan_tree", "forward_rotary", "backward_rotary", "rotary_to_cache",
-           "rotary_frequencies", "forward_tree", "tree_workspace_bytes"]
+           "rotary_frequencies", "forward_tree", "tree_workspace_bytes", "forward_norm_rotary",
+           "backward_norm_rotary", "norm_rotary_to_cache", "norm_rotary_workspace_bytes",
+           "rotary_axes", "forward_packed", "backward_packed", "packed_workspace_bytes"]

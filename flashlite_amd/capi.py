@@ -45,6 +45,13 @@ EXPORTED = (
     "fl_attn_rotary_cache",
     "fl_attn_tree_workspace_bytes",
     "fl_attn_tree_fwd",
+    "fl_attn_norm_rotary",
+    "fl_attn_norm_rotary_bwd",
+    "fl_attn_norm_rotary_cache",
+    "fl_attn_norm_rotary_workspace_bytes",
+    "fl_attn_packed_fwd",
+    "fl_attn_packed_bwd",
+    "fl_attn_packed_bwd_workspace_bytes",
 )
 
 SCRATCH_BYTES = 8 << 20  # FL_ATTN_SCRATCH_BYTES
@@ -177,6 +184,68 @@ class FlTreeParams(ctypes.Structure):
     ]
 
 
+class FlPackedParams(ctypes.Structure):
+    """Mirrors ``fl_packed_params``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 2),  # {head, row} elements
+        ("k_stride", ctypes.c_int64 * 2),
+        ("v_stride", ctypes.c_int64 * 2),
+        ("o_stride", ctypes.c_int64 * 2),
+        ("starts", ctypes.c_void_p),
+        ("key_starts", ctypes.c_void_p),
+        ("sequences", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("key_rows", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("sm_scale", ctypes.c_double),
+        ("causal", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class FlPackedGrads(ctypes.Structure):
+    """Mirrors ``fl_packed_grads``."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dout", "dq", "dk", "dv")] + [
+        (n + "_stride", ctypes.c_int64 * 2) for n in ("dout", "dq", "dk", "dv")]
+
+
+class FlNormParams(ctypes.Structure):
+    """Mirrors ``fl_norm_params``."""
+
+    _fields_ = [
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_double),
+        ("weight_offset", ctypes.c_double),
+        ("axes", ctypes.c_void_p),
+        ("num_axes", ctypes.c_int64),
+        ("axis_stride", ctypes.c_int64),
+    ]
+
+
+class FlNormGrads(ctypes.Structure):
+    """Mirrors ``fl_norm_grads``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("dq_weight", ctypes.c_void_p),
+        ("dk_weight", ctypes.c_void_p),
+    ]
+
+
 class FlashLiteError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"[{code}] {message}")
@@ -237,7 +306,10 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     for name, args in (("fl_attn_cache_plan", [FlCachePlanParams]),
                        ("fl_attn_tree_plan", [FlTreePlanParams]),
                        ("fl_attn_rotary", [FlRotaryParams]),
-                       ("fl_attn_rotary_cache", [FlRotaryParams, FlCacheStore])):
+                       ("fl_attn_rotary_cache", [FlRotaryParams, FlCacheStore]),
+                       ("fl_attn_norm_rotary", [FlRotaryParams, FlNormParams]),
+                       ("fl_attn_norm_rotary_cache", [FlRotaryParams, FlNormParams, FlCacheStore]),
+                       ("fl_attn_packed_fwd", [FlPackedParams])):
         fn = getattr(lib, name)
         fn.argtypes = [ctypes.POINTER(a) for a in args] + [ctypes.c_void_p]
         fn.restype = ctypes.c_int
@@ -246,6 +318,17 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.fl_attn_tree_fwd.argtypes = [ctypes.POINTER(FlTreeParams), ctypes.c_void_p, ctypes.c_int64,
                                      ctypes.c_void_p]
     lib.fl_attn_tree_fwd.restype = ctypes.c_int
+    for name, args in (("fl_attn_norm_rotary_bwd", [FlRotaryParams, FlNormParams, FlNormGrads]),
+                       ("fl_attn_packed_bwd", [FlPackedParams, FlPackedGrads])):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(a) for a in args] + [ctypes.c_void_p, ctypes.c_int64,
+                                                           ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+    for name, arg in (("fl_attn_norm_rotary_workspace_bytes", FlRotaryParams),
+                      ("fl_attn_packed_bwd_workspace_bytes", FlPackedParams)):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(arg)]
+        fn.restype = ctypes.c_int64
     _lib = lib
     return lib
 

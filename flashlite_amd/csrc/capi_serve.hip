@@ -1,62 +1,12 @@
 // C-ABI entry points of the paged-cache operators: argument checks and the
 // launch.  No counterpart in the reference.
 
-#include <algorithm>
 #include <cmath>
 #include <cstdint>
-#include <utility>
 
-#include "fl_serve.h"
+#include "capi_checks.h"
 
 namespace {
-
-using fl::set_error;
-
-int launched(hipError_t e, const char* who) {
-  if (e == hipSuccess) return FL_OK;
-  return set_error(FL_ERR_LAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
-}
-
-int null_params(const char* who) {
-  return set_error(FL_ERR_INVALID_ARGUMENT, "%s: params is NULL", who);
-}
-
-bool fits32(int64_t x) { return x >= 0 && x <= INT32_MAX; }
-
-bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
-
-// Strides of an [n0, n1, n2, head_dim] view: non-negative, and rows of whole
-// 16-byte pieces.  (Those of one entry step nowhere.)
-int check_view(const int64_t st[3], int64_t n0, int64_t n1, int64_t n2, int64_t unit,
-               const char* name, const char* who) {
-  const int64_t n[3] = {n0, n1, n2};
-  for (int i = 0; i < 3; ++i)
-    if (n[i] > 1 && (st[i] < 0 || st[i] % unit != 0))
-      return set_error(FL_ERR_UNSUPPORTED,
-                       "%s: %s strides must be non-negative multiples of %lld elements (got %lld, "
-                       "%lld, %lld)", who, name, (long long)unit, (long long)st[0],
-                       (long long)st[1], (long long)st[2]);
-  return FL_OK;
-}
-
-// Rows of head_dim columns that are written: no two may share a place.  The
-// dimensions must nest: each stride reaches past everything that the smaller
-// ones span.
-int check_apart(const int64_t st[3], int64_t n0, int64_t n1, int64_t n2, int64_t head_dim,
-                const char* name, const char* who) {
-  if (n0 == 0 || n1 == 0 || n2 == 0) return FL_OK;
-  std::pair<int64_t, int64_t> dim[3] = {{st[0], n0}, {st[1], n1}, {st[2], n2}};
-  std::sort(dim, dim + 3);
-  __int128 span = head_dim;
-  for (const auto& [stride, n] : dim) {
-    if (n <= 1) continue;
-    if (stride < span)
-      return set_error(FL_ERR_INVALID_ARGUMENT, "%s: %s is written, its rows must not overlap", who,
-                       name);
-    span += (__int128)stride * (n - 1);
-  }
-  return FL_OK;
-}
 
 int check_pages(int64_t num_blocks, int64_t block_size, const char* who) {
   if (num_blocks < 1 || block_size < 1)
@@ -116,6 +66,58 @@ int check_rotary_pointers(const fl_rotary_params* p, bool cache, const char* who
     return set_error(FL_ERR_MISALIGNED, "%s: q, k and the outputs must be 16-byte aligned", who);
   if (!aligned(p->freqs, 8) || !aligned(p->positions, p->position_bits / 8))
     return set_error(FL_ERR_MISALIGNED, "%s: freqs and positions must be aligned", who);
+  return FL_OK;
+}
+
+// A call that stores rows in a cache; `empty`: it has no rows.
+int check_rotary_store(const fl_rotary_params* p, const fl_cache_store* c, const char* who,
+                       bool& empty) {
+  int rc = check_rotary(p, true, who);
+  if (rc != FL_OK) return rc;
+  if (c == nullptr) return set_error(FL_ERR_INVALID_ARGUMENT, "%s: the cache is NULL", who);
+  if (p->transpose)
+    return set_error(FL_ERR_INVALID_ARGUMENT, "%s: transpose is not for a cache", who);
+  rc = check_pages(c->num_blocks, c->block_size, who);
+  if (rc == FL_OK) rc = check_view(c->v_stride, p->batch, p->kv_heads, p->rows, 8, "v", who);
+  auto cache = [&](const int64_t st[3], const char* name) {
+    return check_view(st, c->num_blocks, p->kv_heads, c->block_size, 8, name, who);
+  };
+  if (rc == FL_OK) rc = cache(c->k_cache_stride, "k_cache");
+  if (rc == FL_OK) rc = cache(c->v_cache_stride, "v_cache");
+  if (rc == FL_OK)
+    rc = check_apart(c->k_cache_stride, c->num_blocks, p->kv_heads, c->block_size, p->head_dim,
+                     "k_cache", who);
+  if (rc == FL_OK)
+    rc = check_apart(c->v_cache_stride, c->num_blocks, p->kv_heads, c->block_size, p->head_dim,
+                     "v_cache", who);
+  if (rc != FL_OK) return rc;
+  empty = p->batch == 0 || p->rows == 0 || p->heads + p->kv_heads == 0;
+  if (empty) return FL_OK;
+  if (!c->slots || (p->kv_heads > 0 && (!p->k || !c->v || !c->k_cache || !c->v_cache)))
+    return set_error(FL_ERR_INVALID_ARGUMENT, "%s: k, v, the caches and slots must be non-NULL", who);
+  rc = check_rotary_pointers(p, true, who);
+  if (rc != FL_OK) return rc;
+  if (!aligned(c->v, 16) || !aligned(c->k_cache, 16) || !aligned(c->v_cache, 16) ||
+      !aligned(c->slots, 8))
+    return set_error(FL_ERR_MISALIGNED, "%s: v and the caches must be 16-byte aligned, slots 8", who);
+  return FL_OK;
+}
+
+int check_norm(const fl_rotary_params* p, const fl_norm_params* n, const char* who) {
+  if (n == nullptr) return null_params(who);
+  if (n->weight_dtype != FL_DTYPE_F32 && n->weight_dtype != p->dtype)
+    return set_error(FL_ERR_INVALID_ARGUMENT, "%s: weights must be fp32 or of the rows' dtype", who);
+  if (!std::isfinite(n->eps) || n->eps < 0.0 || !std::isfinite((float)n->eps) ||
+      !std::isfinite(n->weight_offset) || !std::isfinite((float)n->weight_offset))
+    return set_error(FL_ERR_INVALID_ARGUMENT,
+                     "%s: eps must be finite and not negative, weight_offset finite", who);
+  const int bytes = n->weight_dtype == FL_DTYPE_F32 ? 4 : 2;
+  if (!aligned(n->q_weight, bytes) || !aligned(n->k_weight, bytes) || !aligned(n->axes, 4))
+    return set_error(FL_ERR_MISALIGNED, "%s: weights and axes must be aligned to their elements",
+                     who);
+  if (n->axes != nullptr && (n->num_axes < 1 || !fits32(n->num_axes)))
+    return set_error(FL_ERR_INVALID_ARGUMENT, "%s: axes need at least one axis (got %lld)", who,
+                     (long long)n->num_axes);
   return FL_OK;
 }
 
@@ -257,34 +259,82 @@ int fl_attn_rotary(const fl_rotary_params* p, void* stream) {
 
 int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, void* stream) {
   const char* who = "fl_attn_rotary_cache";
-  int rc = check_rotary(p, true, who);
-  if (rc != FL_OK) return rc;
-  if (c == nullptr) return set_error(FL_ERR_INVALID_ARGUMENT, "%s: the cache is NULL", who);
-  if (p->transpose)
-    return set_error(FL_ERR_INVALID_ARGUMENT, "%s: transpose is not for a cache", who);
-  rc = check_pages(c->num_blocks, c->block_size, who);
-  if (rc == FL_OK) rc = check_view(c->v_stride, p->batch, p->kv_heads, p->rows, 8, "v", who);
-  auto cache = [&](const int64_t st[3], const char* name) {
-    return check_view(st, c->num_blocks, p->kv_heads, c->block_size, 8, name, who);
-  };
-  if (rc == FL_OK) rc = cache(c->k_cache_stride, "k_cache");
-  if (rc == FL_OK) rc = cache(c->v_cache_stride, "v_cache");
-  if (rc == FL_OK)
-    rc = check_apart(c->k_cache_stride, c->num_blocks, p->kv_heads, c->block_size, p->head_dim,
-                     "k_cache", who);
-  if (rc == FL_OK)
-    rc = check_apart(c->v_cache_stride, c->num_blocks, p->kv_heads, c->block_size, p->head_dim,
-                     "v_cache", who);
-  if (rc != FL_OK) return rc;
-  if (p->batch == 0 || p->rows == 0 || p->heads + p->kv_heads == 0) return FL_OK;
-  if (!c->slots || (p->kv_heads > 0 && (!p->k || !c->v || !c->k_cache || !c->v_cache)))
-    return set_error(FL_ERR_INVALID_ARGUMENT, "%s: k, v, the caches and slots must be non-NULL", who);
-  rc = check_rotary_pointers(p, true, who);
-  if (rc != FL_OK) return rc;
-  if (!aligned(c->v, 16) || !aligned(c->k_cache, 16) || !aligned(c->v_cache, 16) ||
-      !aligned(c->slots, 8))
-    return set_error(FL_ERR_MISALIGNED, "%s: v and the caches must be 16-byte aligned, slots 8", who);
+  bool empty = false;
+  const int rc = check_rotary_store(p, c, who, empty);
+  if (rc != FL_OK || empty) return rc;
   return launched(fl::launch_rotary(*p, c, static_cast<hipStream_t>(stream)), who);
+}
+
+int fl_attn_norm_rotary(const fl_rotary_params* p, const fl_norm_params* n, void* stream) {
+  const char* who = "fl_attn_norm_rotary";
+  int rc = check_rotary(p, false, who);
+  if (rc == FL_OK) rc = check_norm(p, n, who);
+  if (rc != FL_OK) return rc;
+  if (p->batch == 0 || p->rows == 0 || p->heads + (p->k ? p->kv_heads : 0) == 0) return FL_OK;
+  rc = check_rotary_pointers(p, false, who);
+  if (rc != FL_OK) return rc;
+  return launched(fl::launch_norm_rotary(*p, *n, nullptr, nullptr, nullptr,
+                                         static_cast<hipStream_t>(stream)), who);
+}
+
+int fl_attn_norm_rotary_cache(const fl_rotary_params* p, const fl_norm_params* n,
+                              const fl_cache_store* c, void* stream) {
+  const char* who = "fl_attn_norm_rotary_cache";
+  bool empty = false;
+  int rc = check_rotary_store(p, c, who, empty);
+  if (rc == FL_OK) rc = check_norm(p, n, who);
+  if (rc != FL_OK || empty) return rc;
+  return launched(fl::launch_norm_rotary(*p, *n, c, nullptr, nullptr,
+                                         static_cast<hipStream_t>(stream)), who);
+}
+
+int64_t fl_attn_norm_rotary_workspace_bytes(const fl_rotary_params* p) {
+  const char* who = "fl_attn_norm_rotary_workspace_bytes";
+  if (p == nullptr) return null_params(who), -1;
+  if (p->head_dim != 64 && p->head_dim != 128)
+    return set_error(FL_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128 (got %lld)", who,
+                     (long long)p->head_dim), -1;
+  return fl::norm_rotary_workspace_bytes(p->head_dim);
+}
+
+int fl_attn_norm_rotary_bwd(const fl_rotary_params* p, const fl_norm_params* n,
+                            const fl_norm_grads* d, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+  const char* who = "fl_attn_norm_rotary_bwd";
+  int rc = check_rotary(p, false, who);
+  if (rc == FL_OK) rc = check_norm(p, n, who);
+  if (rc != FL_OK) return rc;
+  if (d == nullptr) return null_params(who);
+  const bool q = n->q_weight != nullptr && p->heads > 0;
+  const bool k = n->k_weight != nullptr && p->k != nullptr && p->kv_heads > 0;
+  const int64_t unit = p->dtype == FL_DTYPE_F32 ? 4 : 8;
+  if (q) rc = check_view(d->q_stride, p->batch, p->heads, p->rows, unit, "q", who);
+  if (rc == FL_OK && k)
+    rc = check_view(d->k_stride, p->batch, p->kv_heads, p->rows, unit, "k", who);
+  if (rc != FL_OK) return rc;
+  if (!aligned(d->dq_weight, 4) || !aligned(d->dk_weight, 4))
+    return set_error(FL_ERR_MISALIGNED, "%s: dq_weight and dk_weight must be 4-byte aligned", who);
+  if (p->batch == 0 || p->rows == 0 || p->heads + (p->k ? p->kv_heads : 0) == 0) {
+    // sums over no rows
+    float* const dq = n->q_weight ? d->dq_weight : nullptr;
+    float* const dk = n->k_weight ? d->dk_weight : nullptr;
+    if (!dq && !dk) return FL_OK;
+    return launched(fl::launch_norm_zero(*p, dq, dk, static_cast<hipStream_t>(stream)), who);
+  }
+  rc = check_rotary_pointers(p, false, who);
+  if (rc != FL_OK) return rc;
+  if ((q && !d->q) || (k && !d->k))
+    return set_error(FL_ERR_INVALID_ARGUMENT, "%s: the forward pass' q and k must be non-NULL", who);
+  if (!aligned(d->q, 16) || !aligned(d->k, 16))
+    return set_error(FL_ERR_MISALIGNED, "%s: q and k must be 16-byte aligned", who);
+  const int64_t need = fl::norm_rotary_workspace_bytes(p->head_dim);
+  if ((q || k) && (!workspace || workspace_bytes < need))
+    return set_error(FL_ERR_INVALID_ARGUMENT, "%s: a workspace of %lld bytes is needed (got %lld)",
+                     who, (long long)need, (long long)(workspace ? workspace_bytes : 0));
+  if (!aligned(workspace, 16))
+    return set_error(FL_ERR_MISALIGNED, "%s: workspace must be 16-byte aligned", who);
+  return launched(fl::launch_norm_rotary(*p, *n, nullptr, d, workspace,
+                                         static_cast<hipStream_t>(stream)), who);
 }
 
 int64_t fl_attn_tree_workspace_bytes(const fl_tree_params* p) {

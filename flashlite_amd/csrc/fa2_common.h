@@ -139,6 +139,36 @@ struct Elem<__bf16> {
   }
 };
 
+// NaN and infinities of a V operand become 0.
+template <class T>
+__device__ __forceinline__ typename Elem<T>::v8 finite_only(const typename Elem<T>::v8& v) {
+  constexpr uint32_t kExp = sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7C00u : 0x7F80u;
+  u32x4_t x = __builtin_bit_cast(u32x4_t, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((x[i] & kExp) == kExp) x[i] &= 0xFFFF0000u;
+    if ((x[i] & (kExp << 16)) == (kExp << 16)) x[i] &= 0x0000FFFFu;
+  }
+  return __builtin_bit_cast(typename Elem<T>::v8, x);
+}
+
+// Whether one of a tile's operands is NaN or infinite: the largest of their
+// bits, signs aside.
+template <class T>
+__device__ __forceinline__ bool any_odd(const typename Elem<T>::v8 (&v)[8]) {
+  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+  constexpr uint16_t kExp = __is_same(T, _Float16) ? 0x7C00 : 0x7F80;
+  u16x2_t top = {0, 0};
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const u32x4_t x = __builtin_bit_cast(u32x4_t, v[u]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, x[i] & 0x7FFF7FFFu));
+  }
+  return top[0] >= kExp || top[1] >= kExp;
+}
+
 constexpr int kD = 64;                       // head dim
 constexpr int kBc = 64;                      // keys per KV tile
 constexpr int kRowBytes = kD * 2;            // 128
@@ -180,6 +210,7 @@ __device__ __forceinline__ i32x4_t buffer_rsrc(const void* base, int bytes) {
 // [batch][head][row] (head_dim is unit stride), the sizes, the causal
 // diagonal offset N_k - N_q, and the optional log-sum-exp output.
 struct Geom {
+  static constexpr bool kPacked = false;  // (PackedGeom: packed sequences)
   long long q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, o_sb, o_sh;
   int q_sr, k_sr, v_sr, o_sr;
   int heads, seq_q, seq_k, coff;
@@ -1090,6 +1121,11 @@ struct Rows {
           *reinterpret_cast<V8*>(orow + 32 * db + 16 * hh + 8 * g) = out;
         }
     }
+  }
+  // The log-sum-exp of a row whose sum is NaN is NaN (store() has -inf there).
+  __device__ __forceinline__ void store_nan(float* lse) const {
+    const float l_tot = pair_sum(l);
+    if (lse != nullptr && g == 0 && my_q < seq && l_tot != l_tot) lse[my_q] = l_tot;
   }
   // As store(), through buffer resources whose ranges end at the last valid
   // row: O (rows r0.. of the resource, row_bytes apart) and the log-sum-exp

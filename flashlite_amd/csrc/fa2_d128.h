@@ -128,8 +128,14 @@ struct Rows128 {
   // GEMM2 of one tile: O^T += V^T . P^T.
   __device__ __forceinline__ void gemm2(const uint8_t* vt, const V8 (&pp)[2]) {
     V8 va[8];
+    read_v(vt, va);
+    gemm2(va, pp);
+  }
+  __device__ __forceinline__ void read_v(const uint8_t* vt, V8 (&va)[8]) const {
 #pragma unroll
     for (int u = 0; u < 8; ++u) va[u] = read_v_op(vt, u & 3, u >> 2);
+  }
+  __device__ __forceinline__ void gemm2(const V8 (&va)[8], const V8 (&pp)[2]) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) o[u & 3] = E::mfma(va[u], pp[u >> 2], o[u & 3]);
   }
@@ -253,6 +259,11 @@ struct Rows128 {
       o[db][r + 3] = a0 * o[db][r + 3] + a1 * x.w;
     }
     mc = mm;
+  }
+  // As Rows::store_nan.
+  __device__ __forceinline__ void store_nan(float* lse) const {
+    const float l_tot = pair_sum(l);
+    if (lse != nullptr && g == 0 && my_q < seq && l_tot != l_tot) lse[my_q] = l_tot;
   }
   // O = O^T / l of head-dim blocks [B0, B1), 16-byte stores of 8 contiguous
   // head dims; with block 0 the log-sum-exp as in Rows::store.

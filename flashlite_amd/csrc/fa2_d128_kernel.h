@@ -4,6 +4,7 @@
 #pragma once
 
 #include "fa2_d128.h"
+#include "packed.h"
 
 namespace fl {
 
@@ -45,10 +46,10 @@ namespace {
 // 128-row one.  With one wave per SIMD (64-row groups) reading operands 8
 // slots ahead instead of 4 takes those to 12.8 and 62.2; with two it is 0-4%
 // slower.  The rings hold 4 tiles: 5 measured 0-5% slower.
-template <int W, int FK, bool CAUSAL, class T, int SPLIT = 1, bool PAIR = false>
+template <int W, int FK, bool CAUSAL, class T, int SPLIT = 1, bool PAIR = false, class GeomT = Geom>
 __global__ void __launch_bounds__(64 * W * SPLIT, 2)
 fa2_fwd_d128_kernel(const T* Q, const T* __restrict__ K, const T* __restrict__ V, T* O,
-                    const Geom geom, int nqb, float cq, float cr) {
+                    const GeomT launch, int nqb, float cq, float cr) {
   using RowsT = Rows128<CAUSAL, T>;
   using V8 = typename RowsT::V8;
   constexpr int FV = FK - 2;
@@ -86,14 +87,20 @@ fa2_fwd_d128_kernel(const T* Q, const T* __restrict__ K, const T* __restrict__ V
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int stream = SPLIT == 1 ? 0 : wave / W;  // key-range half
   const int rw = wave - stream * W;              // 32-row block within the work-group
-  int bh, qb, qb2 = 0, nblk = 1;
+  int bh, qb = 0, qb2 = 0, nblk = 1;
+  Geom own;
+  if constexpr (GeomT::kPacked) {
+    if (!packed_problem<(PAIR ? 2 : 1) * kBr>(launch, Q, K, V, O, own, bh, qb)) return;
+    if (PAIR) nqb = (own.seq_q + kBr - 1) / kBr;
+  }
+  const Geom& geom = problem_geom(launch, own);
   if constexpr (PAIR) {
-    int pr;
-    pair_coords(nqb, geom.xcds, bh, pr);
+    int pr = qb;
+    if constexpr (!GeomT::kPacked) pair_coords(nqb, geom.xcds, bh, pr);
     qb = nqb - 1 - pr;
     qb2 = pr;
     nblk = qb2 < qb ? 2 : 1;  // the middle block of an odd count walks alone
-  } else {
+  } else if constexpr (!GeomT::kPacked) {
     wg_coords<CAUSAL, kWgPerCu>(nqb, geom.xcds, geom.cus_per_xcd, bh, qb);
   }
   const HeadPtrs<T> hp = head_ptrs<T, kRowBytes2>(geom, bh, Q, K, V, O);
@@ -296,6 +303,9 @@ fa2_fwd_d128_kernel(const T* Q, const T* __restrict__ K, const T* __restrict__ V
     }
   }
 
+  // (packed: also a block whose O is not finite, as in fa2_fwd_slot_kernel)
+  if constexpr (GeomT::kPacked) out_of_range |= __builtin_amdgcn_ballot_w64(any_odd(rows.o));
+
   // Checked pass (as in fa2_fwd_slot_kernel); the flag lives in the last 16
   // bytes of the V rings.
   __builtin_amdgcn_s_waitcnt(0);
@@ -318,7 +328,17 @@ fa2_fwd_d128_kernel(const T* Q, const T* __restrict__ K, const T* __restrict__ V
       rows.mask(tbeg + t, Sc);
       if (t == 0) rows.first_tile(Sc);
       rows.softmax_checked(Sc, Pc);
-      rows.gemm2(rings.vslot(Ic<0>{}), Pc);
+      if constexpr (GeomT::kPacked) {
+        V8 va[8];
+        rows.read_v(rings.vslot(Ic<0>{}), va);
+        const int lim = min(rows.kv_lim, CAUSAL ? rows.my_d + 1 : rows.kv_lim) - (tbeg + t) * kBc2;
+        add_odd<128, T>(
+            rings.vslot(Ic<0>{}), va, rows.o, rows.g, [&](int j) { return j < lim; }, false,
+            [](int r) { return v_swz128(r); });
+        rows.gemm2(va, Pc);
+      } else {
+        rows.gemm2(rings.vslot(Ic<0>{}), Pc);
+      }
       sync_ring_ahead<0, 0>();
     }
   }
@@ -357,12 +377,14 @@ fa2_fwd_d128_kernel(const T* Q, const T* __restrict__ K, const T* __restrict__ V
     if (stream == 0) {
       rows.template merge_half<0>(xslot(4 + rw), x.x, x.y, lane);
       rows.template store<0, 2>(hp.o, geom.o_sr, hp.lse);
+      if constexpr (GeomT::kPacked) rows.store_nan(hp.lse);
     } else {
       rows.template merge_half<1>(xslot(rw), x.x, x.y, lane);
       rows.template store<2, 4>(hp.o, geom.o_sr, hp.lse);
     }
   } else {
     rows.template store<0, 4>(hp.o, geom.o_sr, hp.lse);
+    if constexpr (GeomT::kPacked) rows.store_nan(hp.lse);
   }
   // every wave past its reads of the exchange before the next block's fetches
   if (PAIR && bi + 1 < nblk) __syncthreads();

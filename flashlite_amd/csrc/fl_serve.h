@@ -49,9 +49,34 @@ hipError_t launch_tree_plan(const fl_tree_plan_params& p, hipStream_t stream);  
 hipError_t launch_rotary(const fl_rotary_params& p, const fl_cache_store* store,
                          hipStream_t stream);
 
+// Norms and rotation (norm_rotary.hip): with `store` the rows also go to the
+// cache, with `grads` the backward pass and its workspace.
+int64_t norm_rotary_workspace_bytes(int64_t head_dim);
+hipError_t launch_norm_rotary(const fl_rotary_params& p, const fl_norm_params& n,
+                              const fl_cache_store* store, const fl_norm_grads* grads, void* ws,
+                              hipStream_t stream);
+// Zeros to the weights' gradients (each may be null).
+hipError_t launch_norm_zero(const fl_rotary_params& p, float* dq, float* dk, hipStream_t stream);
+
 // Bytes of the partial results of a call of these sizes, 0 where it is not
 // split; launch_tree_fwd with ws == nullptr does without (tree_fwd.hip).
 int64_t tree_workspace_bytes(const fl_tree_params& p);
 hipError_t launch_tree_fwd(const fl_tree_params& p, void* ws, hipStream_t stream);
+
+// Packed sequences, by element type (packed_fwd_*.hip, packed_bwd_*.hip), one
+// entry of a dimension with a stride that fits.
+hipError_t launch_packed_fwd_f16(const fl_packed_params& p, hipStream_t stream);
+hipError_t launch_packed_fwd_bf16(const fl_packed_params& p, hipStream_t stream);
+hipError_t launch_packed_bwd_f16(const fl_packed_params& p, const fl_packed_grads& d, void* ws,
+                                 hipStream_t stream);
+hipError_t launch_packed_bwd_bf16(const fl_packed_params& p, const fl_packed_grads& d, void* ws,
+                                  hipStream_t stream);
+
+// The backward pass' workspace: {lse, delta} of every row, then with more than
+// one part [parts][kv_heads][key_rows][2 head_dim] sums (capi_packed.hip).
+int packed_bwd_parts(const fl_packed_params& p);
+inline int64_t packed_stat_bytes(const fl_packed_params& p) {
+  return (p.heads * p.rows * 8 + 255) / 256 * 256;
+}
 
 }  // namespace fl

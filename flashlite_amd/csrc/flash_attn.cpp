@@ -483,12 +483,13 @@ py::object backward_rotary(const torch::Tensor& dq, const OptTensor& dk,
   return rotary(dq, dk, positions, freqs, interleaved, scale, q_out, k_out, true);
 }
 
-torch::Tensor rotary_to_cache(const torch::Tensor& q, const torch::Tensor& k,
-                              const torch::Tensor& v, const torch::Tensor& positions,
-                              const torch::Tensor& slots, const torch::Tensor& freqs,
-                              const torch::Tensor& k_cache, const torch::Tensor& v_cache,
-                              bool interleaved, double scale, const OptTensor& out) {
-  fl_rotary_params p = rotary_params(q, k, positions, freqs, interleaved, scale);
+namespace {
+
+// The caches and slots of a call that stores k and v.
+fl_cache_store cache_store(const fl_rotary_params& p, const torch::Tensor& q,
+                           const torch::Tensor& k, const torch::Tensor& v,
+                           const torch::Tensor& slots, const torch::Tensor& k_cache,
+                           const torch::Tensor& v_cache) {
   TORCH_CHECK(p.dtype != FL_DTYPE_F32, "All tensors must be FP16 (Half), or all BF16");
   fl_cache_store c = {};
   view4(v, q, "v", c.v_stride);
@@ -509,12 +510,194 @@ torch::Tensor rotary_to_cache(const torch::Tensor& q, const torch::Tensor& k,
   c.num_blocks = k_cache.size(0);
   c.block_size = k_cache.size(2);
   c.slots = slots.data_ptr<int64_t>();
+  return c;
+}
+
+// The caller's workspace of at least `need` bytes, or a new one.
+torch::Tensor workspace_of(const OptTensor& workspace, int64_t need, const torch::Tensor& like) {
+  if (!given(workspace))
+    return torch::empty({(need + 3) / 4}, like.options().dtype(torch::kFloat32));
+  const torch::Tensor& ws = *workspace;
+  TORCH_CHECK(ws.is_cuda() && ws.device() == like.device() && ws.is_contiguous(),
+              "workspace must be a contiguous tensor on q's device");
+  TORCH_CHECK((int64_t)ws.nbytes() >= need, "workspace of ", need, " bytes needed (got ",
+              ws.nbytes(), ")");
+  return ws;
+}
+
+}  // namespace
+
+torch::Tensor rotary_to_cache(const torch::Tensor& q, const torch::Tensor& k,
+                              const torch::Tensor& v, const torch::Tensor& positions,
+                              const torch::Tensor& slots, const torch::Tensor& freqs,
+                              const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                              bool interleaved, double scale, const OptTensor& out) {
+  fl_rotary_params p = rotary_params(q, k, positions, freqs, interleaved, scale);
+  const fl_cache_store c = cache_store(p, q, k, v, slots, k_cache, v_cache);
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   const torch::Tensor o = given(out) ? *out : torch::zeros_like(q);
   view4(o, q, "out", p.q_out_stride);
   TORCH_CHECK(o.sizes() == q.sizes(), "out must have q's shape");
   p.q_out = o.data_ptr();
   ok(fl_attn_rotary_cache(&p, &c, current_stream(q)));
+  return o;
+}
+
+namespace {
+
+// Weights, epsilon and axes of a call that norms; `positions` with axes is
+// [A, B, N] (or [A, N]).
+fl_norm_params norm_params(const torch::Tensor& q, const OptTensor& k, const OptTensor& q_weight,
+                           const OptTensor& k_weight, const torch::Tensor& positions,
+                           const OptTensor& axes, int64_t pairs, double eps, double offset) {
+  fl_norm_params n = {};
+  n.weight_dtype = FL_DTYPE_F32;
+  n.eps = eps;
+  n.weight_offset = offset;
+  auto weight = [&](const OptTensor& w, const char* name) -> const void* {
+    if (!given(w)) return nullptr;
+    TORCH_CHECK(w->is_cuda() && w->device() == q.device(), name,
+                " must be on the same device as the others");
+    TORCH_CHECK(w->scalar_type() == torch::kFloat32 || w->scalar_type() == q.scalar_type(), name,
+                " must be FP32 or of q's dtype");
+    TORCH_CHECK(w->dim() == 1 && w->size(0) == q.size(3) && w->is_contiguous(), name,
+                " must be a contiguous [D] tensor");
+    return w->data_ptr();
+  };
+  n.q_weight = weight(q_weight, "q_weight");
+  n.k_weight = weight(k_weight, "k_weight");
+  TORCH_CHECK(given(k) || !given(k_weight), "k_weight= needs k");
+  if (given(q_weight) && given(k_weight))
+    TORCH_CHECK(q_weight->scalar_type() == k_weight->scalar_type(),
+                "q_weight and k_weight must have the same dtype");
+  if (given(q_weight) || given(k_weight))
+    n.weight_dtype = serve_dtype(given(q_weight) ? *q_weight : *k_weight);
+  if (given(axes)) {
+    check_int32(*axes, q.device(), 1, "axes");
+    TORCH_CHECK(axes->size(0) == pairs && axes->is_contiguous(),
+                "axes must be contiguous, an axis for each of freqs");
+    n.axes = axes->data_ptr<int32_t>();
+    n.num_axes = positions.size(0);
+    n.axis_stride = positions.stride(0);
+  }
+  return n;
+}
+
+// The positions of the first axis, as rotary_params takes them.
+torch::Tensor first_axis(const torch::Tensor& positions, const OptTensor& axes) {
+  if (!given(axes)) return positions;
+  TORCH_CHECK((positions.dim() == 2 || positions.dim() == 3) && positions.size(0) >= 1,
+              "positions must be [A, B, N] or [A, N] with axes");
+  return positions.select(0, 0);
+}
+
+}  // namespace
+
+py::object forward_norm_rotary(const torch::Tensor& q, const OptTensor& k,
+                               const OptTensor& q_weight, const OptTensor& k_weight,
+                               const torch::Tensor& positions, const torch::Tensor& freqs,
+                               const OptTensor& axes, double eps, double weight_offset,
+                               bool interleaved, double scale, const OptTensor& q_out,
+                               const OptTensor& k_out) {
+  fl_rotary_params p =
+      rotary_params(q, k, first_axis(positions, axes), freqs, interleaved, scale);
+  const fl_norm_params n =
+      norm_params(q, k, q_weight, k_weight, positions, axes, p.pairs, eps, weight_offset);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  const torch::Tensor qo = given(q_out) ? *q_out : torch::empty_like(q);
+  view4(qo, q, "q_out", p.q_out_stride);
+  TORCH_CHECK(qo.sizes() == q.sizes(), "q_out must have q's shape");
+  p.q_out = qo.data_ptr();
+  torch::Tensor ko;
+  if (given(k)) {
+    ko = given(k_out) ? *k_out : torch::empty_like(*k);
+    view4(ko, q, "k_out", p.k_out_stride);
+    TORCH_CHECK(ko.sizes() == k->sizes(), "k_out must have k's shape");
+    p.k_out = ko.data_ptr();
+  } else {
+    TORCH_CHECK(!given(k_out), "k_out= needs k");
+  }
+  ok(fl_attn_norm_rotary(&p, &n, current_stream(q)));
+  if (given(k)) return py::make_tuple(qo, ko);
+  return py::cast(qo);
+}
+
+py::tuple backward_norm_rotary(const torch::Tensor& dq, const OptTensor& dk, const torch::Tensor& q,
+                               const OptTensor& k, const OptTensor& q_weight,
+                               const OptTensor& k_weight, const torch::Tensor& positions,
+                               const torch::Tensor& freqs, const OptTensor& axes, double eps,
+                               double weight_offset, bool interleaved, double scale,
+                               const OptTensor& q_out, const OptTensor& k_out,
+                               const OptTensor& dq_weight, const OptTensor& dk_weight,
+                               const OptTensor& workspace) {
+  fl_rotary_params p =
+      rotary_params(dq, dk, first_axis(positions, axes), freqs, interleaved, scale);
+  TORCH_CHECK(given(k) == given(dk), "k and dk are given both or not at all");
+  const fl_norm_params n =
+      norm_params(dq, dk, q_weight, k_weight, positions, axes, p.pairs, eps, weight_offset);
+  const auto dev = dq.device();
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  fl_norm_grads d = {};
+  view4(q, dq, "q", d.q_stride);
+  TORCH_CHECK(q.sizes() == dq.sizes(), "q must have dq's shape");
+  d.q = q.data_ptr();
+  const torch::Tensor qo = given(q_out) ? *q_out : torch::empty_like(dq);
+  view4(qo, dq, "q_out", p.q_out_stride);
+  TORCH_CHECK(qo.sizes() == dq.sizes(), "q_out must have dq's shape");
+  p.q_out = qo.data_ptr();
+  torch::Tensor ko;
+  if (given(dk)) {
+    view4(*k, dq, "k", d.k_stride);
+    TORCH_CHECK(k->sizes() == dk->sizes(), "k must have dk's shape");
+    d.k = k->data_ptr();
+    ko = given(k_out) ? *k_out : torch::empty_like(*dk);
+    view4(ko, dq, "k_out", p.k_out_stride);
+    TORCH_CHECK(ko.sizes() == dk->sizes(), "k_out must have dk's shape");
+    p.k_out = ko.data_ptr();
+  } else {
+    TORCH_CHECK(!given(k_out), "k_out= needs dk");
+  }
+  TORCH_CHECK(given(q_weight) || !given(dq_weight), "dq_weight= needs q_weight");
+  TORCH_CHECK(given(k_weight) || !given(dk_weight), "dk_weight= needs k_weight");
+  torch::Tensor dqw, dkw, ws;
+  if (given(q_weight)) {
+    dqw = output(dq_weight, {p.head_dim}, torch::kFloat32, dev, "dq_weight");
+    d.dq_weight = dqw.data_ptr<float>();
+  }
+  if (given(k_weight)) {
+    dkw = output(dk_weight, {p.head_dim}, torch::kFloat32, dev, "dk_weight");
+    d.dk_weight = dkw.data_ptr<float>();
+  }
+  const int64_t need = fl_attn_norm_rotary_workspace_bytes(&p);
+  TORCH_CHECK(need >= 0, "FlashLite HIP error: ", fl_attn_last_error());
+  if (given(q_weight) || given(k_weight)) ws = workspace_of(workspace, need, dq);
+  ok(fl_attn_norm_rotary_bwd(&p, &n, &d, ws.defined() ? ws.data_ptr() : nullptr, need,
+                             current_stream(dq)));
+  auto or_none = [](const torch::Tensor& t) -> py::object {
+    if (t.defined()) return py::cast(t);
+    return py::none();
+  };
+  return py::make_tuple(qo, or_none(ko), or_none(dqw), or_none(dkw));
+}
+
+torch::Tensor norm_rotary_to_cache(const torch::Tensor& q, const torch::Tensor& k,
+                                   const torch::Tensor& v, const OptTensor& q_weight,
+                                   const OptTensor& k_weight, const torch::Tensor& positions,
+                                   const torch::Tensor& slots, const torch::Tensor& freqs,
+                                   const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                                   const OptTensor& axes, double eps, double weight_offset,
+                                   bool interleaved, double scale, const OptTensor& out) {
+  fl_rotary_params p =
+      rotary_params(q, k, first_axis(positions, axes), freqs, interleaved, scale);
+  const fl_norm_params n =
+      norm_params(q, k, q_weight, k_weight, positions, axes, p.pairs, eps, weight_offset);
+  const fl_cache_store c = cache_store(p, q, k, v, slots, k_cache, v_cache);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  const torch::Tensor o = given(out) ? *out : torch::zeros_like(q);
+  view4(o, q, "out", p.q_out_stride);
+  TORCH_CHECK(o.sizes() == q.sizes(), "out must have q's shape");
+  p.q_out = o.data_ptr();
+  ok(fl_attn_norm_rotary_cache(&p, &n, &c, current_stream(q)));
   return o;
 }
 
@@ -596,20 +779,127 @@ py::object forward_tree(const torch::Tensor& q, const torch::Tensor& k_cache,
   const int64_t need = fl_attn_tree_workspace_bytes(&p);
   TORCH_CHECK(need >= 0, "FlashLite HIP error: ", fl_attn_last_error());
   torch::Tensor ws;
-  if (need > 0) {
-    if (given(workspace)) {
-      ws = *workspace;
-      TORCH_CHECK(ws.is_cuda() && ws.device() == dev && ws.is_contiguous(),
-                  "workspace must be a contiguous tensor on q's device");
-      TORCH_CHECK((int64_t)ws.nbytes() >= need, "workspace of ", need, " bytes needed (got ",
-                  ws.nbytes(), ")");
-    } else {
-      ws = torch::empty({(need + 3) / 4}, q.options().dtype(torch::kFloat32));
-    }
-  }
+  if (need > 0) ws = workspace_of(workspace, need, q);
   ok(fl_attn_tree_fwd(&p, need > 0 ? ws.data_ptr() : nullptr, need, current_stream(q)));
   if (return_lse) return py::make_tuple(o, l);
   return py::cast(o);
+}
+
+// ---------------------------------------------------------------------------
+// Attention over packed sequences (include/flashlite_attn.h).
+
+namespace {
+
+// A [1, heads, rows, D] view: strides {head, row}.
+void view_packed(const torch::Tensor& t, const torch::Tensor& like, const char* name,
+                 int64_t st[2]) {
+  int64_t all[3];
+  view4(t, like, name, all);
+  TORCH_CHECK(t.size(0) == 1, name, " must be [1, heads, rows, D]: packed sequences are one batch");
+  st[0] = all[1];
+  st[1] = all[2];
+}
+
+fl_packed_params packed_params(const torch::Tensor& q, const torch::Tensor& k,
+                               const torch::Tensor& v, const torch::Tensor& starts,
+                               const OptTensor& key_starts, double sm_scale, bool is_causal) {
+  TORCH_CHECK(q.is_cuda(), "All tensors must be on CUDA");
+  fl_packed_params p = {};
+  p.dtype = serve_dtype(q);
+  TORCH_CHECK(p.dtype == FL_DTYPE_F16 || p.dtype == FL_DTYPE_BF16,
+              "All tensors must be FP16 (Half), or all BF16");
+  view_packed(q, q, "q", p.q_stride);
+  view_packed(k, q, "k", p.k_stride);
+  view_packed(v, q, "v", p.v_stride);
+  p.heads = q.size(1);
+  p.rows = q.size(2);
+  p.head_dim = q.size(3);
+  p.kv_heads = k.size(1);
+  p.key_rows = k.size(2);
+  TORCH_CHECK(k.size(3) == p.head_dim && v.sizes() == k.sizes(),
+              "k and v must be [1, H_k, T_k, D] with q's D");
+  check_int32(starts, q.device(), 1, "starts");
+  TORCH_CHECK(starts.size(0) >= 1 && starts.is_contiguous(),
+              "starts must be contiguous, [sequences + 1]");
+  p.sequences = starts.size(0) - 1;
+  p.starts = starts.data_ptr<int32_t>();
+  if (given(key_starts)) {
+    check_int32(*key_starts, q.device(), 1, "key_starts");
+    TORCH_CHECK(key_starts->sizes() == starts.sizes() && key_starts->is_contiguous(),
+                "key_starts must be contiguous, with as many entries as starts");
+    p.key_starts = key_starts->data_ptr<int32_t>();
+  } else {
+    TORCH_CHECK(p.key_rows == p.rows, "k must have q's rows without key_starts");
+  }
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  for (int i = 0; i < 2; ++i) p.o_stride[i] = p.q_stride[i];
+  p.sm_scale = sm_scale;
+  p.causal = is_causal ? 1 : 0;
+  return p;
+}
+
+}  // namespace
+
+py::object forward_packed(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                          const torch::Tensor& starts, const OptTensor& key_starts,
+                          double sm_scale, bool is_causal, const OptTensor& out, bool return_lse,
+                          const OptTensor& lse) {
+  fl_packed_params p = packed_params(q, k, v, starts, key_starts, sm_scale, is_causal);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  // Rows of no sequence are not written: new outputs are zeros.
+  const torch::Tensor o = given(out) ? *out : torch::zeros_like(q);
+  view_packed(o, q, "out", p.o_stride);
+  TORCH_CHECK(o.sizes() == q.sizes(), "out must have q's shape");
+  p.o = o.data_ptr();
+  torch::Tensor l;
+  TORCH_CHECK(!given(lse) || return_lse, "lse= needs return_lse=True");
+  if (return_lse) {
+    l = output(lse, {1, p.heads, p.rows}, torch::kFloat32, q.device(), "lse");
+    if (!given(lse)) l.zero_();
+    p.lse = l.data_ptr<float>();
+  }
+  ok(fl_attn_packed_fwd(&p, current_stream(q)));
+  if (return_lse) return py::make_tuple(o, l);
+  return py::cast(o);
+}
+
+py::tuple backward_packed(const torch::Tensor& dout, const torch::Tensor& q, const torch::Tensor& k,
+                          const torch::Tensor& v, const torch::Tensor& out,
+                          const torch::Tensor& lse, const torch::Tensor& starts,
+                          const OptTensor& key_starts, double sm_scale, bool is_causal,
+                          const OptTensor& dq, const OptTensor& dk, const OptTensor& dv,
+                          const OptTensor& workspace) {
+  fl_packed_params p = packed_params(q, k, v, starts, key_starts, sm_scale, is_causal);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  fl_packed_grads d = {};
+  view_packed(out, q, "out", p.o_stride);
+  view_packed(dout, q, "dout", d.dout_stride);
+  TORCH_CHECK(out.sizes() == q.sizes() && dout.sizes() == q.sizes(),
+              "out and dout must have q's shape");
+  p.o = out.data_ptr();
+  d.dout = dout.data_ptr();
+  p.lse = output(lse, {1, p.heads, p.rows}, torch::kFloat32, q.device(), "lse").data_ptr<float>();
+  auto gradient = [&](const OptTensor& t, const torch::Tensor& like, const char* name,
+                      int64_t st[2]) {
+    const torch::Tensor x = given(t) ? *t : torch::zeros_like(like);
+    view_packed(x, q, name, st);
+    TORCH_CHECK(x.sizes() == like.sizes(), name, " must have its input's shape");
+    return x;
+  };
+  const torch::Tensor gq = gradient(dq, q, "dq", d.dq_stride);
+  const torch::Tensor gk = gradient(dk, k, "dk", d.dk_stride);
+  const torch::Tensor gv = gradient(dv, v, "dv", d.dv_stride);
+  d.dq = gq.data_ptr();
+  d.dk = gk.data_ptr();
+  d.dv = gv.data_ptr();
+  const int64_t need = fl_attn_packed_bwd_workspace_bytes(&p);
+  TORCH_CHECK(need >= 0, "FlashLite HIP error: ", fl_attn_last_error());
+  torch::Tensor ws;
+  if (need > 0) ws = workspace_of(workspace, need, q);
+  ok(fl_attn_packed_bwd(&p, &d, need > 0 ? ws.data_ptr() : nullptr, need, current_stream(q)));
+  return py::make_tuple(gq, gk, gv);
 }
 
 }  // namespace flash_attn
@@ -732,4 +1022,85 @@ PYBIND11_MODULE(flash_attn_wmma, m) {
         },
         "Workspace bytes of forward_tree for these q and k_cache (0: none is used)", py::arg("q"),
         py::arg("k_cache"));
+
+  m.def("forward_norm_rotary", &flash_attn::forward_norm_rotary,
+        "Norms of q and k (or None) [B, H, N, D] views for each head and rotary positions in one "
+        "pass: x / sqrt(mean(x x) + eps) * (weight + weight_offset), then the rotation of "
+        "forward_rotary. A weight [D] (FP32 or of q's dtype) of None leaves its tensor without a "
+        "norm. axes: int32, the axis of each pair, with positions [A, B, N] (or [A, N]). The "
+        "outputs may be the inputs. Not recorded by autograd: the gradient is "
+        "backward_norm_rotary",
+        py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"), py::arg("positions"),
+        py::arg("freqs"), py::arg("axes") = py::none(), py::arg("eps") = 1e-6,
+        py::arg("weight_offset") = 0.0, py::arg("interleaved") = false, py::arg("scale") = 1.0,
+        py::arg("q_out") = py::none(), py::arg("k_out") = py::none());
+
+  m.def("backward_norm_rotary", &flash_attn::backward_norm_rotary,
+        "The gradients of forward_norm_rotary from those of its outputs, dq and dk, and its inputs "
+        "q and k: returns (dq, dk, dq_weight, dk_weight), the weights' in FP32, None for what is "
+        "not there. q_out and k_out may be dq and dk. workspace: norm_rotary_workspace_bytes(q, k) "
+        "bytes, or one from the caching allocator; calls that may overlap on the GPU must not "
+        "share one. Not recorded by autograd itself",
+        py::arg("dq"), py::arg("dk"), py::arg("q"), py::arg("k"), py::arg("q_weight"),
+        py::arg("k_weight"), py::arg("positions"), py::arg("freqs"), py::arg("axes") = py::none(),
+        py::arg("eps") = 1e-6, py::arg("weight_offset") = 0.0, py::arg("interleaved") = false,
+        py::arg("scale") = 1.0, py::arg("q_out") = py::none(), py::arg("k_out") = py::none(),
+        py::arg("dq_weight") = py::none(), py::arg("dk_weight") = py::none(),
+        py::arg("workspace") = py::none());
+
+  m.def("norm_rotary_workspace_bytes",
+        [](const torch::Tensor& q, const std::optional<torch::Tensor>& k) {
+          (void)k;
+          TORCH_CHECK(q.dim() == 4, "q must be 4D");
+          fl_rotary_params p = {};
+          p.head_dim = q.size(3);
+          const int64_t b = fl_attn_norm_rotary_workspace_bytes(&p);
+          TORCH_CHECK(b >= 0, "FlashLite HIP error: ", fl_attn_last_error());
+          return b;
+        },
+        "Workspace bytes of backward_norm_rotary for these q and k", py::arg("q"),
+        py::arg("k") = py::none());
+
+  m.def("norm_rotary_to_cache", &flash_attn::norm_rotary_to_cache,
+        "forward_norm_rotary for a step's tokens: q goes into out, and k with v into row "
+        "slots[b][i] of the paged caches, as rotary_to_cache stores them",
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("q_weight"), py::arg("k_weight"),
+        py::arg("positions"), py::arg("slots"), py::arg("freqs"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("axes") = py::none(), py::arg("eps") = 1e-6,
+        py::arg("weight_offset") = 0.0, py::arg("interleaved") = false, py::arg("scale") = 1.0,
+        py::arg("out") = py::none());
+
+  m.def("forward_packed", &flash_attn::forward_packed,
+        "Attention over packed sequences of different lengths: q [1, H, T, D], k and v [1, H_k, "
+        "T_k, D] views (FP16 or BF16, D 64 or 128), sequence i the rows starts[i] .. starts[i + 1] "
+        "- 1 of q and key_starts[i] .. (None: the same) of k and v; starts int32 [sequences + 1]. "
+        "Grouped heads; causal: the last query sees all of its sequence's keys. Rows of no "
+        "sequence are left as they were. Returns out, or (out, lse [1, H, T]). Not recorded by "
+        "autograd: the gradient is backward_packed",
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("starts"),
+        py::arg("key_starts") = py::none(), py::arg("sm_scale") = 0.0,
+        py::arg("is_causal") = false, py::arg("out") = py::none(), py::arg("return_lse") = false,
+        py::arg("lse") = py::none());
+
+  m.def("backward_packed", &flash_attn::backward_packed,
+        "The gradients (dq, dk, dv) of forward_packed from dout and its inputs, out and lse; the "
+        "same inputs give the same bits. workspace: packed_workspace_bytes(q, k, starts) bytes, or "
+        "one from the caching allocator; calls that may overlap on the GPU must not share one. Not "
+        "recorded by autograd itself",
+        py::arg("dout"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"),
+        py::arg("starts"), py::arg("key_starts") = py::none(), py::arg("sm_scale") = 0.0,
+        py::arg("is_causal") = false, py::arg("dq") = py::none(), py::arg("dk") = py::none(),
+        py::arg("dv") = py::none(), py::arg("workspace") = py::none());
+
+  m.def("packed_workspace_bytes",
+        [](const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& starts) {
+          const fl_packed_params p =
+              flash_attn::packed_params(q, k, k, starts, starts, 0.0, false);
+          const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+          const int64_t b = fl_attn_packed_bwd_workspace_bytes(&p);
+          TORCH_CHECK(b >= 0, "FlashLite HIP error: ", fl_attn_last_error());
+          return b;
+        },
+        "Workspace bytes of backward_packed for these q, k and starts", py::arg("q"), py::arg("k"),
+        py::arg("starts"));
 }

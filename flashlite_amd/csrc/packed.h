@@ -1,0 +1,238 @@
+// Packed sequences (fl_attn_packed_fwd, fl_attn_packed_bwd): which rows a
+// work-group has, from the sequences' starts on the GPU.
+#pragma once
+
+#include "fa2_common.h"
+#include "fl_serve.h"
+
+namespace fl {
+
+namespace {
+
+// One launch over packed sequences.  Sequence i has rows starts[i] ..
+// starts[i + 1] - 1 of q and o, key_starts[i] .. of k and v.
+struct PackedGeom {
+  static constexpr bool kPacked = true;
+  long long q_sh, k_sh, v_sh, o_sh;  // elements
+  int q_sr, k_sr, v_sr, o_sr;
+  const int32_t* starts;
+  const int32_t* key_starts;
+  int sequences, rows, key_rows;
+  int heads, group;  // query heads, and those of a key head
+  int xcds;
+  float* lse;        // [heads][rows] or null
+};
+
+__device__ __forceinline__ int wave_sum(int x) {
+  return __builtin_amdgcn_readlane(wave_scan(x), 63);
+}
+
+// The rows [begin, begin + count) of sequence i; starts out of [0, rows] or
+// falling are brought into order, never followed.
+__device__ __forceinline__ void sequence_rows(const int32_t* starts, int i, int rows, int& begin,
+                                              int& count) {
+  begin = min(max(starts[i], 0), rows);
+  count = min(max(starts[i + 1], begin), rows) - begin;
+}
+
+// Block of rank r among the sequences' blocks of BLOCK rows, counted from a
+// sequence's first: the higher its index j, the earlier its rank (under a
+// causal mask the heaviest first, over all sequences), up to kRanked
+// sequences; with more the sequences follow one another.  False past the last
+// block.  The search is the same in every wave and needs no table: f(l) =
+// sum_i max(blocks_i - l, 0) blocks have j >= l.
+constexpr int kRanked = 512;
+
+// The largest of a wave's values, none negative (as wave_scan).
+__device__ __forceinline__ int wave_max(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// Blocks of sequences base + 64 c + lane (0 past the last).
+template <int BLOCK, int N>
+__device__ __forceinline__ void sequence_blocks(const int32_t* starts, int sequences, int rows,
+                                                int base, int (&nb)[N]) {
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    const int i = min(base + 64 * c + (int)(threadIdx.x & 63), sequences);
+    const int begin = min(max(starts[i], 0), rows);
+    const int end = min(max(starts[min(i + 1, sequences)], begin), rows);
+    nb[c] = i < sequences ? (end - begin + BLOCK - 1) / BLOCK : 0;
+  }
+}
+
+template <int N>
+__device__ __forceinline__ bool ranked_block(const int (&nb)[N], int r, int& seq, int& j) {
+  auto above = [&](int l) __attribute__((always_inline)) {
+    int n = 0;
+#pragma unroll
+    for (int c = 0; c < N; ++c) n += max(nb[c] - l, 0);
+    return wave_sum(n);
+  };
+  int most = 0;
+#pragma unroll
+  for (int c = 0; c < N; ++c) most = max(most, nb[c]);
+  if (r >= above(0)) return false;
+  int lo = 0, hi = wave_max(most);  // above(lo) > r >= above(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (above(mid) > r)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  r -= above(lo + 1);  // the r-th sequence with a block lo
+  j = lo;
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    const uint64_t has = __builtin_amdgcn_ballot_w64(nb[c] > lo);
+    const int n = __builtin_popcountll(has);
+    if (r < n) {
+      const int before = (int)__builtin_amdgcn_mbcnt_hi(
+          (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+      seq = 64 * c + __builtin_ctzll(__builtin_amdgcn_ballot_w64(nb[c] > lo && before == r));
+      return true;
+    }
+    r -= n;
+  }
+  return false;
+}
+
+template <int BLOCK>
+__device__ __forceinline__ bool packed_block(const int32_t* starts, int sequences, int rows, int r,
+                                             int& seq, int& j) {
+  if (sequences <= 64) {
+    int nb[1];
+    sequence_blocks<BLOCK>(starts, sequences, rows, 0, nb);
+    return ranked_block(nb, r, seq, j);
+  }
+  int nb[kRanked / 64];
+  if (sequences <= kRanked) {
+    sequence_blocks<BLOCK>(starts, sequences, rows, 0, nb);
+    return ranked_block(nb, r, seq, j);
+  }
+  for (int base = 0; base < sequences; base += kRanked) {
+    sequence_blocks<BLOCK>(starts, sequences, rows, base, nb);
+#pragma unroll
+    for (int c = 0; c < kRanked / 64; ++c) {
+      const int upto = wave_scan(nb[c]);
+      const int n = __builtin_amdgcn_readlane(upto, 63);
+      if (r < n) {
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(r < upto));
+        seq = base + 64 * c + at;
+        j = __builtin_amdgcn_readlane(upto, at) - 1 - r;
+        return true;
+      }
+      r -= n;
+    }
+  }
+  return false;
+}
+
+// Work-groups of blocks of `block` rows: at least what any sequences of these
+// rows need.
+inline int64_t packed_groups(int64_t rows, int64_t sequences, int64_t block, int64_t units) {
+  return (rows / block + sequences) * units;
+}
+
+// Work-group -> (rank, unit) with `units` independent walks of a block (heads):
+// neighbouring units, which share keys, on one XCD where they divide evenly.
+__device__ __forceinline__ void packed_unit(int units, int xcds, int& r, int& unit) {
+  const int i = blockIdx.x;
+  if (units % xcds == 0) {
+    const int per = units / xcds, k = i / xcds;
+    r = k / per;
+    unit = (i - k * xcds) * per + (k - r * per);
+  } else {
+    r = i / units;
+    unit = i - r * units;
+  }
+}
+
+// The forward kernels' problem of this work-group: query block qb (of BLOCK
+// rows) of head bh as a dense problem of one sequence, query heads that share
+// a key head as a batch with key head stride 0.  False: no block.
+template <int BLOCK, class QPtr, class KPtr, class OPtr>
+__device__ __forceinline__ bool packed_problem(const PackedGeom& p, QPtr& Q, KPtr& K, KPtr& V,
+                                               OPtr& O, Geom& g, int& bh, int& qb) {
+  int r, seq;
+  packed_unit(p.heads, p.xcds, r, bh);
+  if (!packed_block<BLOCK>(p.starts, p.sequences, p.rows, r, seq, qb)) return false;
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  int q0, k0;
+  sequence_rows(p.starts, seq, p.rows, q0, g.seq_q);
+  sequence_rows(p.key_starts, seq, p.key_rows, k0, g.seq_k);
+  g.coff = g.seq_k - g.seq_q;
+  g.heads = p.group;
+  g.q_sb = p.q_sh * p.group;
+  g.q_sh = p.q_sh;
+  g.o_sb = p.o_sh * p.group;
+  g.o_sh = p.o_sh;
+  g.k_sb = p.k_sh;
+  g.v_sb = p.v_sh;
+  g.k_sh = g.v_sh = 0;
+  g.q_sr = p.q_sr;
+  g.k_sr = p.k_sr;
+  g.v_sr = p.v_sr;
+  g.o_sr = p.o_sr;
+  Q += (long long)q0 * p.q_sr;
+  K += (long long)k0 * p.k_sr;
+  V += (long long)k0 * p.v_sr;
+  O += (long long)q0 * p.o_sr;
+  // (head_ptrs adds bh * seq_q)
+  g.lse = p.lse ? p.lse + ((long long)bh * (p.rows - g.seq_q) + q0) : nullptr;
+  return true;
+}
+
+__device__ __forceinline__ const Geom& problem_geom(const Geom& g, const Geom&) { return g; }
+__device__ __forceinline__ const Geom& problem_geom(const PackedGeom&, const Geom& own) {
+  return own;
+}
+
+template <int N>
+__device__ __forceinline__ bool any_odd(const float16_t (&x)[N]) {
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) most += x[i][r] * 0.0f;
+  return most != 0.0f;
+}
+
+// A tile's transposed operands `op` (of D columns and 8192 / 2D rows) before
+// a product whose other factor is 0 for rows of the tile that a lane's own row
+// does not see: NaN and infinities become 0, and are added to the lanes that
+// see their row (as NaN where the factor may have any sign).
+template <int D, class T, class Ops, class Sees, class Swizzle>
+__device__ __forceinline__ void add_odd(const uint8_t* tile, Ops& ops, float16_t (&acc)[D / 32],
+                                        int g, Sees&& sees, bool as_nan, Swizzle&& swizzle) {
+  using V8 = typename Elem<T>::v8;
+  V8(&op)[8] = reinterpret_cast<V8(&)[8]>(ops);
+  if (__builtin_amdgcn_ballot_w64(any_odd<T>(op)) == 0) return;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) op[u] = finite_only<T>(op[u]);
+#pragma unroll 1
+  for (int j = 0; j < kTileBytes / (2 * D); ++j) {
+    const bool mine = sees(j);
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const V8 x = *reinterpret_cast<const V8*>(tile + j * 2 * D + 16 * ((2 * c + g) ^ swizzle(j)));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = (float)x[e];
+        if (mine && !(__builtin_fabsf(y) < __builtin_huge_valf()))
+          acc[c >> 1][8 * (c & 1) + e] += as_nan ? y - y : y;
+      }
+    }
+  }
+}
+
+}  // namespace
+
+}  // namespace fl

@@ -53,36 +53,6 @@ __device__ __forceinline__ uint64_t first_bits(int n) {
   return n <= 0 ? 0 : n >= 64 ? ~(uint64_t)0 : ((uint64_t)1 << n) - 1;
 }
 
-// NaN and infinities of a V operand become 0.
-template <class T>
-__device__ __forceinline__ typename Elem<T>::v8 finite_only(const typename Elem<T>::v8& v) {
-  constexpr uint32_t kExp = sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7C00u : 0x7F80u;
-  u32x4_t x = __builtin_bit_cast(u32x4_t, v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if ((x[i] & kExp) == kExp) x[i] &= 0xFFFF0000u;
-    if ((x[i] & (kExp << 16)) == (kExp << 16)) x[i] &= 0x0000FFFFu;
-  }
-  return __builtin_bit_cast(typename Elem<T>::v8, x);
-}
-
-// Whether one of a tile's V operands is NaN or infinite: the largest of their
-// bits, signs aside.
-template <class T>
-__device__ __forceinline__ bool any_odd(const typename Elem<T>::v8 (&v)[8]) {
-  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-  constexpr uint16_t kExp = __is_same(T, _Float16) ? 0x7C00 : 0x7F80;
-  u16x2_t top = {0, 0};
-#pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const u32x4_t x = __builtin_bit_cast(u32x4_t, v[u]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, x[i] & 0x7FFF7FFFu));
-  }
-  return top[0] >= kExp || top[1] >= kExp;
-}
-
 // Where a lane's operands lie: those of Rows (head dim 64) and Rows128.
 template <int D, class T>
 struct TreeLayout;

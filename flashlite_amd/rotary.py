@@ -1,4 +1,5 @@
-"""Frequencies of the rotary operators (``forward_rotary``, ``rotary_to_cache``)."""
+"""Frequencies of the rotary operators (``forward_rotary``, ``rotary_to_cache``,
+``forward_norm_rotary``) and the axes of their pairs."""
 
 from __future__ import annotations
 
@@ -55,3 +56,22 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, method: str | None =
         freqs = freqs * (1.0 - ramp) + freqs / factor * ramp
         scale = 0.1 * math.log(factor) + 1.0
     return freqs.to(device) if device is not None else freqs, scale
+
+
+def rotary_axes(sections, interleaved: bool = False, device=None):
+    """The axis of each pair (int32 [sum(sections)]) where ``sections[a]`` pairs
+    turn by a token's position on axis a.
+
+    The sections follow one another, or with ``interleaved`` the axes take
+    turns, pair after pair, until their sections are used up (every axis then
+    has fast and slow pairs); what is left of the longer ones follows.
+    """
+    sections = [int(s) for s in sections]
+    if not sections or min(sections) < 0:
+        raise ValueError(f"sections must be counts of pairs, not negative (got {sections})")
+    if not interleaved:
+        axes = [a for a, count in enumerate(sections) for _ in range(count)]
+    else:
+        axes = [a for turn in range(max(sections)) for a, count in enumerate(sections)
+                if turn < count]
+    return torch.tensor(axes, dtype=torch.int32, device=device)

@@ -356,6 +356,59 @@ int fl_attn_rotary(const fl_rotary_params* p, void* stream);
 int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, void* stream);
 
 /*
+ * Norms of q and k for each head with the rotary positions in the same pass:
+ * y = R(x r w), r = 1 / sqrt(mean(x x) + eps) over a head's row, w its weight
+ * plus weight_offset, R the rotation above with its scale; products and sums
+ * in 32 bits, rounded once.  q_weight and k_weight are [head_dim], fp32 or of
+ * the rows' dtype (weight_dtype); NULL: that tensor is only rotated.
+ *
+ * Positions may have several axes (time, height and width of a picture's
+ * patches): with axes, int32 [pairs], pair j turns by the token's position on
+ * axis axes[j] (brought into 0 .. num_axes - 1), and positions are [num_axes,
+ * batch, rows], axis_stride elements apart.  axes NULL: one position a token.
+ *
+ * fl_attn_norm_rotary_cache stores the rows of a step's tokens as
+ * fl_attn_rotary_cache does.
+ *
+ * fl_attn_norm_rotary_bwd takes the gradients of the outputs as q and k of `p`
+ * and writes those of the inputs to its q_out and k_out (which may be the
+ * gradients' own memory): with g = R' dy, dx = r (g w - x r r mean(g w x)), and
+ * dq_weight, dk_weight = sum over batch, heads and rows of g x r, fp32
+ * [head_dim] (each NULL: not wanted).  d->q and d->k are the forward pass'
+ * inputs, not read where the weight is NULL.  The same inputs give the same
+ * bits.  The workspace (fl_attn_norm_rotary_workspace_bytes) is 16-byte aligned
+ * device memory that needs no initial values; calls that may overlap must not
+ * share one.  `transpose` is not looked at.
+ */
+typedef struct fl_norm_params {
+  const void* q_weight;
+  const void* k_weight;
+  int32_t weight_dtype;
+  double eps;
+  double weight_offset;
+  const int32_t* axes;
+  int64_t num_axes;
+  int64_t axis_stride;
+} fl_norm_params;
+
+typedef struct fl_norm_grads {
+  const void* q;
+  const void* k;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  float* dq_weight;
+  float* dk_weight;
+} fl_norm_grads;
+
+int fl_attn_norm_rotary(const fl_rotary_params* p, const fl_norm_params* n, void* stream);
+int fl_attn_norm_rotary_cache(const fl_rotary_params* p, const fl_norm_params* n,
+                              const fl_cache_store* c, void* stream);
+int64_t fl_attn_norm_rotary_workspace_bytes(const fl_rotary_params* p);
+int fl_attn_norm_rotary_bwd(const fl_rotary_params* p, const fl_norm_params* n,
+                            const fl_norm_grads* d, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
+/*
  * Attention of drafted tokens over a paged cache (fp16 or bf16, head_dim 64 or
  * 128).  Request b has lengths[b] tokens and counts[b] drafts (counts may be
  * NULL: `drafts` of them), whose keys and values are in the cache behind them,
@@ -415,6 +468,77 @@ typedef struct fl_tree_params {
 int64_t fl_attn_tree_workspace_bytes(const fl_tree_params* p);
 int fl_attn_tree_fwd(const fl_tree_params* p, void* workspace, int64_t workspace_bytes,
                      void* stream);
+
+/*
+ * Attention over packed sequences and its gradient (fp16 or bf16, head_dim 64
+ * or 128).  Sequence i has rows starts[i] .. starts[i + 1] - 1 of q and o and
+ * key_starts[i] .. key_starts[i + 1] - 1 of k and v (key_starts NULL: the same
+ * as starts, with key_rows == rows), and attends to its own keys only; either
+ * may be empty.  starts have sequences + 1 entries, which do not fall and lie in
+ * [0, rows]; others are brought into range, never followed.  q and o are [heads,
+ * rows, head_dim] and k and v [kv_heads, key_rows, head_dim] views with strides
+ * {head, row} in elements (heads in front of or behind the rows, also views of
+ * one projection); heads is a multiple of kv_heads, head h reads key/value head
+ * h / (heads / kv_heads).  With causal, query i of nq sees key j of nk iff
+ * j <= i + nk - nq.  lse: optional (forward) fp32 [heads, rows], contiguous.
+ *
+ * A row that sees nothing is 0 (its log-sum-exp -inf); rows of no sequence are
+ * neither read nor written.  What a row does not see does not reach it, NaN and
+ * infinities included, in the gradients too.
+ *
+ * fl_attn_packed_bwd takes the forward pass' o and lse and the gradient dout
+ * of o, and writes dq, dk and dv (of shared key heads: the sum over their
+ * query heads): with p = exp(s - lse) and s = sm_scale q.k, dv = p' dout,
+ * ds = p (dout v' - dout . o), dq = sm_scale ds k, dk = sm_scale ds' q.  The
+ * same inputs give the same bits.  p and ds are rounded to the element type for
+ * their products, whose sums are fp32.  dq, dk and dv must not overlap the
+ * inputs or each other; o may be q in the forward pass.  The workspace
+ * (fl_attn_packed_bwd_workspace_bytes, from the sizes; -1: `p` is rejected) is
+ * 16-byte aligned device memory that needs no initial values; calls that may
+ * overlap must not share one.
+ *
+ * Row strides are below 2^24 elements, those of q, k, v and o at least head_dim;
+ * rows and key_rows are at most 2^30, and all rows of k and of v lie within 2^31
+ * bytes of a head's first.
+ */
+typedef struct fl_packed_params {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;
+  int64_t q_stride[2];
+  int64_t k_stride[2];
+  int64_t v_stride[2];
+  int64_t o_stride[2];
+  const int32_t* starts;
+  const int32_t* key_starts;
+  int64_t sequences;
+  int64_t rows;
+  int64_t key_rows;
+  int64_t heads;
+  int64_t kv_heads;
+  int64_t head_dim;
+  double sm_scale; /* 0.0 means 1/sqrt(head_dim) */
+  int32_t causal;
+  int32_t dtype;
+} fl_packed_params;
+
+typedef struct fl_packed_grads {
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t dout_stride[2];
+  int64_t dq_stride[2];
+  int64_t dk_stride[2];
+  int64_t dv_stride[2];
+} fl_packed_grads;
+
+int fl_attn_packed_fwd(const fl_packed_params* p, void* stream);
+int64_t fl_attn_packed_bwd_workspace_bytes(const fl_packed_params* p);
+int fl_attn_packed_bwd(const fl_packed_params* p, const fl_packed_grads* d, void* workspace,
+                       int64_t workspace_bytes, void* stream);
 
 /*
  * Un-fused baseline: one work-group per query row, scores staged in LDS.
