@@ -52,6 +52,9 @@ int check_packed(const fl_packed_params* p, const char* who) {
       p->sequences > (INT64_C(1) << 24))
     return set_error(FL_ERR_UNSUPPORTED, "%s: at most 2^30 rows, 16384 heads and 2^24 sequences",
                      who);
+  if (!(std::fabs(s) >= 1e-30))
+    return set_error(FL_ERR_UNSUPPORTED, "%s: sm_scale must be at least 1e-30 in size (got %g)", who,
+                     s);
   if (p->heads > 0 && (std::max(p->rows, p->key_rows) / 32 + p->sequences) >
                           INT32_MAX / 16 / p->heads)
     return set_error(FL_ERR_UNSUPPORTED, "%s: too many work-groups", who);
@@ -99,9 +102,16 @@ int check_packed_pointers(const fl_packed_params* p, const char* who) {
 
 namespace fl {
 
+// Parts that a key block's queries are cut into, each a work-group with sums of
+// its own (packed_bwd.h): as many as bring two work-groups a CU, at most 8.
+// One a CU leaves the chip waiting for the heaviest (B2 H16/2 N7000-8192 D 128
+// causal 2690 us in one part, 1805 in two; B1 H8/1 N8192 2274 against 593 in
+// eight); with enough of them the partial sums only cost (B4 H32/8 N4096 2022
+// in one, 2105 in two).
 int packed_bwd_parts(const fl_packed_params& p) {
-  (void)p;
-  return 1;
+  const int64_t groups = (p.key_rows / 128 + p.sequences) * p.kv_heads;
+  const int64_t want = 2 * device_cus();
+  return (int)std::min<int64_t>(8, std::max<int64_t>(1, (want + groups / 2) / groups));
 }
 
 }  // namespace fl

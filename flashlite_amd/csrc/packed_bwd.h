@@ -29,7 +29,7 @@ struct BwdGeom {
   const void *q, *k, *v, *o, *dout;
   void *dq, *dk, *dv;
   const float* lse;       // [heads][rows]
-  float2* stats;          // [heads][rows]: lse in base 2, delta
+  float2* stats;          // [heads][rows]: -lse / scale, -delta
   float* part;            // [parts][kv_heads][key_rows][2 D], or null
   long long q_sh, k_sh, v_sh, o_sh, do_sh, dq_sh, dk_sh, dv_sh;  // elements
   int q_sr, k_sr, v_sr, o_sr, do_sr, dq_sr, dk_sr, dv_sr;
@@ -120,6 +120,44 @@ struct BwdLane {
   }
 };
 
+// The same operands by LDS address: what varies from lane to lane is kept in
+// registers, a tile's place is added.
+template <int D, class T>
+struct TileOps {
+  using L = BwdLane<D, T>;
+  using V8 = typename L::V8;
+  using V4 = typename L::V4;
+  typedef const V8 __attribute__((address_space(3))) * LdsV8;
+  typedef short4_t __attribute__((address_space(3))) * LdsTr;
+  uint32_t row_at[L::kSteps], col_at[L::kCols][2];
+
+  __device__ __forceinline__ explicit TileOps(const L& ln) {
+#pragma unroll
+    for (int st = 0; st < L::kSteps; ++st)
+      row_at[st] = ln.col * L::kRowB + 16 * ((2 * st + ln.g) ^ both_swz<D>(ln.col));
+#pragma unroll
+    for (int c = 0; c < L::kCols; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = ln.tr_row + 8 * h, x = 32 * c + ln.tr_col;
+        col_at[c][h] = row * L::kRowB + 16 * ((x >> 3) ^ both_swz<D>(row)) + 8 * ((x >> 2) & 1);
+      }
+  }
+  // Rows 32 b .. at columns 16 st .., `off` bytes behind the tile.
+  __device__ __forceinline__ V8 rows(uint32_t tile, int off, int b, int st) const {
+    return *(LdsV8)(uintptr_t)(tile + row_at[st] + (off + 32 * b * L::kRowB));
+  }
+  // Columns 32 c .. of rows 16 t .., transposed.
+  __device__ __forceinline__ V8 cols(uint32_t tile, int off, int c, int t) const {
+    const uint32_t o = off + 16 * t * L::kRowB;
+    const V4 a = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                            (LdsTr)(uintptr_t)(tile + col_at[c][0] + o)));
+    const V4 b = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                            (LdsTr)(uintptr_t)(tile + col_at[c][1] + o)));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
 __device__ __forceinline__ float16_t zero16() {
   return (float16_t){0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 }
@@ -138,13 +176,21 @@ __device__ __forceinline__ i32x4_t rows_rsrc(const void* x, int n, int row_bytes
 
 // At most `most` of the `left` rows (scalar: not a vector median).
 __device__ __forceinline__ int tile_rows(int left, int most) {
-  left = min(left, most);
+  left = __builtin_amdgcn_readfirstlane(min(left, most));
   asm("" : "+s"(left));
   return max(left, 0);
 }
 
-// DMA of tiles: wave w moves kSegs of a tile's 8 segments of 1 KiB, each lane
-// 16 bytes.
+// A pointer that is the same in every lane, in scalar registers.
+__device__ __forceinline__ uint8_t* uniform(uint8_t* x) {
+  const uint64_t a = (uint64_t)(uintptr_t)x;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
+  return (uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+
+// DMA of tiles: wave w moves kSegs segments of 1 KiB of a tile, each lane 16
+// bytes.
 template <int D, int kSegs>
 struct TileFetch {
   int lane[kSegs];
@@ -154,20 +200,26 @@ struct TileFetch {
     for (int i = 0; i < kSegs; ++i) {
       const int row = kSegRows * (wave * kSegs + i) + l / kChunks;
       lane[i] = row * row_bytes + 16 * ((l % kChunks) ^ both_swz<D>(row));
+      asm volatile("" : "+v"(lane[i]));  // (kept, not derived again)
     }
   }
-  // The rows row0 .. of x (those from `rows` on as zeros).
-  template <class T>
-  __device__ __forceinline__ void run(const T* x, int row_bytes, int row0, int rows,
-                                      const uint8_t* slot, int wave) const {
-    constexpr int kRows = kTileBytes / (2 * D);
-    const i32x4_t rs =
-        rows_rsrc<2 * D>(reinterpret_cast<const uint8_t*>(x) + (long long)row0 * row_bytes,
-                         tile_rows(rows - row0, kRows), row_bytes);
+  __device__ __forceinline__ void seg(const i32x4_t& rs, const uint8_t* slot, int wave,
+                                      int i) const {
+    load_lds16(rs, lane[i], slot + 1024 * (wave * kSegs + i));
+  }
+  __device__ __forceinline__ void run(const i32x4_t& rs, const uint8_t* slot, int wave) const {
 #pragma unroll
-    for (int i = 0; i < kSegs; ++i) load_lds16(rs, lane[i], slot + 1024 * (wave * kSegs + i));
+    for (int i = 0; i < kSegs; ++i) seg(rs, slot, wave, i);
   }
 };
+
+// Rows row0 .. of the `rows` rows of x, at most `most`, as a resource.
+template <int kRowB, class T>
+__device__ __forceinline__ i32x4_t tile_rsrc(const T* x, int row_bytes, int row0, int rows,
+                                             int most) {
+  return rows_rsrc<kRowB>(reinterpret_cast<const uint8_t*>(x) + (long long)row0 * row_bytes,
+                          tile_rows(rows - row0, most), row_bytes);
+}
 
 // 4 bytes a lane into LDS at slot + 4 * lane (as load_lds16).
 __device__ __forceinline__ void load_lds4(const i32x4_t& rs, int voff, const uint8_t* slot) {
@@ -176,249 +228,614 @@ __device__ __forceinline__ void load_lds4(const i32x4_t& rs, int voff, const uin
                : : "v"(voff), "s"(rs), "{m0}"(lds_base));
 }
 
-constexpr int kBwdSlots = 3;
+// A block's transposed operands (32 rows from `rows` on) before a product
+// whose other factor is 0 for rows that a lane's own row does not see: NaN and
+// infinities become 0, and are added to the lanes that see their row (as NaN
+// where the factor may have any sign).
+template <int D, class T, class Sees>
+__device__ __forceinline__ void add_odd_block(const uint8_t* rows,
+                                              typename Elem<T>::v8 (&op)[D / 16],
+                                              float16_t (&acc)[D / 32], int g, Sees&& sees,
+                                              bool as_nan) {
+  using V8 = typename Elem<T>::v8;
+#pragma unroll
+  for (int u = 0; u < D / 16; ++u) op[u] = finite_only<T>(op[u]);
+#pragma unroll 1
+  for (int j = 0; j < 32; ++j) {
+    const bool mine = sees(j);
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const V8 x =
+          *reinterpret_cast<const V8*>(rows + j * 2 * D + 16 * ((2 * c + g) ^ both_swz<D>(j)));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = (float)x[e];
+        if (mine && !(__builtin_fabsf(y) < __builtin_huge_valf()))
+          acc[c >> 1][8 * (c & 1) + e] += as_nan ? y - y : y;
+      }
+    }
+  }
+}
 
-// dq of W x 32 query rows, and the rows' lse and delta.
-template <int D, int W, class T>
-__global__ void __launch_bounds__(64 * W, 2) packed_dq_kernel(const BwdGeom p) {
-  using L = BwdLane<D, T>;
-  using V8 = typename L::V8;
-  using E = Elem<T>;
-  constexpr int kSegs = 8 / W;
-  __shared__ __attribute__((aligned(16))) uint8_t ring[kBwdSlots][2][kTileBytes];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const L ln(threadIdx.x & 63);
-  int r, head, seq, qb;
-  packed_unit(p.heads, p.xcds, r, head);
-  if (!packed_block<32 * W>(p.starts, p.sequences, p.rows, r, seq, qb)) return;
+// A work-group's query block of the dq kernel.
+struct DqTask {
+  int head, kv, q0, nq, k0, nk, coff, first, tiles;
+};
+
+template <int D, int W>
+__device__ __forceinline__ bool dq_task(const BwdGeom& p, DqTask& x) {
+  int r, seq, qb;
+  packed_unit(p.heads, p.xcds, r, x.head);
+  if (!packed_block<32 * W>(p.starts, p.sequences, p.rows, r, seq, qb)) return false;
   seq = __builtin_amdgcn_readfirstlane(seq);
-  int q0, nq, k0, nk;
-  sequence_rows(p.starts, seq, p.rows, q0, nq);
-  sequence_rows(p.key_starts, seq, p.key_rows, k0, nk);
-  const int coff = p.causal ? nk - nq : nk;  // query i sees keys up to i + coff
-  const int kv = head / p.group;
-  const T* const K = static_cast<const T*>(p.k) + (kv * p.k_sh + (long long)k0 * p.k_sr);
-  const T* const V = static_cast<const T*>(p.v) + (kv * p.v_sh + (long long)k0 * p.v_sr);
-  const int first = qb * 32 * W, qw = first + 32 * wave, my = qw + ln.col;
-  int tiles = (min(nk, min(first + 32 * W, nq) + coff) + L::kRows - 1) / L::kRows;
-  tiles = max(tiles, 0);
+  sequence_rows(p.starts, seq, p.rows, x.q0, x.nq);
+  sequence_rows(p.key_starts, seq, p.key_rows, x.k0, x.nk);
+  x.coff = p.causal ? x.nk - x.nq : x.nk;  // query i sees keys up to i + coff
+  x.kv = x.head / p.group;
+  x.first = qb * 32 * W;
+  constexpr int kRows = kTileBytes / (2 * D);
+  x.tiles = max((min(x.nk, min(x.first + 32 * W, x.nq) + x.coff) + kRows - 1) / kRows, 0);
+  return true;
+}
 
-  const TileFetch<D, kSegs> fk(wave, ln.lane, 2 * p.k_sr), fv(wave, ln.lane, 2 * p.v_sr);
-  auto fetch = [&](int t) __attribute__((always_inline)) {
-    const int s = t % kBwdSlots, rows = t < tiles ? nk : 0;
-    fk.run(K, 2 * p.k_sr, t * L::kRows, rows, ring[s][0], wave);
-    fv.run(V, 2 * p.v_sr, t * L::kRows, rows, ring[s][1], wave);
-  };
-  fetch(0);
-  fetch(1);
-  V8 qf[L::kSteps], df[L::kSteps];
+// This lane's rows of a query block: q and dout as B operands, lse in base 2
+// and delta.
+template <int D, class T>
+struct DqRows {
+  using L = BwdLane<D, T>;
+  typename L::V8 qf[L::kSteps], df[L::kSteps];
   float lse2, delta;
-  {
-    V8 of[L::kSteps];
-    ln.own_rows(static_cast<const T*>(p.q) + (head * p.q_sh + (long long)q0 * p.q_sr), p.q_sr, my,
-                nq, qf);
-    ln.own_rows(static_cast<const T*>(p.dout) + (head * p.do_sh + (long long)q0 * p.do_sr),
-                p.do_sr, my, nq, df);
-    ln.own_rows(static_cast<const T*>(p.o) + (head * p.o_sh + (long long)q0 * p.o_sr), p.o_sr, my,
-                nq, of);
+
+  __device__ __forceinline__ void load(const BwdGeom& p, const DqTask& x, const L& ln, int my) {
+    typename L::V8 of[L::kSteps];
+    ln.own_rows(static_cast<const T*>(p.q) + (x.head * p.q_sh + (long long)x.q0 * p.q_sr), p.q_sr,
+                my, x.nq, qf);
+    ln.own_rows(static_cast<const T*>(p.dout) + (x.head * p.do_sh + (long long)x.q0 * p.do_sr),
+                p.do_sr, my, x.nq, df);
+    ln.own_rows(static_cast<const T*>(p.o) + (x.head * p.o_sh + (long long)x.q0 * p.o_sr), p.o_sr,
+                my, x.nq, of);
     float sum = 0.0f;
 #pragma unroll
     for (int st = 0; st < L::kSteps; ++st)
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)df[st][e], (float)of[st][e], sum);
     delta = pair_sum(sum);
-    const long long at = (long long)head * p.rows + q0 + my;
-    const float lse = my < nq ? p.lse[at] : 0.0f;
+    const float lse = my < x.nq ? p.lse[(long long)x.head * p.rows + x.q0 + my] : 0.0f;
     // (a row that sees nothing: p = 2^-inf)
     lse2 = lse == ninf() ? -ninf() : lse * 1.44269504088896341f;
-    if (my < nq && ln.g == 0) p.stats[at] = make_float2(lse2, delta);
   }
-  // (what the compiler sees of the loads is then done: no waits in the loop)
-  __builtin_amdgcn_s_waitcnt(0);
-  float16_t acc[L::kCols];
-#pragma unroll
-  for (int c = 0; c < L::kCols; ++c) acc[c] = zero16();
-  const int lim = min(nk, my + coff + 1);  // keys that this lane's row sees
-  for (int t = 0; t < tiles; ++t) {
-    sync_ring<2 * kSegs>();
-    fetch(t + 2);
-    const int base = t * L::kRows;
-    if (base > min(qw + 31, nq - 1) + coff || qw >= nq) continue;  // nothing seen by this wave
-    const uint8_t* const kt = ring[t % kBwdSlots][0];
-    const uint8_t* const vt = ring[t % kBwdSlots][1];
-    const bool edge = base + L::kRows > min(nk, qw + coff + 1);
-    V8 ds[L::kBlocks][2];
-#pragma unroll
-    for (int b = 0; b < L::kBlocks; ++b) {
-      float16_t s = zero16(), dp = zero16();
-#pragma unroll
-      for (int st = 0; st < L::kSteps; ++st) s = E::mfma(ln.rows_op(kt, b, st), qf[st], s);
-#pragma unroll
-      for (int st = 0; st < L::kSteps; ++st) dp = E::mfma(ln.rows_op(vt, b, st), df[st], dp);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], p.scale_log2, -lse2));
-        float x = e * (dp[i] - delta);
-        if (edge && base + 32 * b + 8 * (i >> 2) + 4 * ln.g + (i & 3) >= lim) x = 0.0f;
-        ds[b][i >> 3][i & 7] = (T)x;
-      }
-    }
-    V8 ka[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) ka[u] = ln.cols_op(kt, u % L::kCols, u / L::kCols);
-    if (edge)
-      add_odd<D, T>(
-          kt, ka, acc, ln.g, [&](int j) { return base + j < lim; }, true,
-          [](int row) { return both_swz<D>(row); });
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int tt = u / L::kCols;
-      acc[u % L::kCols] = E::mfma(ka[u], ds[tt >> 1][tt & 1], acc[u % L::kCols]);
-    }
-  }
-  __builtin_amdgcn_s_waitcnt(0);
-  ln.store(static_cast<T*>(p.dq) + (head * p.dq_sh + (long long)q0 * p.dq_sr), p.dq_sr, my, nq,
-           p.scale, acc);
-}
+};
 
-// dk and dv of W x 32 keys over part `part` of the queries that see them, of
-// all heads of the group one after the other.
-template <int D, int W, class T, int OCC>
-__global__ void __launch_bounds__(64 * W, OCC) packed_dkv_kernel(const BwdGeom p) {
+// The dq kernel's block walked again, with NaN and infinities of keys that rows
+// do not see kept from them.  (A function of its own: its registers are not
+// the kernel's.)
+template <int D, int W, class T>
+__device__ __attribute__((noinline)) void dq_checked(const void* geom, uint8_t* lds) {
   using L = BwdLane<D, T>;
   using V8 = typename L::V8;
   using E = Elem<T>;
-  constexpr int kSegs = 8 / W;
-  constexpr int kStatB = 2 * 4 * L::kRows, kStatLoads = L::kRows / 32;
-  constexpr int kLoads = 2 * kSegs + kStatLoads;
-  __shared__ __attribute__((aligned(16))) uint8_t ring[kBwdSlots][2][kTileBytes];
-  __shared__ __attribute__((aligned(16))) uint8_t stat[kBwdSlots][kStatB];
+  lds = uniform(lds);
+  BwdGeom p;
+  __builtin_memcpy(&p, geom, sizeof p);
+  DqTask x;
+  if (!dq_task<D, W>(p, x)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const L ln(threadIdx.x & 63);
-  int r, unit, seq, kb;
-  packed_unit(p.kv_heads * p.parts, p.xcds, r, unit);
-  if (!packed_block<32 * W>(p.key_starts, p.sequences, p.key_rows, r, seq, kb)) return;
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  const int kv = unit / p.parts, part = unit - kv * p.parts;
-  int q0, nq, k0, nk;
-  sequence_rows(p.starts, seq, p.rows, q0, nq);
-  sequence_rows(p.key_starts, seq, p.key_rows, k0, nk);
-  // (the last index is the heaviest under a causal mask: the first keys)
-  kb = (nk + 32 * W - 1) / (32 * W) - 1 - kb;
-  const int coff = p.causal ? nk - nq : nk;
-  const int first = kb * 32 * W, kw = first + 32 * wave, my = kw + ln.col;
-  const int tbeg = max(first - coff, 0) / L::kRows;
-  const int per = max((nq + L::kRows - 1) / L::kRows - tbeg, 0);  // tiles a head
-  const int all = per * p.group;
-  const int s0 = (int)((long long)all * part / p.parts);
-  const int s1 = (int)((long long)all * (part + 1) / p.parts);
-  const int h0 = per > 0 ? s0 / per : 0;
+  const int my = x.first + 32 * wave + ln.col;
+  const T* const K = static_cast<const T*>(p.k) + (x.kv * p.k_sh + (long long)x.k0 * p.k_sr);
+  const T* const V = static_cast<const T*>(p.v) + (x.kv * p.v_sh + (long long)x.k0 * p.v_sr);
+  const TileFetch<D, 8 / W> fk(wave, ln.lane, 2 * p.k_sr), fv(wave, ln.lane, 2 * p.v_sr);
+  DqRows<D, T> rows;
+  rows.load(p, x, ln, my);
+  float16_t acc[L::kCols];
+#pragma unroll
+  for (int c = 0; c < L::kCols; ++c) acc[c] = zero16();
+  const int lim = min(x.nk, my + x.coff + 1);  // keys that this lane's row sees
+#pragma unroll 1
+  for (int t = 0; t < x.tiles; ++t) {
+    const int base = t * L::kRows;
+    fk.run(tile_rsrc<2 * D>(K, 2 * p.k_sr, base, x.nk, L::kRows), lds, wave);
+    fv.run(tile_rsrc<2 * D>(V, 2 * p.v_sr, base, x.nk, L::kRows), lds + kTileBytes, wave);
+    sync_ring<0>();
+#pragma unroll 1
+    for (int b = 0; b < L::kBlocks; ++b) {
+      float16_t s = zero16(), dp = zero16();
+      V8 ds[2], ka[D / 16];
+#pragma unroll
+      for (int st = 0; st < L::kSteps; ++st) s = E::mfma(ln.rows_op(lds, b, st), rows.qf[st], s);
+#pragma unroll
+      for (int st = 0; st < L::kSteps; ++st)
+        dp = E::mfma(ln.rows_op(lds + kTileBytes, b, st), rows.df[st], dp);
+      auto sees = [&](int j) { return base + 32 * b + j < lim; };
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], p.scale_log2, -rows.lse2));
+        const float y = e * (dp[i] - rows.delta);
+        ds[i >> 3][i & 7] = (T)(sees(8 * (i >> 2) + 4 * ln.g + (i & 3)) ? y : 0.0f);
+      }
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u)
+        ka[u] = ln.cols_op(lds, u % L::kCols, 2 * b + u / L::kCols);
+      add_odd_block<D, T>(lds + 32 * b * L::kRowB, ka, acc, ln.g, sees, true);
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u)
+        acc[u % L::kCols] = E::mfma(ka[u], ds[u / L::kCols], acc[u % L::kCols]);
+    }
+    sync_ring<0>();
+  }
+  ln.store(static_cast<T*>(p.dq) + (x.head * p.dq_sh + (long long)x.q0 * p.dq_sr), p.dq_sr, my,
+           x.nq, p.scale, acc);
+}
 
-  const TileFetch<D, kSegs> fq(wave, ln.lane, 2 * p.q_sr), fd(wave, ln.lane, 2 * p.do_sr);
-  // The fetched step's head of the group and tile, kFetch steps ahead.
-  int fh = h0, ft = tbeg + (s0 - h0 * per), fs = s0;
-  auto fetch = [&]() __attribute__((always_inline)) {
-    const int s = (fs - s0) % kBwdSlots, rows = fs < s1 ? nq : 0;
-    const long long head = kv * p.group + min(fh, p.group - 1);
-    fq.run(static_cast<const T*>(p.q) + (head * p.q_sh + (long long)q0 * p.q_sr), 2 * p.q_sr,
-           ft * L::kRows, rows, ring[s][0], wave);
-    fd.run(static_cast<const T*>(p.dout) + (head * p.do_sh + (long long)q0 * p.do_sr),
-           2 * p.do_sr, ft * L::kRows, rows, ring[s][1], wave);
-    // every wave all of them, to the same place: its own wait then covers them
-    const i32x4_t rs =
-        rows_rsrc<8>(p.stats + (head * p.rows + q0 + (long long)ft * L::kRows),
-                     tile_rows(rows - ft * L::kRows, L::kRows), 8);
-#pragma unroll
-    for (int i = 0; i < kStatLoads; ++i) {
-      const int x = 64 * i + ln.lane;
-      load_lds4(rs, 8 * (x % L::kRows) + 4 * (x / L::kRows), stat[s] + 256 * i);
-    }
-    ++fs;
-    if (++ft == tbeg + per) {
-      ft = tbeg;
-      ++fh;
-    }
+// dq of W x 32 query rows, and the rows' {-lse / scale, -delta}.
+template <int D, int W, class T>
+__global__ void __launch_bounds__(64 * W, 2) packed_dq_kernel(const BwdGeom p) {
+  using L = BwdLane<D, T>;
+  using V8 = typename L::V8;
+  using E = Elem<T>;
+  constexpr int kSegs = 8 / W, kSlots = 3;
+  __shared__ __attribute__((aligned(16))) uint8_t ring[kSlots][2][kTileBytes];
+  const void* const geom = (const void*)__builtin_amdgcn_kernarg_segment_ptr();
+  DqTask x;
+  if (!dq_task<D, W>(p, x)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const L ln(threadIdx.x & 63);
+  const int qw = x.first + 32 * wave, my = qw + ln.col;
+  const T* const K = static_cast<const T*>(p.k) + (x.kv * p.k_sh + (long long)x.k0 * p.k_sr);
+  const T* const V = static_cast<const T*>(p.v) + (x.kv * p.v_sh + (long long)x.k0 * p.v_sr);
+  const TileFetch<D, kSegs> fk(wave, ln.lane, 2 * p.k_sr), fv(wave, ln.lane, 2 * p.v_sr);
+  auto fetch = [&](int t, int s) __attribute__((always_inline)) {
+    const int rows = t < x.tiles ? x.nk : 0;
+    fk.run(tile_rsrc<2 * D>(K, 2 * p.k_sr, t * L::kRows, rows, L::kRows), ring[s][0], wave);
+    fv.run(tile_rsrc<2 * D>(V, 2 * p.v_sr, t * L::kRows, rows, L::kRows), ring[s][1], wave);
   };
-  fetch();
-  fetch();
-  V8 kf[L::kSteps], vf[L::kSteps];
-  ln.own_rows(static_cast<const T*>(p.k) + (kv * p.k_sh + (long long)k0 * p.k_sr), p.k_sr, my, nk,
-              kf);
-  ln.own_rows(static_cast<const T*>(p.v) + (kv * p.v_sh + (long long)k0 * p.v_sr), p.v_sr, my, nk,
-              vf);
+  fetch(0, 0);
+  fetch(1, 1);
+  DqRows<D, T> rows;
+  rows.load(p, x, ln, my);
+  if (my < x.nq && ln.g == 0) {
+    const float lse = rows.lse2 * 0.693147180559945309f;
+    const float start = lse == -ninf() ? (p.scale > 0.0f ? ninf() : -ninf()) : -lse / p.scale;
+    p.stats[(long long)x.head * p.rows + x.q0 + my] = make_float2(start, -rows.delta);
+  }
+  // (what the compiler sees of the loads is then done: no waits in the loop)
   __builtin_amdgcn_s_waitcnt(0);
-  float16_t dk[L::kCols], dv[L::kCols];
+  const TileOps<D, T> ops(ln);
+  const uint32_t lds = (uint32_t)(uintptr_t)&ring[0][0][0];
+  float16_t acc[L::kCols];
 #pragma unroll
-  for (int c = 0; c < L::kCols; ++c) dk[c] = dv[c] = zero16();
-  int t = tbeg + (s0 - h0 * per);
-  for (int step = s0; step < s1; ++step) {
-    sync_ring<kLoads>();
-    fetch();
-    const int base = t * L::kRows, s = (step - s0) % kBwdSlots;
-    if (++t == tbeg + per) t = tbeg;
-    // (queries of the tile that see one of this wave's keys)
-    if (min(base + L::kRows, nq) - 1 + coff < kw || kw >= nk) continue;
-    const uint8_t* const qt = ring[s][0];
-    const uint8_t* const dt = ring[s][1];
-    const float* const st_lse = reinterpret_cast<const float*>(stat[s]);
-    const float* const st_delta = st_lse + L::kRows;
-    const bool edge = base + L::kRows > nq || base + coff < kw + 31;
-    const int lo = my - coff;  // queries from lo on see this lane's key
-    V8 pp[L::kBlocks][2], ds[L::kBlocks][2];
+  for (int c = 0; c < L::kCols; ++c) acc[c] = zero16();
+  const int lim = min(x.nk, my + x.coff + 1);  // keys that this lane's row sees
+  int s = 0;
+  for (int t = 0; t < x.tiles; ++t) {
+    sync_ring<2 * kSegs>();
+    fetch(t + 2, s == 0 ? 2 : s - 1);
+    const int base = t * L::kRows;
+    const uint32_t kt = lds + s * 2 * kTileBytes;
+    s = s == 2 ? 0 : s + 1;
+    if (base > min(qw + 31, x.nq - 1) + x.coff || qw >= x.nq) continue;  // nothing seen here
+    const bool edge = base + L::kRows > min(x.nk, qw + x.coff + 1);
 #pragma unroll
     for (int b = 0; b < L::kBlocks; ++b) {
       float16_t sc = zero16(), dp = zero16();
+      V8 ds[2];
 #pragma unroll
-      for (int st = 0; st < L::kSteps; ++st) sc = E::mfma(ln.rows_op(qt, b, st), kf[st], sc);
+      for (int st = 0; st < L::kSteps; ++st)
+        sc = E::mfma(ops.rows(kt, 0, b, st), rows.qf[st], sc);
 #pragma unroll
-      for (int st = 0; st < L::kSteps; ++st) dp = E::mfma(ln.rows_op(dt, b, st), vf[st], dp);
+      for (int st = 0; st < L::kSteps; ++st)
+        dp = E::mfma(ops.rows(kt, kTileBytes, b, st), rows.df[st], dp);
+      if (edge) {
+        const float hidden = p.scale > 0.0f ? ninf() : -ninf();
 #pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        const int at = 32 * b + 8 * i4 + 4 * ln.g;
-        const float4 ls = *reinterpret_cast<const float4*>(st_lse + at);
-        const float4 de = *reinterpret_cast<const float4*>(st_delta + at);
-        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dev[4] = {de.x, de.y, de.z, de.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 4 * i4 + e, q = base + at + e;
-          float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.scale_log2, -lsv[e]));
-          float y = x * (dp[i] - dev[e]);
-          if (edge && (q < lo || q >= nq)) x = y = 0.0f;
-          pp[b][i >> 3][i & 7] = (T)x;
-          ds[b][i >> 3][i & 7] = (T)y;
-        }
+        for (int i = 0; i < 16; ++i)
+          if (base + 32 * b + 8 * (i >> 2) + 4 * ln.g + (i & 3) >= lim) sc[i] = hidden;
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.scale_log2, -rows.lse2));
+        ds[i >> 3][i & 7] = (T)(e * (dp[i] - rows.delta));
+      }
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u)
+        acc[u % L::kCols] = E::mfma(ops.cols(kt, 0, u % L::kCols, 2 * b + u / L::kCols),
+                                    ds[u / L::kCols], acc[u % L::kCols]);
     }
-    auto add = [&](const uint8_t* tile, float16_t (&acc)[L::kCols], const V8 (&w)[L::kBlocks][2],
-                   bool as_nan) __attribute__((always_inline)) {
-      V8 a[8];
+  }
+  // A block with a row whose sum is not finite is walked again.
+  __builtin_amdgcn_s_waitcnt(0);
+  int* const redo = reinterpret_cast<int*>(ring);
+  __syncthreads();
+  if (threadIdx.x == 0) *redo = 0;
+  __syncthreads();
+  if (my < x.nq && any_odd(acc)) *redo = 1;
+  __syncthreads();
+  const bool again = *redo != 0;
+  __syncthreads();
+  if (again)
+    dq_checked<D, W, T>(geom, &ring[0][0][0]);
+  else
+    ln.store(static_cast<T*>(p.dq) + (x.head * p.dq_sh + (long long)x.q0 * p.dq_sr), p.dq_sr, my,
+             x.nq, p.scale, acc);
+}
+
+// A work-group's key block, and its share of the queries that see it.
+struct DkvTask {
+  int kv, part, q0, nq, k0, nk, coff, first;
+  int tbeg, per, steps, h0, t0;  // a head's first tile and tiles; steps from head h0, tile t0 on
+};
+
+constexpr int kDkvWaves = 4, kDkvRows = 64;  // query rows of a tile
+
+__device__ __forceinline__ bool dkv_task(const BwdGeom& p, DkvTask& x) {
+  int r, unit, seq, kb;
+  packed_unit(p.kv_heads * p.parts, p.xcds, r, unit);
+  constexpr int kBlock = 32 * kDkvWaves;
+  if (!packed_block<kBlock>(p.key_starts, p.sequences, p.key_rows, r, seq, kb)) return false;
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  x.kv = unit / p.parts;
+  x.part = unit - x.kv * p.parts;
+  sequence_rows(p.starts, seq, p.rows, x.q0, x.nq);
+  sequence_rows(p.key_starts, seq, p.key_rows, x.k0, x.nk);
+  // (the last index is the heaviest under a causal mask: the first keys)
+  x.first = ((x.nk + kBlock - 1) / kBlock - 1 - kb) * kBlock;
+  x.coff = p.causal ? x.nk - x.nq : x.nk;
+  x.tbeg = max(x.first - x.coff, 0) / kDkvRows;
+  x.per = max((x.nq + kDkvRows - 1) / kDkvRows - x.tbeg, 0);
+  const int all = x.per * p.group;
+  const int s0 = (int)((long long)all * x.part / p.parts);
+  x.steps = (int)((long long)all * (x.part + 1) / p.parts) - s0;
+  x.h0 = x.per > 0 ? s0 / x.per : 0;
+  x.t0 = x.tbeg + (s0 - x.h0 * x.per);
+  return true;
+}
+
+// The tiles of a walk, one after the other: the queries of a head, then those
+// of the next.  A wave moves its share of q's and dout's rows and all of the
+// statistics (every wave to the same place: its own wait then covers them).
+template <int D, class T>
+struct DkvFetch {
+  static constexpr int kTileB = kDkvRows * 2 * D, kSegs = kTileB / 1024 / kDkvWaves;
+  static constexpr int kDma = 2 * kSegs + 2;  // instructions of a wave
+  const TileFetch<D, kSegs> fq, fd;
+  int step, head, tile, wave, lane;
+  i32x4_t rq, rd, rst;
+
+  __device__ __forceinline__ DkvFetch(const BwdGeom& p, const DkvTask& x, int wave_, int lane_)
+      : fq(wave_, lane_, 2 * p.q_sr), fd(wave_, lane_, 2 * p.do_sr) {
+    wave = wave_;
+    lane = lane_;
+    step = 0;
+    head = x.kv * p.group + x.h0;
+    tile = x.t0;
+  }
+  // On to the next tile (past the last: zeros).
+  __device__ __forceinline__ void next(const BwdGeom& p, const DkvTask& x) {
+    const int rows = step < x.steps ? x.nq : 0;
+    const long long h = min(head, p.heads - 1);
+    rq = tile_rsrc<2 * D>(static_cast<const T*>(p.q) + (h * p.q_sh + (long long)x.q0 * p.q_sr),
+                          2 * p.q_sr, tile * kDkvRows, rows, kDkvRows);
+    rd = tile_rsrc<2 * D>(
+        static_cast<const T*>(p.dout) + (h * p.do_sh + (long long)x.q0 * p.do_sr), 2 * p.do_sr,
+        tile * kDkvRows, rows, kDkvRows);
+    rst = tile_rsrc<8>(p.stats + (h * p.rows + x.q0), 8, tile * kDkvRows, rows, kDkvRows);
+    ++step;
+    if (++tile == x.tbeg + x.per) {
+      tile = x.tbeg;
+      ++head;
+    }
+  }
+  // Its i-th instruction.
+  __device__ __forceinline__ void dma(const uint8_t* slot, const uint8_t* stat, int i) const {
+    if (i < kSegs)
+      fq.seg(rq, slot, wave, i);
+    else if (i < 2 * kSegs)
+      fd.seg(rd, slot + kTileB, wave, i - kSegs);
+    else
+      load_lds4(rst, 8 * lane + 4 * (i - 2 * kSegs), stat + 256 * (i - 2 * kSegs));
+  }
+  __device__ __forceinline__ void run(const BwdGeom& p, const DkvTask& x, const uint8_t* slot,
+                                      const uint8_t* stat) {
+    next(p, x);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) a[u] = ln.cols_op(tile, u % L::kCols, u / L::kCols);
-      if (edge)
-        add_odd<D, T>(
-            tile, a, acc, ln.g, [&](int j) { return base + j >= lo && base + j < nq; }, as_nan,
-            [](int row) { return both_swz<D>(row); });
+    for (int i = 0; i < kDma; ++i) dma(slot, stat, i);
+  }
+};
+
+template <int D, class T>
+__device__ __forceinline__ void dkv_store(const BwdGeom& p, const DkvTask& x,
+                                          const BwdLane<D, T>& ln, int my,
+                                          const float16_t (&dk)[D / 32],
+                                          const float16_t (&dv)[D / 32]) {
+  if (p.parts > 1) {
+    float* const to =
+        p.part + (((long long)x.part * p.kv_heads + x.kv) * p.key_rows + x.k0) * (2 * D);
+    ln.store_part(to, my, x.nk, dk);
+    ln.store_part(to + D, my, x.nk, dv);
+  } else {
+    ln.store(static_cast<T*>(p.dk) + (x.kv * p.dk_sh + (long long)x.k0 * p.dk_sr), p.dk_sr, my,
+             x.nk, p.scale, dk);
+    ln.store(static_cast<T*>(p.dv) + (x.kv * p.dv_sh + (long long)x.k0 * p.dv_sr), p.dv_sr, my,
+             x.nk, 1.0f, dv);
+  }
+}
+
+// The dk and dv kernel's block walked again, with NaN and infinities of queries
+// that do not see a key kept from it.
+template <int D, class T>
+__device__ __attribute__((noinline)) void dkv_checked(const void* geom, uint8_t* lds,
+                                                      uint8_t* stat) {
+  using L = BwdLane<D, T>;
+  using V8 = typename L::V8;
+  using E = Elem<T>;
+  lds = uniform(lds);
+  stat = uniform(stat);
+  BwdGeom p;
+  __builtin_memcpy(&p, geom, sizeof p);
+  DkvTask x;
+  if (!dkv_task(p, x)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const L ln(threadIdx.x & 63);
+  const int my = x.first + 32 * wave + ln.col;
+  DkvFetch<D, T> tiles(p, x, wave, ln.lane);
+  V8 kf[L::kSteps], vf[L::kSteps];
+  ln.own_rows(static_cast<const T*>(p.k) + (x.kv * p.k_sh + (long long)x.k0 * p.k_sr), p.k_sr, my,
+              x.nk, kf);
+  ln.own_rows(static_cast<const T*>(p.v) + (x.kv * p.v_sh + (long long)x.k0 * p.v_sr), p.v_sr, my,
+              x.nk, vf);
+  float16_t dk[L::kCols], dv[L::kCols];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int tt = u / L::kCols;
-        acc[u % L::kCols] = E::mfma(a[u], w[tt >> 1][tt & 1], acc[u % L::kCols]);
+  for (int c = 0; c < L::kCols; ++c) dk[c] = dv[c] = zero16();
+  const int lo = my - x.coff;  // queries from lo on see this lane's key
+  const float* const st = reinterpret_cast<const float*>(stat);
+  const uint8_t *const qt = lds, *const dt = lds + DkvFetch<D, T>::kTileB;
+  int t = x.t0;
+#pragma unroll 1
+  for (int step = 0; step < x.steps; ++step) {
+    tiles.run(p, x, lds, stat);
+    sync_ring<0>();
+#pragma unroll 1
+    for (int b = 0; b < 2; ++b) {
+      const int base = t * kDkvRows + 32 * b;
+      float16_t sc, dp;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int at = 32 * b + 8 * (i >> 2) + 4 * ln.g + (i & 3);
+        sc[i] = st[at];
+        dp[i] = st[kDkvRows + at];
+      }
+#pragma unroll
+      for (int u = 0; u < L::kSteps; ++u) sc = E::mfma(ln.rows_op(qt, b, u), kf[u], sc);
+#pragma unroll
+      for (int u = 0; u < L::kSteps; ++u) dp = E::mfma(ln.rows_op(dt, b, u), vf[u], dp);
+      V8 pp[2], ds[2];
+      auto sees = [&](int j) { return base + j >= lo && base + j < x.nq; };
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool seen = sees(8 * (i >> 2) + 4 * ln.g + (i & 3));
+        const float e = __builtin_amdgcn_exp2f(sc[i] * p.scale_log2), y = e * dp[i];
+        pp[i >> 3][i & 7] = (T)(seen ? e : 0.0f);
+        ds[i >> 3][i & 7] = (T)(seen ? y : 0.0f);
+      }
+      auto add = [&](const uint8_t* tile, float16_t (&acc)[L::kCols], const V8 (&w)[2],
+                     bool as_nan) __attribute__((always_inline)) {
+        V8 a[D / 16];
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u)
+          a[u] = ln.cols_op(tile, u % L::kCols, 2 * b + u / L::kCols);
+        add_odd_block<D, T>(tile + 32 * b * L::kRowB, a, acc, ln.g, sees, as_nan);
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u)
+          acc[u % L::kCols] = E::mfma(a[u], w[u / L::kCols], acc[u % L::kCols]);
+      };
+      add(dt, dv, pp, false);
+      add(qt, dk, ds, true);
+    }
+    if (++t == x.tbeg + x.per) t = x.tbeg;
+    sync_ring<0>();
+  }
+  dkv_store<D, T>(p, x, ln, my, dk, dv);
+}
+
+// dk and dv of 128 keys (4 waves of 32) over part `part` of the queries that
+// see them, of all heads of the group one after the other, in tiles of 64
+// query rows: blocks of 32, i = 0, 1, ...
+//
+// A slot schedule as in the forward kernels: iteration i has 4 D / 16 MFMAs,
+// the even ones s and dout v' of block i + 1, the odd ones dv and dk of block
+// i - 1, and block i's exponentials, p and ds spread between them.  s and dout
+// v' start from {-lse / scale, -delta} as accumulators, so p = 2^(s c) and
+// ds = p dp' need no further subtraction, and where a block has hidden pairs
+// those start from -inf.  A slot's operand is read kAhead slots before.  Each
+// pair of iterations reads the tiles m - 1, m and m + 1 and fetches m + 2 into
+// a ring of 4.
+template <int D, class T, int OCC>
+__global__ void __launch_bounds__(256, OCC) packed_dkv_kernel(const BwdGeom p) {
+  using L = BwdLane<D, T>;
+  using V8 = typename L::V8;
+  using E = Elem<T>;
+  using F = DkvFetch<D, T>;
+  constexpr int kTileB = F::kTileB, kRing = 4, kSlots = 4 * L::kSteps, kAhead = 8;
+  constexpr int kStatB = 8 * kDkvRows;
+  typedef const float4_t __attribute__((address_space(3))) * LdsF4;
+  __shared__ __attribute__((aligned(16))) uint8_t ring[kRing][2][kTileB];
+  __shared__ __attribute__((aligned(16))) uint8_t stat[kRing][kStatB];
+  const void* const geom = (const void*)__builtin_amdgcn_kernarg_segment_ptr();
+  DkvTask x;
+  if (!dkv_task(p, x)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const L ln(threadIdx.x & 63);
+  const int kw = x.first + 32 * wave, my = kw + ln.col;
+  float16_t dk[L::kCols], dv[L::kCols];
+#pragma unroll
+  for (int c = 0; c < L::kCols; ++c) dk[c] = dv[c] = zero16();
+  bool again = false;
+  if (x.steps > 0) {
+    F tiles(p, x, wave, ln.lane);
+    tiles.run(p, x, ring[0][0], stat[0]);
+    tiles.run(p, x, ring[1][0], stat[1]);
+    {  // tile -1: zeros
+      const i32x4_t none = rows_rsrc<2 * D>(p.q, 0, 0);
+      tiles.fq.run(none, ring[kRing - 1][0], wave);
+      tiles.fd.run(none, ring[kRing - 1][1], wave);
+    }
+    V8 kf[L::kSteps], vf[L::kSteps];
+    ln.own_rows(static_cast<const T*>(p.k) + (x.kv * p.k_sh + (long long)x.k0 * p.k_sr), p.k_sr,
+                my, x.nk, kf);
+    ln.own_rows(static_cast<const T*>(p.v) + (x.kv * p.v_sh + (long long)x.k0 * p.v_sr), p.v_sr,
+                my, x.nk, vf);
+    __builtin_amdgcn_s_waitcnt(0);
+    sync_ring<0>();
+
+    const TileOps<D, T> ops(ln);
+    const uint32_t lds_ring = (uint32_t)(uintptr_t)&ring[0][0][0];
+    const uint32_t lds_stat = (uint32_t)(uintptr_t)&stat[0][0] + 16 * ln.g;
+    // Slot 2u: s (u even) or dout v' (odd), step u / 2; slot 2u + 1: dv (even)
+    // or dk, columns u / 2 % kCols, rows 16 (u / 2 / kCols).
+    auto read_slot = [&](auto sl, uint32_t rows_t, int rows_b, uint32_t cols_t, int cols_b)
+                         __attribute__((always_inline)) {
+      constexpr int Lc = decltype(sl)::value, u = Lc >> 1, half = u & 1, idx = u >> 1;
+      if constexpr ((Lc & 1) == 0)
+        return ops.rows(rows_t, half * kTileB, rows_b, idx);
+      else
+        return ops.cols(cols_t, (1 - half) * kTileB, idx % L::kCols, 2 * cols_b + idx / L::kCols);
+    };
+    // Accumulators of s (which: 0) or dout v' (1) of a tile's block b, rows 8 g4 ..
+    auto start4 = [&](float16_t& to, uint32_t st, int b, int which, int g4)
+                      __attribute__((always_inline)) {
+      const float4_t y =
+          *(LdsF4)(uintptr_t)(st + 4 * (kDkvRows * which + 32 * b + 8 * g4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[4 * g4 + e] = y[e];
+    };
+    // Hidden pairs of the block whose first row is `base`.
+    const int lo = my - x.coff;  // queries from lo on see this lane's key
+    auto hide = [&](float16_t& to, int base) __attribute__((always_inline)) {
+      if (base + 32 <= x.nq && base + x.coff >= kw + 31) return;
+      const float hidden = p.scale > 0.0f ? ninf() : -ninf();
+      const int from = lo - base - 4 * ln.g, end = x.nq - base - 4 * ln.g;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int at = 8 * (e >> 2) + (e & 3);
+        if (at < from || at >= end) to[e] = hidden;
       }
     };
-    add(dt, dv, pp, false);
-    add(qt, dk, ds, true);
+
+    float16_t S[2], X[2];  // scores and dout v', by the block's parity
+    V8 P[2][2], Q[2][2];   // p and ds
+    V8 ahead[kAhead];
+    int t = x.t0;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        start4(S[b], lds_stat, b, 0, g4);
+        start4(X[b], lds_stat, b, 1, g4);
+      }
+      hide(S[b], t * kDkvRows + 32 * b);
+    }
+#pragma unroll
+    for (int st = 0; st < L::kSteps; ++st) {
+      S[0] = E::mfma(ops.rows(lds_ring, 0, 0, st), kf[st], S[0]);
+      X[0] = E::mfma(ops.rows(lds_ring, kTileB, 0, st), vf[st], X[0]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) P[1][i] = Q[1][i] = (V8){0, 0, 0, 0, 0, 0, 0, 0};
+    static_for(std::make_integer_sequence<int, kAhead>{}, [&](auto i) __attribute__((always_inline)) {
+      ahead[decltype(i)::value] =
+          read_slot(i, lds_ring, 1, lds_ring + (kRing - 1) * 2 * kTileB, 1);
+    });
+
+    // Iteration i of parity `par`: rows_t / rows_b hold block i + 1, next_t /
+    // next_b block i + 2 (st_next its statistics, next_base its first row),
+    // cols_t / cols_b block i - 1, own_t / own_b block i.
+    auto block = [&](auto par, uint32_t rows_t, int rows_b, uint32_t next_t, int next_b,
+                     uint32_t cols_t, int cols_b, uint32_t own_t, int own_b, uint32_t st_next,
+                     int next_base, int slot) __attribute__((always_inline)) {
+      constexpr int kPar = decltype(par)::value, kOther = 1 - kPar;
+      V8 op[kSlots];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) op[a] = ahead[a];
+      static_for(std::make_integer_sequence<int, kSlots>{}, [&](auto sl) __attribute__((always_inline)) {
+        constexpr int Lc = decltype(sl)::value, u = Lc >> 1, half = u & 1, idx = u >> 1;
+        if constexpr ((Lc & 1) == 0) {
+          if constexpr (half == 0)
+            S[kOther] = E::mfma(op[Lc], kf[idx], S[kOther]);
+          else
+            X[kOther] = E::mfma(op[Lc], vf[idx], X[kOther]);
+        } else {
+          constexpr int c = idx % L::kCols, tt = idx / L::kCols;
+          if constexpr (half == 0)
+            dv[c] = E::mfma(op[Lc], P[kOther][tt], dv[c]);
+          else
+            dk[c] = E::mfma(op[Lc], Q[kOther][tt], dk[c]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // the next tile's fetches, spread over the first iteration of a tile
+        if constexpr (kPar == 0) {
+          constexpr int every = kSlots / F::kDma;
+          if constexpr (Lc % every == 0 && Lc / every < F::kDma)
+            tiles.dma(ring[slot][0], stat[slot], Lc / every);
+        }
+        constexpr int La = Lc + kAhead;
+        if constexpr (La < kSlots)
+          op[La] = read_slot(Ic<La>{}, rows_t, rows_b, cols_t, cols_b);
+        else
+          ahead[La - kSlots] = read_slot(Ic<La - kSlots>{}, next_t, next_b, own_t, own_b);
+        // block i's elements, done 4 slots before the end, and the start of
+        // block i + 2 in their place
+        static_for(std::make_integer_sequence<int, 16>{}, [&](auto el) __attribute__((always_inline)) {
+          constexpr int e = decltype(el)::value;
+          if constexpr (e * (kSlots - 4) / 16 == Lc) {
+            const float y = __builtin_amdgcn_exp2f(S[kPar][e] * p.scale_log2);
+            P[kPar][e >> 3][e & 7] = (T)y;
+            Q[kPar][e >> 3][e & 7] = (T)(y * X[kPar][e]);
+            if constexpr (e % 4 == 3) {
+              start4(S[kPar], st_next, next_b, 0, e / 4);
+              start4(X[kPar], st_next, next_b, 1, e / 4);
+            }
+          }
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      hide(S[kPar], next_base);
+    };
+#pragma unroll 1
+    for (int m = 0; m < x.steps; ++m) {
+      const uint32_t before = lds_ring + ((m + 3) & 3) * 2 * kTileB;
+      const uint32_t here = lds_ring + (m & 3) * 2 * kTileB;
+      const uint32_t after = lds_ring + ((m + 1) & 3) * 2 * kTileB;
+      const uint32_t st = lds_stat + ((m + 1) & 3) * kStatB;
+      const int slot = (m + 2) & 3;
+      if (++t == x.tbeg + x.per) t = x.tbeg;
+      const int base = t * kDkvRows;  // of tile m + 1
+      tiles.next(p, x);
+      block(Ic<0>{}, here, 1, after, 0, before, 1, here, 0, st, base, slot);
+      block(Ic<1>{}, after, 0, after, 1, here, 0, here, 1, st, base + 32, slot);
+      sync_ring_ahead<0, 15>();
+    }
+    // dv and dk of the last block
+    const uint32_t last = lds_ring + ((x.steps - 1) & 3) * 2 * kTileB;
+#pragma unroll
+    for (int u = 0; u < D / 16; ++u) {
+      const int c = u % L::kCols, tt = u / L::kCols;
+      dv[c] = E::mfma(ops.cols(last, kTileB, c, 2 + tt), P[1][tt], dv[c]);
+      dk[c] = E::mfma(ops.cols(last, 0, c, 2 + tt), Q[1][tt], dk[c]);
+    }
+    // A block with a key whose sums are not finite is walked again.
+    int* const redo = reinterpret_cast<int*>(stat);
+    __syncthreads();
+    if (threadIdx.x == 0) *redo = 0;
+    __syncthreads();
+    if (my < x.nk && (any_odd(dk) || any_odd(dv))) *redo = 1;
+    __syncthreads();
+    again = *redo != 0;
+    __syncthreads();
   }
-  __builtin_amdgcn_s_waitcnt(0);
-  if (p.parts > 1) {
-    float* const x =
-        p.part + (((long long)part * p.kv_heads + kv) * p.key_rows + k0) * (2 * D);
-    ln.store_part(x, my, nk, dk);
-    ln.store_part(x + D, my, nk, dv);
-  } else {
-    ln.store(static_cast<T*>(p.dk) + (kv * p.dk_sh + (long long)k0 * p.dk_sr), p.dk_sr, my, nk,
-             p.scale, dk);
-    ln.store(static_cast<T*>(p.dv) + (kv * p.dv_sh + (long long)k0 * p.dv_sr), p.dv_sr, my, nk,
-             1.0f, dv);
-  }
+  if (again)
+    dkv_checked<D, T>(geom, &ring[0][0][0], &stat[0][0]);
+  else
+    dkv_store<D, T>(p, x, ln, my, dk, dv);
 }
 
 // Sums the parts: a thread 4 columns of a key's dk and dv.
@@ -464,7 +881,7 @@ hipError_t launch_bwd_dim(const BwdGeom& g, hipStream_t st) {
                      dim3((unsigned)packed_groups(g.rows, g.sequences, 32 * W, g.heads)),
                      dim3(64 * W), 0, st, g);
   hipLaunchKernelGGL(
-      (packed_dkv_kernel<D, W, T, 1>),
+      (packed_dkv_kernel<D, T, 1>),
       dim3((unsigned)packed_groups(g.key_rows, g.sequences, 32 * W, g.kv_heads * g.parts)),
       dim3(64 * W), 0, st, g);
   if (g.parts > 1)

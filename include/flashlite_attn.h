@@ -497,7 +497,7 @@ int fl_attn_tree_fwd(const fl_tree_params* p, void* workspace, int64_t workspace
  * 16-byte aligned device memory that needs no initial values; calls that may
  * overlap must not share one.
  *
- * Row strides are below 2^24 elements, those of q, k, v and o at least head_dim;
+ * sm_scale is at least 1e-30 in size.  Row strides are below 2^24 elements, those of q, k, v and o at least head_dim;
  * rows and key_rows are at most 2^30, and all rows of k and of v lie within 2^31
  * bytes of a head's first.
  */

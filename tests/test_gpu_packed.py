@@ -201,3 +201,11 @@ def test_starts_out_of_range_are_not_followed(cuda):
     assert torch.equal(out[:, :, 90:], one)
     grads = fl.backward_packed(torch.ones_like(q), q, k, v, out, lse, starts, is_causal=True)
     assert all(torch.isfinite(g[:, :, 90:]).all() for g in grads)
+
+
+@pytest.mark.parametrize("dtype,d", BOTH)
+@pytest.mark.parametrize("h,hk,lengths,causal", [
+    (7, 1, [400], True), (3, 3, [257, 31], False), (8, 2, [1500], True), (2, 1, [1, 700, 0], True)])
+def test_key_blocks_in_parts(cuda, dtype, d, h, hk, lengths, causal):
+    """Few key blocks: their queries are dealt to several work-groups."""
+    run(Problem(sum(lengths), dtype, d, h, hk, lengths, None, causal, "heads", 3), cuda)

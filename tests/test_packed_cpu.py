@@ -48,6 +48,7 @@ PACKED = [
     (dict(heads=0), capi.FL_ERR_INVALID_ARGUMENT, "multiple"),
     (dict(sm_scale=math.nan), capi.FL_ERR_INVALID_ARGUMENT, "sm_scale"),
     (dict(sm_scale=1e-60), capi.FL_ERR_INVALID_ARGUMENT, "sm_scale"),
+    (dict(sm_scale=1e-31), capi.FL_ERR_UNSUPPORTED, "1e-30"),
     (dict(key_starts=0), capi.FL_ERR_INVALID_ARGUMENT, "key_starts"),
     (dict(rows=1 << 31), capi.FL_ERR_UNSUPPORTED, "2^30"),
     (dict(sequences=1 << 25), capi.FL_ERR_UNSUPPORTED, "2^24"),
