@@ -327,8 +327,10 @@ int fl_attn_norm_rotary_bwd(const fl_rotary_params* p, const fl_norm_params* n,
     return set_error(FL_ERR_INVALID_ARGUMENT, "%s: the forward pass' q and k must be non-NULL", who);
   if (!aligned(d->q, 16) || !aligned(d->k, 16))
     return set_error(FL_ERR_MISALIGNED, "%s: q and k must be 16-byte aligned", who);
+  // (the weights' gradients pass through it)
+  const bool sums = (n->q_weight && d->dq_weight) || (n->k_weight && d->dk_weight);
   const int64_t need = fl::norm_rotary_workspace_bytes(p->head_dim);
-  if ((q || k) && (!workspace || workspace_bytes < need))
+  if (sums && (!workspace || workspace_bytes < need))
     return set_error(FL_ERR_INVALID_ARGUMENT, "%s: a workspace of %lld bytes is needed (got %lld)",
                      who, (long long)need, (long long)(workspace ? workspace_bytes : 0));
   if (!aligned(workspace, 16))

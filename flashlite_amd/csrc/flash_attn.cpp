@@ -311,7 +311,7 @@ void view4(const torch::Tensor& t, const torch::Tensor& like, const char* name, 
               " must be on the same device as the others");
   TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must have the dtype of the others");
   TORCH_CHECK(t.dim() == 4, name, " must be 4D");
-  TORCH_CHECK(t.stride(3) == 1 || t.size(3) == 1, name,
+  TORCH_CHECK(t.stride(3) == 1 || t.size(3) == 1 || t.numel() == 0, name,
               " must have a unit-stride head dimension");
   for (int i = 0; i < 3; ++i) st[i] = t.stride(i);
 }

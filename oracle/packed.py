@@ -99,12 +99,9 @@ def turn(x, positions, freqs, axes=None, interleaved=False, scale=1.0, transpose
         return rotary(x, positions, freqs, interleaved, scale, transpose)
     out = np.array(x, np.float64)
     for j, (f, a) in enumerate(zip(freqs, axes)):
-        one = np.zeros(len(freqs))
-        one[j] = f
         a = min(max(int(a), 0), len(positions) - 1)
-        y = rotary(x, positions[a], one, interleaved, scale, transpose)
         cols = [2 * j, 2 * j + 1] if interleaved else [j, j + len(freqs)]
-        out[..., cols] = y[..., cols]
+        out[..., cols] = rotary(x[..., cols], positions[a], [f], True, scale, transpose)
     return out
 
 

@@ -93,10 +93,32 @@ def problem(rs, cuda, dtype, b, h, hk, n, d, pairs, layout, first, axes, weight)
             torch.from_numpy(freqs).to(cuda), freqs)
 
 
+# More rows than a work-group for each step of the heads: walks over whole tiles of
+# tokens, all heads of a tile or shares of them.
+MANY = [
+    (1, 24, 8, 2501, 128, 64, "bnhd", 0, 1.0, 3),
+    (2, 13, 3, 4099, 64, 32, "bnhd", 10, 1.1, 0),
+    (3, 9, 2, 1801, 64, 10, "bhnd", 7, 1.0, 2),
+    (1, 3, 0, 20000, 64, 32, "bhnd", 0, 1.0, 0),
+    (1, 40, 40, 333, 64, 1, "bnhd", 0, 1.0, 2),
+]
+
+
+@pytest.mark.parametrize("dtype,inter", [("float16", True), ("bfloat16", False), ("float32", False),
+                                         ("float32", True)])
+@pytest.mark.parametrize("b,h,hk,n,d,pairs,layout,first,scale,axes", MANY)
+def test_many_rows(cuda, dtype, inter, b, h, hk, n, d, pairs, layout, first, scale, axes):
+    check_forward_and_backward(cuda, dtype, inter, b, h, hk, n, d, pairs, layout, first, scale, axes)
+
+
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("b,h,hk,n,d,pairs,layout,first,scale,axes", CASES)
 def test_forward_and_backward(cuda, dtype, inter, b, h, hk, n, d, pairs, layout, first, scale, axes):
+    check_forward_and_backward(cuda, dtype, inter, b, h, hk, n, d, pairs, layout, first, scale, axes)
+
+
+def check_forward_and_backward(cuda, dtype, inter, b, h, hk, n, d, pairs, layout, first, scale, axes):
     rs = np.random.RandomState(n + d)
     weight = dtype if n % 3 else "float32"
     eps, offset = (1e-6, 0.0) if n % 2 else (1e-2, 1.0)
@@ -256,6 +278,8 @@ def test_rows_of_zeros_and_far_values(cuda):
     (2, 37, 3, 3, 128, 64, 20, 3, True),
     (3, 9, 4, 1, 128, 10, 8, 2, False),
     (1, 300, 32, 8, 64, 16, 64, 0, True),
+    (2, 2100, 12, 4, 128, 64, 64, 3, True),
+    (1, 9001, 3, 2, 64, 10, 32, 0, False),
 ])
 def test_rows_of_the_cache(cuda, dtype, b, n, h, hk, d, pairs, block, axes, paged_rows):
     """As forward_norm_rotary, in the rows of the slots; passed-over tokens and

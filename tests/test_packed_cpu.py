@@ -313,3 +313,13 @@ def test_oracle_norm_gradients_are_torchs(axes, inter):
     (out * torch.from_numpy(dy)).sum().backward()
     np.testing.assert_allclose(dx, xl.grad.numpy(), atol=1e-12)
     np.testing.assert_allclose(dw, wl.grad.numpy(), atol=1e-12)
+
+
+def test_norm_gradient_workspace_follows_the_sums():
+    """Sums over no heads of q pass through the workspace too."""
+    lib = capi.load()
+    p = rotary_params(heads=0)
+    n = norm_params(k_weight=0)
+    refused(lib.fl_attn_norm_rotary_bwd(ctypes.byref(p), ctypes.byref(n),
+                                        ctypes.byref(norm_grads(dk_weight=0)), None, 0, None),
+            capi.FL_ERR_INVALID_ARGUMENT, "workspace")
