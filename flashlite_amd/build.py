@@ -41,8 +41,9 @@ EXT_NAME = "flash_attn_wmma"
 
 HIP_SOURCES = ["fa2_fwd.hip", "fa2_pipe.hip", "fa2_slot.hip", "fa2_stream.hip", "fa2_short.hip",
                "fa2_rows32.hip", "fa2_d128.hip", "fa2_d128_bf16.hip", "naive_fwd.hip", "cache_plan.hip",
-               "rotary.hip", "norm_rotary.hip", "tree_fwd.hip", "packed_fwd_f16.hip",
-               "packed_fwd_bf16.hip", "packed_bwd_f16.hip", "packed_bwd_bf16.hip", "capi_serve.hip", "capi_packed.hip",
+               "rotary.hip", "norm_rotary.hip", "tree_fwd.hip", "packed_fwd_d64_f16.hip",
+               "packed_fwd_d64_bf16.hip", "packed_fwd_d128_f16.hip", "packed_fwd_d128_bf16.hip",
+               "packed_bwd_f16.hip", "packed_bwd_bf16.hip", "capi_serve.hip", "capi_packed.hip",
                "capi.hip"]
 DIAG_SOURCES = ["diag.hip", "diag_timeline.hip"]
 

@@ -128,8 +128,11 @@ int fl_attn_packed_fwd(const fl_packed_params* p, void* stream) {
   if (rc != FL_OK) return rc;
   const fl_packed_params x = normal(*p);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  return launched(p->dtype == FL_DTYPE_BF16 ? fl::launch_packed_fwd_bf16(x, st)
-                                            : fl::launch_packed_fwd_f16(x, st), who);
+  const bool bf16 = p->dtype == FL_DTYPE_BF16;
+  return launched(p->head_dim == 128 ? (bf16 ? fl::launch_packed_fwd_d128_bf16(x, st)
+                                             : fl::launch_packed_fwd_d128_f16(x, st))
+                                     : (bf16 ? fl::launch_packed_fwd_d64_bf16(x, st)
+                                             : fl::launch_packed_fwd_d64_f16(x, st)), who);
 }
 
 int64_t fl_attn_packed_bwd_workspace_bytes(const fl_packed_params* p) {

@@ -63,10 +63,12 @@ hipError_t launch_norm_zero(const fl_rotary_params& p, float* dq, float* dk, hip
 int64_t tree_workspace_bytes(const fl_tree_params& p);
 hipError_t launch_tree_fwd(const fl_tree_params& p, void* ws, hipStream_t stream);
 
-// Packed sequences, by element type (packed_fwd_*.hip, packed_bwd_*.hip), one
-// entry of a dimension with a stride that fits.
-hipError_t launch_packed_fwd_f16(const fl_packed_params& p, hipStream_t stream);
-hipError_t launch_packed_fwd_bf16(const fl_packed_params& p, hipStream_t stream);
+// Packed sequences, by head dim and element type (packed_fwd_*.hip) or by
+// element type (packed_bwd_*.hip); dimensions of one entry have strides that fit.
+hipError_t launch_packed_fwd_d64_f16(const fl_packed_params& p, hipStream_t stream);
+hipError_t launch_packed_fwd_d64_bf16(const fl_packed_params& p, hipStream_t stream);
+hipError_t launch_packed_fwd_d128_f16(const fl_packed_params& p, hipStream_t stream);
+hipError_t launch_packed_fwd_d128_bf16(const fl_packed_params& p, hipStream_t stream);
 hipError_t launch_packed_bwd_f16(const fl_packed_params& p, const fl_packed_grads& d, void* ws,
                                  hipStream_t stream);
 hipError_t launch_packed_bwd_bf16(const fl_packed_params& p, const fl_packed_grads& d, void* ws,
