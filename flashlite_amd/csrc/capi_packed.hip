@@ -103,15 +103,16 @@ int check_packed_pointers(const fl_packed_params* p, const char* who) {
 namespace fl {
 
 // Parts that a key block's queries are cut into, each a work-group with sums of
-// its own (packed_bwd.h): as many as bring two work-groups a CU, at most 8.
-// One a CU leaves the chip waiting for the heaviest (B2 H16/2 N7000-8192 D 128
-// causal 2690 us in one part, 1805 in two; B1 H8/1 N8192 2274 against 593 in
-// eight); with enough of them the partial sums only cost (B4 H32/8 N4096 2022
-// in one, 2105 in two).
+// its own (packed_bwd.h): as many as bring the work-groups that the chip holds
+// at once, two a CU, or under a causal mask over long keys, where they differ
+// most, twice that (us).  B2 H16/2 N7000-8192 D 128 causal 3169 with one a CU,
+// 2117 with two, 1691 with four; B1 H8 N2048 D 64 causal 82.7, 74.5, 82.2; 8
+// sequences of 300-700, H16, not causal, with two 80, with four 101.
 int packed_bwd_parts(const fl_packed_params& p) {
   const int64_t groups = (p.key_rows / 128 + p.sequences) * p.kv_heads;
-  const int64_t want = 2 * device_cus();
-  return (int)std::min<int64_t>(8, std::max<int64_t>(1, (want + groups / 2) / groups));
+  const int64_t a_cu = p.causal && p.key_rows / p.sequences >= 4096 ? 4 : 2;
+  const int64_t want = a_cu * device_cus();
+  return (int)std::min<int64_t>(4 * a_cu, std::max<int64_t>(1, (want + groups / 2) / groups));
 }
 
 }  // namespace fl
@@ -138,7 +139,12 @@ int fl_attn_packed_fwd(const fl_packed_params* p, void* stream) {
 int64_t fl_attn_packed_bwd_workspace_bytes(const fl_packed_params* p) {
   if (check_packed(p, "fl_attn_packed_bwd_workspace_bytes") != FL_OK) return -1;
   if (p->sequences == 0 || p->heads == 0) return 0;
-  const int64_t parts = fl::packed_bwd_parts(*p);
+  // (whichever the mask)
+  fl_packed_params x = *p;
+  x.causal = 0;
+  int64_t parts = fl::packed_bwd_parts(x);
+  x.causal = 1;
+  parts = std::max<int64_t>(parts, fl::packed_bwd_parts(x));
   return fl::packed_stat_bytes(*p) +
          (parts > 1 ? parts * p->kv_heads * p->key_rows * 2 * p->head_dim * 4 : 0);
 }

@@ -12,6 +12,18 @@
 // dk).  14 D flops a pair of a row and a key, 7 products where one kernel with
 // atomics would do with 5.
 //
+// Bound by the matrix cores and what feeds them: B4 H32/8 N4096 D 128 bf16 causal
+// 1810 us, 1.06 PFLOP/s of the 7 products, where a large library product has
+// 1.2; 16 sequences of 64-2000, H32/8 718 (a block's triangle and the sequences'
+// ends are walked whole), B2 H16/2 N7000-8192 fp16 1630; few short ones by
+// three launches (4 of 33-257, H8/2 D 64 26 us).
+//
+// Both kernels keep two waves a SIMD, the products of one among the exponentials
+// of the other.  One wave with 64 bytes more registers a lane, dv and dk one
+// block behind s and dout v' and the exponentials spread over all products, took
+// 2020 where two waves take 1810 (16 sequences 830 against 718: a work-group
+// alone on its CU leaves it idle at its start and end).
+//
 // Operands as in the forward kernels: a wave's own 32 rows stay in registers
 // as B operands, tiles of the others come into LDS by DMA and are read as rows
 // (A of the score products) and transposed (A of the products that sum over
@@ -373,7 +385,7 @@ __global__ void __launch_bounds__(64 * W, 2) packed_dq_kernel(const BwdGeom p) {
   using L = BwdLane<D, T>;
   using V8 = typename L::V8;
   using E = Elem<T>;
-  constexpr int kSegs = 8 / W, kSlots = 3;
+  constexpr int kSegs = 8 / W, kSlots = 3, kAhead = 4;
   __shared__ __attribute__((aligned(16))) uint8_t ring[kSlots][2][kTileBytes];
   const void* const geom = (const void*)__builtin_amdgcn_kernarg_segment_ptr();
   DqTask x;
@@ -417,29 +429,57 @@ __global__ void __launch_bounds__(64 * W, 2) packed_dq_kernel(const BwdGeom p) {
     const bool edge = base + L::kRows > min(x.nk, qw + x.coff + 1);
 #pragma unroll
     for (int b = 0; b < L::kBlocks; ++b) {
+      // 3 kSteps slots of a product each: s, dout v', dq.  A slot's operand is
+      // read kAhead slots before; p is taken beside dout v'.
+      constexpr int N = L::kSteps;
       float16_t sc = zero16(), dp = zero16();
-      V8 ds[2];
+      V8 op[3 * N], ds[2];
+      auto read = [&](auto sl) __attribute__((always_inline)) {
+        constexpr int i = decltype(sl)::value, of = i / N, u = i % N;
+        if constexpr (of < 2)
+          op[i] = ops.rows(kt, of * kTileBytes, b, u);
+        else
+          op[i] = ops.cols(kt, 0, u % L::kCols, 2 * b + u / L::kCols);
+      };
+      auto minus = [&](int e) __attribute__((always_inline)) {  // element e of ds
+        ds[e >> 3][e & 7] = (T)(sc[e] * (dp[e] - rows.delta));
+      };
+      static_for(std::make_integer_sequence<int, kAhead>{}, read);
+      static_for(std::make_integer_sequence<int, 3 * N>{}, [&](auto sl) __attribute__((always_inline)) {
+        constexpr int i = decltype(sl)::value, of = i / N, u = i % N, kEach = 16 / N;
+        constexpr int c = u % L::kCols, tt = u / L::kCols;
+        if constexpr (of == 0)
+          sc = E::mfma(op[i], rows.qf[u], sc);
+        else if constexpr (of == 1)
+          dp = E::mfma(op[i], rows.df[u], dp);
+        else
+          acc[c] = E::mfma(op[i], ds[tt], acc[c]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (i + kAhead < 3 * N) read(Ic<i + kAhead>{});
+        if constexpr (i == N - 1) {
+          if (edge) {
+            const float hidden = p.scale > 0.0f ? ninf() : -ninf();
 #pragma unroll
-      for (int st = 0; st < L::kSteps; ++st)
-        sc = E::mfma(ops.rows(kt, 0, b, st), rows.qf[st], sc);
+            for (int e = 0; e < 16; ++e)
+              if (base + 32 * b + 8 * (e >> 2) + 4 * ln.g + (e & 3) >= lim) sc[e] = hidden;
+          }
+        }
+        if constexpr (of == 1) {
 #pragma unroll
-      for (int st = 0; st < L::kSteps; ++st)
-        dp = E::mfma(ops.rows(kt, kTileBytes, b, st), rows.df[st], dp);
-      if (edge) {
-        const float hidden = p.scale > 0.0f ? ninf() : -ninf();
+          for (int e = u * kEach; e < (u + 1) * kEach; ++e)
+            sc[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.scale_log2, -rows.lse2));
+        }
+        // (the first 8 rows' before the products that take them, the others among those)
+        if constexpr (i == 2 * N - 1) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (base + 32 * b + 8 * (i >> 2) + 4 * ln.g + (i & 3) >= lim) sc[i] = hidden;
-      }
+          for (int e = 0; e < 8; ++e) minus(e);
+        } else if constexpr (of == 2 && tt == 0) {
+          constexpr int kSome = 8 / L::kCols;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.scale_log2, -rows.lse2));
-        ds[i >> 3][i & 7] = (T)(e * (dp[i] - rows.delta));
-      }
-#pragma unroll
-      for (int u = 0; u < D / 16; ++u)
-        acc[u % L::kCols] = E::mfma(ops.cols(kt, 0, u % L::kCols, 2 * b + u / L::kCols),
-                                    ds[u / L::kCols], acc[u % L::kCols]);
+          for (int e = 8 + u * kSome; e < 8 + (u + 1) * kSome; ++e) minus(e);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
     }
   }
   // A block with a row whose sum is not finite is walked again.
@@ -465,8 +505,9 @@ struct DkvTask {
   int tbeg, per, steps, h0, t0;  // a head's first tile and tiles; steps from head h0, tile t0 on
 };
 
-constexpr int kDkvWaves = 4, kDkvRows = 64;  // query rows of a tile
+constexpr int kDkvWaves = 4;
 
+template <int R>  // query rows of a tile
 __device__ __forceinline__ bool dkv_task(const BwdGeom& p, DkvTask& x) {
   int r, unit, seq, kb;
   packed_unit(p.kv_heads * p.parts, p.xcds, r, unit);
@@ -480,8 +521,8 @@ __device__ __forceinline__ bool dkv_task(const BwdGeom& p, DkvTask& x) {
   // (the last index is the heaviest under a causal mask: the first keys)
   x.first = ((x.nk + kBlock - 1) / kBlock - 1 - kb) * kBlock;
   x.coff = p.causal ? x.nk - x.nq : x.nk;
-  x.tbeg = max(x.first - x.coff, 0) / kDkvRows;
-  x.per = max((x.nq + kDkvRows - 1) / kDkvRows - x.tbeg, 0);
+  x.tbeg = max(x.first - x.coff, 0) / R;
+  x.per = max((x.nq + R - 1) / R - x.tbeg, 0);
   const int all = x.per * p.group;
   const int s0 = (int)((long long)all * x.part / p.parts);
   x.steps = (int)((long long)all * (x.part + 1) / p.parts) - s0;
@@ -493,10 +534,11 @@ __device__ __forceinline__ bool dkv_task(const BwdGeom& p, DkvTask& x) {
 // The tiles of a walk, one after the other: the queries of a head, then those
 // of the next.  A wave moves its share of q's and dout's rows and all of the
 // statistics (every wave to the same place: its own wait then covers them).
-template <int D, class T>
+template <int D, int R, class T>
 struct DkvFetch {
-  static constexpr int kTileB = kDkvRows * 2 * D, kSegs = kTileB / 1024 / kDkvWaves;
-  static constexpr int kDma = 2 * kSegs + 2;  // instructions of a wave
+  static constexpr int kTileB = R * 2 * D, kSegs = kTileB / 1024 / kDkvWaves;
+  static constexpr int kStats = R / 32;
+  static constexpr int kDma = 2 * kSegs + kStats;  // instructions of a wave
   const TileFetch<D, kSegs> fq, fd;
   int step, head, tile, wave, lane;
   i32x4_t rq, rd, rst;
@@ -514,11 +556,11 @@ struct DkvFetch {
     const int rows = step < x.steps ? x.nq : 0;
     const long long h = min(head, p.heads - 1);
     rq = tile_rsrc<2 * D>(static_cast<const T*>(p.q) + (h * p.q_sh + (long long)x.q0 * p.q_sr),
-                          2 * p.q_sr, tile * kDkvRows, rows, kDkvRows);
+                          2 * p.q_sr, tile * R, rows, R);
     rd = tile_rsrc<2 * D>(
         static_cast<const T*>(p.dout) + (h * p.do_sh + (long long)x.q0 * p.do_sr), 2 * p.do_sr,
-        tile * kDkvRows, rows, kDkvRows);
-    rst = tile_rsrc<8>(p.stats + (h * p.rows + x.q0), 8, tile * kDkvRows, rows, kDkvRows);
+        tile * R, rows, R);
+    rst = tile_rsrc<8>(p.stats + (h * p.rows + x.q0), 8, tile * R, rows, R);
     ++step;
     if (++tile == x.tbeg + x.per) {
       tile = x.tbeg;
@@ -532,7 +574,10 @@ struct DkvFetch {
     else if (i < 2 * kSegs)
       fd.seg(rd, slot + kTileB, wave, i - kSegs);
     else
-      load_lds4(rst, 8 * lane + 4 * (i - 2 * kSegs), stat + 256 * (i - 2 * kSegs));
+      {
+      const int at = 64 * (i - 2 * kSegs) + lane;  // {starts of s, of dout v'} [R]
+      load_lds4(rst, 8 * (at % R) + 4 * (at / R), stat + 256 * (i - 2 * kSegs));
+    }
   }
   __device__ __forceinline__ void run(const BwdGeom& p, const DkvTask& x, const uint8_t* slot,
                                       const uint8_t* stat) {
@@ -562,7 +607,7 @@ __device__ __forceinline__ void dkv_store(const BwdGeom& p, const DkvTask& x,
 
 // The dk and dv kernel's block walked again, with NaN and infinities of queries
 // that do not see a key kept from it.
-template <int D, class T>
+template <int D, int R, class T>
 __device__ __attribute__((noinline)) void dkv_checked(const void* geom, uint8_t* lds,
                                                       uint8_t* stat) {
   using L = BwdLane<D, T>;
@@ -573,11 +618,11 @@ __device__ __attribute__((noinline)) void dkv_checked(const void* geom, uint8_t*
   BwdGeom p;
   __builtin_memcpy(&p, geom, sizeof p);
   DkvTask x;
-  if (!dkv_task(p, x)) return;
+  if (!dkv_task<R>(p, x)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const L ln(threadIdx.x & 63);
   const int my = x.first + 32 * wave + ln.col;
-  DkvFetch<D, T> tiles(p, x, wave, ln.lane);
+  DkvFetch<D, R, T> tiles(p, x, wave, ln.lane);
   V8 kf[L::kSteps], vf[L::kSteps];
   ln.own_rows(static_cast<const T*>(p.k) + (x.kv * p.k_sh + (long long)x.k0 * p.k_sr), p.k_sr, my,
               x.nk, kf);
@@ -588,21 +633,21 @@ __device__ __attribute__((noinline)) void dkv_checked(const void* geom, uint8_t*
   for (int c = 0; c < L::kCols; ++c) dk[c] = dv[c] = zero16();
   const int lo = my - x.coff;  // queries from lo on see this lane's key
   const float* const st = reinterpret_cast<const float*>(stat);
-  const uint8_t *const qt = lds, *const dt = lds + DkvFetch<D, T>::kTileB;
+  const uint8_t *const qt = lds, *const dt = lds + DkvFetch<D, R, T>::kTileB;
   int t = x.t0;
 #pragma unroll 1
   for (int step = 0; step < x.steps; ++step) {
     tiles.run(p, x, lds, stat);
     sync_ring<0>();
 #pragma unroll 1
-    for (int b = 0; b < 2; ++b) {
-      const int base = t * kDkvRows + 32 * b;
+    for (int b = 0; b < R / 32; ++b) {
+      const int base = t * R + 32 * b;
       float16_t sc, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int at = 32 * b + 8 * (i >> 2) + 4 * ln.g + (i & 3);
         sc[i] = st[at];
-        dp[i] = st[kDkvRows + at];
+        dp[i] = st[R + at];
       }
 #pragma unroll
       for (int u = 0; u < L::kSteps; ++u) sc = E::mfma(ln.rows_op(qt, b, u), kf[u], sc);
@@ -638,31 +683,27 @@ __device__ __attribute__((noinline)) void dkv_checked(const void* geom, uint8_t*
 }
 
 // dk and dv of 128 keys (4 waves of 32) over part `part` of the queries that
-// see them, of all heads of the group one after the other, in tiles of 64
-// query rows: blocks of 32, i = 0, 1, ...
-//
-// A slot schedule as in the forward kernels: iteration i has 4 D / 16 MFMAs,
-// the even ones s and dout v' of block i + 1, the odd ones dv and dk of block
-// i - 1, and block i's exponentials, p and ds spread between them.  s and dout
-// v' start from {-lse / scale, -delta} as accumulators, so p = 2^(s c) and
-// ds = p dp' need no further subtraction, and where a block has hidden pairs
-// those start from -inf.  A slot's operand is read kAhead slots before.  Each
-// pair of iterations reads the tiles m - 1, m and m + 1 and fetches m + 2 into
-// a ring of 4.
-template <int D, class T, int OCC>
-__global__ void __launch_bounds__(256, OCC) packed_dkv_kernel(const BwdGeom p) {
+// see them, of all heads of the group one after the other, in tiles of R query
+// rows.  K's operands stay in registers and V's in LDS, which leaves registers
+// for two waves a SIMD: the products of one run among the exponentials of the
+// other.  s and dout v' start from {-lse / scale, -delta} as accumulators, so p =
+// 2^(s c) and ds = p dp' need no further subtraction, and where a block has
+// hidden pairs those start from -inf.
+template <int D, int R, class T>
+__global__ void __launch_bounds__(256, 2) packed_dkv_kernel(const BwdGeom p) {
   using L = BwdLane<D, T>;
   using V8 = typename L::V8;
   using E = Elem<T>;
-  using F = DkvFetch<D, T>;
-  constexpr int kTileB = F::kTileB, kRing = 4, kSlots = 4 * L::kSteps, kAhead = 8;
-  constexpr int kStatB = 8 * kDkvRows;
+  using F = DkvFetch<D, R, T>;
+  constexpr int kTileB = F::kTileB, kRing = D == 128 ? 2 : 3;
+  constexpr int kVSegs = 128 * 2 * D / 1024 / 4, kAhead = 3;
   typedef const float4_t __attribute__((address_space(3))) * LdsF4;
   __shared__ __attribute__((aligned(16))) uint8_t ring[kRing][2][kTileB];
-  __shared__ __attribute__((aligned(16))) uint8_t stat[kRing][kStatB];
+  __shared__ __attribute__((aligned(16))) uint8_t vblk[128 * 2 * D];
+  __shared__ __attribute__((aligned(16))) uint8_t stat[kRing][8 * R];
   const void* const geom = (const void*)__builtin_amdgcn_kernarg_segment_ptr();
   DkvTask x;
-  if (!dkv_task(p, x)) return;
+  if (!dkv_task<R>(p, x)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const L ln(threadIdx.x & 63);
   const int kw = x.first + 32 * wave, my = kw + ln.col;
@@ -671,159 +712,104 @@ __global__ void __launch_bounds__(256, OCC) packed_dkv_kernel(const BwdGeom p) {
   for (int c = 0; c < L::kCols; ++c) dk[c] = dv[c] = zero16();
   bool again = false;
   if (x.steps > 0) {
-    F tiles(p, x, wave, ln.lane);
-    tiles.run(p, x, ring[0][0], stat[0]);
-    tiles.run(p, x, ring[1][0], stat[1]);
-    {  // tile -1: zeros
-      const i32x4_t none = rows_rsrc<2 * D>(p.q, 0, 0);
-      tiles.fq.run(none, ring[kRing - 1][0], wave);
-      tiles.fd.run(none, ring[kRing - 1][1], wave);
+    {
+      const TileFetch<D, kVSegs> f(wave, ln.lane, 2 * p.v_sr);
+      f.run(tile_rsrc<2 * D>(static_cast<const T*>(p.v) + (x.kv * p.v_sh + (long long)x.k0 * p.v_sr),
+                             2 * p.v_sr, x.first, x.nk, 128),
+            vblk, wave);
     }
-    V8 kf[L::kSteps], vf[L::kSteps];
+    F tiles(p, x, wave, ln.lane);
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) tiles.run(p, x, ring[i][0], stat[i]);
+    V8 kf[L::kSteps];
     ln.own_rows(static_cast<const T*>(p.k) + (x.kv * p.k_sh + (long long)x.k0 * p.k_sr), p.k_sr,
                 my, x.nk, kf);
-    ln.own_rows(static_cast<const T*>(p.v) + (x.kv * p.v_sh + (long long)x.k0 * p.v_sr), p.v_sr,
-                my, x.nk, vf);
     __builtin_amdgcn_s_waitcnt(0);
-    sync_ring<0>();
-
     const TileOps<D, T> ops(ln);
     const uint32_t lds_ring = (uint32_t)(uintptr_t)&ring[0][0][0];
+    const uint32_t lds_v = (uint32_t)(uintptr_t)&vblk[0] + wave * 32 * L::kRowB;
     const uint32_t lds_stat = (uint32_t)(uintptr_t)&stat[0][0] + 16 * ln.g;
-    // Slot 2u: s (u even) or dout v' (odd), step u / 2; slot 2u + 1: dv (even)
-    // or dk, columns u / 2 % kCols, rows 16 (u / 2 / kCols).
-    auto read_slot = [&](auto sl, uint32_t rows_t, int rows_b, uint32_t cols_t, int cols_b)
-                         __attribute__((always_inline)) {
-      constexpr int Lc = decltype(sl)::value, u = Lc >> 1, half = u & 1, idx = u >> 1;
-      if constexpr ((Lc & 1) == 0)
-        return ops.rows(rows_t, half * kTileB, rows_b, idx);
-      else
-        return ops.cols(cols_t, (1 - half) * kTileB, idx % L::kCols, 2 * cols_b + idx / L::kCols);
-    };
-    // Accumulators of s (which: 0) or dout v' (1) of a tile's block b, rows 8 g4 ..
-    auto start4 = [&](float16_t& to, uint32_t st, int b, int which, int g4)
-                      __attribute__((always_inline)) {
-      const float4_t y =
-          *(LdsF4)(uintptr_t)(st + 4 * (kDkvRows * which + 32 * b + 8 * g4));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) to[4 * g4 + e] = y[e];
-    };
-    // Hidden pairs of the block whose first row is `base`.
     const int lo = my - x.coff;  // queries from lo on see this lane's key
-    auto hide = [&](float16_t& to, int base) __attribute__((always_inline)) {
-      if (base + 32 <= x.nq && base + x.coff >= kw + 31) return;
-      const float hidden = p.scale > 0.0f ? ninf() : -ninf();
-      const int from = lo - base - 4 * ln.g, end = x.nq - base - 4 * ln.g;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int at = 8 * (e >> 2) + (e & 3);
-        if (at < from || at >= end) to[e] = hidden;
+    int t = x.t0, s = 0;
+#pragma unroll 1
+    for (int step = 0; step < x.steps; ++step) {
+      sync_ring<(kRing - 2) * F::kDma>();
+      {
+        const int to = s == 0 ? kRing - 1 : s - 1;
+        tiles.run(p, x, ring[to][0], stat[to]);
       }
-    };
-
-    float16_t S[2], X[2];  // scores and dout v', by the block's parity
-    V8 P[2][2], Q[2][2];   // p and ds
-    V8 ahead[kAhead];
-    int t = x.t0;
+      const uint32_t tile = lds_ring + s * 2 * kTileB, st = lds_stat + s * 8 * R;
+      s = s == kRing - 1 ? 0 : s + 1;
+      const int first = t * R;
+      if (++t == x.tbeg + x.per) t = x.tbeg;
+      // (queries of the tile that see one of this wave's keys)
+      if (min(first + R, x.nq) - 1 + x.coff < kw || kw >= x.nk) continue;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < R / 32; ++b) {
+        const int base = first + 32 * b;
+        float16_t S, X;
 #pragma unroll
-      for (int g4 = 0; g4 < 4; ++g4) {
-        start4(S[b], lds_stat, b, 0, g4);
-        start4(X[b], lds_stat, b, 1, g4);
-      }
-      hide(S[b], t * kDkvRows + 32 * b);
-    }
+        for (int g4 = 0; g4 < 4; ++g4) {
+          const float4_t y = *(LdsF4)(uintptr_t)(st + 4 * (32 * b + 8 * g4));
+          const float4_t z = *(LdsF4)(uintptr_t)(st + 4 * (R + 32 * b + 8 * g4));
 #pragma unroll
-    for (int st = 0; st < L::kSteps; ++st) {
-      S[0] = E::mfma(ops.rows(lds_ring, 0, 0, st), kf[st], S[0]);
-      X[0] = E::mfma(ops.rows(lds_ring, kTileB, 0, st), vf[st], X[0]);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) P[1][i] = Q[1][i] = (V8){0, 0, 0, 0, 0, 0, 0, 0};
-    static_for(std::make_integer_sequence<int, kAhead>{}, [&](auto i) __attribute__((always_inline)) {
-      ahead[decltype(i)::value] =
-          read_slot(i, lds_ring, 1, lds_ring + (kRing - 1) * 2 * kTileB, 1);
-    });
-
-    // Iteration i of parity `par`: rows_t / rows_b hold block i + 1, next_t /
-    // next_b block i + 2 (st_next its statistics, next_base its first row),
-    // cols_t / cols_b block i - 1, own_t / own_b block i.
-    auto block = [&](auto par, uint32_t rows_t, int rows_b, uint32_t next_t, int next_b,
-                     uint32_t cols_t, int cols_b, uint32_t own_t, int own_b, uint32_t st_next,
-                     int next_base, int slot) __attribute__((always_inline)) {
-      constexpr int kPar = decltype(par)::value, kOther = 1 - kPar;
-      V8 op[kSlots];
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) op[a] = ahead[a];
-      static_for(std::make_integer_sequence<int, kSlots>{}, [&](auto sl) __attribute__((always_inline)) {
-        constexpr int Lc = decltype(sl)::value, u = Lc >> 1, half = u & 1, idx = u >> 1;
-        if constexpr ((Lc & 1) == 0) {
-          if constexpr (half == 0)
-            S[kOther] = E::mfma(op[Lc], kf[idx], S[kOther]);
-          else
-            X[kOther] = E::mfma(op[Lc], vf[idx], X[kOther]);
-        } else {
-          constexpr int c = idx % L::kCols, tt = idx / L::kCols;
-          if constexpr (half == 0)
-            dv[c] = E::mfma(op[Lc], P[kOther][tt], dv[c]);
-          else
-            dk[c] = E::mfma(op[Lc], Q[kOther][tt], dk[c]);
+          for (int e = 0; e < 4; ++e) {
+            S[4 * g4 + e] = y[e];
+            X[4 * g4 + e] = z[e];
+          }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        // the next tile's fetches, spread over the first iteration of a tile
-        if constexpr (kPar == 0) {
-          constexpr int every = kSlots / F::kDma;
-          if constexpr (Lc % every == 0 && Lc / every < F::kDma)
-            tiles.dma(ring[slot][0], stat[slot], Lc / every);
+        if (base + 32 > x.nq || base + x.coff < kw + 31) {
+          const float hidden = p.scale > 0.0f ? ninf() : -ninf();
+          const int from = lo - base - 4 * ln.g, end = x.nq - base - 4 * ln.g;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int at = 8 * (e >> 2) + (e & 3);
+            if (at < from || at >= end) S[e] = hidden;
+          }
         }
-        constexpr int La = Lc + kAhead;
-        if constexpr (La < kSlots)
-          op[La] = read_slot(Ic<La>{}, rows_t, rows_b, cols_t, cols_b);
-        else
-          ahead[La - kSlots] = read_slot(Ic<La - kSlots>{}, next_t, next_b, own_t, own_b);
-        // block i's elements, done 4 slots before the end, and the start of
-        // block i + 2 in their place
-        static_for(std::make_integer_sequence<int, 16>{}, [&](auto el) __attribute__((always_inline)) {
-          constexpr int e = decltype(el)::value;
-          if constexpr (e * (kSlots - 4) / 16 == Lc) {
-            const float y = __builtin_amdgcn_exp2f(S[kPar][e] * p.scale_log2);
-            P[kPar][e >> 3][e & 7] = (T)y;
-            Q[kPar][e >> 3][e & 7] = (T)(y * X[kPar][e]);
-            if constexpr (e % 4 == 3) {
-              start4(S[kPar], st_next, next_b, 0, e / 4);
-              start4(X[kPar], st_next, next_b, 1, e / 4);
+// 4 kSteps slots of a product each: s, dout v', dv, dk.  A slot's operand
+        // is read kAhead slots before; p is taken beside dout v', ds beside dv.
+        constexpr int N = L::kSteps;
+        V8 op[4 * N], vo[N], P[2], Q[2];
+        auto read = [&](auto sl) __attribute__((always_inline)) {
+          constexpr int i = decltype(sl)::value, of = i / N, u = i % N;
+          if constexpr (of < 2) {
+            op[i] = ops.rows(tile, of * kTileB, b, u);
+            if constexpr (of == 1) vo[u] = ops.rows(lds_v, 0, 0, u);
+          } else {
+            op[i] = ops.cols(tile, (3 - of) * kTileB, u % L::kCols, 2 * b + u / L::kCols);
+          }
+        };
+        static_for(std::make_integer_sequence<int, kAhead>{}, read);
+        static_for(std::make_integer_sequence<int, 4 * N>{}, [&](auto sl) __attribute__((always_inline)) {
+          constexpr int i = decltype(sl)::value, of = i / N, u = i % N;
+          constexpr int c = u % L::kCols, tt = u / L::kCols, kEach = 16 / N;
+          if constexpr (of == 0)
+            S = E::mfma(op[i], kf[u], S);
+          else if constexpr (of == 1)
+            X = E::mfma(op[i], vo[u], X);
+          else if constexpr (of == 2)
+            dv[c] = E::mfma(op[i], P[tt], dv[c]);
+          else
+            dk[c] = E::mfma(op[i], Q[tt], dk[c]);
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (i + kAhead < 4 * N) read(Ic<i + kAhead>{});
+#pragma unroll
+          for (int e = u * kEach; e < (u + 1) * kEach; ++e) {
+            if constexpr (of == 1) {
+              S[e] = __builtin_amdgcn_exp2f(S[e] * p.scale_log2);
+              P[e >> 3][e & 7] = (T)S[e];
+            } else if constexpr (of == 2) {
+              Q[e >> 3][e & 7] = (T)(S[e] * X[e]);
             }
           }
+          __builtin_amdgcn_sched_barrier(0);
         });
-        __builtin_amdgcn_sched_barrier(0);
-      });
-      hide(S[kPar], next_base);
-    };
-#pragma unroll 1
-    for (int m = 0; m < x.steps; ++m) {
-      const uint32_t before = lds_ring + ((m + 3) & 3) * 2 * kTileB;
-      const uint32_t here = lds_ring + (m & 3) * 2 * kTileB;
-      const uint32_t after = lds_ring + ((m + 1) & 3) * 2 * kTileB;
-      const uint32_t st = lds_stat + ((m + 1) & 3) * kStatB;
-      const int slot = (m + 2) & 3;
-      if (++t == x.tbeg + x.per) t = x.tbeg;
-      const int base = t * kDkvRows;  // of tile m + 1
-      tiles.next(p, x);
-      block(Ic<0>{}, here, 1, after, 0, before, 1, here, 0, st, base, slot);
-      block(Ic<1>{}, after, 0, after, 1, here, 0, here, 1, st, base + 32, slot);
-      sync_ring_ahead<0, 15>();
-    }
-    // dv and dk of the last block
-    const uint32_t last = lds_ring + ((x.steps - 1) & 3) * 2 * kTileB;
-#pragma unroll
-    for (int u = 0; u < D / 16; ++u) {
-      const int c = u % L::kCols, tt = u / L::kCols;
-      dv[c] = E::mfma(ops.cols(last, kTileB, c, 2 + tt), P[1][tt], dv[c]);
-      dk[c] = E::mfma(ops.cols(last, 0, c, 2 + tt), Q[1][tt], dk[c]);
+      }
     }
     // A block with a key whose sums are not finite is walked again.
-    int* const redo = reinterpret_cast<int*>(stat);
+    __builtin_amdgcn_s_waitcnt(0);
+    int* const redo = reinterpret_cast<int*>(vblk);
     __syncthreads();
     if (threadIdx.x == 0) *redo = 0;
     __syncthreads();
@@ -833,7 +819,7 @@ __global__ void __launch_bounds__(256, OCC) packed_dkv_kernel(const BwdGeom p) {
     __syncthreads();
   }
   if (again)
-    dkv_checked<D, T>(geom, &ring[0][0][0], &stat[0][0]);
+    dkv_checked<D, R, T>(geom, &ring[0][0][0], &stat[0][0]);
   else
     dkv_store<D, T>(p, x, ln, my, dk, dv);
 }
@@ -881,7 +867,7 @@ hipError_t launch_bwd_dim(const BwdGeom& g, hipStream_t st) {
                      dim3((unsigned)packed_groups(g.rows, g.sequences, 32 * W, g.heads)),
                      dim3(64 * W), 0, st, g);
   hipLaunchKernelGGL(
-      (packed_dkv_kernel<D, T, 1>),
+      (packed_dkv_kernel<D, D == 128 ? 32 : 64, T>),
       dim3((unsigned)packed_groups(g.key_rows, g.sequences, 32 * W, g.kv_heads * g.parts)),
       dim3(64 * W), 0, st, g);
   if (g.parts > 1)
