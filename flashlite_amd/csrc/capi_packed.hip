@@ -103,16 +103,29 @@ int check_packed_pointers(const fl_packed_params* p, const char* who) {
 namespace fl {
 
 // Parts that a key block's queries are cut into, each a work-group with sums of
-// its own (packed_bwd.h): as many as bring the work-groups that the chip holds
-// at once, two a CU, or under a causal mask over long keys, where they differ
-// most, twice that (us).  B2 H16/2 N7000-8192 D 128 causal 3169 with one a CU,
-// 2117 with two, 1691 with four; B1 H8 N2048 D 64 causal 82.7, 74.5, 82.2; 8
-// sequences of 300-700, H16, not causal, with two 80, with four 101.
+// its own (packed_bwd.h): at most as many as bring the work-groups that the chip
+// holds at once, two a CU, or under a causal mask over long keys, where they
+// differ most, twice that (us).  B2 H16/2 N7000-8192 D 128 causal 3169 with one
+// a CU, 2117 with two, 1691 with four; B1 H8 N2048 D 64 causal 82.7, 74.5, 82.2;
+// 8 sequences of 300-700, H16, not causal, with two 80, with four 101.  Fewer
+// where the partial sums cost more than the shorter walks save: a tile of the
+// walk takes about 1 us, the join's launch 5, a part 0.3 a MB written and read
+// (4 sequences of 300-700, H8 D 64: one part 36.4, two 41.8, four 45.7; 4 of
+// 33-257, H8/2: one 39.7, two 31.5, four 27.1, eight 26.3; one of 300, H16/4
+// D 128: one 64.5, eight 37.9).
 int packed_bwd_parts(const fl_packed_params& p) {
   const int64_t groups = (p.key_rows / 128 + p.sequences) * p.kv_heads;
   const int64_t a_cu = p.causal && p.key_rows / p.sequences >= 4096 ? 4 : 2;
   const int64_t want = a_cu * device_cus();
-  return (int)std::min<int64_t>(4 * a_cu, std::max<int64_t>(1, (want + groups / 2) / groups));
+  const int64_t most = std::min<int64_t>(4 * a_cu, (want + groups / 2) / groups);
+  const int64_t tile = p.head_dim == 128 ? 32 : 64;
+  const double walk =
+      (double)(p.heads / p.kv_heads) * ((p.rows / p.sequences + tile - 1) / tile);
+  const double part = 0.3e-6 * p.kv_heads * p.key_rows * 2 * p.head_dim * 4;
+  int best = 1;
+  for (int n = 2; n <= most; ++n)
+    if (walk / n + 5 + n * part < walk / best + (best > 1 ? 5 + best * part : 0)) best = n;
+  return best;
 }
 
 }  // namespace fl
