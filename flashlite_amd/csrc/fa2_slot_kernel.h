@@ -139,7 +139,8 @@ fa2_fwd_slot_kernel(const T* Q, const T* __restrict__ K, const T* __restrict__ V
   int bh, qb = 0, qb2 = 0, nblk = 1;
   Geom own;
   if constexpr (GeomT::kPacked) {
-    if (!packed_problem<(PAIR ? 2 : 1) * kBr>(launch, Q, K, V, O, own, bh, qb)) return;
+    if (!packed_problem<(PAIR ? 2 : 1) * kBr, CAUSAL>(launch, Q, K, V, O, own, bh, qb))
+      return;
     if (PAIR) nqb = (own.seq_q + kBr - 1) / kBr;
   }
   const Geom& geom = problem_geom(launch, own);
@@ -453,7 +454,7 @@ fa2_fwd_slot_kernel(const T* Q, const T* __restrict__ K, const T* __restrict__ V
         if constexpr (GeomT::kPacked) {
           const int lim = min(rows.kv_lim, CAUSAL ? rows.my_d + 1 : rows.kv_lim) - (tbeg + t) * kBc;
           add_odd<64, T>(
-              rings.vslot(Ic<0>{}), va, rows.o, rows.g, [&](int j) { return j < lim; }, false,
+              rings.vslot(Ic<0>{}), va, rows.o, rows.g, [&](int j) { return j < lim; },
               [](int r) { return v_swz(r); });
         }
         rows.gemm2(va, Pc);

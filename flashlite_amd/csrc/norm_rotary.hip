@@ -380,13 +380,11 @@ __global__ void __launch_bounds__(256) norm_rotary_step_kernel(const NormGeom g)
 
 // Many rows: a work-group walks the heads of a tile of tokens (g.tile of
 // them), q's, then k's, then v's, 1 << g.across_log2 side by side, or blockIdx.y's
-// share of them.  The tile's
-// sines and cosines are computed once, into LDS: done by each thread for its
-// own pairs, with the loads of positions and frequencies, they cost as much as
-// the rows of several heads.
+// share of them.  The tile's sines and cosines are computed once, into LDS: done
+// by each thread for its own pairs, with the loads of positions and frequencies,
+// they cost as much as the rows of several heads.
 template <class T, int D, bool INTER, int V, int MODE>
-__global__ void __launch_bounds__(256, 4)
-    norm_rotary_kernel(const NormGeom g) {
+__global__ void __launch_bounds__(256, 4) norm_rotary_kernel(const NormGeom g) {
   constexpr int kThreads = D / (2 * V);  // a row
   constexpr bool kBack = MODE == kBackward;
   __shared__ float2 table[256 * V];  // {cosine, sine} [token][pair]
@@ -479,8 +477,7 @@ __global__ void __launch_bounds__(256, 4)
       while (end - step >= kMost) steps(std::integral_constant<int, kMost>{});
       if constexpr (kMost == 4)
         if (end - step >= 2) steps(std::integral_constant<int, 2>{});
-      if constexpr (kMost > 1)
-        if (end > step) steps(std::integral_constant<int, 1>{});
+      if (end > step) steps(std::integral_constant<int, 1>{});
     };
     walk(std::integral_constant<int, 0>{});
     walk(std::integral_constant<int, 1>{});
@@ -512,7 +509,6 @@ __global__ void __launch_bounds__(1024) norm_weight_kernel(const float* part, in
   }
   if (r == 0) out[c] = sums[0][threadIdx.x];
 }
-
 
 // Neighbouring threads go on to the next token, or where heads lie closer
 // together than rows first to the next of up to kAcross heads, so that a wave's

@@ -35,14 +35,6 @@ __device__ __forceinline__ void sequence_rows(const int32_t* starts, int i, int 
   count = min(max(starts[i + 1], begin), rows) - begin;
 }
 
-// Block of rank r among the sequences' blocks of BLOCK rows, counted from a
-// sequence's first: the higher its index j, the earlier its rank (under a
-// causal mask the heaviest first, over all sequences), up to kRanked
-// sequences; with more the sequences follow one another.  False past the last
-// block.  The search is the same in every wave and needs no table: f(l) =
-// sum_i max(blocks_i - l, 0) blocks have j >= l.
-constexpr int kRanked = 512;
-
 // The largest of a wave's values, none negative (as wave_scan).
 __device__ __forceinline__ int wave_max(int x) {
   x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));
@@ -54,32 +46,52 @@ __device__ __forceinline__ int wave_max(int x) {
   return __builtin_amdgcn_readlane(x, 63);
 }
 
-// Blocks of sequences base + 64 c + lane (0 past the last).
-template <int BLOCK, int N>
-__device__ __forceinline__ void sequence_blocks(const int32_t* starts, int sequences, int rows,
-                                                int base, int (&nb)[N]) {
-#pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const int i = min(base + 64 * c + (int)(threadIdx.x & 63), sequences);
-    const int begin = min(max(starts[i], 0), rows);
-    const int end = min(max(starts[min(i + 1, sequences)], begin), rows);
-    nb[c] = i < sequences ? (end - begin + BLOCK - 1) / BLOCK : 0;
-  }
-}
+// Block of rank r among the sequences' blocks of BLOCK rows, counted from a
+// sequence's first, which is the same in every wave and needs no table.  False:
+// no block.
+//
+// Under a causal mask, up to kRanked sequences, a lane each: the higher a
+// block's index j, the earlier its rank (the heaviest first, over all
+// sequences); f(l) = sum_i max(blocks_i - l, 0) blocks have j >= l.  More
+// sequences, and any without that mask, follow one another, the last block of
+// each first, which keeps neighbours in the L2 (us, ranked against one after
+// the other; causal bf16 H32/8 D 128: gradients of 16 sequences of 500-1500 593
+// and 649, of 32 of 64-2000 1402 and 1511, of 64 2945 and 2943, of 100 4879 and
+// 4560; not causal, of 32 2617 and 2454, of 8 of 1000-3000 1936 and 1843, of one
+// of 4096 844 and 863).
+constexpr int kRanked = 64;
 
-template <int N>
-__device__ __forceinline__ bool ranked_block(const int (&nb)[N], int r, int& seq, int& j) {
-  auto above = [&](int l) __attribute__((always_inline)) {
-    int n = 0;
-#pragma unroll
-    for (int c = 0; c < N; ++c) n += max(nb[c] - l, 0);
-    return wave_sum(n);
-  };
-  int most = 0;
-#pragma unroll
-  for (int c = 0; c < N; ++c) most = max(most, nb[c]);
+template <int BLOCK>
+__device__ __forceinline__ bool packed_block(const int32_t* starts, int sequences, int rows, int r,
+                                             bool ranked, int& seq, int& j) {
+  const int lane = threadIdx.x & 63;
+  int begin, count;
+  if (!ranked || sequences > kRanked) {
+    // Sequence i has the ranks from begin_i / BLOCK + i on, one more than it
+    // may need: the last i that starts at or before r, 64 places a look.
+    int lo = 0, hi = sequences;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64, i = lo + step * lane;
+      const bool past = i >= hi || min(max(starts[i], 0), rows) / BLOCK + i > r;
+      const uint64_t at = __builtin_amdgcn_ballot_w64(past);
+      if (at & 1) return false;
+      lo += step * ((at == 0 ? 64 : __builtin_ctzll(at)) - 1);
+      hi = min(hi, lo + step);
+    }
+    sequence_rows(starts, lo, rows, begin, count);
+    seq = lo;
+    r -= begin / BLOCK + lo;
+    j = (count + BLOCK - 1) / BLOCK - 1 - r;
+    return r >= 0 && j >= 0;
+  }
+  int nb = 0;
+  if (lane < sequences) {
+    sequence_rows(starts, lane, rows, begin, count);
+    nb = (count + BLOCK - 1) / BLOCK;
+  }
+  auto above = [&](int l) __attribute__((always_inline)) { return wave_sum(max(nb - l, 0)); };
   if (r >= above(0)) return false;
-  int lo = 0, hi = wave_max(most);  // above(lo) > r >= above(hi)
+  int lo = 0, hi = wave_max(nb);  // above(lo) > r >= above(hi)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (above(mid) > r)
@@ -89,50 +101,11 @@ __device__ __forceinline__ bool ranked_block(const int (&nb)[N], int r, int& seq
   }
   r -= above(lo + 1);  // the r-th sequence with a block lo
   j = lo;
-#pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const uint64_t has = __builtin_amdgcn_ballot_w64(nb[c] > lo);
-    const int n = __builtin_popcountll(has);
-    if (r < n) {
-      const int before = (int)__builtin_amdgcn_mbcnt_hi(
-          (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
-      seq = 64 * c + __builtin_ctzll(__builtin_amdgcn_ballot_w64(nb[c] > lo && before == r));
-      return true;
-    }
-    r -= n;
-  }
-  return false;
-}
-
-template <int BLOCK>
-__device__ __forceinline__ bool packed_block(const int32_t* starts, int sequences, int rows, int r,
-                                             int& seq, int& j) {
-  if (sequences <= 64) {
-    int nb[1];
-    sequence_blocks<BLOCK>(starts, sequences, rows, 0, nb);
-    return ranked_block(nb, r, seq, j);
-  }
-  int nb[kRanked / 64];
-  if (sequences <= kRanked) {
-    sequence_blocks<BLOCK>(starts, sequences, rows, 0, nb);
-    return ranked_block(nb, r, seq, j);
-  }
-  for (int base = 0; base < sequences; base += kRanked) {
-    sequence_blocks<BLOCK>(starts, sequences, rows, base, nb);
-#pragma unroll
-    for (int c = 0; c < kRanked / 64; ++c) {
-      const int upto = wave_scan(nb[c]);
-      const int n = __builtin_amdgcn_readlane(upto, 63);
-      if (r < n) {
-        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(r < upto));
-        seq = base + 64 * c + at;
-        j = __builtin_amdgcn_readlane(upto, at) - 1 - r;
-        return true;
-      }
-      r -= n;
-    }
-  }
-  return false;
+  const uint64_t has = __builtin_amdgcn_ballot_w64(nb > lo);
+  const int before = (int)__builtin_amdgcn_mbcnt_hi(
+      (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+  seq = __builtin_ctzll(__builtin_amdgcn_ballot_w64(nb > lo && before == r));
+  return true;
 }
 
 // Work-groups of blocks of `block` rows: at least what any sequences of these
@@ -158,12 +131,12 @@ __device__ __forceinline__ void packed_unit(int units, int xcds, int& r, int& un
 // The forward kernels' problem of this work-group: query block qb (of BLOCK
 // rows) of head bh as a dense problem of one sequence, query heads that share
 // a key head as a batch with key head stride 0.  False: no block.
-template <int BLOCK, class QPtr, class KPtr, class OPtr>
+template <int BLOCK, bool CAUSAL, class QPtr, class KPtr, class OPtr>
 __device__ __forceinline__ bool packed_problem(const PackedGeom& p, QPtr& Q, KPtr& K, KPtr& V,
                                                OPtr& O, Geom& g, int& bh, int& qb) {
   int r, seq;
   packed_unit(p.heads, p.xcds, r, bh);
-  if (!packed_block<BLOCK>(p.starts, p.sequences, p.rows, r, seq, qb)) return false;
+  if (!packed_block<BLOCK>(p.starts, p.sequences, p.rows, r, CAUSAL, seq, qb)) return false;
   seq = __builtin_amdgcn_readfirstlane(seq);
   int q0, k0;
   sequence_rows(p.starts, seq, p.rows, q0, g.seq_q);
@@ -208,10 +181,10 @@ __device__ __forceinline__ bool any_odd(const float16_t (&x)[N]) {
 // A tile's transposed operands `op` (of D columns and 8192 / 2D rows) before
 // a product whose other factor is 0 for rows of the tile that a lane's own row
 // does not see: NaN and infinities become 0, and are added to the lanes that
-// see their row (as NaN where the factor may have any sign).
+// see their row.
 template <int D, class T, class Ops, class Sees, class Swizzle>
 __device__ __forceinline__ void add_odd(const uint8_t* tile, Ops& ops, float16_t (&acc)[D / 32],
-                                        int g, Sees&& sees, bool as_nan, Swizzle&& swizzle) {
+                                        int g, Sees&& sees, Swizzle&& swizzle) {
   using V8 = typename Elem<T>::v8;
   V8(&op)[8] = reinterpret_cast<V8(&)[8]>(ops);
   if (__builtin_amdgcn_ballot_w64(any_odd<T>(op)) == 0) return;
@@ -227,7 +200,7 @@ __device__ __forceinline__ void add_odd(const uint8_t* tile, Ops& ops, float16_t
       for (int e = 0; e < 8; ++e) {
         const float y = (float)x[e];
         if (mine && !(__builtin_fabsf(y) < __builtin_huge_valf()))
-          acc[c >> 1][8 * (c & 1) + e] += as_nan ? y - y : y;
+          acc[c >> 1][8 * (c & 1) + e] += y;
       }
     }
   }

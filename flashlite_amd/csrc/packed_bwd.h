@@ -278,7 +278,7 @@ template <int D, int W>
 __device__ __forceinline__ bool dq_task(const BwdGeom& p, DqTask& x) {
   int r, seq, qb;
   packed_unit(p.heads, p.xcds, r, x.head);
-  if (!packed_block<32 * W>(p.starts, p.sequences, p.rows, r, seq, qb)) return false;
+  if (!packed_block<32 * W>(p.starts, p.sequences, p.rows, r, p.causal, seq, qb)) return false;
   seq = __builtin_amdgcn_readfirstlane(seq);
   sequence_rows(p.starts, seq, p.rows, x.q0, x.nq);
   sequence_rows(p.key_starts, seq, p.key_rows, x.k0, x.nk);
@@ -512,7 +512,8 @@ __device__ __forceinline__ bool dkv_task(const BwdGeom& p, DkvTask& x) {
   int r, unit, seq, kb;
   packed_unit(p.kv_heads * p.parts, p.xcds, r, unit);
   constexpr int kBlock = 32 * kDkvWaves;
-  if (!packed_block<kBlock>(p.key_starts, p.sequences, p.key_rows, r, seq, kb)) return false;
+  if (!packed_block<kBlock>(p.key_starts, p.sequences, p.key_rows, r, p.causal, seq, kb))
+    return false;
   seq = __builtin_amdgcn_readfirstlane(seq);
   x.kv = unit / p.parts;
   x.part = unit - x.kv * p.parts;
@@ -573,8 +574,7 @@ struct DkvFetch {
       fq.seg(rq, slot, wave, i);
     else if (i < 2 * kSegs)
       fd.seg(rd, slot + kTileB, wave, i - kSegs);
-    else
-      {
+    else {
       const int at = 64 * (i - 2 * kSegs) + lane;  // {starts of s, of dout v'} [R]
       load_lds4(rst, 8 * (at % R) + 4 * (at / R), stat + 256 * (i - 2 * kSegs));
     }
@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(256, 2) packed_dkv_kernel(const BwdGeom p) {
             if (at < from || at >= end) S[e] = hidden;
           }
         }
-// 4 kSteps slots of a product each: s, dout v', dv, dk.  A slot's operand
+        // 4 kSteps slots of a product each: s, dout v', dv, dk.  A slot's operand
         // is read kAhead slots before; p is taken beside dout v', ds beside dv.
         constexpr int N = L::kSteps;
         V8 op[4 * N], vo[N], P[2], Q[2];

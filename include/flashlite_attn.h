@@ -359,8 +359,9 @@ int fl_attn_rotary_cache(const fl_rotary_params* p, const fl_cache_store* c, voi
  * Norms of q and k for each head with the rotary positions in the same pass:
  * y = R(x r w), r = 1 / sqrt(mean(x x) + eps) over a head's row, w its weight
  * plus weight_offset, R the rotation above with its scale; products and sums
- * in 32 bits, rounded once.  q_weight and k_weight are [head_dim], fp32 or of
- * the rows' dtype (weight_dtype); NULL: that tensor is only rotated.
+ * in 32 bits, rounded once (mean(x x) + eps below 2^-126 counts as 0).  q_weight
+ * and k_weight are [head_dim], fp32 or of the rows' dtype (weight_dtype); NULL:
+ * that tensor is only rotated.
  *
  * Positions may have several axes (time, height and width of a picture's
  * patches): with axes, int32 [pairs], pair j turns by the token's position on
@@ -497,9 +498,10 @@ int fl_attn_tree_fwd(const fl_tree_params* p, void* workspace, int64_t workspace
  * 16-byte aligned device memory that needs no initial values; calls that may
  * overlap must not share one.
  *
- * sm_scale is at least 1e-30 in size.  Row strides are below 2^24 elements, those of q, k, v and o at least head_dim;
- * rows and key_rows are at most 2^30, and all rows of k and of v lie within 2^31
- * bytes of a head's first.
+ * sm_scale is at least 1e-30 in size.  Row strides are below 2^24 elements,
+ * those of q, k, v and o at least head_dim; rows and key_rows are at most 2^30,
+ * sequences 2^24, and all rows of k and of v lie within 2^31 bytes of a head's
+ * first.
  */
 typedef struct fl_packed_params {
   const void* q;

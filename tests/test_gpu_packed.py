@@ -74,6 +74,16 @@ def test_packed_other_keys(cuda, dtype, d, causal, h, hk, lengths, keys):
     run(Problem(sum(keys) + d, dtype, d, h, hk, lengths, keys, causal, "rows", 1), cuda)
 
 
+@pytest.mark.parametrize("dtype,d", [("float16", 64), ("bfloat16", 128)])
+@pytest.mark.parametrize("lengths,keys", [
+    ([0, 1, 130, 5, 0, 0, 257, 2] * 66, [3, 0, 200, 5, 1, 0, 20, 300] * 66),
+    ([1, 0, 2] * 1500, None),
+])
+def test_packed_many_sequences(cuda, dtype, d, lengths, keys):
+    """More than a wave or eight of them look at once."""
+    run(Problem(6, dtype, d, 2, 1, lengths, keys, True, "rows", 3), cuda)
+
+
 @pytest.mark.parametrize("dtype,d", BOTH)
 @pytest.mark.parametrize("scale,q_scale", [(-0.3, 1.0), (1.0, 3.0), (0.02, 0.1)])
 def test_packed_scales(cuda, dtype, d, scale, q_scale):

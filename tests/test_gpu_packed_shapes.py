@@ -68,3 +68,44 @@ def test_more_keys_than_rows_over_long_sequences(cuda):
         p = Problem(h, "bfloat16", 128, h, h // 2, lengths, keys, True, "heads", 1)
         out, lse = fl.forward_packed(**p.device(cuda), return_lse=True)
         check(out, lse, p, reference(p, cuda))
+
+
+@pytest.mark.parametrize("dtype,d", [("float16", 64), ("bfloat16", 128)])
+@pytest.mark.parametrize("nan", [False, True])
+@pytest.mark.parametrize("h,hk,lengths,causal", [
+    (4, 1, [130, 0, 61], True), (2, 1, [700], True), (8, 2, [1450, 533, 1100, 900], True),
+    (8, 2, [4077], True), (8, 2, [4000, 4111], True), (16, 4, [4200], True),
+    (16, 16, [2301, 2050], False)])
+def test_out_over_q(cuda, dtype, d, nan, h, hk, lengths, causal):
+    """The output in q's own place, in each shape."""
+    import torch
+
+    p = Problem(sum(lengths) + 1, dtype, d, h, hk, lengths, None, causal, "heads", 2)
+    if nan:
+        p.v[0, 2 + lengths[0] // 2, 7] = float("nan")
+    a = p.device(cuda)
+    want = fl.forward_packed(**a)
+    a["q"] = a["q"].clone()
+    got = fl.forward_packed(**a, out=a["q"])
+    there = torch.from_numpy(p.inside()).to(cuda)
+    assert got.data_ptr() == a["q"].data_ptr()
+    assert torch.equal(torch.nan_to_num(got[:, :, there]), torch.nan_to_num(want[:, :, there]))
+    assert torch.equal(got.isnan()[:, :, there], want.isnan()[:, :, there])
+
+
+@pytest.mark.parametrize("dtype,d", [("float16", 64), ("bfloat16", 128)])
+@pytest.mark.parametrize("lengths", [[40, 0, 7], [300, 129]])
+def test_gradient_of_a_broadcast(cuda, dtype, d, lengths):
+    """dout of stride 0 along the heads, the rows, both: as one that is spelled
+    out, bit for bit."""
+    import torch
+
+    p = Problem(sum(lengths), dtype, d, 4, 2, lengths, None, True, "rows", 1)
+    a = p.device(cuda)
+    out, lse = fl.forward_packed(**a, return_lse=True)
+    dout = p.dout.nan_to_num().to(cuda)[None]
+    how = (a["q"], a["k"], a["v"], out, lse, a["starts"], None, a["sm_scale"], True)
+    for part in (dout[:, :1], dout[:, :, 3:4], dout[:, :1, 3:4]):
+        wide = part.expand_as(a["q"])
+        for x, y in zip(fl.backward_packed(wide, *how), fl.backward_packed(wide.contiguous(), *how)):
+            assert torch.equal(x.nan_to_num(), y.nan_to_num())
