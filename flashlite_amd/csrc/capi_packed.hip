@@ -110,9 +110,9 @@ namespace fl {
 // 8 sequences of 300-700, H16, not causal, with two 80, with four 101.  Fewer
 // where the partial sums cost more than the shorter walks save: a tile of the
 // walk takes about 1 us, the join's launch 5, a part 0.3 a MB written and read
-// (4 sequences of 300-700, H8 D 64: one part 36.4, two 41.8, four 45.7; 4 of
-// 33-257, H8/2: one 39.7, two 31.5, four 27.1, eight 26.3; one of 300, H16/4
-// D 128: one 64.5, eight 37.9).
+// (with dq and dk, dv in two launches, 4 sequences of 300-700, H8 D 64: one part
+// 36.4, two 41.8, four 45.7; 4 of 33-257, H8/2: one 39.7, two 31.5, four 27.1,
+// eight 26.3; one of 300, H16/4 D 128: one 64.5, eight 37.9).
 int packed_bwd_parts(const fl_packed_params& p) {
   const int64_t groups = (p.key_rows / 128 + p.sequences) * p.kv_heads;
   const int64_t a_cu = p.causal && p.key_rows / p.sequences >= 4096 ? 4 : 2;

@@ -116,8 +116,7 @@ inline int64_t packed_groups(int64_t rows, int64_t sequences, int64_t block, int
 
 // Work-group -> (rank, unit) with `units` independent walks of a block (heads):
 // neighbouring units, which share keys, on one XCD where they divide evenly.
-__device__ __forceinline__ void packed_unit(int units, int xcds, int& r, int& unit) {
-  const int i = blockIdx.x;
+__device__ __forceinline__ void packed_unit(int i, int units, int xcds, int& r, int& unit) {
   if (units % xcds == 0) {
     const int per = units / xcds, k = i / xcds;
     r = k / per;
@@ -135,7 +134,7 @@ template <int BLOCK, bool CAUSAL, class QPtr, class KPtr, class OPtr>
 __device__ __forceinline__ bool packed_problem(const PackedGeom& p, QPtr& Q, KPtr& K, KPtr& V,
                                                OPtr& O, Geom& g, int& bh, int& qb) {
   int r, seq;
-  packed_unit(p.heads, p.xcds, r, bh);
+  packed_unit(blockIdx.x, p.heads, p.xcds, r, bh);
   if (!packed_block<BLOCK>(p.starts, p.sequences, p.rows, r, CAUSAL, seq, qb)) return false;
   seq = __builtin_amdgcn_readfirstlane(seq);
   int q0, k0;

@@ -5,23 +5,24 @@
 // ds = p (dout v' - delta):
 //   dv = p' dout    dk = scale ds' q    dq = scale ds k
 // p is taken again from q, k and lse, so nothing of the size of the scores is
-// kept.  Two kernels, each of which owns what it sums, so no atomics and the
-// same bits every time: one walks a query block's keys (3 products a pair: s,
-// dout v', dq) and leaves lse and delta in base 2 for the other, which walks a
-// key block's queries over all heads of its group (4 products: s, dout v', dv,
-// dk).  14 D flops a pair of a row and a key, 7 products where one kernel with
-// atomics would do with 5.
+// kept.  Two kinds of work-groups, each of which owns what it sums, so no atomics
+// and the same bits every time: one walks a query block's keys (3 products a
+// pair: s, dout v', dq) and leaves -lse / scale and -delta of its rows for the
+// other, which walks a key block's queries over all heads of its group (4
+// products: s, dout v', dv, dk) in a launch behind it.  14 D flops a pair of a row
+// and a key, 7 products where one kernel with atomics would do with 5.  Little
+// work is one launch of both kinds, with delta taken by either.
 //
 // Bound by the matrix cores and what feeds them: B4 H32/8 N4096 D 128 bf16 causal
-// 1810 us, 1.06 PFLOP/s of the 7 products, where a large library product has
-// 1.2; 16 sequences of 64-2000, H32/8 718 (a block's triangle and the sequences'
-// ends are walked whole), B2 H16/2 N7000-8192 fp16 1630; few short ones by
-// three launches (4 of 33-257, H8/2 D 64 26 us).
+// 1780 us, 1.08 PFLOP/s of the 7 products, where a large library product has
+// 1.2; 16 sequences of 64-2000, H32/8 690 (a block's triangle and the sequences'
+// ends are walked whole), B2 H16/2 N7000-8192 fp16 1580; few short ones by
+// launches and chains of loads (4 of 33-257, H8/2 D 64 17.5 us).
 //
 // Both kernels keep two waves a SIMD, the products of one among the exponentials
 // of the other.  One wave with 64 bytes more registers a lane, dv and dk one
 // block behind s and dout v' and the exponentials spread over all products, took
-// 2020 where two waves take 1810 (16 sequences 830 against 718: a work-group
+// 2020 where two waves then took 1810 (16 sequences 830 against 718: a work-group
 // alone on its CU leaves it idle at its start and end).
 //
 // Operands as in the forward kernels: a wave's own 32 rows stay in registers
@@ -275,9 +276,9 @@ struct DqTask {
 };
 
 template <int D, int W>
-__device__ __forceinline__ bool dq_task(const BwdGeom& p, DqTask& x) {
+__device__ __forceinline__ bool dq_task(const BwdGeom& p, int group, DqTask& x) {
   int r, seq, qb;
-  packed_unit(p.heads, p.xcds, r, x.head);
+  packed_unit(group, p.heads, p.xcds, r, x.head);
   if (!packed_block<32 * W>(p.starts, p.sequences, p.rows, r, p.causal, seq, qb)) return false;
   seq = __builtin_amdgcn_readfirstlane(seq);
   sequence_rows(p.starts, seq, p.rows, x.q0, x.nq);
@@ -296,7 +297,7 @@ template <int D, class T>
 struct DqRows {
   using L = BwdLane<D, T>;
   typename L::V8 qf[L::kSteps], df[L::kSteps];
-  float lse2, delta;
+  float lse, lse2, delta;
 
   __device__ __forceinline__ void load(const BwdGeom& p, const DqTask& x, const L& ln, int my) {
     typename L::V8 of[L::kSteps];
@@ -312,7 +313,7 @@ struct DqRows {
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)df[st][e], (float)of[st][e], sum);
     delta = pair_sum(sum);
-    const float lse = my < x.nq ? p.lse[(long long)x.head * p.rows + x.q0 + my] : 0.0f;
+    lse = my < x.nq ? p.lse[(long long)x.head * p.rows + x.q0 + my] : 0.0f;
     // (a row that sees nothing: p = 2^-inf)
     lse2 = lse == ninf() ? -ninf() : lse * 1.44269504088896341f;
   }
@@ -322,15 +323,16 @@ struct DqRows {
 // do not see kept from them.  (A function of its own: its registers are not
 // the kernel's.)
 template <int D, int W, class T>
-__device__ __attribute__((noinline)) void dq_checked(const void* geom, uint8_t* lds) {
+__device__ __attribute__((noinline)) void dq_checked(const void* geom, int group, uint8_t* lds) {
   using L = BwdLane<D, T>;
   using V8 = typename L::V8;
   using E = Elem<T>;
   lds = uniform(lds);
+  group = __builtin_amdgcn_readfirstlane(group);
   BwdGeom p;
   __builtin_memcpy(&p, geom, sizeof p);
   DqTask x;
-  if (!dq_task<D, W>(p, x)) return;
+  if (!dq_task<D, W>(p, group, x)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const L ln(threadIdx.x & 63);
   const int my = x.first + 32 * wave + ln.col;
@@ -379,17 +381,24 @@ __device__ __attribute__((noinline)) void dq_checked(const void* geom, uint8_t* 
            x.nq, p.scale, acc);
 }
 
-// dq of W x 32 query rows, and the rows' {-lse / scale, -delta}.
-template <int D, int W, class T>
-__global__ void __launch_bounds__(64 * W, 2) packed_dq_kernel(const BwdGeom p) {
+// What a row's scores and dout v' start from.
+__device__ __forceinline__ float2 row_stats(float lse, float delta, float scale) {
+  // (a row that sees nothing: p = 2^-inf)
+  return make_float2(lse == ninf() ? (scale > 0.0f ? ninf() : -ninf()) : -lse / scale, -delta);
+}
+
+using DqRing = uint8_t[3][2][kTileBytes];
+
+// dq of W x 32 query rows, and with STATS the rows' {-lse / scale, -delta}.
+template <int D, int W, bool STATS, class T>
+__device__ __forceinline__ void dq_body(const BwdGeom& p, int group, DqRing& ring) {
   using L = BwdLane<D, T>;
   using V8 = typename L::V8;
   using E = Elem<T>;
-  constexpr int kSegs = 8 / W, kSlots = 3, kAhead = 4;
-  __shared__ __attribute__((aligned(16))) uint8_t ring[kSlots][2][kTileBytes];
+  constexpr int kSegs = 8 / W, kAhead = 4;
   const void* const geom = (const void*)__builtin_amdgcn_kernarg_segment_ptr();
   DqTask x;
-  if (!dq_task<D, W>(p, x)) return;
+  if (!dq_task<D, W>(p, group, x)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const L ln(threadIdx.x & 63);
   const int qw = x.first + 32 * wave, my = qw + ln.col;
@@ -405,11 +414,8 @@ __global__ void __launch_bounds__(64 * W, 2) packed_dq_kernel(const BwdGeom p) {
   fetch(1, 1);
   DqRows<D, T> rows;
   rows.load(p, x, ln, my);
-  if (my < x.nq && ln.g == 0) {
-    const float lse = rows.lse2 * 0.693147180559945309f;
-    const float start = lse == -ninf() ? (p.scale > 0.0f ? ninf() : -ninf()) : -lse / p.scale;
-    p.stats[(long long)x.head * p.rows + x.q0 + my] = make_float2(start, -rows.delta);
-  }
+  if (STATS && my < x.nq && ln.g == 0)
+    p.stats[(long long)x.head * p.rows + x.q0 + my] = row_stats(rows.lse, rows.delta, p.scale);
   // (what the compiler sees of the loads is then done: no waits in the loop)
   __builtin_amdgcn_s_waitcnt(0);
   const TileOps<D, T> ops(ln);
@@ -493,10 +499,16 @@ __global__ void __launch_bounds__(64 * W, 2) packed_dq_kernel(const BwdGeom p) {
   const bool again = *redo != 0;
   __syncthreads();
   if (again)
-    dq_checked<D, W, T>(geom, &ring[0][0][0]);
+    dq_checked<D, W, T>(geom, group, &ring[0][0][0]);
   else
     ln.store(static_cast<T*>(p.dq) + (x.head * p.dq_sh + (long long)x.q0 * p.dq_sr), p.dq_sr, my,
              x.nq, p.scale, acc);
+}
+
+template <int D, int W, class T>
+__global__ void __launch_bounds__(64 * W, 2) packed_dq_kernel(const BwdGeom p) {
+  __shared__ __attribute__((aligned(16))) DqRing ring;
+  dq_body<D, W, true, T>(p, blockIdx.x, ring);
 }
 
 // A work-group's key block, and its share of the queries that see it.
@@ -508,9 +520,9 @@ struct DkvTask {
 constexpr int kDkvWaves = 4;
 
 template <int R>  // query rows of a tile
-__device__ __forceinline__ bool dkv_task(const BwdGeom& p, DkvTask& x) {
+__device__ __forceinline__ bool dkv_task(const BwdGeom& p, int group, DkvTask& x) {
   int r, unit, seq, kb;
-  packed_unit(p.kv_heads * p.parts, p.xcds, r, unit);
+  packed_unit(group, p.kv_heads * p.parts, p.xcds, r, unit);
   constexpr int kBlock = 32 * kDkvWaves;
   if (!packed_block<kBlock>(p.key_starts, p.sequences, p.key_rows, r, p.causal, seq, kb))
     return false;
@@ -534,11 +546,12 @@ __device__ __forceinline__ bool dkv_task(const BwdGeom& p, DkvTask& x) {
 
 // The tiles of a walk, one after the other: the queries of a head, then those
 // of the next.  A wave moves its share of q's and dout's rows and all of the
-// statistics (every wave to the same place: its own wait then covers them).
-template <int D, int R, class T>
+// statistics (every wave to the same place: its own wait then covers them), or
+// with OWN none of those.
+template <int D, int R, bool OWN, class T>
 struct DkvFetch {
   static constexpr int kTileB = R * 2 * D, kSegs = kTileB / 1024 / kDkvWaves;
-  static constexpr int kStats = R / 32;
+  static constexpr int kStats = OWN ? 0 : R / 32;
   static constexpr int kDma = 2 * kSegs + kStats;  // instructions of a wave
   const TileFetch<D, kSegs> fq, fd;
   int step, head, tile, wave, lane;
@@ -561,7 +574,7 @@ struct DkvFetch {
     rd = tile_rsrc<2 * D>(
         static_cast<const T*>(p.dout) + (h * p.do_sh + (long long)x.q0 * p.do_sr), 2 * p.do_sr,
         tile * R, rows, R);
-    rst = tile_rsrc<8>(p.stats + (h * p.rows + x.q0), 8, tile * R, rows, R);
+    if constexpr (!OWN) rst = tile_rsrc<8>(p.stats + (h * p.rows + x.q0), 8, tile * R, rows, R);
     ++step;
     if (++tile == x.tbeg + x.per) {
       tile = x.tbeg;
@@ -574,7 +587,7 @@ struct DkvFetch {
       fq.seg(rq, slot, wave, i);
     else if (i < 2 * kSegs)
       fd.seg(rd, slot + kTileB, wave, i - kSegs);
-    else {
+    else if constexpr (!OWN) {
       const int at = 64 * (i - 2 * kSegs) + lane;  // {starts of s, of dout v'} [R]
       load_lds4(rst, 8 * (at % R) + 4 * (at / R), stat + 256 * (i - 2 * kSegs));
     }
@@ -586,6 +599,54 @@ struct DkvFetch {
     for (int i = 0; i < kDma; ++i) dma(slot, stat, i);
   }
 };
+
+// Tiles whose statistics a work-group takes at a time, where it does so itself.
+constexpr int kOwnSteps = 16;
+
+// The statistics {starts of s, of dout v'} [R] of the next tiles of a walk, at
+// most kOwnSteps from `step` on, by all threads: D / 16 a row.  (Rows past the
+// last: 0, as loads give.)
+template <int D, int R, class T>
+__device__ __forceinline__ void own_stats(const BwdGeom& p, const DkvTask& x, int step, int& head,
+                                          int& t, float* stat) {
+  using V8 = typename Elem<T>::v8;
+  constexpr int kThreads = D / 16;
+  static_assert(R * kThreads == 256);
+  const int row = (int)threadIdx.x / kThreads, c = 16 * ((int)threadIdx.x % kThreads);
+  const int count = min(x.steps - step, kOwnSteps);
+#pragma unroll 2
+  for (int i = 0; i < count; ++i) {
+    const int r = t * R + row;
+    float2 s = make_float2(0.0f, 0.0f);
+    float sum = 0.0f, lse = 0.0f;
+    if (r < x.nq) {
+      const T* const d = static_cast<const T*>(p.dout) + (head * p.do_sh +
+                                                          (long long)(x.q0 + r) * p.do_sr + c);
+      const T* const o =
+          static_cast<const T*>(p.o) + (head * p.o_sh + (long long)(x.q0 + r) * p.o_sr + c);
+      lse = p.lse[(long long)head * p.rows + x.q0 + r];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const V8 a = *reinterpret_cast<const V8*>(d + 8 * h);
+        const V8 b = *reinterpret_cast<const V8*>(o + 8 * h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)a[e], (float)b[e], sum);
+      }
+    }
+#pragma unroll
+    for (int m = 1; m < kThreads; m *= 2) sum += __shfl_xor(sum, m);
+    if (r < x.nq) s = row_stats(lse, sum, p.scale);
+    if (c == 0) {
+      stat[2 * R * i + row] = s.x;
+      stat[2 * R * i + R + row] = s.y;
+    }
+    if (++t == x.tbeg + x.per) {
+      t = x.tbeg;
+      ++head;
+    }
+  }
+  __syncthreads();
+}
 
 template <int D, class T>
 __device__ __forceinline__ void dkv_store(const BwdGeom& p, const DkvTask& x,
@@ -607,22 +668,23 @@ __device__ __forceinline__ void dkv_store(const BwdGeom& p, const DkvTask& x,
 
 // The dk and dv kernel's block walked again, with NaN and infinities of queries
 // that do not see a key kept from it.
-template <int D, int R, class T>
-__device__ __attribute__((noinline)) void dkv_checked(const void* geom, uint8_t* lds,
+template <int D, int R, bool OWN, class T>
+__device__ __attribute__((noinline)) void dkv_checked(const void* geom, int group, uint8_t* lds,
                                                       uint8_t* stat) {
   using L = BwdLane<D, T>;
   using V8 = typename L::V8;
   using E = Elem<T>;
   lds = uniform(lds);
   stat = uniform(stat);
+  group = __builtin_amdgcn_readfirstlane(group);
   BwdGeom p;
   __builtin_memcpy(&p, geom, sizeof p);
   DkvTask x;
-  if (!dkv_task<R>(p, x)) return;
+  if (!dkv_task<R>(p, group, x)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const L ln(threadIdx.x & 63);
   const int my = x.first + 32 * wave + ln.col;
-  DkvFetch<D, R, T> tiles(p, x, wave, ln.lane);
+  DkvFetch<D, R, OWN, T> tiles(p, x, wave, ln.lane);
   V8 kf[L::kSteps], vf[L::kSteps];
   ln.own_rows(static_cast<const T*>(p.k) + (x.kv * p.k_sh + (long long)x.k0 * p.k_sr), p.k_sr, my,
               x.nk, kf);
@@ -632,12 +694,13 @@ __device__ __attribute__((noinline)) void dkv_checked(const void* geom, uint8_t*
 #pragma unroll
   for (int c = 0; c < L::kCols; ++c) dk[c] = dv[c] = zero16();
   const int lo = my - x.coff;  // queries from lo on see this lane's key
-  const float* const st = reinterpret_cast<const float*>(stat);
-  const uint8_t *const qt = lds, *const dt = lds + DkvFetch<D, R, T>::kTileB;
-  int t = x.t0;
+  float* const st = reinterpret_cast<float*>(stat);
+  const uint8_t *const qt = lds, *const dt = lds + DkvFetch<D, R, OWN, T>::kTileB;
+  int t = x.t0, own_head = x.kv * p.group + x.h0, own_t = x.t0;
 #pragma unroll 1
   for (int step = 0; step < x.steps; ++step) {
     tiles.run(p, x, lds, stat);
+    if (OWN && step % kOwnSteps == 0) own_stats<D, R, T>(p, x, step, own_head, own_t, st);
     sync_ring<0>();
 #pragma unroll 1
     for (int b = 0; b < R / 32; ++b) {
@@ -645,7 +708,7 @@ __device__ __attribute__((noinline)) void dkv_checked(const void* geom, uint8_t*
       float16_t sc, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int at = 32 * b + 8 * (i >> 2) + 4 * ln.g + (i & 3);
+        const int at = (OWN ? 2 * R * (step % kOwnSteps) : 0) + 32 * b + 8 * (i >> 2) + 4 * ln.g + (i & 3);
         sc[i] = st[at];
         dp[i] = st[R + at];
       }
@@ -688,22 +751,31 @@ __device__ __attribute__((noinline)) void dkv_checked(const void* geom, uint8_t*
 // for two waves a SIMD: the products of one run among the exponentials of the
 // other.  s and dout v' start from {-lse / scale, -delta} as accumulators, so p =
 // 2^(s c) and ds = p dp' need no further subtraction, and where a block has
-// hidden pairs those start from -inf.
-template <int D, int R, class T>
-__global__ void __launch_bounds__(256, 2) packed_dkv_kernel(const BwdGeom p) {
+// hidden pairs those start from -inf.  With OWN the work-group takes the
+// statistics of its few tiles itself, into LDS.
+template <int D, int R, bool OWN>
+struct DkvLds {
+  static constexpr int kRing = D == 128 ? 2 : 3;
+  uint8_t ring[kRing][2][R * 2 * D];
+  uint8_t vblk[128 * 2 * D];
+  uint8_t stat[OWN ? kOwnSteps : kRing][8 * R];
+};
+
+template <int D, int R, bool OWN, class T>
+__device__ __forceinline__ void dkv_body(const BwdGeom& p, int group, DkvLds<D, R, OWN>& lds) {
   using L = BwdLane<D, T>;
   using V8 = typename L::V8;
   using E = Elem<T>;
-  using F = DkvFetch<D, R, T>;
-  constexpr int kTileB = F::kTileB, kRing = D == 128 ? 2 : 3;
+  using F = DkvFetch<D, R, OWN, T>;
+  constexpr int kTileB = F::kTileB, kRing = DkvLds<D, R, OWN>::kRing;
+  auto& ring = lds.ring;
+  auto& vblk = lds.vblk;
+  auto& stat = lds.stat;
   constexpr int kVSegs = 128 * 2 * D / 1024 / 4, kAhead = 3;
   typedef const float4_t __attribute__((address_space(3))) * LdsF4;
-  __shared__ __attribute__((aligned(16))) uint8_t ring[kRing][2][kTileB];
-  __shared__ __attribute__((aligned(16))) uint8_t vblk[128 * 2 * D];
-  __shared__ __attribute__((aligned(16))) uint8_t stat[kRing][8 * R];
   const void* const geom = (const void*)__builtin_amdgcn_kernarg_segment_ptr();
   DkvTask x;
-  if (!dkv_task<R>(p, x)) return;
+  if (!dkv_task<R>(p, group, x)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const L ln(threadIdx.x & 63);
   const int kw = x.first + 32 * wave, my = kw + ln.col;
@@ -730,15 +802,17 @@ __global__ void __launch_bounds__(256, 2) packed_dkv_kernel(const BwdGeom p) {
     const uint32_t lds_v = (uint32_t)(uintptr_t)&vblk[0] + wave * 32 * L::kRowB;
     const uint32_t lds_stat = (uint32_t)(uintptr_t)&stat[0][0] + 16 * ln.g;
     const int lo = my - x.coff;  // queries from lo on see this lane's key
-    int t = x.t0, s = 0;
+    int t = x.t0, s = 0, own_head = x.kv * p.group + x.h0, own_t = x.t0;
 #pragma unroll 1
     for (int step = 0; step < x.steps; ++step) {
       sync_ring<(kRing - 2) * F::kDma>();
+      if (OWN && step % kOwnSteps == 0)
+        own_stats<D, R, T>(p, x, step, own_head, own_t, reinterpret_cast<float*>(&stat[0][0]));
       {
         const int to = s == 0 ? kRing - 1 : s - 1;
         tiles.run(p, x, ring[to][0], stat[to]);
       }
-      const uint32_t tile = lds_ring + s * 2 * kTileB, st = lds_stat + s * 8 * R;
+      const uint32_t tile = lds_ring + s * 2 * kTileB, st = lds_stat + (OWN ? step % kOwnSteps : s) * 8 * R;
       s = s == kRing - 1 ? 0 : s + 1;
       const int first = t * R;
       if (++t == x.tbeg + x.per) t = x.tbeg;
@@ -819,9 +893,29 @@ __global__ void __launch_bounds__(256, 2) packed_dkv_kernel(const BwdGeom p) {
     __syncthreads();
   }
   if (again)
-    dkv_checked<D, R, T>(geom, &ring[0][0][0], &stat[0][0]);
+    dkv_checked<D, R, OWN, T>(geom, group, &ring[0][0][0], &stat[0][0]);
   else
     dkv_store<D, T>(p, x, ln, my, dk, dv);
+}
+
+template <int D, int R, class T>
+__global__ void __launch_bounds__(256, 2) packed_dkv_kernel(const BwdGeom p) {
+  __shared__ __attribute__((aligned(16))) DkvLds<D, R, false> lds;
+  dkv_body<D, R, false, T>(p, blockIdx.x, lds);
+}
+
+// Little work: the work-groups of both kernels in one launch, `first` of them
+// dq's, none of which waits for another.
+template <int D, int R, class T>
+__global__ void __launch_bounds__(256, 2) packed_both_kernel(const BwdGeom p, int first) {
+  __shared__ __attribute__((aligned(16))) union {
+    DqRing ring;
+    DkvLds<D, R, true> lds;
+  } u;
+  if ((int)blockIdx.x < first)
+    dq_body<D, 4, false, T>(p, blockIdx.x, u.ring);
+  else
+    dkv_body<D, R, true, T>(p, blockIdx.x - first, u.lds);
 }
 
 // Sums the parts: a thread 4 columns of a key's dk and dv.
@@ -862,14 +956,21 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const BwdGeom p) {
 
 template <int D, class T>
 hipError_t launch_bwd_dim(const BwdGeom& g, hipStream_t st) {
-  constexpr int W = 4;
-  hipLaunchKernelGGL((packed_dq_kernel<D, W, T>),
-                     dim3((unsigned)packed_groups(g.rows, g.sequences, 32 * W, g.heads)),
-                     dim3(64 * W), 0, st, g);
-  hipLaunchKernelGGL(
-      (packed_dkv_kernel<D, D == 128 ? 32 : 64, T>),
-      dim3((unsigned)packed_groups(g.key_rows, g.sequences, 32 * W, g.kv_heads * g.parts)),
-      dim3(64 * W), 0, st, g);
+  constexpr int W = 4, R = D == 128 ? 32 : 64;
+  const int64_t a = packed_groups(g.rows, g.sequences, 32 * W, g.heads);
+  const int64_t b = packed_groups(g.key_rows, g.sequences, 32 * W, g.kv_heads * g.parts);
+  // One launch up to two rounds of two work-groups a CU, one and a half without
+  // a causal mask (us; two launches, one): 4 sequences of 33-257, H8/2 D 64 25.8,
+  // 17.5; 4 of 300-700, H8 36.2, 26.2; one of 2048, H4 58.8, 42.7; of 1024, H32/8
+  // D 128 81.9, 72.2; of 8192, H1 257, 218; above: 8 of 100-300, H32/8 60.2, 66.8;
+  // 16 of 64-2000 686, 904; not causal, 4096, H8 D 64 159, 169.
+  if (a + b <= (g.causal ? 4 : 3) * device_cus()) {
+    hipLaunchKernelGGL((packed_both_kernel<D, R, T>), dim3((unsigned)(a + b)), dim3(64 * W), 0, st,
+                       g, (int)a);
+  } else {
+    hipLaunchKernelGGL((packed_dq_kernel<D, W, T>), dim3((unsigned)a), dim3(64 * W), 0, st, g);
+    hipLaunchKernelGGL((packed_dkv_kernel<D, R, T>), dim3((unsigned)b), dim3(64 * W), 0, st, g);
+  }
   if (g.parts > 1)
     hipLaunchKernelGGL(
         (packed_join_kernel<D, T>),

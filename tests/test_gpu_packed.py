@@ -122,6 +122,24 @@ def test_nan_and_infinities_stay_where_they_are_seen(cuda, dtype, d):
         run(other, cuda)
 
 
+@pytest.mark.parametrize("dtype,d", BOTH)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("h,hk,lengths", [
+    (2, 1, [33, 67, 50] + [0] * 600),            # beyond what is ranked over all sequences
+    (18, 1, [110, 129, 0, 40] + [0] * 58),       # key blocks in parts
+])
+def test_gradients_in_two_launches(cuda, dtype, d, causal, h, hk, lengths):
+    """More work-groups than one launch takes for dq with dk and dv (empty
+    sequences have work-groups too), with and without NaN and infinities."""
+    for plant in (None, ("v", 40, np.nan)) if h > 2 else (None, ("dout", 70, np.inf),
+                                                          ("k", 99, np.nan)):
+        p = Problem(h + d, dtype, d, h, hk, lengths, None, causal, "rows", 2)
+        if plant is not None:
+            name, row, value = plant
+            getattr(p, name)[0, 2 + row, 5] = value
+        run(p, cuda)
+
+
 def test_gradient_against_differences(cuda):
     """Directional differences of sum(dout out) in 64 bits of the oracle, which
     the kernel's gradients must follow: |g . e - slope| within the step's third
