@@ -46,9 +46,14 @@ __device__ __forceinline__ int wave_max(int x) {
   return __builtin_amdgcn_readlane(x, 63);
 }
 
-// Block of rank r among the sequences' blocks of BLOCK rows, counted from a
-// sequence's first, which is the same in every wave and needs no table.  False:
-// no block.
+// A block of a sequence's rows (its j-th, of those that are cut into blocks), and
+// the sequence's rows among those and among the others.
+struct PackedAt {
+  int j, begin, count, other, others;
+};
+
+// Block of rank r among the sequences' blocks of BLOCK rows, which is the same in
+// every wave and needs no table.  False: no block.
 //
 // Under a causal mask, up to kRanked sequences, a lane each: the higher a
 // block's index j, the earlier its rank (the heaviest first, over all
@@ -62,11 +67,12 @@ __device__ __forceinline__ int wave_max(int x) {
 constexpr int kRanked = 64;
 
 template <int BLOCK>
-__device__ __forceinline__ bool packed_block(const int32_t* starts, int sequences, int rows, int r,
-                                             bool ranked, int& seq, int& j) {
+__device__ __forceinline__ bool packed_block(const int32_t* starts, int rows,
+                                             const int32_t* other_starts, int others,
+                                             int sequences, int r, bool ranked, PackedAt& x) {
   const int lane = threadIdx.x & 63;
-  int begin, count;
-  if (!ranked || sequences > kRanked) {
+  int begin = rows, count = 0;
+  if (sequences > kRanked) {
     // Sequence i has the ranks from begin_i / BLOCK + i on, one more than it
     // may need: the last i that starts at or before r, 64 places a look.
     int lo = 0, hi = sequences;
@@ -78,33 +84,49 @@ __device__ __forceinline__ bool packed_block(const int32_t* starts, int sequence
       lo += step * ((at == 0 ? 64 : __builtin_ctzll(at)) - 1);
       hi = min(hi, lo + step);
     }
-    sequence_rows(starts, lo, rows, begin, count);
-    seq = lo;
-    r -= begin / BLOCK + lo;
-    j = (count + BLOCK - 1) / BLOCK - 1 - r;
-    return r >= 0 && j >= 0;
+    sequence_rows(starts, lo, rows, x.begin, x.count);
+    sequence_rows(other_starts, lo, others, x.other, x.others);
+    r -= x.begin / BLOCK + lo;
+    x.j = (x.count + BLOCK - 1) / BLOCK - 1 - r;
+    return r >= 0 && x.j >= 0;
   }
-  int nb = 0;
+  // A lane a sequence: what the block needs of its own is then read across
+  // lanes, not loaded behind the search.
+  int other = 0, of_other = 0, seq;
   if (lane < sequences) {
     sequence_rows(starts, lane, rows, begin, count);
-    nb = (count + BLOCK - 1) / BLOCK;
+    sequence_rows(other_starts, lane, others, other, of_other);
   }
-  auto above = [&](int l) __attribute__((always_inline)) { return wave_sum(max(nb - l, 0)); };
-  if (r >= above(0)) return false;
-  int lo = 0, hi = wave_max(nb);  // above(lo) > r >= above(hi)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (above(mid) > r)
-      lo = mid;
-    else
-      hi = mid;
+  const int nb = (count + BLOCK - 1) / BLOCK;
+  if (ranked) {
+    auto above = [&](int l) __attribute__((always_inline)) { return wave_sum(max(nb - l, 0)); };
+    if (r >= above(0)) return false;
+    int lo = 0, hi = wave_max(nb);  // above(lo) > r >= above(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (above(mid) > r)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    r -= above(lo + 1);  // the r-th sequence with a block lo
+    x.j = lo;
+    const uint64_t has = __builtin_amdgcn_ballot_w64(nb > lo);
+    const int before = (int)__builtin_amdgcn_mbcnt_hi(
+        (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+    seq = __builtin_ctzll(__builtin_amdgcn_ballot_w64(nb > lo && before == r));
+  } else {
+    const int first = begin / BLOCK + lane;
+    const uint64_t past = __builtin_amdgcn_ballot_w64(lane >= sequences || first > r);
+    if (past & 1) return false;
+    seq = (past == 0 ? 64 : __builtin_ctzll(past)) - 1;
+    x.j = __builtin_amdgcn_readlane(first + nb, seq) - 1 - r;
+    if (x.j < 0) return false;
   }
-  r -= above(lo + 1);  // the r-th sequence with a block lo
-  j = lo;
-  const uint64_t has = __builtin_amdgcn_ballot_w64(nb > lo);
-  const int before = (int)__builtin_amdgcn_mbcnt_hi(
-      (uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
-  seq = __builtin_ctzll(__builtin_amdgcn_ballot_w64(nb > lo && before == r));
+  x.begin = __builtin_amdgcn_readlane(begin, seq);
+  x.count = __builtin_amdgcn_readlane(count, seq);
+  x.other = __builtin_amdgcn_readlane(other, seq);
+  x.others = __builtin_amdgcn_readlane(of_other, seq);
   return true;
 }
 
@@ -133,13 +155,15 @@ __device__ __forceinline__ void packed_unit(int i, int units, int xcds, int& r, 
 template <int BLOCK, bool CAUSAL, class QPtr, class KPtr, class OPtr>
 __device__ __forceinline__ bool packed_problem(const PackedGeom& p, QPtr& Q, KPtr& K, KPtr& V,
                                                OPtr& O, Geom& g, int& bh, int& qb) {
-  int r, seq;
+  int r;
+  PackedAt x;
   packed_unit(blockIdx.x, p.heads, p.xcds, r, bh);
-  if (!packed_block<BLOCK>(p.starts, p.sequences, p.rows, r, CAUSAL, seq, qb)) return false;
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  int q0, k0;
-  sequence_rows(p.starts, seq, p.rows, q0, g.seq_q);
-  sequence_rows(p.key_starts, seq, p.key_rows, k0, g.seq_k);
+  if (!packed_block<BLOCK>(p.starts, p.rows, p.key_starts, p.key_rows, p.sequences, r, CAUSAL, x))
+    return false;
+  qb = x.j;
+  const int q0 = x.begin, k0 = x.other;
+  g.seq_q = x.count;
+  g.seq_k = x.others;
   g.coff = g.seq_k - g.seq_q;
   g.heads = p.group;
   g.q_sb = p.q_sh * p.group;

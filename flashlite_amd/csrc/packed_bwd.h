@@ -277,15 +277,19 @@ struct DqTask {
 
 template <int D, int W>
 __device__ __forceinline__ bool dq_task(const BwdGeom& p, int group, DqTask& x) {
-  int r, seq, qb;
+  int r;
+  PackedAt at;
   packed_unit(group, p.heads, p.xcds, r, x.head);
-  if (!packed_block<32 * W>(p.starts, p.sequences, p.rows, r, p.causal, seq, qb)) return false;
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  sequence_rows(p.starts, seq, p.rows, x.q0, x.nq);
-  sequence_rows(p.key_starts, seq, p.key_rows, x.k0, x.nk);
+  if (!packed_block<32 * W>(p.starts, p.rows, p.key_starts, p.key_rows, p.sequences, r, p.causal,
+                            at))
+    return false;
+  x.q0 = at.begin;
+  x.nq = at.count;
+  x.k0 = at.other;
+  x.nk = at.others;
   x.coff = p.causal ? x.nk - x.nq : x.nk;  // query i sees keys up to i + coff
   x.kv = x.head / p.group;
-  x.first = qb * 32 * W;
+  x.first = at.j * 32 * W;
   constexpr int kRows = kTileBytes / (2 * D);
   x.tiles = max((min(x.nk, min(x.first + 32 * W, x.nq) + x.coff) + kRows - 1) / kRows, 0);
   return true;
@@ -521,18 +525,21 @@ constexpr int kDkvWaves = 4;
 
 template <int R>  // query rows of a tile
 __device__ __forceinline__ bool dkv_task(const BwdGeom& p, int group, DkvTask& x) {
-  int r, unit, seq, kb;
+  int r, unit;
+  PackedAt at;
   packed_unit(group, p.kv_heads * p.parts, p.xcds, r, unit);
   constexpr int kBlock = 32 * kDkvWaves;
-  if (!packed_block<kBlock>(p.key_starts, p.sequences, p.key_rows, r, p.causal, seq, kb))
+  if (!packed_block<kBlock>(p.key_starts, p.key_rows, p.starts, p.rows, p.sequences, r, p.causal,
+                            at))
     return false;
-  seq = __builtin_amdgcn_readfirstlane(seq);
   x.kv = unit / p.parts;
   x.part = unit - x.kv * p.parts;
-  sequence_rows(p.starts, seq, p.rows, x.q0, x.nq);
-  sequence_rows(p.key_starts, seq, p.key_rows, x.k0, x.nk);
+  x.q0 = at.other;
+  x.nq = at.others;
+  x.k0 = at.begin;
+  x.nk = at.count;
   // (the last index is the heaviest under a causal mask: the first keys)
-  x.first = ((x.nk + kBlock - 1) / kBlock - 1 - kb) * kBlock;
+  x.first = ((x.nk + kBlock - 1) / kBlock - 1 - at.j) * kBlock;
   x.coff = p.causal ? x.nk - x.nq : x.nk;
   x.tbeg = max(x.first - x.coff, 0) / R;
   x.per = max((x.nq + R - 1) / R - x.tbeg, 0);
