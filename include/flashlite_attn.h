@@ -500,8 +500,8 @@ int fl_attn_tree_fwd(const fl_tree_params* p, void* workspace, int64_t workspace
  *
  * sm_scale is at least 1e-30 in size.  Row strides are below 2^24 elements,
  * those of q, k, v and o at least head_dim; rows and key_rows are at most 2^30,
- * sequences 2^24, and all rows of k and of v lie within 2^31 bytes of a head's
- * first.
+ * sequences 2^24, and all rows of k and of v, and 128 more, lie within 2^31 bytes
+ * of a head's first.
  */
 typedef struct fl_packed_params {
   const void* q;

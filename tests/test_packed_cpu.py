@@ -58,6 +58,8 @@ PACKED = [
     (dict(v_stride=T2(64, 0)), capi.FL_ERR_UNSUPPORTED, "row stride of v"),
     (dict(q_stride=T2(64, 1 << 24)), capi.FL_ERR_UNSUPPORTED, "row stride of q"),
     (dict(key_rows=1 << 24), capi.FL_ERR_UNSUPPORTED, "2^31 bytes"),
+    (dict(key_rows=65, v_stride=T2(64, (1 << 30) // 65 // 8 * 8)), capi.FL_ERR_UNSUPPORTED,
+     "128 more"),
     (dict(k_stride=T2(-64, 128)), capi.FL_ERR_UNSUPPORTED, "k strides"),
 ]
 
