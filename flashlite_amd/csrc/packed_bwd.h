@@ -15,7 +15,7 @@
 //
 // Bound by the matrix cores and what feeds them: B4 H32/8 N4096 D 128 bf16 causal
 // 1780 us, 1.08 PFLOP/s of the 7 products, where a large library product has
-// 1.2; 16 sequences of 64-2000, H32/8 690 (a block's triangle and the sequences'
+// 1.2; 16 sequences of 64-2000, H32/8 675 (a block's triangle and the sequences'
 // ends are walked whole), B2 H16/2 N7000-8192 fp16 1580; few short ones by
 // launches and chains of loads (4 of 33-257, H8/2 D 64 17.5 us).
 //
@@ -621,7 +621,6 @@ __device__ __forceinline__ void own_stats(const BwdGeom& p, const DkvTask& x, in
   static_assert(R * kThreads == 256);
   const int row = (int)threadIdx.x / kThreads, c = 16 * ((int)threadIdx.x % kThreads);
   const int count = min(x.steps - step, kOwnSteps);
-#pragma unroll 2
   for (int i = 0; i < count; ++i) {
     const int r = t * R + row;
     float2 s = make_float2(0.0f, 0.0f);
